@@ -45,6 +45,11 @@ extern "C" {
 #define QSTE_E_BLOCK (-5)
 #define QSTE_E_ALIGN (-6)
 #define QSTE_E_SCRATCH (-7)
+#define QSTE_E_VALUE (-8)
+
+/* most tokens qste_token_logprobs lists, most entries a row of qste_distill has */
+#define QSTE_MAX_TOP 128
+#define QSTE_MAX_ENTRIES 1024
 
 /* Library version; bumps when an entry point's contract changes. */
 int qste_version(void);
@@ -475,6 +480,68 @@ int qste_embedding_backward(const int64_t* ids, int64_t count, const void* grad,
                             const uint8_t* packed, const float* scale, float* evidence,
                             float* grad_scale, int64_t rows, int64_t cols, void* workspace,
                             size_t workspace_bytes, void* stream);
+
+/* ---- scores of tokens, distillation from a teacher's top tokens ---------- */
+
+/* Rows of logits, in the four entry points below: outer * inner rows of
+ * `vocab` columns (at most 2^30), row (o, i) starting at element o *
+ * outer_stride + i * inner_stride of `logits` (any element: no alignment past
+ * the type's own; strides may be 0 or negative), its columns one element apart.  Everything per row is
+ * contiguous, row o * inner + i at that index.  z is a row of logits over
+ * `temperature` > 0, p its softmax, all computed in fp32; logits of -inf
+ * (masked tokens) have p = 0.  Row offsets are 64-bit.  No counterparts in
+ * the reference, which ends at a model's logits. */
+
+/* Per row: logprobs = ln p[tokens[row]]; entropy = -sum p ln p;
+ * top_tokens int64 [rows, top] the `top` (0 .. QSTE_MAX_TOP, at most vocab)
+ * largest logits' tokens in falling order, equal ones by the lowest token
+ * (-0 equals 0; NaN is the largest), and top_logprobs [rows, top] their ln p.
+ * tokens int64 may be NULL (logprobs is not written then).  A negative token
+ * marks a row that is not scored and not read: logprob and entropy 0, top
+ * tokens -1 with -inf.  A token >= vocab gives a NaN logprob.  A row of only
+ * -inf has logprobs -inf and entropy 0.  stats fp32 [rows, 2], or NULL, is
+ * what the backward reads. */
+int qste_token_logprobs(const void* logits, int dtype, int64_t outer, int64_t inner, int64_t outer_stride,
+                        int64_t inner_stride, int64_t vocab, const int64_t* tokens, double temperature, int64_t top,
+                        float* logprobs, float* entropy, float* top_logprobs, int64_t* top_tokens, float* stats,
+                        void* stream);
+
+/* grad [rows, vocab] in dtype (16-byte aligned), every element written: the
+ * logits' gradient (g ([j = token] - p_j) - h p_j (ln p_j + entropy)) /
+ * temperature for g = logprob_grad[row] and h = entropy_grad[row] (fp32; NULL
+ * is zeros), with the forward's entropy and stats.  Zeros where nothing
+ * flows back (g = h = 0, a row that is not scored, a row of only -inf). */
+int qste_token_logprobs_backward(const void* logits, int dtype, int64_t outer, int64_t inner, int64_t outer_stride,
+                                 int64_t inner_stride, int64_t vocab, const int64_t* tokens, double temperature,
+                                 const float* logprob_grad, const float* entropy_grad, const float* entropy,
+                                 const float* stats, void* grad, void* stream);
+
+/* Distillation from a teacher's top tokens.  Per row the teacher's log
+ * probabilities top_logprobs fp32 [rows, k] of top_tokens int64 [rows, k] (k 1
+ * .. QSTE_MAX_ENTRIES; a negative token is no entry, a token listed twice
+ * counts with the sum), taken at the same temperature.
+ *   tail = 0: q = softmax(top_logprobs), q_r = 0
+ *   tail = 1: q = exp(top_logprobs), q_r = max(0, 1 - sum q) against the
+ *             student's mass p_r outside the list (left out when p_r = 0)
+ *   losses = temperature^2 (sum q (ln q - ln p[token]) + q_r (ln q_r - ln p_r))
+ * A row without entries has the loss 0 and no gradient, and is not read; one
+ * with a token >= vocab a NaN loss and gradient; one of only -inf logits the loss inf
+ * and no gradient.  stats fp32 [rows, 4] (16-byte aligned), or NULL, is what
+ * qste_distill_backward reads.  With grad ([rows, vocab] in dtype, 16-byte
+ * aligned; NULL: the loss alone) the logits' gradient for the row weights
+ * loss_grad fp32 [rows] is written by the same pass:
+ *   loss_grad temperature (s p - q) for a listed token, loss_grad temperature
+ *   p (s - q_r / p_r) for another, s = sum q + q_r; zeros where loss_grad is 0. */
+int qste_distill(const void* logits, int dtype, int64_t outer, int64_t inner, int64_t outer_stride,
+                 int64_t inner_stride, int64_t vocab, const int64_t* top_tokens, const float* top_logprobs, int64_t k,
+                 double temperature, int tail, float* losses, float* stats, const float* loss_grad, void* grad,
+                 void* stream);
+
+/* The same gradient from an earlier call's stats, for weights known later. */
+int qste_distill_backward(const void* logits, int dtype, int64_t outer, int64_t inner, int64_t outer_stride,
+                          int64_t inner_stride, int64_t vocab, const int64_t* top_tokens, const float* top_logprobs,
+                          int64_t k, double temperature, int tail, const float* stats, const float* loss_grad,
+                          void* grad, void* stream);
 
 #ifdef __cplusplus
 }

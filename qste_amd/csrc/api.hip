@@ -3,6 +3,7 @@
 // synchronizes; every launch goes on the caller's stream.
 #include "common.hpp"
 #include "prep.hpp"
+#include "vocab_row.hpp"
 
 namespace qste {
 int launch_pack_coordinate(const int8_t*, uint8_t*, int64_t, int64_t, hipStream_t);
@@ -73,6 +74,14 @@ int launch_swiglu_backward_sums(const void*, const void*, const void*, int, void
 int launch_step_finish(float* const*, const int64_t*, int, const int64_t* const*, int, float, float, int64_t*,
                        hipStream_t);
 int launch_row_scale_backward(const void*, const void*, int, void*, int64_t, float, float, hipStream_t);
+int launch_token_logprobs(const vocab::Logits&, int, int64_t, const int64_t*, double, int64_t, float*, float*, float*,
+                          int64_t*, float*, hipStream_t);
+int launch_token_logprobs_backward(const vocab::Logits&, int, int64_t, const int64_t*, double, const float*,
+                                   const float*, const float*, const float*, void*, hipStream_t);
+int launch_distill(const vocab::Logits&, int, int64_t, const int64_t*, const float*, int64_t, double, int, float*,
+                   float*, const float*, void*, hipStream_t);
+int launch_distill_backward(const vocab::Logits&, int, int64_t, const int64_t*, const float*, int64_t, double, int,
+                            const float*, const float*, void*, hipStream_t);
 // fp32 products through bf16 limbs (gemm_mfma.hip): 0 bytes / return 1 when
 // the shape is not for them
 size_t f32_forward_workspace(int64_t, int64_t, int64_t);
@@ -125,6 +134,19 @@ bool ragged_backward(int dtype, int64_t samples, int64_t rows, int64_t cols, boo
                         static_cast<double>(rows) * cols * 4.0 / 17e6 + (rows % 64 ? 19.0 : 0.0) +
                         (cols % 64 ? 5.4 : 0.0) + (with_dx ? 3.2 + 0.0036 * rows : 0.0);
   return matrix < scalar;
+}
+
+// Whether rows of logits are what vocab_row.hpp's kernels take: every index
+// inside a row fits an int, and a row is a workgroup.
+int logits_ok(const void* logits, int dtype, int64_t outer, int64_t inner, int64_t vocab, double temperature) {
+  if (!dtype_ok(dtype)) return QSTE_E_DTYPE;
+  if (outer < 0 || inner < 0 || vocab <= 0 || vocab > vocab::kMaxVocab) return QSTE_E_SHAPE;
+  if (inner > 0 && outer > INT32_MAX / inner) return QSTE_E_SHAPE;
+  if (!(temperature > 0.0) || !(temperature < 1e30) || temperature < 1e-30) return QSTE_E_VALUE;
+  if (outer * inner == 0) return 0;
+  if (!logits) return QSTE_E_NULL;
+  if (reinterpret_cast<uintptr_t>(logits) % (dtype == QSTE_F32 ? 4 : 2)) return QSTE_E_ALIGN;
+  return 0;
 }
 
 struct BackwardLayout {
@@ -301,7 +323,7 @@ int fill_zero(float* p, int64_t n, hipStream_t s) {
 
 extern "C" {
 
-int qste_version(void) { return 2; }
+int qste_version(void) { return 3; }
 
 const char* qste_error_string(int code) {
   switch (code) {
@@ -312,6 +334,7 @@ const char* qste_error_string(int code) {
     case QSTE_E_WORKSPACE: return "qste: workspace missing or smaller than the *_workspace_bytes query";
     case QSTE_E_BLOCK: return "qste: momentum block size must be positive";
     case QSTE_E_ALIGN: return "qste: pointer alignment not supported";
+    case QSTE_E_VALUE: return "qste: temperature must be positive and finite";
     case QSTE_E_SCRATCH:
       return "qste: surface too large for the library's static scratch (qste_coordinate_update_static_limit)";
     default: return hipGetErrorString(static_cast<hipError_t>(code));
@@ -785,6 +808,60 @@ int qste_row_scale_backward(const void* exp_value, const void* grad, int dtype, 
   if (n == 0) return 0;
   if (!exp_value || !grad || !grad_log_scale) return QSTE_E_NULL;
   return launch_row_scale_backward(exp_value, grad, dtype, grad_log_scale, n, lo, hi, as_stream(stream));
+}
+
+int qste_token_logprobs(const void* logits, int dtype, int64_t outer, int64_t inner, int64_t outer_stride,
+                        int64_t inner_stride, int64_t vocab, const int64_t* tokens, double temperature, int64_t top,
+                        float* logprobs, float* entropy, float* top_logprobs, int64_t* top_tokens, float* stats,
+                        void* stream) {
+  if (int rc = logits_ok(logits, dtype, outer, inner, vocab, temperature)) return rc;
+  if (top < 0 || top > vocab || top > QSTE_MAX_TOP) return QSTE_E_SHAPE;
+  if (outer * inner == 0) return 0;
+  if (!entropy || (tokens && !logprobs) || (top && (!top_logprobs || !top_tokens))) return QSTE_E_NULL;
+  const vocab::Logits l{logits, inner, outer_stride, inner_stride, static_cast<int>(vocab)};
+  return launch_token_logprobs(l, dtype, outer * inner, tokens, temperature, top, logprobs, entropy, top_logprobs,
+                               top_tokens, stats, as_stream(stream));
+}
+
+int qste_token_logprobs_backward(const void* logits, int dtype, int64_t outer, int64_t inner, int64_t outer_stride,
+                                 int64_t inner_stride, int64_t vocab, const int64_t* tokens, double temperature,
+                                 const float* logprob_grad, const float* entropy_grad, const float* entropy,
+                                 const float* stats, void* grad, void* stream) {
+  if (int rc = logits_ok(logits, dtype, outer, inner, vocab, temperature)) return rc;
+  if (outer * inner == 0) return 0;
+  if (!entropy || !stats || !grad) return QSTE_E_NULL;
+  if (reinterpret_cast<uintptr_t>(grad) % 16) return QSTE_E_ALIGN;
+  const vocab::Logits l{logits, inner, outer_stride, inner_stride, static_cast<int>(vocab)};
+  return launch_token_logprobs_backward(l, dtype, outer * inner, tokens, temperature, logprob_grad, entropy_grad,
+                                        entropy, stats, grad, as_stream(stream));
+}
+
+int qste_distill(const void* logits, int dtype, int64_t outer, int64_t inner, int64_t outer_stride,
+                 int64_t inner_stride, int64_t vocab, const int64_t* top_tokens, const float* top_logprobs, int64_t k,
+                 double temperature, int tail, float* losses, float* stats, const float* loss_grad, void* grad,
+                 void* stream) {
+  if (int rc = logits_ok(logits, dtype, outer, inner, vocab, temperature)) return rc;
+  if (k < 1 || k > QSTE_MAX_ENTRIES) return QSTE_E_SHAPE;
+  if (outer * inner == 0) return 0;
+  if (!top_tokens || !top_logprobs || !losses || (grad && !loss_grad)) return QSTE_E_NULL;
+  if (reinterpret_cast<uintptr_t>(stats) % 16 || reinterpret_cast<uintptr_t>(grad) % 16) return QSTE_E_ALIGN;
+  const vocab::Logits l{logits, inner, outer_stride, inner_stride, static_cast<int>(vocab)};
+  return launch_distill(l, dtype, outer * inner, top_tokens, top_logprobs, k, temperature, tail != 0, losses, stats,
+                        loss_grad, grad, as_stream(stream));
+}
+
+int qste_distill_backward(const void* logits, int dtype, int64_t outer, int64_t inner, int64_t outer_stride,
+                          int64_t inner_stride, int64_t vocab, const int64_t* top_tokens, const float* top_logprobs,
+                          int64_t k, double temperature, int tail, const float* stats, const float* loss_grad,
+                          void* grad, void* stream) {
+  if (int rc = logits_ok(logits, dtype, outer, inner, vocab, temperature)) return rc;
+  if (k < 1 || k > QSTE_MAX_ENTRIES) return QSTE_E_SHAPE;
+  if (outer * inner == 0) return 0;
+  if (!top_tokens || !top_logprobs || !stats || !loss_grad || !grad) return QSTE_E_NULL;
+  if (reinterpret_cast<uintptr_t>(stats) % 16 || reinterpret_cast<uintptr_t>(grad) % 16) return QSTE_E_ALIGN;
+  const vocab::Logits l{logits, inner, outer_stride, inner_stride, static_cast<int>(vocab)};
+  return launch_distill_backward(l, dtype, outer * inner, top_tokens, top_logprobs, k, temperature, tail != 0, stats,
+                                 loss_grad, grad, as_stream(stream));
 }
 
 size_t qste_coordinate_update_static_limit(void) { return coordinate_update_static_limit(); }

@@ -34,6 +34,8 @@ __all__ = [
     "unpack_bits",
     "coordinate_update",
     "cuda_available",
+    "distill_backward",
+    "distill_forward",
     "embedding_backward",
     "packed_embedding",
     "evidence_from_packed",
@@ -47,6 +49,8 @@ __all__ = [
     "status",
     "swiglu_backward",
     "swiglu_forward",
+    "token_logprobs_backward",
+    "token_logprobs_forward",
     "unpack_rows",
 ]
 
@@ -903,3 +907,168 @@ def embedding_backward(ids: Tensor, grad: Tensor, packed: Tensor, scale: Tensor,
         _ptr(evidence), _ptr(grad_scale), rows, int(columns), _ptr(ws), ws.numel(), _stream(device))
     _lib.check(code, "embedding_backward")
     return evidence, grad_scale
+
+
+# ---------------------------------------------------------------------------
+# scores of tokens, distillation from a teacher's top tokens (no counterparts
+# in the reference)
+# ---------------------------------------------------------------------------
+
+MAX_TOP, MAX_ENTRIES, MAX_VOCAB = 128, 1024, 1 << 30
+
+
+def _logit_rows(logits: Tensor) -> tuple[Tensor, tuple[int, int, int, int, int]]:
+    """``logits`` and its rows as (outer, inner, outer_stride, inner_stride, vocab):
+    itself where the leading dimensions come down to two strides (any view
+    whose columns are adjacent, such as ``logits[:, :-1]``), else a copy."""
+
+    if logits.dim() == 0 or not 0 < logits.shape[-1] <= MAX_VOCAB:
+        raise ValueError(f"logits need a last dimension of 1 to {MAX_VOCAB} columns")
+    vocab = int(logits.shape[-1])
+    if logits.numel() == 0:
+        return logits, (0, 0, 0, 0, vocab)
+    groups = _merged_rows(logits)
+    if len(groups) > 2 or (vocab > 1 and logits.stride(-1) != 1):
+        logits = logits.contiguous()
+        groups = _merged_rows(logits)
+    (outer, outer_stride), (inner, inner_stride) = [(1, 0)] * (2 - len(groups)) + groups
+    return logits, (outer, inner, outer_stride, inner_stride, vocab)
+
+
+def _merged_rows(t: Tensor) -> list[tuple[int, int]]:
+    """(size, stride) of the leading dimensions, those that step alike as one."""
+
+    groups: list[tuple[int, int]] = []
+    for size, stride in zip(t.shape[:-1], t.stride()[:-1]):
+        if size == 1:
+            continue
+        if groups and groups[-1][1] == size * stride:
+            size *= groups.pop()[0]
+        groups.append((size, stride))
+    return groups
+
+
+def _temperature(value: float) -> float:
+    value = float(value)
+    if not 1e-30 <= value < 1e30:
+        raise ValueError(f"temperature must be positive and finite, got {value}")
+    return value
+
+
+def _row_tokens(tokens: Tensor, shape, what: str) -> Tensor:
+    """Token numbers of the given shape as contiguous int64."""
+
+    if tokens.dtype not in (torch.int64, torch.int32, torch.int16, torch.uint8):
+        raise TypeError(f"{what} must be integers, got {tokens.dtype}")
+    if tuple(tokens.shape) != tuple(shape):
+        raise ValueError(f"{what} have shape {tuple(tokens.shape)}, expected {tuple(shape)}")
+    return tokens.to(torch.int64).contiguous()
+
+
+def _row_weights(weights: Tensor | None, shape, what: str) -> Tensor | None:
+    if weights is None:
+        return None
+    if tuple(weights.shape) != tuple(shape):
+        raise ValueError(f"{what} has shape {tuple(weights.shape)}, expected {tuple(shape)}")
+    return _f32(weights)
+
+
+def token_logprobs_forward(logits: Tensor, tokens: Tensor | None, *, top: int = 0, temperature: float = 1.0,
+                           want_stats: bool = False):
+    """``(logprobs, entropy, top_logprobs, top_tokens, stats)`` of the rows of logits.
+
+    ``logits`` [..., vocab], ``tokens`` [...] or None (logprobs is None then); a
+    negative token marks a row that is not scored.  ``top_logprobs`` and
+    ``top_tokens`` [..., top] are None for ``top = 0``; ``stats`` fp32 [..., 2], what
+    ``token_logprobs_backward`` reads, is None unless asked for.  All but
+    ``top_tokens`` (int64) are fp32.
+    """
+
+    device = _require_gpu(logits, tokens)
+    code = _dtype_code(logits)
+    rows, layout = _logit_rows(logits.detach())
+    shape, vocab, top, temperature = logits.shape[:-1], layout[4], int(top), _temperature(temperature)
+    if not 0 <= top <= min(MAX_TOP, vocab):
+        raise ValueError(f"top must lie in 0 .. {min(MAX_TOP, vocab)}, got {top}")
+    tokens_i64 = None if tokens is None else _row_tokens(tokens, shape, "tokens")
+    entropy = torch.empty(shape, dtype=torch.float32, device=device)
+    logprobs = None if tokens is None else torch.empty_like(entropy)
+    top_logprobs = torch.empty(*shape, top, dtype=torch.float32, device=device) if top else None
+    top_tokens = torch.empty(*shape, top, dtype=torch.int64, device=device) if top else None
+    stats = torch.empty(*shape, 2, dtype=torch.float32, device=device) if want_stats else None
+    _lib.check(_lib.load().qste_token_logprobs(
+        _ptr(rows), code, *layout, _ptr(tokens_i64), temperature, top, _ptr(logprobs), _ptr(entropy),
+        _ptr(top_logprobs), _ptr(top_tokens), _ptr(stats), _stream(device)), "token_logprobs")
+    return logprobs, entropy, top_logprobs, top_tokens, stats
+
+
+def token_logprobs_backward(logits: Tensor, tokens: Tensor | None, logprob_grad: Tensor | None,
+                            entropy_grad: Tensor | None, entropy: Tensor, stats: Tensor, *,
+                            temperature: float = 1.0) -> Tensor:
+    """The logits' gradient, contiguous in their dtype, for gradients [...] of the
+    log probabilities and the entropies (None: zeros)."""
+
+    device = _require_gpu(logits, tokens, logprob_grad, entropy_grad, entropy, stats)
+    code = _dtype_code(logits)
+    rows, layout = _logit_rows(logits.detach())
+    shape, temperature = logits.shape[:-1], _temperature(temperature)
+    tokens_i64 = None if tokens is None else _row_tokens(tokens, shape, "tokens")
+    g = _row_weights(logprob_grad, shape, "logprob_grad")
+    h = _row_weights(entropy_grad, shape, "entropy_grad")
+    entropy_f32 = _row_weights(entropy, shape, "entropy")
+    stats_f32 = _row_weights(stats, (*shape, 2), "stats")
+    grad = torch.empty(logits.shape, dtype=logits.dtype, device=device)
+    _lib.check(_lib.load().qste_token_logprobs_backward(
+        _ptr(rows), code, *layout, _ptr(tokens_i64), temperature, _ptr(g), _ptr(h), _ptr(entropy_f32),
+        _ptr(stats_f32), _ptr(grad), _stream(device)), "token_logprobs_backward")
+    return grad
+
+
+def _teacher(logits: Tensor, top_tokens: Tensor, top_logprobs: Tensor) -> tuple[Tensor, Tensor]:
+    if top_tokens.dim() != logits.dim() or not 1 <= top_tokens.shape[-1] <= MAX_ENTRIES:
+        raise ValueError(f"top_tokens need the logits' leading dimensions and 1 to {MAX_ENTRIES} entries, "
+                         f"got {tuple(top_tokens.shape)}")
+    if not top_logprobs.dtype.is_floating_point:
+        raise TypeError(f"top_logprobs must be floating point, got {top_logprobs.dtype}")
+    shape = (*logits.shape[:-1], top_tokens.shape[-1])
+    return (_row_tokens(top_tokens, shape, "top_tokens"), _row_weights(top_logprobs, shape, "top_logprobs"))
+
+
+def distill_forward(logits: Tensor, top_tokens: Tensor, top_logprobs: Tensor, *, temperature: float = 1.0,
+                    tail: bool = False, loss_grad: Tensor | None = None, want_stats: bool = False):
+    """``(losses, stats, grad)``: the losses fp32 [...] of logits [..., vocab] against
+    a teacher's ``top_tokens`` and ``top_logprobs`` [..., k]; ``stats`` fp32 [..., 4], what
+    ``distill_backward`` reads, if asked for; and with ``loss_grad`` [...] the
+    logits' gradient for these weights, from the same pass, else None."""
+
+    device = _require_gpu(logits, top_tokens, top_logprobs, loss_grad)
+    code = _dtype_code(logits)
+    rows, layout = _logit_rows(logits.detach())
+    shape, temperature = logits.shape[:-1], _temperature(temperature)
+    tokens_i64, values = _teacher(logits, top_tokens, top_logprobs)
+    weights = _row_weights(loss_grad, shape, "loss_grad")
+    losses = torch.empty(shape, dtype=torch.float32, device=device)
+    stats = torch.empty(*shape, 4, dtype=torch.float32, device=device) if want_stats else None
+    grad = torch.empty(logits.shape, dtype=logits.dtype, device=device) if weights is not None else None
+    _lib.check(_lib.load().qste_distill(
+        _ptr(rows), code, *layout, _ptr(tokens_i64), _ptr(values), tokens_i64.shape[-1], temperature, int(tail),
+        _ptr(losses), _ptr(stats), _ptr(weights), _ptr(grad), _stream(device)), "distill")
+    return losses, stats, grad
+
+
+def distill_backward(logits: Tensor, top_tokens: Tensor, top_logprobs: Tensor, loss_grad: Tensor, stats: Tensor, *,
+                     temperature: float = 1.0, tail: bool = False) -> Tensor:
+    """The logits' gradient, contiguous in their dtype, for the weights ``loss_grad`` [...]."""
+
+    device = _require_gpu(logits, top_tokens, top_logprobs, loss_grad, stats)
+    code = _dtype_code(logits)
+    rows, layout = _logit_rows(logits.detach())
+    shape, temperature = logits.shape[:-1], _temperature(temperature)
+    tokens_i64, values = _teacher(logits, top_tokens, top_logprobs)
+    weights = _row_weights(loss_grad, shape, "loss_grad")
+    stats_f32 = _row_weights(stats, (*shape, 4), "stats")
+    grad = torch.empty(logits.shape, dtype=logits.dtype, device=device)
+    _lib.check(_lib.load().qste_distill_backward(
+        _ptr(rows), code, *layout, _ptr(tokens_i64), _ptr(values), tokens_i64.shape[-1], temperature, int(tail),
+        _ptr(stats_f32), _ptr(weights), _ptr(grad), _stream(device)), "distill_backward")
+    return grad

@@ -26,6 +26,7 @@ from torch.autograd import Function
 
 from . import kernels
 from .functional import swiglu
+from .losses import TokenScores, distillation_loss, distillation_loss_and_grad, token_logprobs
 
 # The originals, bound before ``packed_activations`` can patch them: the
 # wrappers call these for values the kernels do not produce, and a patched
@@ -780,6 +781,7 @@ __all__ = [
     "CELU", "Dropout", "ELU", "EXACT_REPLACEMENTS", "GELU", "Hardsigmoid", "Hardswish", "Hardtanh",
     "LeakyReLU", "Mish", "REPLACEMENTS", "ReLU", "ReLU6", "SELU", "SMOOTH_REPLACEMENTS", "SiLU",
     "Sigmoid", "Softplus", "Tanh", "celu", "dropout", "elementwise", "elu", "gelu", "hardsigmoid", "swiglu", "swiglu_mlp",
+    "TokenScores", "distillation_loss", "distillation_loss_and_grad", "token_logprobs",
     "hardswish", "hardtanh", "leaky_relu", "mish", "packed", "packed_activations", "relu",
     "relu6", "relu_square", "replace", "selu", "sigmoid", "silu", "softplus", "tanh",
 ]
