@@ -499,12 +499,15 @@ int qste_embedding_backward(const int64_t* ids, int64_t count, const void* grad,
  * tokens int64 may be NULL (logprobs is not written then).  A negative token
  * marks a row that is not scored and not read: logprob and entropy 0, top
  * tokens -1 with -inf.  A token >= vocab gives a NaN logprob.  A row of only
- * -inf has logprobs -inf and entropy 0.  stats fp32 [rows, 2], or NULL, is
- * what the backward reads. */
+ * -inf has logprobs -inf and entropy 0.  stats fp32 [rows, 2] (8-byte
+ * aligned), or NULL, is what the backward reads.  Needs
+ * qste_token_logprobs_workspace_bytes(outer * inner, vocab, dtype, top) bytes of
+ * workspace, 8-byte aligned (0 where rows are not cut into parts). */
+size_t qste_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int dtype, int64_t top);
 int qste_token_logprobs(const void* logits, int dtype, int64_t outer, int64_t inner, int64_t outer_stride,
                         int64_t inner_stride, int64_t vocab, const int64_t* tokens, double temperature, int64_t top,
                         float* logprobs, float* entropy, float* top_logprobs, int64_t* top_tokens, float* stats,
-                        void* stream);
+                        void* workspace, size_t workspace_bytes, void* stream);
 
 /* grad [rows, vocab] in dtype (16-byte aligned), every element written: the
  * logits' gradient (g ([j = token] - p_j) - h p_j (ln p_j + entropy)) /

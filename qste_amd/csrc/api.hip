@@ -74,8 +74,9 @@ int launch_swiglu_backward_sums(const void*, const void*, const void*, int, void
 int launch_step_finish(float* const*, const int64_t*, int, const int64_t* const*, int, float, float, int64_t*,
                        hipStream_t);
 int launch_row_scale_backward(const void*, const void*, int, void*, int64_t, float, float, hipStream_t);
+size_t token_logprobs_workspace(int64_t, int64_t, int, int64_t);
 int launch_token_logprobs(const vocab::Logits&, int, int64_t, const int64_t*, double, int64_t, float*, float*, float*,
-                          int64_t*, float*, hipStream_t);
+                          int64_t*, float*, void*, hipStream_t);
 int launch_token_logprobs_backward(const vocab::Logits&, int, int64_t, const int64_t*, double, const float*,
                                    const float*, const float*, const float*, void*, hipStream_t);
 int launch_distill(const vocab::Logits&, int, int64_t, const int64_t*, const float*, int64_t, double, int, float*,
@@ -810,17 +811,27 @@ int qste_row_scale_backward(const void* exp_value, const void* grad, int dtype, 
   return launch_row_scale_backward(exp_value, grad, dtype, grad_log_scale, n, lo, hi, as_stream(stream));
 }
 
+size_t qste_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int dtype, int64_t top) {
+  if (!dtype_ok(dtype) || rows <= 0 || rows > INT32_MAX || vocab <= 0 || vocab > vocab::kMaxVocab || top < 0 ||
+      top > QSTE_MAX_TOP)
+    return 0;
+  return token_logprobs_workspace(rows, vocab, dtype, top);
+}
+
 int qste_token_logprobs(const void* logits, int dtype, int64_t outer, int64_t inner, int64_t outer_stride,
                         int64_t inner_stride, int64_t vocab, const int64_t* tokens, double temperature, int64_t top,
                         float* logprobs, float* entropy, float* top_logprobs, int64_t* top_tokens, float* stats,
-                        void* stream) {
+                        void* workspace, size_t workspace_bytes, void* stream) {
   if (int rc = logits_ok(logits, dtype, outer, inner, vocab, temperature)) return rc;
   if (top < 0 || top > vocab || top > QSTE_MAX_TOP) return QSTE_E_SHAPE;
   if (outer * inner == 0) return 0;
   if (!entropy || (tokens && !logprobs) || (top && (!top_logprobs || !top_tokens))) return QSTE_E_NULL;
+  if (reinterpret_cast<uintptr_t>(stats) % 8 || reinterpret_cast<uintptr_t>(workspace) % 8) return QSTE_E_ALIGN;
+  const size_t need = token_logprobs_workspace(outer * inner, vocab, dtype, top);
+  if (need && (!workspace || workspace_bytes < need)) return QSTE_E_WORKSPACE;
   const vocab::Logits l{logits, inner, outer_stride, inner_stride, static_cast<int>(vocab)};
   return launch_token_logprobs(l, dtype, outer * inner, tokens, temperature, top, logprobs, entropy, top_logprobs,
-                               top_tokens, stats, as_stream(stream));
+                               top_tokens, stats, workspace, as_stream(stream));
 }
 
 int qste_token_logprobs_backward(const void* logits, int dtype, int64_t outer, int64_t inner, int64_t outer_stride,

@@ -123,8 +123,8 @@ __global__ __launch_bounds__(THREADS) void forward_kernel(Args a) {
   using T = typename W::T;
   const int64_t r = blockIdx.x;
   const int tid = threadIdx.x;
-  const Row<DT, THREADS> row(a.logits, r);
-  const int vocab = row.vocab;
+  const Row<DT, THREADS, 0> row(a.logits.row<T>(r), a.logits.vocab);
+  const int vocab = row.count;
   T* out = static_cast<T*>(a.grad) + r * vocab;
   float log_q[kMaxEntries / THREADS];
   const float mass = load_entries<THREADS>(a, r, t, log_q);
@@ -245,9 +245,9 @@ __global__ __launch_bounds__(kBackThreads) void backward_kernel(Args a, int part
   const int64_t r = blockIdx.x / parts;
   constexpr int kPart = kBackThreads * kBackRuns * W::E;
   const int from = static_cast<int>(blockIdx.x % parts) * kPart;
-  const Row<DT, kBackThreads> row(a.logits, r);
-  const int to = min(row.vocab, from + kPart);
-  T* out = static_cast<T*>(a.grad) + r * row.vocab;
+  const Row<DT, kBackThreads, 0> row(a.logits.row<T>(r), a.logits.vocab);
+  const int to = min(row.count, from + kPart);
+  T* out = static_cast<T*>(a.grad) + r * row.count;
   const float4 st = reinterpret_cast<const float4*>(a.stats)[r];
   const float m = st.x, sum = st.y, weight = st.z;
   const float g = a.loss_grad[r];
@@ -259,7 +259,7 @@ __global__ __launch_bounds__(kBackThreads) void backward_kernel(Args a, int part
   const float per_q = g * a.temperature, per_p = per_q / sum, per_other = per_p * st.w;
   row.each(from, to, [&](int first, auto& x) {
     constexpr int N = sizeof(x) / sizeof(x[0]);
-    if (first >= row.vocab) return;
+    if (first >= row.count) return;
 #pragma unroll
     for (int j = 0; j < N; ++j) x[j] = ex.of(ex.power(x[j])) * per_other;
     W::store(out + first, x);

@@ -8,14 +8,18 @@
 //   dz_j = (g ([j = token] - p_j) - h p_j (ln p_j + H)) / T
 // for the gradients g of the logprob and h of the entropy.
 #include "vocab_row.hpp"
+#ifndef SPLIT_ROWS
+#define SPLIT_ROWS 128
+#endif
 
 namespace qste {
 namespace scores {
 
 using namespace vocab;
 
-constexpr int kThreads = 512;
-constexpr int kCandidates = 1024;
+constexpr int kThreads = 256;
+constexpr int kCandidates = 1024, kRuns = 384;
+constexpr int kMaxParts = 32;
 
 struct Args {
   Logits logits;
@@ -27,6 +31,10 @@ struct Args {
   float* top_logprobs;
   int64_t* top_tokens;
   float* stats;  // [rows, 2]: m and the sum of the exponentials
+  // rows cut into parts: columns a part, and what each part leaves
+  int parts, part;
+  float* part_stats;       // [rows, parts, 3]: m, sum, moment
+  uint64_t* part_entries;  // [rows, parts, top], falling, zeros past a part's columns
 };
 
 // ---------------------------------------------------------------------------
@@ -34,9 +42,10 @@ struct Args {
 // ---------------------------------------------------------------------------
 
 struct Candidates {
-  int count;
-  uint32_t bound[16];
-  int scan[16];
+  int count, runs;
+  int scan[kThreads / kWave];
+  int first[kRuns];
+  float run[kRuns][8];
   uint64_t entry[kCandidates];  // key above ~column: larger is better, and no two are equal
 };
 
@@ -49,8 +58,7 @@ __device__ __forceinline__ void push(Candidates& c, float x, int column) {
   if (at < kCandidates) c.entry[at] = entry_of(x, column);
 }
 
-// The workgroup's count of `flag`s summed over its threads' v
-template <int THREADS>
+// The sum of the threads' v
 __device__ __forceinline__ int block_count(int v, int* scratch) {
   v = wave_sum(v);
   __syncthreads();
@@ -58,13 +66,13 @@ __device__ __forceinline__ int block_count(int v, int* scratch) {
   __syncthreads();
   int total = 0;
 #pragma unroll
-  for (int w = 0; w < THREADS / kWave; ++w) total += scratch[w];
+  for (int w = 0; w < kThreads / kWave; ++w) total += scratch[w];
   return total;
 }
 
 // The k-th largest key of the row, bit by bit from the top: one pass over
 // the row for each.
-template <int THREADS, int BITS, class R>
+template <int BITS, class R>
 __device__ uint32_t kth_key(const R& row, int k, int* scratch) {
   uint32_t found = 0;
   for (int bit = BITS - 1; bit >= 0; --bit) {
@@ -72,59 +80,47 @@ __device__ uint32_t kth_key(const R& row, int k, int* scratch) {
     int n = 0;
     row.each([&](int first, auto& x) {
       constexpr int N = sizeof(x) / sizeof(x[0]);
-      if (first < row.vocab)
+      if (first < row.count)
 #pragma unroll
         for (int j = 0; j < N; ++j) n += (key_of(x[j]) >> (32 - BITS)) >= at_least;
     });
-    if (block_count<THREADS>(n, scratch) >= k) found = at_least;
+    if (block_count(n, scratch) >= k) found = at_least;
   }
   return found;
 }
 
-// Fills c with at least the k best values of the row (few more).  A bound
-// that k values are sure to reach: with `waves` waves whose every lane holds
-// values, the r-th largest of a wave's lane maxima, r = ceil(k / waves), has r
-// values of that wave at or above it, so the least of them over the waves has
-// k.  What is at or above the bound is kept; where that is too much (long runs
-// of equal values, or rows in order), only what is above it, and its equals
-// from the lowest column up.
-template <int DT, int THREADS, class R>
-__device__ void collect(const R& row, float lane_max, int k, Candidates& c) {
-  constexpr int BITS = kKeyBits<DT>, SHIFT = 32 - BITS, E = R::E;
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-  const int whole_waves = min(THREADS / kWave, row.vocab / (kWave * E));
+// A key that k values of the row are sure to reach.  With `waves` waves whose
+// every lane holds values, the r-th largest of a wave's lane maxima, r = ceil(k
+// / waves), has r values of that wave at or above it, so the least of these
+// over the waves has k.  This is a wave's; 0 says that it knows none.
+template <int BITS>
+__device__ __forceinline__ uint32_t wave_bound(float lane_max, int r) {
+  const uint32_t mine = key_of(lane_max) >> (32 - BITS);
   uint32_t bound = 0;
-  if (whole_waves > 0 && wave < whole_waves) {
-    const int r = (k + whole_waves - 1) / whole_waves;
-    const uint32_t mine = key_of(lane_max) >> SHIFT;
 #pragma unroll
-    for (int bit = BITS - 1; bit >= 0; --bit) {
-      const uint32_t at_least = bound | 1u << bit;
-      if (__popcll(__ballot(mine >= at_least)) >= r) bound = at_least;
-    }
+  for (int bit = BITS - 1; bit >= 0; --bit) {
+    const uint32_t at_least = bound | 1u << bit;
+    if (__popcll(__ballot(mine >= at_least)) >= r) bound = at_least;
   }
-  __syncthreads();
-  if (lane == 0) c.bound[wave] = wave < whole_waves ? bound : 0xFFFFFFFFu;
-  if (threadIdx.x == 0) c.count = 0;
-  __syncthreads();
-  bound = c.bound[0];
-  for (int w = 1; w < whole_waves; ++w) bound = min(bound, c.bound[w]);
-  if (whole_waves == 0) bound = 0;
-  auto value = [](uint32_t b) {
-    const uint32_t full = b << SHIFT;
-    return b == 0 ? -INFINITY : value_of(full & 0x80000000u ? full : full | ((1u << SHIFT) - 1u));
-  };
-  float edge = value(bound);
-  row.each([&](int first, auto& x) {
-    constexpr int N = sizeof(x) / sizeof(x[0]);
-    if (first < row.vocab)
-#pragma unroll
-      for (int j = 0; j < N; ++j)
-        if (!(x[j] < edge)) push(c, x[j], first + j);
-  });
-  __syncthreads();
-  if (c.count <= kCandidates) return;
+  return bound;
+}
 
+// the value of such a key
+template <int BITS>
+__device__ __forceinline__ float edge_of(uint32_t bound) {
+  constexpr int SHIFT = 32 - BITS;
+  const uint32_t full = bound << SHIFT;
+  return bound == 0 ? -INFINITY : value_of(full & 0x80000000u ? full : full | ((1u << SHIFT) - 1u));
+}
+
+// More than kCandidates values at or above the edge (long runs of equal values,
+// or rows in order): at least the k best into c again, from what is above
+// the edge, raised to the k-th key where that is still too much, and its equals
+// from the lowest column up.
+template <int DT, class R>
+__device__ __forceinline__ void collect_many(const R& row, int from, float edge, int k, Candidates& c) {
+  constexpr int BITS = kKeyBits<DT>;
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   bool nan_edge = false;
   auto above = [&] {  // only what is above the edge
     __syncthreads();
@@ -132,19 +128,19 @@ __device__ void collect(const R& row, float lane_max, int k, Candidates& c) {
     __syncthreads();
     row.each([&](int first, auto& x) {
       constexpr int N = sizeof(x) / sizeof(x[0]);
-      if (first < row.vocab && !nan_edge)
+      if (first < row.count && !nan_edge)
 #pragma unroll
         for (int j = 0; j < N; ++j)
-          if (!(x[j] <= edge)) push(c, x[j], first + j);
+          if (!(x[j] <= edge)) push(c, x[j], from + first + j);
     });
     __syncthreads();
     return c.count;
   };
   int have = above();
   if (have > kCandidates) {
-    const uint32_t key = kth_key<THREADS, BITS>(row, k, c.scan);
-    nan_edge = key == 0xFFFFFFFFu >> SHIFT;
-    edge = value(key);
+    const uint32_t key = kth_key<BITS>(row, k, c.scan);
+    nan_edge = key == 0xFFFFFFFFu >> (32 - BITS);
+    edge = edge_of<BITS>(key);
     have = above();  // fewer than k
   }
   if (have >= k) return;
@@ -153,7 +149,7 @@ __device__ void collect(const R& row, float lane_max, int k, Candidates& c) {
     constexpr int N = sizeof(x) / sizeof(x[0]);
     if (have >= k) return;
     int mine = 0;
-    if (first < row.vocab)
+    if (first < row.count)
 #pragma unroll
       for (int j = 0; j < N; ++j) mine += nan_edge ? x[j] != x[j] : x[j] == edge;
     int upto = mine;  // this lane's and the lower lanes' of its wave
@@ -166,15 +162,15 @@ __device__ void collect(const R& row, float lane_max, int k, Candidates& c) {
     if (lane == kWave - 1) c.scan[wave] = upto;
     __syncthreads();
     int at = have + upto - mine, total = 0;
-    for (int w = 0; w < THREADS / kWave; ++w) {
+    for (int w = 0; w < kThreads / kWave; ++w) {
       if (w < wave) at += c.scan[w];
       total += c.scan[w];
     }
-    if (first < row.vocab)
+    if (first < row.count)
 #pragma unroll
       for (int j = 0; j < N; ++j)
         if (nan_edge ? x[j] != x[j] : x[j] == edge) {
-          if (at < k) c.entry[at] = entry_of(x[j], first + j);
+          if (at < k) c.entry[at] = entry_of(x[j], from + first + j);
           ++at;
         }
     have += total;
@@ -185,43 +181,111 @@ __device__ void collect(const R& row, float lane_max, int k, Candidates& c) {
 }
 
 // ---------------------------------------------------------------------------
-// forward: one workgroup a row
+// forward: one workgroup a row, or one for each part of it and one that joins them
 // ---------------------------------------------------------------------------
 
-template <int DT, int THREADS>
-__global__ __launch_bounds__(THREADS) void forward_kernel(Args a) {
-  __shared__ float scratch[THREADS / kWave];
+// A row that is not to be scored
+__device__ __forceinline__ void unscored(const Args& a, int64_t r) {
+  if (threadIdx.x == 0) {
+    a.logprobs[r] = 0.0f;
+    a.entropy[r] = 0.0f;
+    if (a.stats) reinterpret_cast<float2*>(a.stats)[r] = make_float2(0.0f, 1.0f);
+  }
+  for (int i = threadIdx.x; i < a.top; i += kThreads) {
+    a.top_logprobs[r * a.top + i] = -INFINITY;
+    a.top_tokens[r * a.top + i] = -1;
+  }
+}
+
+// A row's results but for its top tokens; returns ln S
+template <int DT>
+__device__ __forceinline__ float scored(const Args& a, int64_t r, int64_t token, float m, float sum, float moment) {
+  const float log_sum = logf(sum);
+  if (threadIdx.x == 0) {
+    if (a.tokens) {
+      float lp = -INFINITY;
+      if (token >= a.logits.vocab)
+        lp = NAN;
+      else if (sum != 0.0f)
+        lp = (Elem<DT>::load(a.logits.row<typename Elem<DT>::T>(r), token) - m) * a.inverse - log_sum;
+      a.logprobs[r] = lp;
+    }
+    const float h = sum == 0.0f ? 0.0f : log_sum - kLn2 * (moment / sum);
+    a.entropy[r] = h < 0.0f ? 0.0f : h;
+    if (a.stats) reinterpret_cast<float2*>(a.stats)[r] = make_float2(m, sum);
+  }
+  return log_sum;
+}
+
+__device__ __forceinline__ void write_top(const Args& a, int64_t r, int rank, uint64_t entry, float m, float sum,
+                                          float log_sum) {
+  const float x = value_of(static_cast<uint32_t>(entry >> 32));
+  a.top_logprobs[r * a.top + rank] = sum == 0.0f ? -INFINITY : (x - m) * a.inverse - log_sum;
+  a.top_tokens[r * a.top + rank] = static_cast<int64_t>(~static_cast<uint32_t>(entry));
+}
+
+template <int DT, int HELD, int WAVES_A_SIMD, bool SPLIT>
+__global__ __launch_bounds__(kThreads, WAVES_A_SIMD) void forward_kernel(Args a) {
+  constexpr int WAVES = kThreads / kWave, BITS = kKeyBits<DT>;
+  using R = Row<DT, kThreads, HELD>;
+  __shared__ float maxima[WAVES], sums[WAVES], moments[WAVES];
+  __shared__ uint32_t bounds[WAVES];
   __shared__ Candidates c;
-  const int64_t r = blockIdx.x;
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
+  const int64_t r = SPLIT ? blockIdx.x / static_cast<uint32_t>(a.parts) : blockIdx.x;
+  const int part = SPLIT ? blockIdx.x % static_cast<uint32_t>(a.parts) : 0;
   const int64_t token = a.tokens ? a.tokens[r] : 0;
-  if (token < 0) {  // not to be scored
-    if (tid == 0) {
-      a.logprobs[r] = 0.0f;
-      a.entropy[r] = 0.0f;
-      if (a.stats) {
-        a.stats[2 * r] = 0.0f;
-        a.stats[2 * r + 1] = 1.0f;
-      }
-    }
-    for (int i = tid; i < a.top; i += THREADS) {
-      a.top_logprobs[r * a.top + i] = -INFINITY;
-      a.top_tokens[r * a.top + i] = -1;
-    }
+  if (token < 0) {
+    if (!SPLIT) unscored(a, r);
     return;
   }
-  const Row<DT, THREADS> row(a.logits, r);
+  const int from = SPLIT ? part * a.part : 0;
+  const int to = SPLIT && part < a.parts - 1 ? from + a.part : a.logits.vocab;
+  const typename R::T* columns = a.logits.row<typename R::T>(r) + from;
+  const R row(columns, to - from);
+  const int top = min(a.top, row.count);
   float lane_max = -INFINITY;
-  row.each([&](int, auto& x) {
-    constexpr int N = sizeof(x) / sizeof(x[0]);
+  row.each([&](int, auto& x) { lane_max = max_of(lane_max, x); });
+
+  // the maximum, and an edge that `top` values reach
+  const int whole_waves = min(WAVES, row.count / (kWave * R::E));
+  const float wave_top = fold_max(lane_max);
+  uint32_t bound = 0;
+  if (top > 0 && whole_waves > 0) bound = wave_bound<BITS>(lane_max, (top + whole_waves - 1) / whole_waves);
+  if (lane == 0) {
+    maxima[wave] = wave_top;
+    bounds[wave] = wave < whole_waves ? bound : 0xFFFFFFFFu;
+  }
+  if (tid == 0) c.count = c.runs = 0;
+  __syncthreads();
+  float m = maxima[0];
+  bound = bounds[0];
 #pragma unroll
-    for (int j = 0; j < N; ++j) lane_max = fmaxf(lane_max, x[j]);
-  });
-  const float m = block_max<THREADS>(lane_max, scratch);
+  for (int w = 1; w < WAVES; ++w) {
+    m = fmaxf(m, maxima[w]);
+    bound = min(bound, bounds[w]);
+  }
+  if (whole_waves == 0) bound = 0;
+  const float edge = edge_of<BITS>(bound);
+
   const Exponent ex(m, a.scale);
   float sum = 0.0f, moment = 0.0f;
-  row.each([&](int, auto& x) {
+  row.each([&](int first, auto& x) {
     constexpr int N = sizeof(x) / sizeof(x[0]);
+    if (top > 0 && !(max_of(-INFINITY, x) < edge)) {
+      if (first < row.count) {
+        if constexpr (N == 1) {
+          push(c, x[0], from + first);
+        } else {  // kept whole, looked through below
+          const int at = atomicAdd(&c.runs, 1);
+          if (at < kRuns) {
+            c.first[at] = first;
+#pragma unroll
+            for (int j = 0; j < N; ++j) c.run[at][j] = x[j];
+          }
+        }
+      }
+    }
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       const float power = ex.power(x[j]), e = ex.of(power);
@@ -229,38 +293,155 @@ __global__ __launch_bounds__(THREADS) void forward_kernel(Args a) {
       moment = fmaf(e, fmaxf(power, -200.0f), moment);  // 0 where e is 0
     }
   });
-  sum = block_sum(sum, scratch);
-  moment = block_sum(moment, scratch);
-  const float log_sum = logf(sum);
-  if (tid == 0) {
-    if (a.tokens) {
-      float lp = -INFINITY;
-      if (token >= row.vocab)
-        lp = NAN;
-      else if (sum != 0.0f)
-        lp = (Elem<DT>::load(row.p, token) - m) * a.inverse - log_sum;
-      a.logprobs[r] = lp;
-    }
-    const float h = sum == 0.0f ? 0.0f : log_sum - kLn2 * (moment / sum);
-    a.entropy[r] = h < 0.0f ? 0.0f : h;
-    if (a.stats) {
-      a.stats[2 * r] = m;
-      a.stats[2 * r + 1] = sum;
-    }
+  sum = fold_sum(sum);
+  moment = fold_sum(moment);
+  if (lane == 0) {
+    sums[wave] = sum;
+    moments[wave] = moment;
   }
-  if (a.top == 0) return;
-  collect<DT, THREADS>(row, lane_max, a.top, c);
+  __syncthreads();
+  sum = sums[0];
+  moment = moments[0];
+#pragma unroll
+  for (int w = 1; w < WAVES; ++w) {
+    sum += sums[w];
+    moment += moments[w];
+  }
+  float log_sum = 0.0f;
+  const int64_t slot = r * a.parts + part;
+  if constexpr (SPLIT) {
+    if (tid < 3) a.part_stats[3 * slot + tid] = tid == 0 ? m : tid == 1 ? sum : moment;
+  } else {
+    log_sum = scored<DT>(a, r, token, m, sum, moment);
+  }
+  if (top == 0) return;
+
+  const int runs = c.runs;
+  if (runs <= kRuns) {
+    for (int i = tid; i < runs; i += kThreads) {
+      const int first = c.first[i];
+#pragma unroll
+      for (int j = 0; j < R::E; ++j)
+        if (!(c.run[i][j] < edge)) push(c, c.run[i][j], from + first + j);
+    }
+    __syncthreads();
+  }
+  if (runs > kRuns || c.count > kCandidates || sum != sum)  // a run's maximum passes over NaN
+    collect_many<DT>(Row<DT, kThreads, 0>(columns, to - from), from, edge, top, c);
   const int n = c.count;
-  for (int i = tid; i < n; i += THREADS) {
+  for (int i = tid; i < n; i += kThreads) {
     const uint64_t mine = c.entry[i];
     int rank = 0;
     for (int j = 0; j < n; ++j) rank += c.entry[j] > mine;
-    if (rank < a.top) {
-      const float x = value_of(static_cast<uint32_t>(mine >> 32));
-      a.top_logprobs[r * a.top + rank] = sum == 0.0f ? -INFINITY : (x - m) * a.inverse - log_sum;
-      a.top_tokens[r * a.top + rank] = static_cast<int64_t>(~static_cast<uint32_t>(mine));
+    if (rank >= top) continue;
+    if constexpr (SPLIT)
+      a.part_entries[slot * a.top + rank] = mine;
+    else
+      write_top(a, r, rank, mine, m, sum, log_sum);
+  }
+  if constexpr (SPLIT)
+    for (int i = top + tid; i < a.top; i += kThreads) a.part_entries[slot * a.top + i] = 0;
+}
+
+// The parts of a row as one: their sums against the common maximum, and the
+// best of their lists.  An entry's rank is its own place and, by a search
+// in each other list, how many there are larger.  With r = ceil(top / parts), r entries
+// of every part are at or above the least of the parts' r-th, so what lies
+// below that is left out beforehand.
+template <int DT>
+__global__ __launch_bounds__(kThreads) void join_kernel(Args a) {
+  extern __shared__ uint64_t lists[];  // [parts, top], then a rank for each
+  __shared__ float stats[3 * kMaxParts];
+  __shared__ unsigned long long edge;
+  const int tid = threadIdx.x, k = a.top, n = a.parts * k;
+  const int64_t r = blockIdx.x;
+  const int64_t token = a.tokens ? a.tokens[r] : 0;
+  if (token < 0) {
+    unscored(a, r);
+    return;
+  }
+  int* ranks = reinterpret_cast<int*>(lists + n);
+  if (tid < 3 * a.parts) stats[tid] = a.part_stats[3 * r * a.parts + tid];
+  for (int i = tid; i < n; i += kThreads) {
+    lists[i] = a.part_entries[r * n + i];
+    ranks[i] = 0;
+  }
+  if (tid == 0) edge = ~0ull;
+  __syncthreads();
+  if (k > 0 && tid < a.parts) atomicMin(&edge, static_cast<unsigned long long>(lists[tid * k + (k + a.parts - 1) / a.parts - 1]));
+  float m = -INFINITY;
+  for (int p = 0; p < a.parts; ++p) m = fmaxf(m, stats[3 * p]);
+  const Exponent ex(m, a.scale);
+  float sum = 0.0f, moment = 0.0f;
+  for (int p = 0; p < a.parts; ++p) {
+    const float lower = fmaxf(ex.power(stats[3 * p]), -200.0f), weight = ex.of(lower);  // a part of -inf only: its sums are 0
+    sum = fmaf(stats[3 * p + 1], weight, sum);
+    moment += weight * fmaf(stats[3 * p + 1], lower, stats[3 * p + 2]);
+  }
+  const float log_sum = scored<DT>(a, r, token, m, sum, moment);
+  if (k == 0) return;
+  __syncthreads();
+  for (int i = tid; i < n * a.parts; i += kThreads) {
+    const int at = i / a.parts, p = i - at * a.parts;
+    const uint64_t mine = lists[at];
+    if (mine < edge || mine == 0) continue;
+    int lo = 0, hi = k;  // entries of list p larger than mine
+    while (lo < hi) {
+      const int mid = (lo + hi) / 2;
+      if (lists[p * k + mid] > mine)
+        lo = mid + 1;
+      else
+        hi = mid;
+    }
+    if (lo) atomicAdd(&ranks[at], lo);
+  }
+  __syncthreads();
+  for (int i = tid; i < n; i += kThreads) {
+    const uint64_t mine = lists[i];
+    if (mine >= edge && mine != 0 && ranks[i] < k) write_top(a, r, ranks[i], mine, m, sum, log_sum);
+  }
+}
+
+struct Plan {
+  int parts, part;  // parts a row, columns a part (the last has the rest)
+};
+
+Plan forward_plan(int64_t rows, int64_t vocab, int dtype) {
+  const int64_t runs = runs_of(vocab, dtype), e = dtype == QSTE_F32 ? 4 : 8;
+  int64_t most = rows < SPLIT_ROWS ? 256 * 8 : 256 * 25;
+  Plan plan{1, 0};
+  if (runs > most) {
+    plan.parts = static_cast<int>((runs + most - 1) / most);
+    if (plan.parts > kMaxParts) plan.parts = static_cast<int>((runs + 256 * 25 - 1) / (256 * 25));
+    if (plan.parts > kMaxParts) plan.parts = 0;  // too long: one workgroup reads the row for each pass
+  }
+  if (plan.parts > 1) plan.part = static_cast<int>((runs + plan.parts - 1) / plan.parts * e);
+  return plan;
+}
+
+template <int DT, int HELD, int WAVES_A_SIMD>
+int forward_as(const Args& a, int64_t rows, hipStream_t s) {
+  if constexpr (HELD > 0) {
+    if (a.parts > 1) {
+      forward_kernel<DT, HELD, WAVES_A_SIMD, true><<<static_cast<unsigned>(rows * a.parts), kThreads, 0, s>>>(a);
+      if (int rc = static_cast<int>(hipGetLastError())) return rc;
+      join_kernel<DT><<<static_cast<unsigned>(rows), kThreads, static_cast<size_t>(a.parts) * a.top * 12, s>>>(a);
+      return static_cast<int>(hipGetLastError());
     }
   }
+  forward_kernel<DT, HELD, WAVES_A_SIMD, false><<<static_cast<unsigned>(rows), kThreads, 0, s>>>(a);
+  return static_cast<int>(hipGetLastError());
+}
+
+template <int DT>
+int forward(Args a, int64_t rows, const Plan& plan, hipStream_t s) {
+  a.parts = plan.parts ? plan.parts : 1;
+  a.part = plan.part;
+  if (plan.parts == 0) return forward_as<DT, 0, 4>(a, rows, s);
+  const int64_t runs = plan.parts > 1 ? plan.part / (DT == QSTE_F32 ? 4 : 8) : runs_of(a.logits.vocab, DT);
+  if (runs <= 256 * 8) return forward_as<DT, 8, 7>(a, rows, s);
+  if (runs <= 256 * 16) return forward_as<DT, 16, 5>(a, rows, s);
+  return forward_as<DT, 25, 4>(a, rows, s);
 }
 
 // ---------------------------------------------------------------------------
@@ -288,9 +469,9 @@ __global__ __launch_bounds__(kBackThreads) void backward_kernel(BackArgs a, int 
   const int64_t r = blockIdx.x / parts;
   constexpr int kPart = kBackThreads * kBackRuns * W::E;
   const int from = static_cast<int>(blockIdx.x % parts) * kPart;
-  const Row<DT, kBackThreads> row(a.logits, r);
-  const int to = min(row.vocab, from + kPart);
-  T* out = static_cast<T*>(a.grad) + r * row.vocab;
+  const Row<DT, kBackThreads, 0> row(a.logits.row<T>(r), a.logits.vocab);
+  const int to = min(row.count, from + kPart);
+  T* out = static_cast<T*>(a.grad) + r * row.count;
   const int64_t token = a.tokens ? a.tokens[r] : -1;
   const float m = a.stats[2 * r], sum = a.stats[2 * r + 1];
   float g = a.logprob_grad && token >= 0 ? a.logprob_grad[r] : 0.0f;
@@ -299,7 +480,7 @@ __global__ __launch_bounds__(kBackThreads) void backward_kernel(BackArgs a, int 
     zero_row<DT, kBackThreads>(out, from, to);
     return;
   }
-  if (token >= row.vocab) g = NAN;
+  if (token >= row.count) g = NAN;
   const Exponent ex(m, a.scale);
   // dz = e (flat + slope power), from p = e / S and ln p = ln2 power - ln S
   const float per = -a.inverse / sum;
@@ -308,7 +489,7 @@ __global__ __launch_bounds__(kBackThreads) void backward_kernel(BackArgs a, int 
   const float extra = g * a.inverse;
   row.each(from, to, [&](int first, auto& x) {
     constexpr int N = sizeof(x) / sizeof(x[0]);
-    if (first >= row.vocab) return;
+    if (first >= row.count) return;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       const float power = ex.power(x[j]), e = ex.of(power);
@@ -320,21 +501,27 @@ __global__ __launch_bounds__(kBackThreads) void backward_kernel(BackArgs a, int 
 
 }  // namespace scores
 
+size_t token_logprobs_workspace(int64_t rows, int64_t vocab, int dtype, int64_t top) {
+  const scores::Plan plan = scores::forward_plan(rows, vocab, dtype);
+  return plan.parts > 1 ? static_cast<size_t>(rows) * plan.parts * (top * 8 + 12) : 0;
+}
+
 int launch_token_logprobs(const vocab::Logits& logits, int dtype, int64_t rows, const int64_t* tokens,
                           double temperature, int64_t top, float* logprobs, float* entropy, float* top_logprobs,
-                          int64_t* top_tokens, float* stats, hipStream_t s) {
+                          int64_t* top_tokens, float* stats, void* workspace, hipStream_t s) {
   using namespace scores;
+  const Plan plan = forward_plan(rows, logits.vocab, dtype);
+  if (rows * (plan.parts > 1 ? plan.parts : 1) > INT32_MAX) return QSTE_E_SHAPE;
+  uint64_t* entries = plan.parts > 1 ? static_cast<uint64_t*>(workspace) : nullptr;
+  float* part_stats = plan.parts > 1 ? reinterpret_cast<float*>(entries + rows * plan.parts * top) : nullptr;
   const Args a{logits, tokens, static_cast<float>(1.4426950408889634 / temperature),
                static_cast<float>(1.0 / temperature), static_cast<int>(top), logprobs, entropy, top_logprobs,
-               top_tokens, stats};
-  const dim3 grid(static_cast<unsigned>(rows));
-  if (dtype == QSTE_F32)
-    forward_kernel<QSTE_F32, kThreads><<<grid, kThreads, 0, s>>>(a);
-  else if (dtype == QSTE_F16)
-    forward_kernel<QSTE_F16, kThreads><<<grid, kThreads, 0, s>>>(a);
-  else
-    forward_kernel<QSTE_BF16, kThreads><<<grid, kThreads, 0, s>>>(a);
-  return static_cast<int>(hipGetLastError());
+               top_tokens, stats, 1, 0, part_stats, entries};
+  switch (dtype) {
+    case QSTE_F32: return forward<QSTE_F32>(a, rows, plan, s);
+    case QSTE_F16: return forward<QSTE_F16>(a, rows, plan, s);
+    default: return forward<QSTE_BF16>(a, rows, plan, s);
+  }
 }
 
 int launch_token_logprobs_backward(const vocab::Logits& logits, int dtype, int64_t rows, const int64_t* tokens,

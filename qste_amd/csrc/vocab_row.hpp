@@ -24,8 +24,8 @@ struct Logits {
 
   template <class T>
   __device__ __forceinline__ const T* row(int64_t r) const {
-    const int64_t o = r / inner;
-    return static_cast<const T*>(p) + o * outer_stride + (r - o * inner) * inner_stride;
+    const uint32_t n = static_cast<uint32_t>(r), o = n / static_cast<uint32_t>(inner);  // rows fit 31 bits
+    return static_cast<const T*>(p) + o * outer_stride + (n - o * static_cast<uint32_t>(inner)) * inner_stride;
   }
 };
 
@@ -80,44 +80,85 @@ struct Wide {
   __device__ __forceinline__ static void store(T* p, const float (&x)[1]) { Elem<DT>::store(p, 0, x[0]); }
 };
 
-// A workgroup's view of one row: `each` calls f(first, x) for every run of E
-// columns (x: their values; -inf and first >= vocab where a thread has none)
-// and once more for the row's last vocab % E columns, one a thread.  The calls
-// go up through the columns by thread and then by call, and all threads make
-// the same calls, so f may hold barriers.
-template <int DT, int THREADS>
+// A workgroup's view of one row, or of a part of one: `each` calls f(first, x)
+// for every run of E columns (x: their values; -inf and first >= count where a
+// thread has none) and once more for the last count % E columns, one a thread.
+// The calls go up through the columns by thread and then by call, and all
+// threads make the same calls, so f may hold barriers.
+//
+// With HELD > 0 the columns are loaded once, HELD 16-byte runs a thread, and
+// stay in registers for every pass (up to THREADS * HELD runs); with HELD = 0
+// each pass reads them again.
+template <int DT, int THREADS, int HELD>
 struct Row {
   using W = Wide<DT>;
   using T = typename W::T;
   static constexpr int E = W::E;
+  static constexpr int kStep = THREADS * E;
   const T* p;
-  int vocab;
+  int count;
+  uint4 held[HELD > 0 ? HELD : 1];
+  float last;
 
-  __device__ __forceinline__ Row(const Logits& l, int64_t r) : p(l.row<T>(r)), vocab(l.vocab) {}
+  __device__ __forceinline__ Row(const T* columns, int n) : p(columns), count(n) {
+    if constexpr (HELD > 0) {
+      const int whole = count - count % E, mine = static_cast<int>(threadIdx.x) * E;
+#pragma unroll
+      for (int i = 0; i < HELD; ++i) {
+        held[i] = W::none();
+        if ((i + 1) * kStep <= whole)
+          held[i] = W::load(p + i * kStep + mine);
+        else if (i * kStep + mine < whole)
+          held[i] = W::load(p + i * kStep + mine);
+      }
+      const int at = whole + static_cast<int>(threadIdx.x);
+      last = at < count ? Elem<DT>::load(p, at) : -INFINITY;
+    }
+  }
 
-  // over the columns [from, to): `from` a multiple of THREADS * E, and `to` one or the row's end
+  // over the columns [from, to): `from` a multiple of kStep, and `to` one or the row's end
   template <class F>
   __device__ __forceinline__ void each(int from, int to, F&& f) const {
-    const int whole = vocab - vocab % E;
-    for (int at = from; at < to && at < whole; at += THREADS * E) {
-      const int first = at + static_cast<int>(threadIdx.x) * E;
-      const bool mine = first < whole;
-      float x[E];
-      W::unpack(mine ? W::load(p + first) : W::none(), x);
-      f(mine ? first : vocab, x);
+    const int whole = count - count % E;
+    int mine = static_cast<int>(threadIdx.x) * E;
+    if constexpr (HELD > 0) {
+      // a pass works its columns out anew: carried from pass to pass they would take a register for each run
+      asm volatile("" : "+v"(mine));
+#pragma unroll
+      for (int i = 0; i < HELD; ++i) {
+        if (i * kStep < whole) {
+          const int first = i * kStep + mine;
+          float x[E];
+          W::unpack(held[i], x);
+          f(first < whole ? first : count, x);
+        }
+      }
+    } else {
+      for (int at = from; at < to && at < whole; at += kStep) {
+        const int first = at + mine;
+        float x[E];
+        W::unpack(first < whole ? W::load(p + first) : W::none(), x);
+        f(first < whole ? first : count, x);
+      }
     }
-    if (to >= vocab && whole < vocab) {
-      const int first = whole + static_cast<int>(threadIdx.x);
-      const bool mine = first < vocab;
-      float x[1] = {mine ? Elem<DT>::load(p, first) : -INFINITY};
-      f(mine ? first : vocab, x);
+    if (to >= count && whole < count) {
+      const int at = whole + static_cast<int>(threadIdx.x);
+      float x[1];
+      if constexpr (HELD > 0)
+        x[0] = last;
+      else
+        x[0] = at < count ? Elem<DT>::load(p, at) : -INFINITY;
+      f(at < count ? at : count, x);
     }
   }
   template <class F>
   __device__ __forceinline__ void each(F&& f) const {
-    each(0, vocab, f);
+    each(0, count, f);
   }
 };
+
+// the 16-byte runs that a row of `vocab` columns has
+inline int64_t runs_of(int64_t vocab, int dtype) { return vocab / (dtype == QSTE_F32 ? 4 : 8); }
 
 // Zeros in the columns [from, to) of a row of gradients, from = 0 or a multiple of
 // 16-byte accesses past it.
@@ -130,6 +171,31 @@ __device__ __forceinline__ void zero_row(typename Elem<DT>::T* out, int from, in
   for (int i = whole + static_cast<int>(threadIdx.x); i < to; i += THREADS) W::store(out + i, zero);
 }
 
+// Reductions over a wave in data-parallel moves: lanes 1, 2, 4 and 8 apart
+// within rows of 16, then a row's last lane into the next one's, then the
+// lower half's last into the upper's; lane 63 ends with all.  A lane that
+// nothing reaches takes `idle`, the operation's neutral value.
+template <class F>
+__device__ __forceinline__ float wave_fold(float v, float idle, F&& f) {
+#define QSTE_FOLD(ctrl, rows)                                                                                  \
+  v = f(v, __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(idle), __float_as_int(v), ctrl, rows, 0xf, \
+                                                      false)))
+  QSTE_FOLD(0x111, 0xf);
+  QSTE_FOLD(0x112, 0xf);
+  QSTE_FOLD(0x114, 0xf);
+  QSTE_FOLD(0x118, 0xf);
+  QSTE_FOLD(0x142, 0xa);
+  QSTE_FOLD(0x143, 0xc);
+#undef QSTE_FOLD
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), kWave - 1));
+}
+__device__ __forceinline__ float fold_max(float v) {
+  return wave_fold(v, -INFINITY, [](float a, float b) { return fmaxf(a, b); });
+}
+__device__ __forceinline__ float fold_sum(float v) {
+  return wave_fold(v, 0.0f, [](float a, float b) { return a + b; });
+}
+
 template <int THREADS>
 __device__ __forceinline__ float block_max(float v, float* scratch) {
   v = wave_max(v);
@@ -140,6 +206,24 @@ __device__ __forceinline__ float block_max(float v, float* scratch) {
 #pragma unroll
   for (int w = 1; w < THREADS / kWave; ++w) best = fmaxf(best, scratch[w]);
   return best;
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c));
+  return d;
+}
+
+// The largest of m and x (NaN where x holds a signalling one, else the numbers')
+template <int N>
+__device__ __forceinline__ float max_of(float m, const float (&x)[N]) {
+  if constexpr (N == 1) {
+    return fmaxf(m, x[0]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; j += 2) m = max3(m, x[j], x[j + 1]);
+    return m;
+  }
 }
 
 // The exponentials of a row, 2^((z - m) c) with m the row's maximum and c =

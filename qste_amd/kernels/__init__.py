@@ -996,9 +996,12 @@ def token_logprobs_forward(logits: Tensor, tokens: Tensor | None, *, top: int = 
     top_logprobs = torch.empty(*shape, top, dtype=torch.float32, device=device) if top else None
     top_tokens = torch.empty(*shape, top, dtype=torch.int64, device=device) if top else None
     stats = torch.empty(*shape, 2, dtype=torch.float32, device=device) if want_stats else None
-    _lib.check(_lib.load().qste_token_logprobs(
+    lib = _lib.load()
+    nbytes = lib.qste_token_logprobs_workspace_bytes(entropy.numel(), vocab, code, top)
+    work = _workspace(nbytes, device) if nbytes else None
+    _lib.check(lib.qste_token_logprobs(
         _ptr(rows), code, *layout, _ptr(tokens_i64), temperature, top, _ptr(logprobs), _ptr(entropy),
-        _ptr(top_logprobs), _ptr(top_tokens), _ptr(stats), _stream(device)), "token_logprobs")
+        _ptr(top_logprobs), _ptr(top_tokens), _ptr(stats), _ptr(work), nbytes, _stream(device)), "token_logprobs")
     return logprobs, entropy, top_logprobs, top_tokens, stats
 
 

@@ -83,8 +83,9 @@ SIGNATURES = {
     "qste_embedding_backward_workspace_bytes": (_sz, [_i64, _i64]),
     "qste_embedding_backward": (_int, [_vp, _i64, _vp, _int, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _sz,
                                        _vp]),
+    "qste_token_logprobs_workspace_bytes": (_sz, [_i64, _i64, _int, _i64]),
     "qste_token_logprobs": (_int, [_vp, _int, _i64, _i64, _i64, _i64, _i64, _vp, _dbl, _i64, _vp, _vp, _vp, _vp, _vp,
-                                   _vp]),
+                                   _vp, _sz, _vp]),
     "qste_token_logprobs_backward": (_int, [_vp, _int, _i64, _i64, _i64, _i64, _i64, _vp, _dbl, _vp, _vp, _vp, _vp,
                                             _vp, _vp]),
     "qste_distill": (_int, [_vp, _int, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _dbl, _int, _vp, _vp, _vp, _vp,

@@ -17,7 +17,7 @@ def test_c_entry_points_refuse_before_any_launch():
     assert b"temperature" in lib.qste_error_string(-8)
 
     def score(*logits, temperature=1.0, top=0, entropy=16):
-        return lib.qste_token_logprobs(*logits, None, temperature, top, None, entropy, None, None, None, None)
+        return lib.qste_token_logprobs(*logits, None, temperature, top, None, entropy, None, None, None, None, 0, None)
 
     def score_back(*logits, temperature=1.0, grad=16):
         return lib.qste_token_logprobs_backward(*logits, None, temperature, None, None, 16, 16, grad, None)
