@@ -8,9 +8,6 @@
 //   dz_j = (g ([j = token] - p_j) - h p_j (ln p_j + H)) / T
 // for the gradients g of the logprob and h of the entropy.
 #include "vocab_row.hpp"
-#ifndef SPLIT_ROWS
-#define SPLIT_ROWS 128
-#endif
 
 namespace qste {
 namespace scores {
@@ -344,15 +341,16 @@ __global__ __launch_bounds__(kThreads, WAVES_A_SIMD) void forward_kernel(Args a)
 }
 
 // The parts of a row as one: their sums against the common maximum, and the
-// best of their lists.  An entry's rank is its own place and, by a search
-// in each other list, how many there are larger.  With r = ceil(top / parts), r entries
-// of every part are at or above the least of the parts' r-th, so what lies
-// below that is left out beforehand.
+// best of their lists.  With r = ceil(top / parts), r entries of every part are
+// at or above the least of the parts' r-th, so only what is not below that
+// stays.  An entry's rank is its own place and, by a search in each other
+// list, how many there are larger.
 template <int DT>
 __global__ __launch_bounds__(kThreads) void join_kernel(Args a) {
-  extern __shared__ uint64_t lists[];  // [parts, top], then a rank for each
+  extern __shared__ uint64_t lists[];  // [parts, top], then a rank and a place of those that stay for each
   __shared__ float stats[3 * kMaxParts];
   __shared__ unsigned long long edge;
+  __shared__ int stay;
   const int tid = threadIdx.x, k = a.top, n = a.parts * k;
   const int64_t r = blockIdx.x;
   const int64_t token = a.tokens ? a.tokens[r] : 0;
@@ -361,14 +359,16 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Args a) {
     return;
   }
   int* ranks = reinterpret_cast<int*>(lists + n);
+  int* places = ranks + n;
   if (tid < 3 * a.parts) stats[tid] = a.part_stats[3 * r * a.parts + tid];
-  for (int i = tid; i < n; i += kThreads) {
-    lists[i] = a.part_entries[r * n + i];
-    ranks[i] = 0;
+  for (int i = tid; i < n; i += kThreads) lists[i] = a.part_entries[r * n + i];
+  if (tid == 0) {
+    edge = ~0ull;
+    stay = 0;
   }
-  if (tid == 0) edge = ~0ull;
   __syncthreads();
-  if (k > 0 && tid < a.parts) atomicMin(&edge, static_cast<unsigned long long>(lists[tid * k + (k + a.parts - 1) / a.parts - 1]));
+  if (k > 0 && tid < a.parts)
+    atomicMin(&edge, static_cast<unsigned long long>(lists[tid * k + (k + a.parts - 1) / a.parts - 1]));
   float m = -INFINITY;
   for (int p = 0; p < a.parts; ++p) m = fmaxf(m, stats[3 * p]);
   const Exponent ex(m, a.scale);
@@ -381,10 +381,17 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Args a) {
   const float log_sum = scored<DT>(a, r, token, m, sum, moment);
   if (k == 0) return;
   __syncthreads();
-  for (int i = tid; i < n * a.parts; i += kThreads) {
-    const int at = i / a.parts, p = i - at * a.parts;
+  for (int i = tid; i < n; i += kThreads) {
+    if (lists[i] == 0 || lists[i] < edge) continue;
+    ranks[i] = i % k;
+    places[atomicAdd(&stay, 1)] = i;
+  }
+  __syncthreads();
+  const int pairs = stay * a.parts;
+  for (int i = tid; i < pairs; i += kThreads) {
+    const int at = places[i / a.parts], p = i % a.parts;
+    if (at / k == p) continue;
     const uint64_t mine = lists[at];
-    if (mine < edge || mine == 0) continue;
     int lo = 0, hi = k;  // entries of list p larger than mine
     while (lo < hi) {
       const int mid = (lo + hi) / 2;
@@ -396,9 +403,9 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Args a) {
     if (lo) atomicAdd(&ranks[at], lo);
   }
   __syncthreads();
-  for (int i = tid; i < n; i += kThreads) {
-    const uint64_t mine = lists[i];
-    if (mine >= edge && mine != 0 && ranks[i] < k) write_top(a, r, ranks[i], mine, m, sum, log_sum);
+  for (int i = tid; i < stay; i += kThreads) {
+    const int at = places[i];
+    if (ranks[at] < k) write_top(a, r, ranks[at], lists[at], m, sum, log_sum);
   }
 }
 
@@ -406,17 +413,30 @@ struct Plan {
   int parts, part;  // parts a row, columns a part (the last has the rest)
 };
 
-Plan forward_plan(int64_t rows, int64_t vocab, int dtype) {
+// Up to 25 runs a thread stay in registers with four waves on a SIMD (120 to
+// 126 of 128 registers), so a row has up to kLong runs in one workgroup, or is
+// cut into parts of as many.  Shorter parts, of kShort runs, bring in more
+// workgroups where there are few:
+//   50257 bf16 logits a row, top 20, whole / in 4: 1 row 11.5 / 11.2 us, 8
+//   13.8 / 12.2, 40 14.3 / 12.3, 128 14.4 / 14.0; but 200 14.9 / 16.5, 500
+//   20.4 / 22.4 and 4096 97 / 110, where the join costs more than it gives;
+//   131072, where the row is cut in any case, in 3 / in 8: 1 row 14.3 / 12.4,
+//   128 21.2 / 18.7, 600 44.3 / 40.8; but 2048 107 / 111.
+// With many tokens to list the join decides: 16 rows of 131072 fp32 logits,
+// top 128, in 6 / in 16: 28 / 36 us.
+constexpr int kShort = kThreads * 8, kMiddle = kThreads * 16, kLong = kThreads * 25;
+constexpr int64_t kGroupsWhole = 512, kGroupsCut = 4800, kListed = 1024;
+
+Plan forward_plan(int64_t rows, int64_t vocab, int dtype, int64_t top) {
   const int64_t runs = runs_of(vocab, dtype), e = dtype == QSTE_F32 ? 4 : 8;
-  int64_t most = rows < SPLIT_ROWS ? 256 * 8 : 256 * 25;
-  Plan plan{1, 0};
-  if (runs > most) {
-    plan.parts = static_cast<int>((runs + most - 1) / most);
-    if (plan.parts > kMaxParts) plan.parts = static_cast<int>((runs + 256 * 25 - 1) / (256 * 25));
-    if (plan.parts > kMaxParts) plan.parts = 0;  // too long: one workgroup reads the row for each pass
-  }
-  if (plan.parts > 1) plan.part = static_cast<int>((runs + plan.parts - 1) / plan.parts * e);
-  return plan;
+  int64_t parts = runs > kLong ? (runs + kLong - 1) / kLong : 1;
+  const int64_t more = (runs + kShort - 1) / kShort;
+  if (runs > kMiddle && more <= kMaxParts && rows * more <= (parts > 1 ? kGroupsCut : kGroupsWhole) &&
+      more * top <= kListed)
+    parts = more;
+  if (parts > kMaxParts) return {0, 0};  // one workgroup reads the row again for each pass
+  // no part is empty: runs > parts * parts
+  return {static_cast<int>(parts), parts > 1 ? static_cast<int>((runs + parts - 1) / parts * e) : 0};
 }
 
 template <int DT, int HELD, int WAVES_A_SIMD>
@@ -425,7 +445,7 @@ int forward_as(const Args& a, int64_t rows, hipStream_t s) {
     if (a.parts > 1) {
       forward_kernel<DT, HELD, WAVES_A_SIMD, true><<<static_cast<unsigned>(rows * a.parts), kThreads, 0, s>>>(a);
       if (int rc = static_cast<int>(hipGetLastError())) return rc;
-      join_kernel<DT><<<static_cast<unsigned>(rows), kThreads, static_cast<size_t>(a.parts) * a.top * 12, s>>>(a);
+      join_kernel<DT><<<static_cast<unsigned>(rows), kThreads, static_cast<size_t>(a.parts) * a.top * 16, s>>>(a);
       return static_cast<int>(hipGetLastError());
     }
   }
@@ -439,8 +459,8 @@ int forward(Args a, int64_t rows, const Plan& plan, hipStream_t s) {
   a.part = plan.part;
   if (plan.parts == 0) return forward_as<DT, 0, 4>(a, rows, s);
   const int64_t runs = plan.parts > 1 ? plan.part / (DT == QSTE_F32 ? 4 : 8) : runs_of(a.logits.vocab, DT);
-  if (runs <= 256 * 8) return forward_as<DT, 8, 7>(a, rows, s);
-  if (runs <= 256 * 16) return forward_as<DT, 16, 5>(a, rows, s);
+  if (runs <= kShort) return forward_as<DT, 8, 7>(a, rows, s);
+  if (runs <= kMiddle) return forward_as<DT, 16, 5>(a, rows, s);
   return forward_as<DT, 25, 4>(a, rows, s);
 }
 
@@ -502,7 +522,7 @@ __global__ __launch_bounds__(kBackThreads) void backward_kernel(BackArgs a, int 
 }  // namespace scores
 
 size_t token_logprobs_workspace(int64_t rows, int64_t vocab, int dtype, int64_t top) {
-  const scores::Plan plan = scores::forward_plan(rows, vocab, dtype);
+  const scores::Plan plan = scores::forward_plan(rows, vocab, dtype, top);
   return plan.parts > 1 ? static_cast<size_t>(rows) * plan.parts * (top * 8 + 12) : 0;
 }
 
@@ -510,7 +530,7 @@ int launch_token_logprobs(const vocab::Logits& logits, int dtype, int64_t rows, 
                           double temperature, int64_t top, float* logprobs, float* entropy, float* top_logprobs,
                           int64_t* top_tokens, float* stats, void* workspace, hipStream_t s) {
   using namespace scores;
-  const Plan plan = forward_plan(rows, logits.vocab, dtype);
+  const Plan plan = forward_plan(rows, logits.vocab, dtype, top);
   if (rows * (plan.parts > 1 ? plan.parts : 1) > INT32_MAX) return QSTE_E_SHAPE;
   uint64_t* entries = plan.parts > 1 ? static_cast<uint64_t*>(workspace) : nullptr;
   float* part_stats = plan.parts > 1 ? reinterpret_cast<float*>(entries + rows * plan.parts * top) : nullptr;

@@ -265,6 +265,28 @@ def test_layouts(dtype):
     check(flat, random_tokens((4,), 1013, 7).to(torch.int32), top=2)
 
 
+@pytest.mark.parametrize("dtype,vocab", [(torch.bfloat16, 1_700_003), (torch.float32, 900_001), (torch.float16, 500_000)])
+def test_very_long_rows(dtype, vocab):
+    """In parts as long as registers hold, and past what so many parts hold."""
+
+    print(f"long {vocab} {dtype}", flush=True)
+    logits = random_logits((3, vocab), dtype, 14)
+    logits[1] = torch.arange(vocab, device=DEV).float() / vocab  # in order, with long runs of equals
+    logits[2, 5:] = -math.inf
+    check(logits, torch.tensor([vocab - 1, 17, 3], device=DEV), top=100)
+
+
+@pytest.mark.parametrize("rows,vocab", [(300, 32776), (150, 51200), (150, 51208), (1300, 65536)])
+def test_many_long_rows(rows, vocab):
+    """Both sides of where a row is cut, and of how many rows are cut into short parts."""
+
+    print(f"many {rows} x {vocab}", flush=True)
+    logits = random_logits((rows, vocab), torch.bfloat16, rows)
+    tokens = random_tokens((rows,), vocab, rows)
+    tokens[5] = -1
+    check(logits, tokens, top=7)
+
+
 def test_rows_far_apart():
     """Offsets past 32 bits, in elements and in bytes."""
 
