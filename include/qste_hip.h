@@ -50,6 +50,8 @@ extern "C" {
 /* most tokens qste_token_logprobs lists, most entries a row of qste_distill has */
 #define QSTE_MAX_TOP 128
 #define QSTE_MAX_ENTRIES 1024
+/* floats a row in the statistics of qste_distill */
+#define QSTE_DISTILL_STATS 5
 
 /* Library version; bumps when an entry point's contract changes. */
 int qste_version(void);
@@ -525,20 +527,23 @@ int qste_token_logprobs_backward(const void* logits, int dtype, int64_t outer, i
  * counts with the sum), taken at the same temperature.
  *   tail = 0: q = softmax(top_logprobs), q_r = 0
  *   tail = 1: q = exp(top_logprobs), q_r = max(0, 1 - sum q) against the
- *             student's mass p_r outside the list (left out when p_r = 0)
+ *             student's mass p_r outside the list (left out when p_r < 2^-100)
  *   losses = temperature^2 (sum q (ln q - ln p[token]) + q_r (ln q_r - ln p_r))
- * A row without entries has the loss 0 and no gradient, and is not read; one
- * with a token >= vocab a NaN loss and gradient; one of only -inf logits the loss inf
- * and no gradient.  stats fp32 [rows, 4] (16-byte aligned), or NULL, is what
- * qste_distill_backward reads.  With grad ([rows, vocab] in dtype, 16-byte
+ * A row without entries (tail = 0: without one of mass) has the loss 0 and no
+ * gradient, whatever its logits hold; one with a token >= vocab a NaN loss and
+ * gradient; one of only -inf logits the loss inf and no gradient.  stats fp32
+ * [rows, QSTE_DISTILL_STATS], or NULL, is what qste_distill_backward reads.  With grad ([rows, vocab] in dtype, 16-byte
  * aligned; NULL: the loss alone) the logits' gradient for the row weights
  * loss_grad fp32 [rows] is written by the same pass:
  *   loss_grad temperature (s p - q) for a listed token, loss_grad temperature
- *   p (s - q_r / p_r) for another, s = sum q + q_r; zeros where loss_grad is 0. */
+ *   p (s - q_r / p_r) for another, s = sum q + q_r; zeros where loss_grad is 0.
+ * Needs qste_distill_workspace_bytes(outer * inner, vocab, dtype, grad != NULL)
+ * bytes of workspace, 4-byte aligned (0 where rows are not cut into parts). */
+size_t qste_distill_workspace_bytes(int64_t rows, int64_t vocab, int dtype, int with_grad);
 int qste_distill(const void* logits, int dtype, int64_t outer, int64_t inner, int64_t outer_stride,
                  int64_t inner_stride, int64_t vocab, const int64_t* top_tokens, const float* top_logprobs, int64_t k,
                  double temperature, int tail, float* losses, float* stats, const float* loss_grad, void* grad,
-                 void* stream);
+                 void* workspace, size_t workspace_bytes, void* stream);
 
 /* The same gradient from an earlier call's stats, for weights known later. */
 int qste_distill_backward(const void* logits, int dtype, int64_t outer, int64_t inner, int64_t outer_stride,

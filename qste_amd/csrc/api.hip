@@ -79,8 +79,9 @@ int launch_token_logprobs(const vocab::Logits&, int, int64_t, const int64_t*, do
                           int64_t*, float*, void*, hipStream_t);
 int launch_token_logprobs_backward(const vocab::Logits&, int, int64_t, const int64_t*, double, const float*,
                                    const float*, const float*, const float*, void*, hipStream_t);
+size_t distill_workspace(int64_t, int64_t, int, int);
 int launch_distill(const vocab::Logits&, int, int64_t, const int64_t*, const float*, int64_t, double, int, float*,
-                   float*, const float*, void*, hipStream_t);
+                   float*, const float*, void*, void*, hipStream_t);
 int launch_distill_backward(const vocab::Logits&, int, int64_t, const int64_t*, const float*, int64_t, double, int,
                             const float*, const float*, void*, hipStream_t);
 // fp32 products through bf16 limbs (gemm_mfma.hip): 0 bytes / return 1 when
@@ -847,18 +848,25 @@ int qste_token_logprobs_backward(const void* logits, int dtype, int64_t outer, i
                                         entropy, stats, grad, as_stream(stream));
 }
 
+size_t qste_distill_workspace_bytes(int64_t rows, int64_t vocab, int dtype, int with_grad) {
+  if (!dtype_ok(dtype) || rows <= 0 || rows > INT32_MAX || vocab <= 0 || vocab > vocab::kMaxVocab) return 0;
+  return distill_workspace(rows, vocab, dtype, with_grad);
+}
+
 int qste_distill(const void* logits, int dtype, int64_t outer, int64_t inner, int64_t outer_stride,
                  int64_t inner_stride, int64_t vocab, const int64_t* top_tokens, const float* top_logprobs, int64_t k,
                  double temperature, int tail, float* losses, float* stats, const float* loss_grad, void* grad,
-                 void* stream) {
+                 void* workspace, size_t workspace_bytes, void* stream) {
   if (int rc = logits_ok(logits, dtype, outer, inner, vocab, temperature)) return rc;
   if (k < 1 || k > QSTE_MAX_ENTRIES) return QSTE_E_SHAPE;
   if (outer * inner == 0) return 0;
   if (!top_tokens || !top_logprobs || !losses || (grad && !loss_grad)) return QSTE_E_NULL;
-  if (reinterpret_cast<uintptr_t>(stats) % 16 || reinterpret_cast<uintptr_t>(grad) % 16) return QSTE_E_ALIGN;
+  if (reinterpret_cast<uintptr_t>(grad) % 16 || reinterpret_cast<uintptr_t>(workspace) % 4) return QSTE_E_ALIGN;
+  const size_t need = distill_workspace(outer * inner, vocab, dtype, grad != nullptr);
+  if (need && (!workspace || workspace_bytes < need)) return QSTE_E_WORKSPACE;
   const vocab::Logits l{logits, inner, outer_stride, inner_stride, static_cast<int>(vocab)};
   return launch_distill(l, dtype, outer * inner, top_tokens, top_logprobs, k, temperature, tail != 0, losses, stats,
-                        loss_grad, grad, as_stream(stream));
+                        loss_grad, grad, workspace, as_stream(stream));
 }
 
 int qste_distill_backward(const void* logits, int dtype, int64_t outer, int64_t inner, int64_t outer_stride,
@@ -869,7 +877,7 @@ int qste_distill_backward(const void* logits, int dtype, int64_t outer, int64_t 
   if (k < 1 || k > QSTE_MAX_ENTRIES) return QSTE_E_SHAPE;
   if (outer * inner == 0) return 0;
   if (!top_tokens || !top_logprobs || !stats || !loss_grad || !grad) return QSTE_E_NULL;
-  if (reinterpret_cast<uintptr_t>(stats) % 16 || reinterpret_cast<uintptr_t>(grad) % 16) return QSTE_E_ALIGN;
+  if (reinterpret_cast<uintptr_t>(grad) % 16) return QSTE_E_ALIGN;
   const vocab::Logits l{logits, inner, outer_stride, inner_stride, static_cast<int>(vocab)};
   return launch_distill_backward(l, dtype, outer * inner, top_tokens, top_logprobs, k, temperature, tail != 0, stats,
                                  loss_grad, grad, as_stream(stream));

@@ -95,6 +95,7 @@ struct Row {
   using T = typename W::T;
   static constexpr int E = W::E;
   static constexpr int kStep = THREADS * E;
+  static constexpr bool kHeld = HELD > 0;
   const T* p;
   int count;
   uint4 held[HELD > 0 ? HELD : 1];
@@ -198,7 +199,7 @@ __device__ __forceinline__ float fold_sum(float v) {
 
 template <int THREADS>
 __device__ __forceinline__ float block_max(float v, float* scratch) {
-  v = wave_max(v);
+  v = fold_max(v);
   __syncthreads();
   if ((threadIdx.x & (kWave - 1)) == 0) scratch[threadIdx.x / kWave] = v;
   __syncthreads();

@@ -914,7 +914,7 @@ def embedding_backward(ids: Tensor, grad: Tensor, packed: Tensor, scale: Tensor,
 # in the reference)
 # ---------------------------------------------------------------------------
 
-MAX_TOP, MAX_ENTRIES, MAX_VOCAB = 128, 1024, 1 << 30
+MAX_TOP, MAX_ENTRIES, MAX_VOCAB, DISTILL_STATS = 128, 1024, 1 << 30, 5  # as in include/qste_hip.h
 
 
 def _logit_rows(logits: Tensor) -> tuple[Tensor, tuple[int, int, int, int, int]]:
@@ -1040,7 +1040,7 @@ def _teacher(logits: Tensor, top_tokens: Tensor, top_logprobs: Tensor) -> tuple[
 def distill_forward(logits: Tensor, top_tokens: Tensor, top_logprobs: Tensor, *, temperature: float = 1.0,
                     tail: bool = False, loss_grad: Tensor | None = None, want_stats: bool = False):
     """``(losses, stats, grad)``: the losses fp32 [...] of logits [..., vocab] against
-    a teacher's ``top_tokens`` and ``top_logprobs`` [..., k]; ``stats`` fp32 [..., 4], what
+    a teacher's ``top_tokens`` and ``top_logprobs`` [..., k]; ``stats`` fp32 [..., 5], what
     ``distill_backward`` reads, if asked for; and with ``loss_grad`` [...] the
     logits' gradient for these weights, from the same pass, else None."""
 
@@ -1051,11 +1051,14 @@ def distill_forward(logits: Tensor, top_tokens: Tensor, top_logprobs: Tensor, *,
     tokens_i64, values = _teacher(logits, top_tokens, top_logprobs)
     weights = _row_weights(loss_grad, shape, "loss_grad")
     losses = torch.empty(shape, dtype=torch.float32, device=device)
-    stats = torch.empty(*shape, 4, dtype=torch.float32, device=device) if want_stats else None
+    stats = torch.empty(*shape, DISTILL_STATS, dtype=torch.float32, device=device) if want_stats else None
     grad = torch.empty(logits.shape, dtype=logits.dtype, device=device) if weights is not None else None
-    _lib.check(_lib.load().qste_distill(
+    lib = _lib.load()
+    nbytes = lib.qste_distill_workspace_bytes(losses.numel(), layout[4], code, int(grad is not None))
+    work = _workspace(nbytes, device) if nbytes else None
+    _lib.check(lib.qste_distill(
         _ptr(rows), code, *layout, _ptr(tokens_i64), _ptr(values), tokens_i64.shape[-1], temperature, int(tail),
-        _ptr(losses), _ptr(stats), _ptr(weights), _ptr(grad), _stream(device)), "distill")
+        _ptr(losses), _ptr(stats), _ptr(weights), _ptr(grad), _ptr(work), nbytes, _stream(device)), "distill")
     return losses, stats, grad
 
 
@@ -1069,7 +1072,7 @@ def distill_backward(logits: Tensor, top_tokens: Tensor, top_logprobs: Tensor, l
     shape, temperature = logits.shape[:-1], _temperature(temperature)
     tokens_i64, values = _teacher(logits, top_tokens, top_logprobs)
     weights = _row_weights(loss_grad, shape, "loss_grad")
-    stats_f32 = _row_weights(stats, (*shape, 4), "stats")
+    stats_f32 = _row_weights(stats, (*shape, DISTILL_STATS), "stats")
     grad = torch.empty(logits.shape, dtype=logits.dtype, device=device)
     _lib.check(_lib.load().qste_distill_backward(
         _ptr(rows), code, *layout, _ptr(tokens_i64), _ptr(values), tokens_i64.shape[-1], temperature, int(tail),

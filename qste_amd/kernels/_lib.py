@@ -88,8 +88,9 @@ SIGNATURES = {
                                    _vp, _sz, _vp]),
     "qste_token_logprobs_backward": (_int, [_vp, _int, _i64, _i64, _i64, _i64, _i64, _vp, _dbl, _vp, _vp, _vp, _vp,
                                             _vp, _vp]),
+    "qste_distill_workspace_bytes": (_sz, [_i64, _i64, _int, _int]),
     "qste_distill": (_int, [_vp, _int, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _dbl, _int, _vp, _vp, _vp, _vp,
-                            _vp]),
+                            _vp, _sz, _vp]),
     "qste_distill_backward": (_int, [_vp, _int, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _dbl, _int, _vp, _vp,
                                      _vp, _vp]),
 }

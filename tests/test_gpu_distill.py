@@ -194,6 +194,29 @@ def test_a_student_sure_of_the_list(dtype):
     check(logits, tokens, values, tail=True)
 
 
+def test_tails_that_vanish():
+    """Down to 2^-100 of the mass the tail counts; below, it is left out."""
+
+    vocab, k = 5003, 8
+    tokens, values = random_teacher((3,), vocab, k, 15)
+    logits = random_logits((3, vocab), torch.float32, 15, 1.0)
+    rest = torch.ones(3, vocab, dtype=torch.bool, device=DEV).scatter_(1, tokens, False)
+    logits[0, rest[0]] -= 60.0  # 5000 e^-60 = 2^-74
+    logits[1, rest[1]] -= 85.0  # 2^-110
+    logits[2, rest[2]] -= 1e4
+    check(logits[:1], tokens[:1], values[:1], tail=True)
+    import qste_amd as qste
+
+    inside = values[1:] - values[1:].logsumexp(1, keepdim=True)
+    for r in (1, 2):
+        losses, grad = qste.nn.distillation_loss_and_grad(logits[r:r + 1], tokens[r:r + 1], values[r:r + 1], tail=True)
+        # over the list alone the teacher is its mass times the same one renormalised
+        mass = float(values[r].double().exp().sum())
+        alone, _, _, _ = distilled(logits[r:r + 1], tokens[r:r + 1], inside[r - 1:r], torch.ones(1))
+        assert abs(float(losses) - mass * (float(alone) + math.log(mass))) < 1e-4
+        assert grad.isfinite().all() and float(grad[0, rest[r]].abs().max()) < 1e-30
+
+
 @pytest.mark.parametrize("tail", [False, True])
 def test_masked_students(tail):
     vocab, k = 1500, 12
@@ -266,6 +289,19 @@ def test_broadcast_weights():
     for weight in (0.1, torch.tensor(0.1, device=DEV), torch.full((5,), 0.1, device=DEV), torch.full((2, 1), 0.1, device=DEV)):
         _, grad = qste.nn.distillation_loss_and_grad(logits.detach(), tokens, values, loss_grad=weight, tail=True)
         near(grad, dz, LOG * size + 2.0 ** -23 * dz.abs())
+
+
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("dtype,rows,vocab", [(torch.bfloat16, 1, 1_700_003), (torch.float32, 2, 900_001),
+                                              (torch.float16, 300, 32776), (torch.bfloat16, 60, 51200),
+                                              (torch.bfloat16, 60, 51208)])
+def test_long_rows(dtype, rows, vocab, tail):
+    """Past what registers hold in one workgroup, and past what they hold in parts."""
+
+    print(f"long {rows} x {vocab} {dtype}", flush=True)
+    tokens, values = random_teacher((rows,), vocab, 40, 16)
+    tokens[-1, 20:] = -1
+    check(random_logits((rows, vocab), dtype, 16), tokens, values, tail=tail)
 
 
 def test_rows_far_apart():

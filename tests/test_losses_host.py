@@ -23,7 +23,7 @@ def test_c_entry_points_refuse_before_any_launch():
         return lib.qste_token_logprobs_backward(*logits, None, temperature, None, None, 16, 16, grad, None)
 
     def distill(*logits, temperature=1.0, k=4, losses=16):
-        return lib.qste_distill(*logits, 16, 16, k, temperature, 0, losses, None, None, None, None)
+        return lib.qste_distill(*logits, 16, 16, k, temperature, 0, losses, None, None, None, None, 0, None)
 
     def distill_back(*logits, temperature=1.0, k=4, grad=16):
         return lib.qste_distill_backward(*logits, 16, 16, k, temperature, 0, 16, 16, grad, None)
