@@ -51,7 +51,7 @@ extern "C" {
 #define QSTE_MAX_TOP 128
 #define QSTE_MAX_ENTRIES 1024
 /* floats a row in the statistics of qste_distill */
-#define QSTE_DISTILL_STATS 5
+#define QSTE_DISTILL_STATS 6
 
 /* Library version; bumps when an entry point's contract changes. */
 int qste_version(void);
@@ -538,7 +538,7 @@ int qste_token_logprobs_backward(const void* logits, int dtype, int64_t outer, i
  *   loss_grad temperature (s p - q) for a listed token, loss_grad temperature
  *   p (s - q_r / p_r) for another, s = sum q + q_r; zeros where loss_grad is 0.
  * Needs qste_distill_workspace_bytes(outer * inner, vocab, dtype, grad != NULL)
- * bytes of workspace, 4-byte aligned (0 where rows are not cut into parts). */
+ * bytes of workspace, 16-byte aligned (0 where rows are not cut into parts). */
 size_t qste_distill_workspace_bytes(int64_t rows, int64_t vocab, int dtype, int with_grad);
 int qste_distill(const void* logits, int dtype, int64_t outer, int64_t inner, int64_t outer_stride,
                  int64_t inner_stride, int64_t vocab, const int64_t* top_tokens, const float* top_logprobs, int64_t k,

@@ -861,7 +861,7 @@ int qste_distill(const void* logits, int dtype, int64_t outer, int64_t inner, in
   if (k < 1 || k > QSTE_MAX_ENTRIES) return QSTE_E_SHAPE;
   if (outer * inner == 0) return 0;
   if (!top_tokens || !top_logprobs || !losses || (grad && !loss_grad)) return QSTE_E_NULL;
-  if (reinterpret_cast<uintptr_t>(grad) % 16 || reinterpret_cast<uintptr_t>(workspace) % 4) return QSTE_E_ALIGN;
+  if (reinterpret_cast<uintptr_t>(grad) % 16 || reinterpret_cast<uintptr_t>(workspace) % 16) return QSTE_E_ALIGN;
   const size_t need = distill_workspace(outer * inner, vocab, dtype, grad != nullptr);
   if (need && (!workspace || workspace_bytes < need)) return QSTE_E_WORKSPACE;
   const vocab::Logits l{logits, inner, outer_stride, inner_stride, static_cast<int>(vocab)};

@@ -26,7 +26,8 @@ constexpr int kWaves = kThreads / kWave;
 constexpr int kMaxParts = 32;
 // columns whose membership in the list is held in LDS at a time, one bit each
 constexpr int kSpan = 1 << 17;
-constexpr int kStats = 5;
+constexpr int kSingles = 128;  // more than a Row's columns outside its runs
+constexpr int kStats = QSTE_DISTILL_STATS;
 
 struct Args {
   Logits logits;
@@ -35,16 +36,28 @@ struct Args {
   int k, tail;
   float scale, inverse, temperature;
   float* losses;
-  float* stats;            // [rows, kStats]: m, the sum of the exponentials, s, s - q_r / p_r, and what ln q is below the values
+  // [rows, kStats]: m, the sum of the exponentials, s, s - q_r / p_r, what ln q is below the values, and whether a token is repeated
+  float* stats;
   const float* loss_grad;  // [rows] or NULL
   void* grad;              // NULL: the loss alone
   // rows cut into parts: columns a part, and what each part leaves
   int parts, part;
-  float* part_stats;  // [rows, parts, 3]: m, sum, the sum outside the list
+  float* part_stats;  // [rows, parts, 4]: m, sum, the sum outside the list, whether a token is repeated
 };
 
-// The row's entries in LDS, k of each: its tokens (-1: none) and ln q, then the
-// bits of the listed columns.
+// What the entries come to: the mass of q (0: the row has no entry, without
+// the tail also none with mass; NaN: a token is past the vocabulary) and what
+// it leaves of 1, what ln q is below the values, whether there is an entry and
+// whether one is repeated.
+struct Teacher {
+  float mass, rest, shift;
+  int any, repeated;
+  __device__ __forceinline__ bool none(int tail) const { return mass == 0.0f && !(tail && any); }
+};
+
+// The row's entries in LDS, k of each: its tokens (-1: none) and ln q; then the
+// bits of the listed columns, by their place in a Row (columns before the runs come
+// after the others).
 struct Entries {
   int* token;
   float* log_q;
@@ -53,26 +66,40 @@ struct Entries {
       : token(reinterpret_cast<int*>(lds)), log_q(reinterpret_cast<float*>(lds) + k), listed(lds + 2 * k) {}
 };
 
-inline size_t entries_bytes(int64_t k, int64_t columns, int tail) {
-  const int64_t span = columns < kSpan ? columns : kSpan;
-  return static_cast<size_t>(k * 8 + (tail ? (span + 31) / 32 * 4 : 0));
+inline size_t entries_bytes(int64_t k, int64_t columns) {
+  const int64_t span = columns < kSpan + kSingles ? columns : kSpan + kSingles;
+  return static_cast<size_t>(k * 8 + (span + 31) / 32 * 4);
 }
 
-// What the entries come to: the mass of q (0: the row has no entry, outside
-// the tail also none with mass; NaN: a token is past the vocabulary) and what
-// ln q is below the values.  `any`: whether there is an entry.
-struct Teacher {
-  float mass, shift;
-  bool any;
-  __device__ __forceinline__ bool none(int tail) const { return mass == 0.0f && !(tail && any); }
-};
+// exp(v) to 1e-11: the mass of a list is near 1, and what it leaves of 1 has to
+// be right to its own size, which sums of fp32 exponentials are not.  2^(n + f)
+// with |f| <= 1/2, and the exponential series in f ln 2 up to its ninth power (the
+// next term is under 1e-11).
+__device__ __forceinline__ double exp_exactly(float v) {
+  if (v <= -100.0f) return 0.0;
+  const double t = static_cast<double>(v) * 1.4426950408889634074, n = rint(t), x = (t - n) * 0.69314718055994530942;
+  double p = 1.0 / 362880;
+  p = fma(p, x, 1.0 / 40320);
+  p = fma(p, x, 1.0 / 5040);
+  p = fma(p, x, 1.0 / 720);
+  p = fma(p, x, 1.0 / 120);
+  p = fma(p, x, 1.0 / 24);
+  p = fma(p, x, 1.0 / 6);
+  p = fma(p, x, 0.5);
+  p = fma(p, x, 1.0);
+  p = fma(p, x, 1.0);
+  return ldexp(p, static_cast<int>(fmin(n, 1024.0)));
+}
 
-__device__ __forceinline__ Teacher load_entries(const Args& a, int64_t r, const Entries& t, float* scratch) {
+// One wave reads the entries, while the others' loads of the row are on
+// their way: token and ln q to LDS, the rest in every lane.
+__device__ __forceinline__ Teacher load_entries(const Args& a, int64_t r, const Entries& t) {
+  const int lane = threadIdx.x & (kWave - 1);
   const int64_t* tokens = a.tokens + r * a.k;
   const float* values = a.values + r * a.k;
   float top = -INFINITY;
   bool any = false, bad = false;
-  for (int k = threadIdx.x; k < a.k; k += kThreads) {
+  for (int k = lane; k < a.k; k += kWave) {
     const int64_t at = tokens[k];
     const bool there = at >= 0 && at < a.logits.vocab;
     any |= there;
@@ -82,80 +109,138 @@ __device__ __forceinline__ Teacher load_entries(const Args& a, int64_t r, const 
     t.log_q[k] = v;
     top = fmaxf(top, v);
   }
-  any = __syncthreads_or(any);
-  bad = __syncthreads_or(bad);
-  top = a.tail ? 0.0f : block_max<kThreads>(top, scratch);
+  top = a.tail ? 0.0f : fold_max(top);
   if (top == -INFINITY) top = 0.0f;
-  float sum = 0.0f;
-  for (int k = threadIdx.x; k < a.k; k += kThreads) sum += expf(t.log_q[k] - top);
-  sum = block_sum(sum, scratch);
-  Teacher out{sum, 0.0f, any};
+  double total = 0.0;
+  for (int k = lane; k < a.k; k += kWave) total += exp_exactly(t.log_q[k] - top);
+  total = wave_sum(total);
+  const float sum = static_cast<float>(total);
+  Teacher out{sum, total > 1.0 ? 0.0f : static_cast<float>(1.0 - total), 0.0f, __any(any), 0};
   if (!a.tail && sum > 0.0f) {
     out.shift = top + logf(sum);
     out.mass = 1.0f;
-    for (int k = threadIdx.x; k < a.k; k += kThreads) t.log_q[k] -= out.shift;
+    for (int k = lane; k < a.k; k += kWave) t.log_q[k] -= out.shift;
   }
-  if (bad) out.mass = NAN;
-  __syncthreads();
+  if (__any(bad)) out.mass = NAN;
   return out;
 }
 
-__device__ __forceinline__ void set_stats(const Args& a, int64_t r, float m, float sum, float listed, float other,
-                                          float shift) {
-  if (!a.stats) return;
-  const float v[kStats] = {m, sum, listed, other, shift};
-#pragma unroll
-  for (int i = 0; i < kStats; ++i) a.stats[kStats * r + i] = v[i];
-}
-
-// The bits of the listed columns in [from, to)
-__device__ __forceinline__ void mark_listed(const Args& a, const Entries& t, int from, int to) {
-  __syncthreads();
-  for (int i = threadIdx.x; i < (to - from + 31) / 32; i += kThreads) t.listed[i] = 0;
-  __syncthreads();
-  for (int k = threadIdx.x; k < a.k; k += kThreads) {
-    const int at = t.token[k];
-    if (at >= from && at < to) atomicOr(&t.listed[(at - from) >> 5], 1u << ((at - from) & 31));
+// By one wave: the bits of the listed columns whose places lie in [from, to),
+// of a view of `count` columns that begins at column `begin` and has `head` before
+// its runs.  Returns whether a token is there twice.
+__device__ __forceinline__ bool mark_listed(const Args& a, const Entries& t, int begin, int count, int head, int from,
+                                            int to) {
+  const int lane = threadIdx.x & (kWave - 1);
+  for (int i = lane; i < (to - from + 31) / 32; i += kWave) t.listed[i] = 0;
+  __builtin_amdgcn_wave_barrier();
+  bool twice = false;
+  for (int k = lane; k < a.k; k += kWave) {
+    const int column = t.token[k] - begin;
+    if (t.token[k] < 0 || column < 0 || column >= count) continue;
+    const int at = column - head + (column < head ? count : 0) - from;
+    if (at < 0 || at >= to - from) continue;
+    const uint32_t bit = 1u << (at & 31);
+    twice |= (atomicOr(&t.listed[at >> 5], bit) & bit) != 0;
   }
-  __syncthreads();
+  return __any(twice);
 }
 
 // A thread's sums of the exponentials over the columns, all and outside the
-// list.  `from`: the row's column that they begin at.
+// list; `from` and the bits as in mark_listed.
 template <class R>
-__device__ __forceinline__ void sums(const Args& a, const R& row, const Entries& t, int from, const Exponent& ex,
-                                     float& sum, float& outside) {
+__device__ __forceinline__ void sums(const Args& a, const R& row, const Entries& t, int from, int to,
+                                     const Exponent& ex, float& sum, float& outside) {
   if (!a.tail) {
-    row.each([&](int, auto& x) {
+    row.each(from, to, [&](int, auto& x) {
       constexpr int N = sizeof(x) / sizeof(x[0]);
 #pragma unroll
       for (int j = 0; j < N; ++j) sum += ex.of(ex.power(x[j]));
     });
     return;
   }
-  for (int at = 0; at < row.count; at += kSpan) {  // a row in registers has one span
-    const int end = min(row.count, at + kSpan);
-    mark_listed(a, t, from + at, from + end);
-    row.each(at, end, [&](int first, auto& x) {
-      constexpr int N = sizeof(x) / sizeof(x[0]);
-      uint32_t bits = first < row.count ? t.listed[(first - at) >> 5] >> ((first - at) & 31) : 0;
-      bits &= (1u << N) - 1;
-      float all = 0.0f;
+  row.each(from, to, [&](int first, auto& x) {
+    constexpr int N = sizeof(x) / sizeof(x[0]);
+    const int at = first - row.head + (N == 1 && first < row.head ? row.count : 0) - from;
+    uint32_t bits = first < row.count && at >= 0 && at < to - from ? t.listed[at >> 5] >> (at & 31) : 0;
+    bits &= (1u << N) - 1;
+    float all = 0.0f;
 #pragma unroll
-      for (int j = 0; j < N; ++j) {
-        x[j] = ex.of(ex.power(x[j]));
-        all += x[j];
-      }
-      sum += all;
-      if (__any(bits)) {  // few waves' runs hold a listed column
-        all = 0.0f;
+    for (int j = 0; j < N; ++j) {
+      x[j] = ex.of(ex.power(x[j]));
+      all += x[j];
+    }
+    sum += all;
+    if (__any(bits)) {  // few waves' runs hold a listed column
+      all = 0.0f;
 #pragma unroll
-        for (int j = 0; j < N; ++j) all += bits >> j & 1 ? 0.0f : x[j];
-      }
-      outside += all;
-    });
-    if constexpr (R::kHeld) break;
+      for (int j = 0; j < N; ++j) all += bits >> j & 1 ? 0.0f : x[j];
+    }
+    outside += all;
+  });
+}
+
+// The workgroup's folds and the teacher
+struct Shared {
+  float maxima[kWaves], sum[kWaves], outside[kWaves];
+  Teacher teacher;
+};
+
+// The row's or part's maximum and sums, the entries read on the way (all of
+// them by the first wave).
+template <class R>
+__device__ __forceinline__ void reduce(const Args& a, int64_t r, const R& row, const Entries& t, int begin, Shared& sh,
+                                       float& m, float& sum, float& outside) {
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  if (wave == 0) {
+    Teacher teacher = load_entries(a, r, t);
+    if (R::kHeld) teacher.repeated = mark_listed(a, t, begin, row.count, row.head, 0, row.count);
+    if (lane == 0) sh.teacher = teacher;
   }
+  m = -INFINITY;
+  row.each([&](int, auto& x) { m = max_of(m, x); });
+  m = fold_max(m);
+  if (lane == 0) sh.maxima[wave] = m;
+  __syncthreads();
+  m = sh.maxima[0];
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) m = fmaxf(m, sh.maxima[w]);
+  const Exponent ex(m, a.scale);
+  sum = outside = 0.0f;
+  if constexpr (R::kHeld) {
+    sums(a, row, t, 0, row.count, ex, sum, outside);
+  } else {
+    int to = 0;
+    for (int from = 0; to < row.count; from += kSpan) {
+      to = row.count - from <= kSpan + kSingles ? row.count : from + kSpan;  // the single columns in the last span
+      __syncthreads();
+      if (wave == 0 && mark_listed(a, t, begin, row.count, row.head, from, to) && lane == 0) sh.teacher.repeated = 1;
+      __syncthreads();
+      sums(a, row, t, from, to, ex, sum, outside);
+    }
+  }
+  sum = fold_sum(sum);
+  outside = fold_sum(outside);
+  if (lane == 0) {
+    sh.sum[wave] = sum;
+    sh.outside[wave] = outside;
+  }
+  __syncthreads();
+  sum = sh.sum[0];
+  outside = sh.outside[0];
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) {
+    sum += sh.sum[w];
+    outside += sh.outside[w];
+  }
+}
+
+__device__ __forceinline__ void set_stats(const Args& a, int64_t r, float m, float sum, const float (&more)[4]) {
+  if (!a.stats) return;
+  float* st = a.stats + kStats * r;
+  st[0] = m;
+  st[1] = sum;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) st[2 + i] = more[i];
 }
 
 // What a row's gradient and loss take from its sums: s and s - q_r / p_r, and
@@ -164,36 +249,38 @@ struct Coefficients {
   float weight, other, rest_loss;
 };
 
-__device__ __forceinline__ Coefficients coefficients(const Args& a, float mass, float sum, float outside) {
+__device__ __forceinline__ Coefficients coefficients(const Args& a, const Teacher& teacher, float sum, float outside) {
+  const float mass = teacher.mass, p_rest = outside / sum;
   if (sum == 0.0f) return {0.0f, 0.0f, 0.0f};  // a row of -inf only
   if (mass != mass) return {mass, mass, mass};
-  const float p_rest = outside / sum;
-  const float rest = a.tail && p_rest >= 0x1p-100f ? fmaxf(0.0f, 1.0f - mass) : p_rest != p_rest ? p_rest : 0.0f;
+  const float rest = a.tail && p_rest >= 0x1p-100f ? teacher.rest : p_rest != p_rest ? p_rest : 0.0f;
   const float weight = mass + rest;
   if (rest == 0.0f) return {weight, weight, 0.0f};
   return {weight, weight - rest / p_rest, rest * (logf(rest) - logf(p_rest))};
 }
 
-// The row's loss and statistics (all threads)
+// The row's loss and statistics, by one wave
 template <int DT>
 __device__ __forceinline__ void write_loss(const Args& a, int64_t r, const Entries& t, const Teacher& teacher, float m,
-                                           float sum, const Coefficients& co, float* scratch) {
+                                           float sum, const Coefficients& co) {
   using T = typename Elem<DT>::T;
+  const int lane = threadIdx.x & (kWave - 1);
   const T* row = a.logits.row<T>(r);
   const float log_sum = logf(sum);
   float loss = 0.0f;
   if (sum != 0.0f)
-    for (int k = threadIdx.x; k < a.k; k += kThreads) {
+    for (int k = lane; k < a.k; k += kWave) {
       const int at = t.token[k];
       const float log_q = t.log_q[k], q = expf(log_q);
       if (at >= 0 && q != 0.0f) loss += q * (log_q - ((Elem<DT>::load(row, at) - m) * a.inverse - log_sum));
     }
-  loss = block_sum(loss, scratch);
-  if (threadIdx.x == 0) {
+  loss = fold_sum(loss);
+  if (lane == 0) {
     loss += co.rest_loss;
     if (sum == 0.0f) loss = teacher.mass == 0.0f ? 0.0f : teacher.mass != teacher.mass ? teacher.mass : INFINITY;
     a.losses[r] = loss * a.temperature * a.temperature;
-    set_stats(a, r, m, sum == 0.0f ? 1.0f : sum, co.weight, co.other, teacher.shift);
+    set_stats(a, r, m, sum == 0.0f ? 1.0f : sum,
+              {co.weight, co.other, teacher.shift, teacher.repeated ? 1.0f : 0.0f});
   }
 }
 
@@ -201,15 +288,15 @@ __device__ __forceinline__ void write_loss(const Args& a, int64_t r, const Entri
 __device__ __forceinline__ void write_none(const Args& a, int64_t r) {
   if (threadIdx.x == 0) {
     a.losses[r] = 0.0f;
-    set_stats(a, r, 0.0f, 1.0f, 0.0f, 0.0f, 0.0f);
+    set_stats(a, r, 0.0f, 1.0f, {0.0f, 0.0f, 0.0f, 0.0f});
   }
 }
 
 // dz of the listed tokens with columns in [from, to), over what the workgroup's
 // first pass wrote there: all of a token's entries add up to its q
 template <int DT>
-__device__ __forceinline__ void write_listed(const Args& a, const Entries& t, int64_t r, const Exponent& ex, float per_p,
-                                             float per_q, int from, int to) {
+__device__ __forceinline__ void write_listed(const Args& a, const Entries& t, bool repeated, int64_t r,
+                                             const Exponent& ex, float per_p, float per_q, int from, int to) {
   using T = typename Elem<DT>::T;
   const T* row = a.logits.row<T>(r);
   T* out = static_cast<T*>(a.grad) + r * a.logits.vocab;
@@ -217,8 +304,11 @@ __device__ __forceinline__ void write_listed(const Args& a, const Entries& t, in
   for (int k = threadIdx.x; k < a.k; k += kThreads) {
     const int at = t.token[k];
     if (at < from || at >= to) continue;
-    float q = 0.0f;
-    for (int i = 0; i < a.k; ++i) q += t.token[i] == at ? expf(t.log_q[i]) : 0.0f;
+    float q = expf(t.log_q[k]);
+    if (repeated) {
+      q = 0.0f;
+      for (int i = 0; i < a.k; ++i) q += t.token[i] == at ? expf(t.log_q[i]) : 0.0f;
+    }
     const float e = ex.of(ex.power(Elem<DT>::load(row, at)));
     Elem<DT>::store(out, at, e * per_p - q * per_q);
   }
@@ -231,29 +321,24 @@ __device__ __forceinline__ void write_listed(const Args& a, const Entries& t, in
 template <int DT, int HELD, int WAVES_A_SIMD>
 __global__ __launch_bounds__(kThreads, WAVES_A_SIMD) void forward_kernel(Args a) {
   extern __shared__ uint32_t lds[];
-  __shared__ float scratch[kWaves];
+  __shared__ Shared sh;
   using R = Row<DT, kThreads, HELD>;
   using W = Wide<DT>;
   const int64_t r = blockIdx.x;
   const int vocab = a.logits.vocab;
   const Entries t(lds, a.k);
   typename R::T* out = static_cast<typename R::T*>(a.grad) + r * vocab;
-  const Teacher teacher = load_entries(a, r, t, scratch);
+  const R row(a.logits.row<typename R::T>(r), vocab, a.grad ? before_line<DT>(out) : 0);
+  float m, sum, outside;
+  reduce(a, r, row, t, 0, sh, m, sum, outside);
+  const Teacher teacher = sh.teacher;
   if (teacher.none(a.tail)) {
     write_none(a, r);
     if (a.grad) zero_row<DT, kThreads>(out, 0, vocab);
     return;
   }
-  const R row(a.logits.row<typename R::T>(r), vocab);
-  float m = -INFINITY;
-  row.each([&](int, auto& x) { m = max_of(m, x); });
-  m = block_max<kThreads>(m, scratch);
   const Exponent ex(m, a.scale);
-  float sum = 0.0f, outside = 0.0f;
-  sums(a, row, t, 0, ex, sum, outside);
-  sum = block_sum(sum, scratch);
-  if (a.tail) outside = block_sum(outside, scratch);
-  const Coefficients co = coefficients(a, teacher.mass, sum, outside);
+  const Coefficients co = coefficients(a, teacher, sum, outside);
   if (a.grad) {
     const float g = a.loss_grad[r];
     if (g == 0.0f || sum == 0.0f) {
@@ -266,10 +351,10 @@ __global__ __launch_bounds__(kThreads, WAVES_A_SIMD) void forward_kernel(Args a)
         for (int j = 0; j < N; ++j) x[j] = ex.of(ex.power(x[j])) * per_other;
         if (first < vocab) W::store(out + first, x);
       });
-      write_listed<DT>(a, t, r, ex, per_p * co.weight, per_q, 0, vocab);
+      write_listed<DT>(a, t, teacher.repeated, r, ex, per_p * co.weight, per_q, 0, vocab);
     }
   }
-  write_loss<DT>(a, r, t, teacher, m, sum, co, scratch);
+  if (threadIdx.x < kWave) write_loss<DT>(a, r, t, teacher, m, sum, co);
 }
 
 // ---------------------------------------------------------------------------
@@ -279,60 +364,54 @@ __global__ __launch_bounds__(kThreads, WAVES_A_SIMD) void forward_kernel(Args a)
 template <int DT, int HELD, int WAVES_A_SIMD>
 __global__ __launch_bounds__(kThreads, WAVES_A_SIMD) void part_kernel(Args a) {
   extern __shared__ uint32_t lds[];
-  __shared__ float scratch[kWaves];
+  __shared__ Shared sh;
   using R = Row<DT, kThreads, HELD>;
   const int64_t r = blockIdx.x / static_cast<uint32_t>(a.parts);
   const int part = blockIdx.x % static_cast<uint32_t>(a.parts);
   const int from = part * a.part, to = part < a.parts - 1 ? from + a.part : a.logits.vocab;
   const Entries t(lds, a.k);
   const R row(a.logits.row<typename R::T>(r) + from, to - from);
-  if (a.tail)
-    for (int k = threadIdx.x; k < a.k; k += kThreads) {
-      const int64_t at = a.tokens[r * a.k + k];
-      t.token[k] = at >= 0 && at < a.logits.vocab ? static_cast<int>(at) : -1;
-    }
-  float m = -INFINITY;
-  row.each([&](int, auto& x) { m = max_of(m, x); });
-  m = block_max<kThreads>(m, scratch);
-  const Exponent ex(m, a.scale);
-  float sum = 0.0f, outside = 0.0f;
-  sums(a, row, t, from, ex, sum, outside);
-  sum = block_sum(sum, scratch);
-  if (a.tail) outside = block_sum(outside, scratch);
-  const int64_t slot = r * a.parts + part;
-  if (threadIdx.x < 3) a.part_stats[3 * slot + threadIdx.x] = threadIdx.x == 0 ? m : threadIdx.x == 1 ? sum : outside;
+  float m, sum, outside;
+  reduce(a, r, row, t, from, sh, m, sum, outside);
+  if (threadIdx.x == 0)
+    reinterpret_cast<float4*>(a.part_stats)[r * a.parts + part] =
+        make_float4(m, sum, outside, sh.teacher.repeated ? 1.0f : 0.0f);
 }
 
+// one wave a row
 template <int DT>
-__global__ __launch_bounds__(kThreads) void join_kernel(Args a) {
+__global__ __launch_bounds__(kWave) void join_kernel(Args a) {
   extern __shared__ uint32_t lds[];
-  __shared__ float scratch[kWaves];
-  __shared__ float stats[3 * kMaxParts];
   const int64_t r = blockIdx.x;
   const Entries t(lds, a.k);
-  if (threadIdx.x < 3 * a.parts) stats[threadIdx.x] = a.part_stats[3 * r * a.parts + threadIdx.x];
-  const Teacher teacher = load_entries(a, r, t, scratch);
+  const float4* parts = reinterpret_cast<const float4*>(a.part_stats) + r * a.parts;
+  Teacher teacher = load_entries(a, r, t);
   if (teacher.none(a.tail)) {
     write_none(a, r);
     return;
   }
   float m = -INFINITY;
-  for (int p = 0; p < a.parts; ++p) m = fmaxf(m, stats[3 * p]);
+  for (int p = 0; p < a.parts; ++p) m = fmaxf(m, parts[p].x);
   const Exponent ex(m, a.scale);
   float sum = 0.0f, outside = 0.0f;
   for (int p = 0; p < a.parts; ++p) {
-    const float weight = ex.of(ex.power(stats[3 * p]));  // a part of -inf only: its sums are 0
-    sum = fmaf(stats[3 * p + 1], weight, sum);
-    outside = fmaf(stats[3 * p + 2], weight, outside);
+    const float4 st = parts[p];
+    const float weight = ex.of(ex.power(st.x));  // a part of -inf only: its sums are 0
+    sum = fmaf(st.y, weight, sum);
+    outside = fmaf(st.z, weight, outside);
+    if (st.w != 0.0f) teacher.repeated = 1;
   }
-  write_loss<DT>(a, r, t, teacher, m, sum, coefficients(a, teacher.mass, sum, outside), scratch);
+  write_loss<DT>(a, r, t, teacher, m, sum, coefficients(a, teacher, sum, outside));
 }
 
 // ---------------------------------------------------------------------------
 // the gradient from a forward's statistics: one workgroup per part of a row
 // ---------------------------------------------------------------------------
 
-constexpr int kBackRuns = 8;  // 16-byte accesses a thread makes
+#ifndef BR
+#define BR 4
+#endif
+constexpr int kBackRuns = BR;  // 16-byte accesses a thread makes
 
 template <int DT>
 __global__ __launch_bounds__(kThreads) void backward_kernel(Args a) {
@@ -340,17 +419,19 @@ __global__ __launch_bounds__(kThreads) void backward_kernel(Args a) {
   using R = Row<DT, kThreads, kBackRuns>;
   using W = Wide<DT>;
   const int64_t r = blockIdx.x / static_cast<uint32_t>(a.parts);
-  const int from = static_cast<int>(blockIdx.x % static_cast<uint32_t>(a.parts)) * a.part;
-  const int to = min(a.logits.vocab, from + a.part);
-  typename R::T* out = static_cast<typename R::T*>(a.grad) + r * a.logits.vocab + from;
+  const int part = blockIdx.x % static_cast<uint32_t>(a.parts), vocab = a.logits.vocab;
+  typename R::T* out = static_cast<typename R::T*>(a.grad) + r * vocab;
+  // parts begin at whole lines of the gradient, but for the first
+  const int head = min(vocab, before_line<DT>(out));
+  const int from = part == 0 ? 0 : min(vocab, head + part * a.part), to = min(vocab, head + (part + 1) * a.part);
   const float* st = a.stats + kStats * r;
   const float m = st[0], sum = st[1], weight = st[2], other = st[3], shift = st[4];
   const float g = a.loss_grad[r];
   if (g == 0.0f || (weight == 0.0f && other == 0.0f)) {  // nothing flows back: the row is not read
-    zero_row<DT, kThreads>(out, 0, to - from);
+    zero_row<DT, kThreads>(out + from, 0, to - from);
     return;
   }
-  const R row(a.logits.row<typename R::T>(r) + from, to - from);
+  const R row(a.logits.row<typename R::T>(r) + from, to - from, part == 0 ? head : 0);
   const Entries t(lds, a.k);
   for (int k = threadIdx.x; k < a.k; k += kThreads) {
     const int64_t at = a.tokens[r * a.k + k];
@@ -363,9 +444,9 @@ __global__ __launch_bounds__(kThreads) void backward_kernel(Args a) {
     constexpr int N = sizeof(x) / sizeof(x[0]);
 #pragma unroll
     for (int j = 0; j < N; ++j) x[j] = ex.of(ex.power(x[j])) * per_other;
-    if (first < row.count) W::store(out + first, x);
+    if (first < row.count) W::store(out + from + first, x);
   });
-  write_listed<DT>(a, t, r, ex, per_p * weight, per_q, from, to);
+  write_listed<DT>(a, t, st[5] != 0.0f, r, ex, per_p * weight, per_q, from, to);
 }
 
 constexpr int kShort = kThreads * 8, kMiddle = kThreads * 16, kLong = kThreads * 25;
@@ -387,14 +468,14 @@ int loss_as(const Args& a, int64_t rows, hipStream_t s) {
   if constexpr (HELD > 0) {
     if (a.parts > 1) {
       part_kernel<DT, HELD, WAVES_A_SIMD>
-          <<<static_cast<unsigned>(rows * a.parts), kThreads, entries_bytes(a.k, a.part, a.tail), s>>>(a);
+          <<<static_cast<unsigned>(rows * a.parts), kThreads, entries_bytes(a.k, a.part + Wide<DT>::E), s>>>(a);
       if (int rc = static_cast<int>(hipGetLastError())) return rc;
-      join_kernel<DT><<<static_cast<unsigned>(rows), kThreads, entries_bytes(a.k, 0, 0), s>>>(a);
+      join_kernel<DT><<<static_cast<unsigned>(rows), kWave, entries_bytes(a.k, 0), s>>>(a);
       return static_cast<int>(hipGetLastError());
     }
   }
   forward_kernel<DT, HELD, WAVES_A_SIMD>
-      <<<static_cast<unsigned>(rows), kThreads, entries_bytes(a.k, a.logits.vocab, a.tail), s>>>(a);
+      <<<static_cast<unsigned>(rows), kThreads, entries_bytes(a.k, a.logits.vocab), s>>>(a);
   return static_cast<int>(hipGetLastError());
 }
 
@@ -412,7 +493,7 @@ int backward(Args a, int64_t rows, hipStream_t s) {
   a.part = kThreads * kBackRuns * Wide<DT>::E;
   a.parts = ceil_div(a.logits.vocab, a.part);
   if (rows * a.parts > INT32_MAX) return QSTE_E_SHAPE;
-  backward_kernel<DT><<<static_cast<unsigned>(rows * a.parts), kThreads, entries_bytes(a.k, 0, 0), s>>>(a);
+  backward_kernel<DT><<<static_cast<unsigned>(rows * a.parts), kThreads, entries_bytes(a.k, 0), s>>>(a);
   return static_cast<int>(hipGetLastError());
 }
 
@@ -427,7 +508,7 @@ Args arguments(const Logits& logits, const int64_t* tokens, const float* values,
 size_t distill_workspace(int64_t rows, int64_t vocab, int dtype, int with_grad) {
   const int parts = distill::forward_plan(rows, vocab, dtype).parts;
   // the parts' sums, and the row statistics that a gradient after the join reads
-  return parts > 1 ? static_cast<size_t>(rows) * 4 * (3 * parts + (with_grad ? distill::kStats : 0)) : 0;
+  return parts > 1 ? static_cast<size_t>(rows) * 4 * (4 * parts + (with_grad ? distill::kStats : 0)) : 0;
 }
 
 int launch_distill_backward(const vocab::Logits& logits, int dtype, int64_t rows, const int64_t* tokens,
@@ -459,7 +540,7 @@ int launch_distill(const vocab::Logits& logits, int dtype, int64_t rows, const i
     a.parts = plan.parts;
     a.part = plan.part;
     a.part_stats = static_cast<float*>(workspace);
-    if (grad && !stats) a.stats = a.part_stats + rows * plan.parts * 3;
+    if (grad && !stats) a.stats = a.part_stats + rows * plan.parts * 4;
   } else {
     a.grad = grad;
   }

@@ -41,7 +41,11 @@ struct Wide {
   static constexpr int E = 16 / sizeof(T);  // elements of a 16-byte access
 
   __device__ __forceinline__ static uint4 load(const T* p) {
+#ifdef NTL
+    const V v = __builtin_nontemporal_load(reinterpret_cast<const V*>(p));
+#else
     const V v = *reinterpret_cast<const V*>(p);
+#endif
     return make_uint4(v.x, v.y, v.z, v.w);
   }
   __device__ __forceinline__ static uint4 none() {  // -inf in every element
@@ -74,7 +78,11 @@ struct Wide {
       else
         v[i] = f32_to_f16(x[2 * i]) | static_cast<uint32_t>(f32_to_f16(x[2 * i + 1])) << 16;
     }
+#ifdef NTS
+    __builtin_nontemporal_store(v, reinterpret_cast<V*>(p));
+#else
     *reinterpret_cast<V*>(p) = v;
+#endif
   }
   // one value
   __device__ __forceinline__ static void store(T* p, const float (&x)[1]) { Elem<DT>::store(p, 0, x[0]); }
@@ -82,9 +90,10 @@ struct Wide {
 
 // A workgroup's view of one row, or of a part of one: `each` calls f(first, x)
 // for every run of E columns (x: their values; -inf and first >= count where a
-// thread has none) and once more for the last count % E columns, one a thread.
-// The calls go up through the columns by thread and then by call, and all
-// threads make the same calls, so f may hold barriers.
+// thread has none) and once more for the columns that no run has, one a thread:
+// the `head` columns before the first run and the fewer than E after the last.
+// All threads make the same calls, so f may hold barriers; without a head the
+// calls go up through the columns by thread and then by call.
 //
 // With HELD > 0 the columns are loaded once, HELD 16-byte runs a thread, and
 // stay in registers for every pass (up to THREADS * HELD runs); with HELD = 0
@@ -97,31 +106,40 @@ struct Row {
   static constexpr int kStep = THREADS * E;
   static constexpr bool kHeld = HELD > 0;
   const T* p;
-  int count;
+  int count, head, whole;  // whole: the columns in runs
   uint4 held[HELD > 0 ? HELD : 1];
   float last;
 
-  __device__ __forceinline__ Row(const T* columns, int n) : p(columns), count(n) {
+  __device__ __forceinline__ Row(const T* columns, int n, int before = 0)
+      : p(columns), count(n), head(min(before, n)), whole((n - min(before, n)) / E * E) {
     if constexpr (HELD > 0) {
-      const int whole = count - count % E, mine = static_cast<int>(threadIdx.x) * E;
+      const T* runs = p + head;
+      const int mine = static_cast<int>(threadIdx.x) * E;
 #pragma unroll
       for (int i = 0; i < HELD; ++i) {
         held[i] = W::none();
         if ((i + 1) * kStep <= whole)
-          held[i] = W::load(p + i * kStep + mine);
+          held[i] = W::load(runs + i * kStep + mine);
         else if (i * kStep + mine < whole)
-          held[i] = W::load(p + i * kStep + mine);
+          held[i] = W::load(runs + i * kStep + mine);
       }
-      const int at = whole + static_cast<int>(threadIdx.x);
+      const int at = single();
       last = at < count ? Elem<DT>::load(p, at) : -INFINITY;
     }
   }
 
-  // over the columns [from, to): `from` a multiple of kStep, and `to` one or the row's end
+  // this thread's column outside the runs
+  __device__ __forceinline__ int single() const {
+    const int at = static_cast<int>(threadIdx.x);
+    return at < head ? at : at + whole;
+  }
+
+  // over the runs that begin in [from, to) columns past the head, `from` and `to`
+  // multiples of kStep; with to = count over the rest, the single columns too
   template <class F>
   __device__ __forceinline__ void each(int from, int to, F&& f) const {
-    const int whole = count - count % E;
-    int mine = static_cast<int>(threadIdx.x) * E;
+    int mine = head + static_cast<int>(threadIdx.x) * E;
+    const int end = head + whole;
     if constexpr (HELD > 0) {
       // a pass works its columns out anew: carried from pass to pass they would take a register for each run
       asm volatile("" : "+v"(mine));
@@ -131,19 +149,19 @@ struct Row {
           const int first = i * kStep + mine;
           float x[E];
           W::unpack(held[i], x);
-          f(first < whole ? first : count, x);
+          f(first < end ? first : count, x);
         }
       }
     } else {
       for (int at = from; at < to && at < whole; at += kStep) {
         const int first = at + mine;
         float x[E];
-        W::unpack(first < whole ? W::load(p + first) : W::none(), x);
-        f(first < whole ? first : count, x);
+        W::unpack(first < end ? W::load(p + first) : W::none(), x);
+        f(first < end ? first : count, x);
       }
     }
     if (to >= count && whole < count) {
-      const int at = whole + static_cast<int>(threadIdx.x);
+      const int at = single();
       float x[1];
       if constexpr (HELD > 0)
         x[0] = last;
@@ -157,6 +175,14 @@ struct Row {
     each(0, count, f);
   }
 };
+
+// The columns of a row of gradients before its first full 128-byte line: from
+// there on a wave's store of 64 runs covers whole lines
+template <int DT>
+__device__ __forceinline__ int before_line(const typename Elem<DT>::T* out) {
+  constexpr int size = sizeof(typename Elem<DT>::T);
+  return static_cast<int>((128 - reinterpret_cast<uintptr_t>(out) % 128) % 128) / size;
+}
 
 // the 16-byte runs that a row of `vocab` columns has
 inline int64_t runs_of(int64_t vocab, int dtype) { return vocab / (dtype == QSTE_F32 ? 4 : 8); }

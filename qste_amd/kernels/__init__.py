@@ -914,7 +914,7 @@ def embedding_backward(ids: Tensor, grad: Tensor, packed: Tensor, scale: Tensor,
 # in the reference)
 # ---------------------------------------------------------------------------
 
-MAX_TOP, MAX_ENTRIES, MAX_VOCAB, DISTILL_STATS = 128, 1024, 1 << 30, 5  # as in include/qste_hip.h
+MAX_TOP, MAX_ENTRIES, MAX_VOCAB, DISTILL_STATS = 128, 1024, 1 << 30, 6  # as in include/qste_hip.h
 
 
 def _logit_rows(logits: Tensor) -> tuple[Tensor, tuple[int, int, int, int, int]]:
@@ -1040,7 +1040,7 @@ def _teacher(logits: Tensor, top_tokens: Tensor, top_logprobs: Tensor) -> tuple[
 def distill_forward(logits: Tensor, top_tokens: Tensor, top_logprobs: Tensor, *, temperature: float = 1.0,
                     tail: bool = False, loss_grad: Tensor | None = None, want_stats: bool = False):
     """``(losses, stats, grad)``: the losses fp32 [...] of logits [..., vocab] against
-    a teacher's ``top_tokens`` and ``top_logprobs`` [..., k]; ``stats`` fp32 [..., 5], what
+    a teacher's ``top_tokens`` and ``top_logprobs`` [..., k]; ``stats`` fp32 [..., 6], what
     ``distill_backward`` reads, if asked for; and with ``loss_grad`` [...] the
     logits' gradient for these weights, from the same pass, else None."""
 

@@ -79,7 +79,7 @@ def token_logprobs(logits: Tensor, tokens: Optional[Tensor] = None, *, top: int 
 
 class DistillationFn(Function):
     """``distillation_loss`` with the logits' gradient; keeps the logits, the
-    teacher's entries and five floats a row."""
+    teacher's entries and six floats a row."""
 
     @staticmethod
     def forward(ctx, logits, top_tokens, top_logprobs, temperature: float, tail: bool):
