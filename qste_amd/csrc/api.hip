@@ -151,6 +151,12 @@ int logits_ok(const void* logits, int dtype, int64_t outer, int64_t inner, int64
   return 0;
 }
 
+vocab::Logits logits_of(const void* logits, int dtype, int64_t outer, int64_t inner, int64_t outer_stride,
+                        int64_t inner_stride, int64_t vocab) {
+  return vocab::streamed({logits, inner, outer_stride, inner_stride, static_cast<int>(vocab), false, false},
+                         outer * inner, dtype);
+}
+
 struct BackwardLayout {
   size_t v_part, db_part, v, gs_part, w_t, x_t, s16, xs16, partial, limbs, limb_bytes, dy_pad, w_pad, total;
   int64_t chunks, tiles;
@@ -830,7 +836,7 @@ int qste_token_logprobs(const void* logits, int dtype, int64_t outer, int64_t in
   if (reinterpret_cast<uintptr_t>(stats) % 8 || reinterpret_cast<uintptr_t>(workspace) % 8) return QSTE_E_ALIGN;
   const size_t need = token_logprobs_workspace(outer * inner, vocab, dtype, top);
   if (need && (!workspace || workspace_bytes < need)) return QSTE_E_WORKSPACE;
-  const vocab::Logits l{logits, inner, outer_stride, inner_stride, static_cast<int>(vocab)};
+  const vocab::Logits l = logits_of(logits, dtype, outer, inner, outer_stride, inner_stride, vocab);
   return launch_token_logprobs(l, dtype, outer * inner, tokens, temperature, top, logprobs, entropy, top_logprobs,
                                top_tokens, stats, workspace, as_stream(stream));
 }
@@ -843,7 +849,7 @@ int qste_token_logprobs_backward(const void* logits, int dtype, int64_t outer, i
   if (outer * inner == 0) return 0;
   if (!entropy || !stats || !grad) return QSTE_E_NULL;
   if (reinterpret_cast<uintptr_t>(grad) % 16) return QSTE_E_ALIGN;
-  const vocab::Logits l{logits, inner, outer_stride, inner_stride, static_cast<int>(vocab)};
+  const vocab::Logits l = logits_of(logits, dtype, outer, inner, outer_stride, inner_stride, vocab);
   return launch_token_logprobs_backward(l, dtype, outer * inner, tokens, temperature, logprob_grad, entropy_grad,
                                         entropy, stats, grad, as_stream(stream));
 }
@@ -864,7 +870,7 @@ int qste_distill(const void* logits, int dtype, int64_t outer, int64_t inner, in
   if (reinterpret_cast<uintptr_t>(grad) % 16 || reinterpret_cast<uintptr_t>(workspace) % 16) return QSTE_E_ALIGN;
   const size_t need = distill_workspace(outer * inner, vocab, dtype, grad != nullptr);
   if (need && (!workspace || workspace_bytes < need)) return QSTE_E_WORKSPACE;
-  const vocab::Logits l{logits, inner, outer_stride, inner_stride, static_cast<int>(vocab)};
+  const vocab::Logits l = logits_of(logits, dtype, outer, inner, outer_stride, inner_stride, vocab);
   return launch_distill(l, dtype, outer * inner, top_tokens, top_logprobs, k, temperature, tail != 0, losses, stats,
                         loss_grad, grad, workspace, as_stream(stream));
 }
@@ -878,7 +884,7 @@ int qste_distill_backward(const void* logits, int dtype, int64_t outer, int64_t 
   if (outer * inner == 0) return 0;
   if (!top_tokens || !top_logprobs || !stats || !loss_grad || !grad) return QSTE_E_NULL;
   if (reinterpret_cast<uintptr_t>(grad) % 16) return QSTE_E_ALIGN;
-  const vocab::Logits l{logits, inner, outer_stride, inner_stride, static_cast<int>(vocab)};
+  const vocab::Logits l = logits_of(logits, dtype, outer, inner, outer_stride, inner_stride, vocab);
   return launch_distill_backward(l, dtype, outer * inner, top_tokens, top_logprobs, k, temperature, tail != 0, stats,
                                  loss_grad, grad, as_stream(stream));
 }

@@ -91,20 +91,30 @@ __device__ __forceinline__ double exp_exactly(float v) {
   return ldexp(p, static_cast<int>(fmin(n, 1024.0)));
 }
 
-// One wave reads the entries, while the others' loads of the row are on
-// their way: token and ln q to LDS, the rest in every lane.
-__device__ __forceinline__ Teacher load_entries(const Args& a, int64_t r, const Entries& t) {
+// A lane's first entry, asked for before the row: loads come back in order
+struct First {
+  int64_t token;
+  float value;
+};
+
+__device__ __forceinline__ First load_first(const Args& a, int64_t r) {
+  const int64_t at = r * a.k + min(static_cast<int>(threadIdx.x), a.k - 1);
+  return {a.tokens[at], a.values[at]};
+}
+
+// One wave takes the entries, while the row's loads are on their way: token
+// and ln q to LDS, the rest in every lane.
+__device__ __forceinline__ Teacher load_entries(const Args& a, int64_t r, const First& first, const Entries& t) {
   const int lane = threadIdx.x & (kWave - 1);
-  const int64_t* tokens = a.tokens + r * a.k;
-  const float* values = a.values + r * a.k;
   float top = -INFINITY;
   bool any = false, bad = false;
   for (int k = lane; k < a.k; k += kWave) {
-    const int64_t at = tokens[k];
+    const int64_t at = k < kWave ? first.token : a.tokens[r * a.k + k];
     const bool there = at >= 0 && at < a.logits.vocab;
     any |= there;
     bad |= at >= a.logits.vocab;
-    const float v = there ? values[k] : -INFINITY;
+    const float given = k < kWave ? first.value : a.values[r * a.k + k];
+    const float v = there ? given : -INFINITY;
     t.token[k] = there ? static_cast<int>(at) : -1;
     t.log_q[k] = v;
     top = fmaxf(top, v);
@@ -188,11 +198,11 @@ struct Shared {
 // The row's or part's maximum and sums, the entries read on the way (all of
 // them by the first wave).
 template <class R>
-__device__ __forceinline__ void reduce(const Args& a, int64_t r, const R& row, const Entries& t, int begin, Shared& sh,
+__device__ __forceinline__ void reduce(const Args& a, int64_t r, const First& first, const R& row, const Entries& t, int begin, Shared& sh,
                                        float& m, float& sum, float& outside) {
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   if (wave == 0) {
-    Teacher teacher = load_entries(a, r, t);
+    Teacher teacher = load_entries(a, r, first, t);
     if (R::kHeld) teacher.repeated = mark_listed(a, t, begin, row.count, row.head, 0, row.count);
     if (lane == 0) sh.teacher = teacher;
   }
@@ -323,14 +333,14 @@ __global__ __launch_bounds__(kThreads, WAVES_A_SIMD) void forward_kernel(Args a)
   extern __shared__ uint32_t lds[];
   __shared__ Shared sh;
   using R = Row<DT, kThreads, HELD>;
-  using W = Wide<DT>;
   const int64_t r = blockIdx.x;
   const int vocab = a.logits.vocab;
   const Entries t(lds, a.k);
   typename R::T* out = static_cast<typename R::T*>(a.grad) + r * vocab;
-  const R row(a.logits.row<typename R::T>(r), vocab, a.grad ? before_line<DT>(out) : 0);
+  const First first = load_first(a, r);
+  const R row(a.logits.row<typename R::T>(r), vocab, a.grad ? before_line<DT>(out) : 0, a.logits.once);
   float m, sum, outside;
-  reduce(a, r, row, t, 0, sh, m, sum, outside);
+  reduce(a, r, first, row, t, 0, sh, m, sum, outside);
   const Teacher teacher = sh.teacher;
   if (teacher.none(a.tail)) {
     write_none(a, r);
@@ -345,11 +355,10 @@ __global__ __launch_bounds__(kThreads, WAVES_A_SIMD) void forward_kernel(Args a)
       zero_row<DT, kThreads>(out, 0, vocab);
     } else {
       const float per_q = g * a.temperature, per_p = per_q / sum, per_other = per_p * co.other;
-      row.each([&](int first, auto& x) {
+      row.map(out, a.logits.write_once, [&](int, auto& x) {
         constexpr int N = sizeof(x) / sizeof(x[0]);
 #pragma unroll
         for (int j = 0; j < N; ++j) x[j] = ex.of(ex.power(x[j])) * per_other;
-        if (first < vocab) W::store(out + first, x);
       });
       write_listed<DT>(a, t, teacher.repeated, r, ex, per_p * co.weight, per_q, 0, vocab);
     }
@@ -370,9 +379,10 @@ __global__ __launch_bounds__(kThreads, WAVES_A_SIMD) void part_kernel(Args a) {
   const int part = blockIdx.x % static_cast<uint32_t>(a.parts);
   const int from = part * a.part, to = part < a.parts - 1 ? from + a.part : a.logits.vocab;
   const Entries t(lds, a.k);
-  const R row(a.logits.row<typename R::T>(r) + from, to - from);
+  const First first = load_first(a, r);
+  const R row(a.logits.row<typename R::T>(r) + from, to - from, 0, a.logits.once);
   float m, sum, outside;
-  reduce(a, r, row, t, from, sh, m, sum, outside);
+  reduce(a, r, first, row, t, from, sh, m, sum, outside);
   if (threadIdx.x == 0)
     reinterpret_cast<float4*>(a.part_stats)[r * a.parts + part] =
         make_float4(m, sum, outside, sh.teacher.repeated ? 1.0f : 0.0f);
@@ -385,7 +395,7 @@ __global__ __launch_bounds__(kWave) void join_kernel(Args a) {
   const int64_t r = blockIdx.x;
   const Entries t(lds, a.k);
   const float4* parts = reinterpret_cast<const float4*>(a.part_stats) + r * a.parts;
-  Teacher teacher = load_entries(a, r, t);
+  Teacher teacher = load_entries(a, r, load_first(a, r), t);
   if (teacher.none(a.tail)) {
     write_none(a, r);
     return;
@@ -408,16 +418,12 @@ __global__ __launch_bounds__(kWave) void join_kernel(Args a) {
 // the gradient from a forward's statistics: one workgroup per part of a row
 // ---------------------------------------------------------------------------
 
-#ifndef BR
-#define BR 4
-#endif
-constexpr int kBackRuns = BR;  // 16-byte accesses a thread makes
+constexpr int kBackRuns = 4;  // 16-byte accesses a thread makes
 
 template <int DT>
 __global__ __launch_bounds__(kThreads) void backward_kernel(Args a) {
   extern __shared__ uint32_t lds[];
   using R = Row<DT, kThreads, kBackRuns>;
-  using W = Wide<DT>;
   const int64_t r = blockIdx.x / static_cast<uint32_t>(a.parts);
   const int part = blockIdx.x % static_cast<uint32_t>(a.parts), vocab = a.logits.vocab;
   typename R::T* out = static_cast<typename R::T*>(a.grad) + r * vocab;
@@ -431,20 +437,20 @@ __global__ __launch_bounds__(kThreads) void backward_kernel(Args a) {
     zero_row<DT, kThreads>(out + from, 0, to - from);
     return;
   }
-  const R row(a.logits.row<typename R::T>(r) + from, to - from, part == 0 ? head : 0);
   const Entries t(lds, a.k);
+  const First first = load_first(a, r);
+  const R row(a.logits.row<typename R::T>(r) + from, to - from, part == 0 ? head : 0, a.logits.once);
   for (int k = threadIdx.x; k < a.k; k += kThreads) {
-    const int64_t at = a.tokens[r * a.k + k];
+    const int64_t at = k < kThreads ? first.token : a.tokens[r * a.k + k];
     t.token[k] = at >= from && at < to ? static_cast<int>(at) : -1;
-    t.log_q[k] = a.values[r * a.k + k] - shift;
+    t.log_q[k] = (k < kThreads ? first.value : a.values[r * a.k + k]) - shift;
   }
   const Exponent ex(m, a.scale);
   const float per_q = g * a.temperature, per_p = per_q / sum, per_other = per_p * other;
-  row.each([&](int first, auto& x) {
+  row.map(out + from, a.logits.write_once, [&](int, auto& x) {
     constexpr int N = sizeof(x) / sizeof(x[0]);
 #pragma unroll
     for (int j = 0; j < N; ++j) x[j] = ex.of(ex.power(x[j])) * per_other;
-    if (first < row.count) W::store(out + from + first, x);
   });
   write_listed<DT>(a, t, st[5] != 0.0f, r, ex, per_p * weight, per_q, from, to);
 }

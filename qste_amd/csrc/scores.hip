@@ -239,7 +239,7 @@ __global__ __launch_bounds__(kThreads, WAVES_A_SIMD) void forward_kernel(Args a)
   const int from = SPLIT ? part * a.part : 0;
   const int to = SPLIT && part < a.parts - 1 ? from + a.part : a.logits.vocab;
   const typename R::T* columns = a.logits.row<typename R::T>(r) + from;
-  const R row(columns, to - from);
+  const R row(columns, to - from, 0, a.logits.once);
   const int top = min(a.top, row.count);
   float lane_max = -INFINITY;
   row.each([&](int, auto& x) { lane_max = max_of(lane_max, x); });
@@ -468,8 +468,7 @@ int forward(Args a, int64_t rows, const Plan& plan, hipStream_t s) {
 // backward: elementwise over (part of a row, row)
 // ---------------------------------------------------------------------------
 
-constexpr int kBackThreads = 256;
-constexpr int kBackRuns = 8;  // 16-byte accesses a thread makes
+constexpr int kBackRuns = 4;  // 16-byte accesses a thread makes
 
 struct BackArgs {
   Logits logits;
@@ -483,39 +482,41 @@ struct BackArgs {
 };
 
 template <int DT>
-__global__ __launch_bounds__(kBackThreads) void backward_kernel(BackArgs a, int parts) {
+__global__ __launch_bounds__(kThreads) void backward_kernel(BackArgs a, int parts) {
   using W = Wide<DT>;
-  using T = typename W::T;
-  const int64_t r = blockIdx.x / parts;
-  constexpr int kPart = kBackThreads * kBackRuns * W::E;
-  const int from = static_cast<int>(blockIdx.x % parts) * kPart;
-  const Row<DT, kBackThreads, 0> row(a.logits.row<T>(r), a.logits.vocab);
-  const int to = min(row.count, from + kPart);
-  T* out = static_cast<T*>(a.grad) + r * row.count;
+  using R = Row<DT, kThreads, kBackRuns>;
+  constexpr int kPart = kThreads * kBackRuns * W::E;
+  const int64_t r = blockIdx.x / static_cast<uint32_t>(parts);
+  const int part = blockIdx.x % static_cast<uint32_t>(parts), vocab = a.logits.vocab;
+  typename R::T* out = static_cast<typename R::T*>(a.grad) + r * vocab;
+  // parts begin at whole lines of the gradient, but for the first
+  const int head = min(vocab, before_line<DT>(out));
+  const int from = part == 0 ? 0 : min(vocab, head + part * kPart), to = min(vocab, head + (part + 1) * kPart);
+  out += from;
   const int64_t token = a.tokens ? a.tokens[r] : -1;
   const float m = a.stats[2 * r], sum = a.stats[2 * r + 1];
   float g = a.logprob_grad && token >= 0 ? a.logprob_grad[r] : 0.0f;
   const float h = a.entropy_grad && (token >= 0 || !a.tokens) ? a.entropy_grad[r] : 0.0f;
   if ((g == 0.0f && h == 0.0f) || sum == 0.0f) {  // nothing flows back: the row is not read
-    zero_row<DT, kBackThreads>(out, from, to);
+    zero_row<DT, kThreads>(out, 0, to - from);
     return;
   }
-  if (token >= row.count) g = NAN;
+  const R row(a.logits.row<typename R::T>(r) + from, to - from, part == 0 ? head : 0, a.logits.once);
+  if (token >= vocab) g = NAN;
   const Exponent ex(m, a.scale);
   // dz = e (flat + slope power), from p = e / S and ln p = ln2 power - ln S
   const float per = -a.inverse / sum;
   const float flat = per * (g + h * (a.entropy[r] - logf(sum)));
   const float slope = per * h * kLn2;
   const float extra = g * a.inverse;
-  row.each(from, to, [&](int first, auto& x) {
+  const int64_t mine = token - from;
+  row.map(out, a.logits.write_once, [&](int first, auto& x) {
     constexpr int N = sizeof(x) / sizeof(x[0]);
-    if (first >= row.count) return;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       const float power = ex.power(x[j]), e = ex.of(power);
-      x[j] = e * fmaf(slope, fmaxf(power, -200.0f), flat) + (first + j == token ? extra : 0.0f);
+      x[j] = e * fmaf(slope, fmaxf(power, -200.0f), flat) + (first + j == mine ? extra : 0.0f);
     }
-    W::store(out + first, x);
   });
 }
 
@@ -550,17 +551,17 @@ int launch_token_logprobs_backward(const vocab::Logits& logits, int dtype, int64
   using namespace scores;
   const BackArgs a{logits, tokens, static_cast<float>(1.4426950408889634 / temperature),
                    static_cast<float>(1.0 / temperature), logprob_grad, entropy_grad, entropy, stats, grad};
-  const int part = kBackThreads * kBackRuns * (dtype == QSTE_F32 ? 4 : 8);
+  const int part = kThreads * kBackRuns * (dtype == QSTE_F32 ? 4 : 8);
   const int parts = ceil_div(logits.vocab, part);
   const int64_t blocks = rows * parts;
   if (blocks > INT32_MAX) return QSTE_E_SHAPE;
   const dim3 grid(static_cast<unsigned>(blocks));
   if (dtype == QSTE_F32)
-    backward_kernel<QSTE_F32><<<grid, kBackThreads, 0, s>>>(a, parts);
+    backward_kernel<QSTE_F32><<<grid, kThreads, 0, s>>>(a, parts);
   else if (dtype == QSTE_F16)
-    backward_kernel<QSTE_F16><<<grid, kBackThreads, 0, s>>>(a, parts);
+    backward_kernel<QSTE_F16><<<grid, kThreads, 0, s>>>(a, parts);
   else
-    backward_kernel<QSTE_BF16><<<grid, kBackThreads, 0, s>>>(a, parts);
+    backward_kernel<QSTE_BF16><<<grid, kThreads, 0, s>>>(a, parts);
   return static_cast<int>(hipGetLastError());
 }
 

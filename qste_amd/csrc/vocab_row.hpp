@@ -21,6 +21,7 @@ struct Logits {
   const void* p;
   int64_t inner, outer_stride, inner_stride;
   int vocab;
+  bool once, write_once;  // read, written without keeping the lines: streamed()
 
   template <class T>
   __device__ __forceinline__ const T* row(int64_t r) const {
@@ -40,12 +41,9 @@ struct Wide {
   using V = std::conditional_t<DT == QSTE_F32, Word16, Half16>;
   static constexpr int E = 16 / sizeof(T);  // elements of a 16-byte access
 
+  template <bool ONCE = false>
   __device__ __forceinline__ static uint4 load(const T* p) {
-#ifdef NTL
-    const V v = __builtin_nontemporal_load(reinterpret_cast<const V*>(p));
-#else
-    const V v = *reinterpret_cast<const V*>(p);
-#endif
+    const V v = ONCE ? __builtin_nontemporal_load(reinterpret_cast<const V*>(p)) : *reinterpret_cast<const V*>(p);
     return make_uint4(v.x, v.y, v.z, v.w);
   }
   __device__ __forceinline__ static uint4 none() {  // -inf in every element
@@ -67,6 +65,7 @@ struct Wide {
       }
     }
   }
+  template <bool ONCE = false>
   __device__ __forceinline__ static void store(T* p, const float (&x)[E]) {
     V v;
 #pragma unroll
@@ -78,14 +77,16 @@ struct Wide {
       else
         v[i] = f32_to_f16(x[2 * i]) | static_cast<uint32_t>(f32_to_f16(x[2 * i + 1])) << 16;
     }
-#ifdef NTS
-    __builtin_nontemporal_store(v, reinterpret_cast<V*>(p));
-#else
-    *reinterpret_cast<V*>(p) = v;
-#endif
+    if constexpr (ONCE)
+      __builtin_nontemporal_store(v, reinterpret_cast<V*>(p));
+    else
+      *reinterpret_cast<V*>(p) = v;
   }
   // one value
-  __device__ __forceinline__ static void store(T* p, const float (&x)[1]) { Elem<DT>::store(p, 0, x[0]); }
+  template <bool ONCE = false>
+  __device__ __forceinline__ static void store(T* p, const float (&x)[1]) {
+    Elem<DT>::store(p, 0, x[0]);
+  }
 };
 
 // A workgroup's view of one row, or of a part of one: `each` calls f(first, x)
@@ -110,21 +111,29 @@ struct Row {
   uint4 held[HELD > 0 ? HELD : 1];
   float last;
 
-  __device__ __forceinline__ Row(const T* columns, int n, int before = 0)
+  __device__ __forceinline__ Row(const T* columns, int n, int before = 0, bool once = false)
       : p(columns), count(n), head(min(before, n)), whole((n - min(before, n)) / E * E) {
     if constexpr (HELD > 0) {
-      const T* runs = p + head;
-      const int mine = static_cast<int>(threadIdx.x) * E;
-#pragma unroll
-      for (int i = 0; i < HELD; ++i) {
-        held[i] = W::none();
-        if ((i + 1) * kStep <= whole)
-          held[i] = W::load(runs + i * kStep + mine);
-        else if (i * kStep + mine < whole)
-          held[i] = W::load(runs + i * kStep + mine);
-      }
+      if (once)
+        hold<true>();
+      else
+        hold<false>();
       const int at = single();
       last = at < count ? Elem<DT>::load(p, at) : -INFINITY;
+    }
+  }
+
+  template <bool ONCE>
+  __device__ __forceinline__ void hold() {
+    const T* runs = p + head;
+    const int mine = static_cast<int>(threadIdx.x) * E;
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) {
+      held[i] = W::none();
+      if ((i + 1) * kStep <= whole)
+        held[i] = W::template load<ONCE>(runs + i * kStep + mine);
+      else if (i * kStep + mine < whole)
+        held[i] = W::template load<ONCE>(runs + i * kStep + mine);
     }
   }
 
@@ -174,7 +183,35 @@ struct Row {
   __device__ __forceinline__ void each(F&& f) const {
     each(0, count, f);
   }
+
+  // f(first, x) leaves in x what goes to `out`, a row of its own
+  template <class F>
+  __device__ __forceinline__ void map(T* out, bool once, F&& f) const {
+    if (once)
+      each([&](int first, auto& x) {
+        f(first, x);
+        if (first < count) W::template store<true>(out + first, x);
+      });
+    else
+      each([&](int first, auto& x) {
+        f(first, x);
+        if (first < count) W::template store<false>(out + first, x);
+      });
+  }
 };
+
+// Whether logits are read, and gradients written, without keeping their lines:
+// what is larger than the 256 MiB last-level cache goes through it unread.
+// 4096 rows of 50257 bf16 logits (412 MB), kept / streamed: the distillation
+// loss 127 / 122 us, with the gradient 191 / 170; but at 4099 columns (34 MB,
+// found in the cache) 24.8 / 28.7.  Stores gain from a size less: 1533 rows of
+// 32003 (98 MB) 48.5 / 44.4 with the stores alone streamed, 48.6 with both.
+inline Logits streamed(Logits l, int64_t rows, int dtype) {
+  const double bytes = static_cast<double>(rows) * l.vocab * (dtype == QSTE_F32 ? 4 : 2);
+  l.once = bytes > 268435456.0;
+  l.write_once = bytes > 67108864.0;
+  return l;
+}
 
 // The columns of a row of gradients before its first full 128-byte line: from
 // there on a wave's store of 64 runs covers whole lines
