@@ -106,6 +106,7 @@ struct Row {
   static constexpr int E = W::E;
   static constexpr int kStep = THREADS * E;
   static constexpr bool kHeld = HELD > 0;
+  static constexpr bool kTight = HELD > 16;  // few registers are left
   const T* p;
   int count, head, whole;  // whole: the columns in runs
   uint4 held[HELD > 0 ? HELD : 1];

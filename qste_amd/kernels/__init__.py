@@ -925,12 +925,12 @@ def _logit_rows(logits: Tensor) -> tuple[Tensor, tuple[int, int, int, int, int]]
     if logits.dim() == 0 or not 0 < logits.shape[-1] <= MAX_VOCAB:
         raise ValueError(f"logits need a last dimension of 1 to {MAX_VOCAB} columns")
     vocab = int(logits.shape[-1])
-    if logits.numel() == 0:
-        return logits, (0, 0, 0, 0, vocab)
+    if logits.is_contiguous():
+        rows = logits.numel() // vocab
+        return logits, (1, rows, 0, vocab, vocab) if rows else (0, 0, 0, 0, vocab)
     groups = _merged_rows(logits)
     if len(groups) > 2 or (vocab > 1 and logits.stride(-1) != 1):
-        logits = logits.contiguous()
-        groups = _merged_rows(logits)
+        return _logit_rows(logits.detach().contiguous())
     (outer, outer_stride), (inner, inner_stride) = [(1, 0)] * (2 - len(groups)) + groups
     return logits, (outer, inner, outer_stride, inner_stride, vocab)
 
@@ -958,18 +958,22 @@ def _temperature(value: float) -> float:
 def _row_tokens(tokens: Tensor, shape, what: str) -> Tensor:
     """Token numbers of the given shape as contiguous int64."""
 
-    if tokens.dtype not in (torch.int64, torch.int32, torch.int16, torch.uint8):
-        raise TypeError(f"{what} must be integers, got {tokens.dtype}")
-    if tuple(tokens.shape) != tuple(shape):
+    if tokens.shape != shape:
         raise ValueError(f"{what} have shape {tuple(tokens.shape)}, expected {tuple(shape)}")
-    return tokens.to(torch.int64).contiguous()
+    if tokens.dtype != torch.int64:
+        if tokens.dtype not in (torch.int32, torch.int16, torch.uint8):
+            raise TypeError(f"{what} must be integers, got {tokens.dtype}")
+        tokens = tokens.to(torch.int64)
+    return tokens.contiguous()
 
 
 def _row_weights(weights: Tensor | None, shape, what: str) -> Tensor | None:
     if weights is None:
         return None
-    if tuple(weights.shape) != tuple(shape):
+    if weights.shape != shape:
         raise ValueError(f"{what} has shape {tuple(weights.shape)}, expected {tuple(shape)}")
+    if weights.dtype == torch.float32 and weights.is_contiguous():
+        return weights
     return _f32(weights)
 
 
@@ -986,7 +990,7 @@ def token_logprobs_forward(logits: Tensor, tokens: Tensor | None, *, top: int = 
 
     device = _require_gpu(logits, tokens)
     code = _dtype_code(logits)
-    rows, layout = _logit_rows(logits.detach())
+    rows, layout = _logit_rows(logits)
     shape, vocab, top, temperature = logits.shape[:-1], layout[4], int(top), _temperature(temperature)
     if not 0 <= top <= min(MAX_TOP, vocab):
         raise ValueError(f"top must lie in 0 .. {min(MAX_TOP, vocab)}, got {top}")
@@ -1013,7 +1017,7 @@ def token_logprobs_backward(logits: Tensor, tokens: Tensor | None, logprob_grad:
 
     device = _require_gpu(logits, tokens, logprob_grad, entropy_grad, entropy, stats)
     code = _dtype_code(logits)
-    rows, layout = _logit_rows(logits.detach())
+    rows, layout = _logit_rows(logits)
     shape, temperature = logits.shape[:-1], _temperature(temperature)
     tokens_i64 = None if tokens is None else _row_tokens(tokens, shape, "tokens")
     g = _row_weights(logprob_grad, shape, "logprob_grad")
@@ -1046,7 +1050,7 @@ def distill_forward(logits: Tensor, top_tokens: Tensor, top_logprobs: Tensor, *,
 
     device = _require_gpu(logits, top_tokens, top_logprobs, loss_grad)
     code = _dtype_code(logits)
-    rows, layout = _logit_rows(logits.detach())
+    rows, layout = _logit_rows(logits)
     shape, temperature = logits.shape[:-1], _temperature(temperature)
     tokens_i64, values = _teacher(logits, top_tokens, top_logprobs)
     weights = _row_weights(loss_grad, shape, "loss_grad")
@@ -1068,7 +1072,7 @@ def distill_backward(logits: Tensor, top_tokens: Tensor, top_logprobs: Tensor, l
 
     device = _require_gpu(logits, top_tokens, top_logprobs, loss_grad, stats)
     code = _dtype_code(logits)
-    rows, layout = _logit_rows(logits.detach())
+    rows, layout = _logit_rows(logits)
     shape, temperature = logits.shape[:-1], _temperature(temperature)
     tokens_i64, values = _teacher(logits, top_tokens, top_logprobs)
     weights = _row_weights(loss_grad, shape, "loss_grad")

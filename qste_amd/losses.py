@@ -139,7 +139,7 @@ def distillation_loss_and_grad(logits: Tensor, top_tokens: Tensor, top_logprobs:
     _constant(top_logprobs)
     shape = logits.shape[:-1]
     if isinstance(loss_grad, Tensor):
-        weights = loss_grad.detach().expand(shape)
+        weights = loss_grad if loss_grad.shape == shape else loss_grad.expand(shape)
     else:
         weights = torch.full(shape, float(loss_grad), dtype=torch.float32, device=logits.device)
     losses, _, grad = kernels.distill_forward(logits, top_tokens, top_logprobs, temperature=temperature, tail=tail,
