@@ -7,6 +7,8 @@
 //   top: the largest z, equal ones by the lowest token (NaN above all)
 //   dz_j = (g ([j = token] - p_j) - h p_j (ln p_j + H)) / T
 // for the gradients g of the logprob and h of the entropy.
+#include <float.h>
+
 #include "vocab_row.hpp"
 
 namespace qste {
@@ -15,6 +17,7 @@ namespace scores {
 using namespace vocab;
 
 constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / kWave;
 constexpr int kCandidates = 1024, kRuns = 384;
 constexpr int kMaxParts = 32;
 
@@ -40,7 +43,7 @@ struct Args {
 
 struct Candidates {
   int count, runs;
-  int scan[kThreads / kWave];
+  int scan[kWaves];
   int first[kRuns];
   float run[kRuns][8];
   uint64_t entry[kCandidates];  // key above ~column: larger is better, and no two are equal
@@ -110,14 +113,53 @@ __device__ __forceinline__ float edge_of(uint32_t bound) {
   return bound == 0 ? -INFINITY : value_of(full & 0x80000000u ? full : full | ((1u << SHIFT) - 1u));
 }
 
-// More than kCandidates values at or above the edge (long runs of equal values,
-// or rows in order): at least the k best into c again, from what is above
-// the edge, raised to the k-th key where that is still too much, and its equals
-// from the lowest column up.
+// `have` entries above the edge are in c, fewer than k: its equals (NaN for
+// nan_edge) from the lowest column up, to make k.
+template <class R>
+__device__ __forceinline__ void add_equals(const R& row, int from, float edge, bool nan_edge, int have, int k,
+                                           Candidates& c) {
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  row.each_while([&](int first, auto& x) {
+    constexpr int N = sizeof(x) / sizeof(x[0]);
+    int mine = 0;
+    if (first < row.count)
+#pragma unroll
+      for (int j = 0; j < N; ++j) mine += nan_edge ? x[j] != x[j] : x[j] == edge;
+    int upto = mine;  // this lane's and the lower lanes' of its wave
+#pragma unroll
+    for (int d = 1; d < kWave; d <<= 1) {
+      const int other = __shfl_up(upto, d, kWave);
+      if (lane >= d) upto += other;
+    }
+    __syncthreads();
+    if (lane == kWave - 1) c.scan[wave] = upto;
+    __syncthreads();
+    int at = have + upto - mine, total = 0;
+    for (int w = 0; w < kWaves; ++w) {
+      if (w < wave) at += c.scan[w];
+      total += c.scan[w];
+    }
+    if (first < row.count)
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (nan_edge ? x[j] != x[j] : x[j] == edge) {
+          if (at < k) c.entry[at] = entry_of(x[j], from + first + j);
+          ++at;
+        }
+    have += total;
+    return have < k;
+  });
+  __syncthreads();
+  if (threadIdx.x == 0) c.count = min(have, k);
+  __syncthreads();
+}
+
+// Too many values at or above the edge (long runs of equal values, or rows in
+// order), or NaN: at least the k best into c again, from what is above the
+// edge, raised to the k-th key where that is still too much, and its equals.
 template <int DT, class R>
 __device__ __forceinline__ void collect_many(const R& row, int from, float edge, int k, Candidates& c) {
   constexpr int BITS = kKeyBits<DT>;
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   bool nan_edge = false;
   auto above = [&] {  // only what is above the edge
     __syncthreads();
@@ -140,41 +182,7 @@ __device__ __forceinline__ void collect_many(const R& row, int from, float edge,
     edge = edge_of<BITS>(key);
     have = above();  // fewer than k
   }
-  if (have >= k) return;
-  // the edge's equals in column order
-  row.each([&](int first, auto& x) {
-    constexpr int N = sizeof(x) / sizeof(x[0]);
-    if (have >= k) return;
-    int mine = 0;
-    if (first < row.count)
-#pragma unroll
-      for (int j = 0; j < N; ++j) mine += nan_edge ? x[j] != x[j] : x[j] == edge;
-    int upto = mine;  // this lane's and the lower lanes' of its wave
-#pragma unroll
-    for (int d = 1; d < kWave; d <<= 1) {
-      const int other = __shfl_up(upto, d, kWave);
-      if (lane >= d) upto += other;
-    }
-    __syncthreads();
-    if (lane == kWave - 1) c.scan[wave] = upto;
-    __syncthreads();
-    int at = have + upto - mine, total = 0;
-    for (int w = 0; w < kThreads / kWave; ++w) {
-      if (w < wave) at += c.scan[w];
-      total += c.scan[w];
-    }
-    if (first < row.count)
-#pragma unroll
-      for (int j = 0; j < N; ++j)
-        if (nan_edge ? x[j] != x[j] : x[j] == edge) {
-          if (at < k) c.entry[at] = entry_of(x[j], from + first + j);
-          ++at;
-        }
-    have += total;
-  });
-  __syncthreads();
-  if (threadIdx.x == 0) c.count = min(have, k);
-  __syncthreads();
+  if (have < k) add_equals(row, from, edge, nan_edge, have, k, c);
 }
 
 // ---------------------------------------------------------------------------
@@ -223,10 +231,10 @@ __device__ __forceinline__ void write_top(const Args& a, int64_t r, int rank, ui
 
 template <int DT, int HELD, int WAVES_A_SIMD, bool SPLIT>
 __global__ __launch_bounds__(kThreads, WAVES_A_SIMD) void forward_kernel(Args a) {
-  constexpr int WAVES = kThreads / kWave, BITS = kKeyBits<DT>;
+  constexpr int BITS = kKeyBits<DT>;
   using R = Row<DT, kThreads, HELD>;
-  __shared__ float maxima[WAVES], sums[WAVES], moments[WAVES];
-  __shared__ uint32_t bounds[WAVES];
+  __shared__ float maxima[kWaves], sums[kWaves], moments[kWaves];
+  __shared__ uint32_t bounds[kWaves];
   __shared__ Candidates c;
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
   const int64_t r = SPLIT ? blockIdx.x / static_cast<uint32_t>(a.parts) : blockIdx.x;
@@ -245,7 +253,7 @@ __global__ __launch_bounds__(kThreads, WAVES_A_SIMD) void forward_kernel(Args a)
   row.each([&](int, auto& x) { lane_max = max_of(lane_max, x); });
 
   // the maximum, and an edge that `top` values reach
-  const int whole_waves = min(WAVES, row.count / (kWave * R::E));
+  const int whole_waves = min(kWaves, row.count / (kWave * R::E));
   const float wave_top = fold_max(lane_max);
   uint32_t bound = 0;
   if (top > 0 && whole_waves > 0) bound = wave_bound<BITS>(lane_max, (top + whole_waves - 1) / whole_waves);
@@ -258,18 +266,19 @@ __global__ __launch_bounds__(kThreads, WAVES_A_SIMD) void forward_kernel(Args a)
   float m = maxima[0];
   bound = bounds[0];
 #pragma unroll
-  for (int w = 1; w < WAVES; ++w) {
+  for (int w = 1; w < kWaves; ++w) {
     m = fmaxf(m, maxima[w]);
     bound = min(bound, bounds[w]);
   }
   if (whole_waves == 0) bound = 0;
   const float edge = edge_of<BITS>(bound);
+  const float least = fmaxf(edge, -FLT_MAX);  // where only -inf is sure to be reached by so many, it waits
 
   const Exponent ex(m, a.scale);
   float sum = 0.0f, moment = 0.0f;
   row.each([&](int first, auto& x) {
     constexpr int N = sizeof(x) / sizeof(x[0]);
-    if (top > 0 && !(max_of(-INFINITY, x) < edge)) {
+    if (top > 0 && !(max_of(-INFINITY, x) < least)) {
       if (first < row.count) {
         if constexpr (N == 1) {
           push(c, x[0], from + first);
@@ -300,7 +309,7 @@ __global__ __launch_bounds__(kThreads, WAVES_A_SIMD) void forward_kernel(Args a)
   sum = sums[0];
   moment = moments[0];
 #pragma unroll
-  for (int w = 1; w < WAVES; ++w) {
+  for (int w = 1; w < kWaves; ++w) {
     sum += sums[w];
     moment += moments[w];
   }
@@ -319,13 +328,17 @@ __global__ __launch_bounds__(kThreads, WAVES_A_SIMD) void forward_kernel(Args a)
       const int first = c.first[i];
 #pragma unroll
       for (int j = 0; j < R::E; ++j)
-        if (!(c.run[i][j] < edge)) push(c, c.run[i][j], from + first + j);
+        if (!(c.run[i][j] < least)) push(c, c.run[i][j], from + first + j);
     }
     __syncthreads();
   }
-  if (runs > kRuns || c.count > kCandidates || sum != sum)  // a run's maximum passes over NaN
-    collect_many<DT>(Row<DT, kThreads, 0>(columns, to - from), from, edge, top, c);
-  const int n = c.count;
+  const Row<DT, kThreads, 0> again(columns, to - from);
+  int n = c.count;
+  if (runs > kRuns || n > kCandidates || sum != sum)  // a run's maximum passes over NaN
+    collect_many<DT>(again, from, edge, top, c);
+  else if (n < top)
+    add_equals(again, from, -INFINITY, false, n, top, c);
+  n = c.count;
   for (int i = tid; i < n; i += kThreads) {
     const uint64_t mine = c.entry[i];
     int rank = 0;
@@ -415,28 +428,24 @@ struct Plan {
 
 // Up to 25 runs a thread stay in registers with four waves on a SIMD (120 to
 // 126 of 128 registers), so a row has up to kLong runs in one workgroup, or is
-// cut into parts of as many.  Shorter parts, of kShort runs, bring in more
-// workgroups where there are few:
-//   50257 bf16 logits a row, top 20, whole / in 4: 1 row 11.5 / 11.2 us, 8
-//   13.8 / 12.2, 40 14.3 / 12.3, 128 14.4 / 14.0; but 200 14.9 / 16.5, 500
-//   20.4 / 22.4 and 4096 97 / 110, where the join costs more than it gives;
-//   131072, where the row is cut in any case, in 3 / in 8: 1 row 14.3 / 12.4,
-//   128 21.2 / 18.7, 600 44.3 / 40.8; but 2048 107 / 111.
-// With many tokens to list the join decides: 16 rows of 131072 fp32 logits,
-// top 128, in 6 / in 16: 28 / 36 us.
+// cut into parts of as many.  Where it is cut in any case, shorter parts, of
+// kShort runs, bring in more workgroups for few rows: 131072 bf16 logits a row,
+// top 20, in 3 / in 8 parts: 1 row 14.3 / 12.4 us, 128 21.2 / 18.7, 600 44.3 /
+// 40.8; but 2048 107 / 111, and with many tokens to list the join decides (16
+// rows of 131072 fp32 logits, top 128, in 6 / in 16: 28 / 36).  A row that one
+// workgroup holds is left whole: cutting 40 rows of 50257 gained 14.3 -> 12.3
+// us on the GPU, less than the second launch takes on the host.
 constexpr int kShort = kThreads * 8, kMiddle = kThreads * 16, kLong = kThreads * 25;
-constexpr int64_t kGroupsWhole = 512, kGroupsCut = 4800, kListed = 1024;
+constexpr int64_t kGroups = 4800, kListed = 1024;
 
 Plan forward_plan(int64_t rows, int64_t vocab, int dtype, int64_t top) {
   const int64_t runs = runs_of(vocab, dtype), e = dtype == QSTE_F32 ? 4 : 8;
-  int64_t parts = runs > kLong ? (runs + kLong - 1) / kLong : 1;
+  if (runs <= kLong) return {1, 0};
+  int64_t parts = (runs + kLong - 1) / kLong;
   const int64_t more = (runs + kShort - 1) / kShort;
-  if (runs > kMiddle && more <= kMaxParts && rows * more <= (parts > 1 ? kGroupsCut : kGroupsWhole) &&
-      more * top <= kListed)
-    parts = more;
+  if (more <= kMaxParts && rows * more <= kGroups && more * top <= kListed) parts = more;
   if (parts > kMaxParts) return {0, 0};  // one workgroup reads the row again for each pass
-  // no part is empty: runs > parts * parts
-  return {static_cast<int>(parts), parts > 1 ? static_cast<int>((runs + parts - 1) / parts * e) : 0};
+  return {static_cast<int>(parts), static_cast<int>((runs + parts - 1) / parts * e)};  // runs > parts * parts: none is empty
 }
 
 template <int DT, int HELD, int WAVES_A_SIMD>

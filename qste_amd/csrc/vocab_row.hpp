@@ -185,6 +185,16 @@ struct Row {
     each(0, count, f);
   }
 
+  // each, for a row that is read again, while f(first, x) is true
+  template <class F>
+  __device__ __forceinline__ void each_while(F&& f) const {
+    static_assert(HELD == 0, "a row in registers has all its runs at hand");
+    bool more = true;
+    for (int at = 0; at < whole && more; at += kStep)
+      each(at, at + kStep < whole ? at + kStep : whole, [&](int first, auto& x) { more = f(first, x); });
+    if (more) each(whole, count, f);
+  }
+
   // f(first, x) leaves in x what goes to `out`, a row of its own
   template <class F>
   __device__ __forceinline__ void map(T* out, bool once, F&& f) const {
