@@ -22,7 +22,6 @@ namespace distill {
 using namespace vocab;
 
 constexpr int kThreads = 256;
-constexpr int kWaves = kThreads / kWave;
 constexpr int kMaxParts = 32;
 // columns whose membership in the list is held in LDS at a time, one bit each
 constexpr int kSpan = 1 << 17;
@@ -196,7 +195,7 @@ __device__ __forceinline__ void sums(const Args& a, const R& row, const Entries&
 
 // The workgroup's folds and the teacher
 struct Shared {
-  float maxima[kWaves], sum[kWaves], outside[kWaves];
+  float maxima[8], sum[8], outside[8];  // of up to 8 waves
   Teacher teacher;
 };
 
@@ -218,7 +217,7 @@ __device__ __forceinline__ void reduce(const Args& a, int64_t r, const First& fi
   __syncthreads();
   m = sh.maxima[0];
 #pragma unroll
-  for (int w = 1; w < kWaves; ++w) m = fmaxf(m, sh.maxima[w]);
+  for (int w = 1; w < R::kWaves; ++w) m = fmaxf(m, sh.maxima[w]);
   const Exponent ex(m, a.scale);
   sum = outside = 0.0f;
   if constexpr (R::kHeld) {
@@ -243,7 +242,7 @@ __device__ __forceinline__ void reduce(const Args& a, int64_t r, const First& fi
   sum = sh.sum[0];
   outside = sh.outside[0];
 #pragma unroll
-  for (int w = 1; w < kWaves; ++w) {
+  for (int w = 1; w < R::kWaves; ++w) {
     sum += sh.sum[w];
     outside += sh.outside[w];
   }
@@ -309,14 +308,14 @@ __device__ __forceinline__ void write_none(const Args& a, int64_t r) {
 
 // dz of the listed tokens with columns in [from, to), over what the workgroup's
 // first pass wrote there: all of a token's entries add up to its q
-template <int DT>
+template <int DT, int THREADS>
 __device__ __forceinline__ void write_listed(const Args& a, const Entries& t, bool repeated, int64_t r,
                                              const Exponent& ex, float per_p, float per_q, int from, int to) {
   using T = typename Elem<DT>::T;
   const T* row = a.logits.row<T>(r);
   T* out = static_cast<T*>(a.grad) + r * a.logits.vocab;
   __syncthreads();
-  for (int k = threadIdx.x; k < a.k; k += kThreads) {
+  for (int k = threadIdx.x; k < a.k; k += THREADS) {
     const int at = t.token[k];
     if (at < from || at >= to) continue;
     float q = expf(t.log_q[k]);
@@ -333,23 +332,24 @@ __device__ __forceinline__ void write_listed(const Args& a, const Entries& t, bo
 // the loss, and with `grad` the gradient too: one workgroup a row
 // ---------------------------------------------------------------------------
 
-template <int DT, int HELD, int WAVES_A_SIMD>
-__global__ __launch_bounds__(kThreads, WAVES_A_SIMD) void forward_kernel(Args a) {
+template <int DT, int THREADS, int HELD, int KEPT, int WAVES_A_SIMD>
+__global__ __launch_bounds__(THREADS, WAVES_A_SIMD) void forward_kernel(Args a) {
   extern __shared__ uint32_t lds[];
   __shared__ Shared sh;
-  using R = Row<DT, kThreads, HELD>;
+  using R = Row<DT, THREADS, HELD, KEPT>;
   const int64_t r = blockIdx.x;
   const int vocab = a.logits.vocab;
-  const Entries t(lds, a.k);
+  const Entries t(lds + KEPT * THREADS * 4, a.k);
   typename R::T* out = static_cast<typename R::T*>(a.grad) + r * vocab;
   const First first = load_first(a, r);
-  const R row(a.logits.row<typename R::T>(r), vocab, a.grad ? before_line<DT>(out) : 0, a.logits.once);
+  const R row(a.logits.row<typename R::T>(r), vocab, a.grad ? before_line<DT>(out) : 0, a.logits.once,
+              reinterpret_cast<uint4*>(lds));
   float m, sum, outside;
   reduce(a, r, first, row, t, 0, sh, m, sum, outside);
   const Teacher teacher = sh.teacher;
   if (teacher.none(a.tail)) {
     write_none(a, r);
-    if (a.grad) zero_row<DT, kThreads>(out, 0, vocab);
+    if (a.grad) zero_row<DT, THREADS>(out, 0, vocab);
     return;
   }
   const Exponent ex(m, a.scale);
@@ -357,7 +357,7 @@ __global__ __launch_bounds__(kThreads, WAVES_A_SIMD) void forward_kernel(Args a)
   if (a.grad) {
     const float g = a.loss_grad[r];
     if (g == 0.0f || sum == 0.0f) {
-      zero_row<DT, kThreads>(out, 0, vocab);
+      zero_row<DT, THREADS>(out, 0, vocab);
     } else {
       const float per_q = g * a.temperature, per_p = per_q / sum, per_other = per_p * co.other;
       row.map(out, a.logits.write_once, [&](int, auto& x) {
@@ -365,7 +365,7 @@ __global__ __launch_bounds__(kThreads, WAVES_A_SIMD) void forward_kernel(Args a)
 #pragma unroll
         for (int j = 0; j < N; ++j) x[j] = ex.of(ex.power(x[j])) * per_other;
       });
-      write_listed<DT>(a, t, teacher.repeated, r, ex, per_p * co.weight, per_q, 0, vocab);
+      write_listed<DT, THREADS>(a, t, teacher.repeated, r, ex, per_p * co.weight, per_q, 0, vocab);
     }
   }
   if (threadIdx.x < kWave) write_loss<DT>(a, r, t, teacher, m, sum, co);
@@ -457,46 +457,62 @@ __global__ __launch_bounds__(kThreads) void backward_kernel(Args a) {
 #pragma unroll
     for (int j = 0; j < N; ++j) x[j] = ex.of(ex.power(x[j])) * per_other;
   });
-  write_listed<DT>(a, t, st[5] != 0.0f, r, ex, per_p * weight, per_q, from, to);
+  write_listed<DT, kThreads>(a, t, st[5] != 0.0f, r, ex, per_p * weight, per_q, from, to);
 }
 
+// Up to 25 runs a thread stay in registers with four waves on a SIMD, so a row
+// of up to kLong runs has one workgroup of 256 threads, four to a CU.  The
+// gradient wants a longer row held too: 512 threads hold up to kWide runs, two
+// workgroups to a CU, and with seven more a thread in LDS (56 KiB and the
+// list's bits: two still fit) kWidest.  Against three launches that read the
+// row twice (in parts, the join, the gradient): 2046 rows of 50257 fp32 logits
+// 209 -> 166 us, 2048 of 65536 bf16 149 -> 119, 8192 of 131072 1072 -> 821;
+// rows of kWidest gain from about 160 of them (128: 31 / 34 us, 200: 41 / 36).
+// The loss alone reads a row once in any case, faster in parts.
 constexpr int kShort = kThreads * 8, kMiddle = kThreads * 16, kLong = kThreads * 25;
+constexpr int kKept = 7, kWide = 2 * kThreads * 25, kWidest = 2 * kThreads * (25 + kKept);
+constexpr int64_t kWidestRows = 160;
 
 struct Plan {
   int parts, part;  // parts a row, columns a part (the last has the rest); 0 parts: one workgroup reads the row again for each pass
 };
 
-Plan forward_plan(int64_t rows, int64_t vocab, int dtype) {
+Plan forward_plan(int64_t rows, int64_t vocab, int dtype, bool with_grad) {
   const int64_t runs = runs_of(vocab, dtype), e = dtype == QSTE_F32 ? 4 : 8;
-  int64_t parts = runs > kLong ? (runs + kLong - 1) / kLong : 1;
+  if (runs <= kLong || (with_grad && (runs <= kWide || (runs <= kWidest && rows >= kWidestRows)))) return {1, 0};
+  const int64_t parts = (runs + kLong - 1) / kLong;
   if (parts > kMaxParts) return {0, 0};
-  // no part is empty: runs > parts * parts
-  return {static_cast<int>(parts), parts > 1 ? static_cast<int>((runs + parts - 1) / parts * e) : 0};
+  return {static_cast<int>(parts), static_cast<int>((runs + parts - 1) / parts * e)};  // runs > parts * parts: none is empty
+}
+
+template <int DT, int THREADS, int HELD, int KEPT, int WAVES_A_SIMD>
+int whole_as(const Args& a, int64_t rows, hipStream_t s) {
+  const size_t lds = entries_bytes(a.k, a.logits.vocab) + static_cast<size_t>(KEPT) * THREADS * 16;
+  forward_kernel<DT, THREADS, HELD, KEPT, WAVES_A_SIMD><<<static_cast<unsigned>(rows), THREADS, lds, s>>>(a);
+  return static_cast<int>(hipGetLastError());
 }
 
 template <int DT, int HELD, int WAVES_A_SIMD>
-int loss_as(const Args& a, int64_t rows, hipStream_t s) {
-  if constexpr (HELD > 0) {
-    if (a.parts > 1) {
-      part_kernel<DT, HELD, WAVES_A_SIMD>
-          <<<static_cast<unsigned>(rows * a.parts), kThreads, entries_bytes(a.k, a.part + Wide<DT>::E), s>>>(a);
-      if (int rc = static_cast<int>(hipGetLastError())) return rc;
-      join_kernel<DT><<<static_cast<unsigned>(rows), kWave, entries_bytes(a.k, 0), s>>>(a);
-      return static_cast<int>(hipGetLastError());
-    }
-  }
-  forward_kernel<DT, HELD, WAVES_A_SIMD>
-      <<<static_cast<unsigned>(rows), kThreads, entries_bytes(a.k, a.logits.vocab), s>>>(a);
+int parts_as(const Args& a, int64_t rows, hipStream_t s) {
+  part_kernel<DT, HELD, WAVES_A_SIMD>
+      <<<static_cast<unsigned>(rows * a.parts), kThreads, entries_bytes(a.k, a.part + Wide<DT>::E), s>>>(a);
+  if (int rc = static_cast<int>(hipGetLastError())) return rc;
+  join_kernel<DT><<<static_cast<unsigned>(rows), kWave, entries_bytes(a.k, 0), s>>>(a);
   return static_cast<int>(hipGetLastError());
 }
 
 template <int DT>
 int loss(const Args& a, const Plan& plan, int64_t rows, hipStream_t s) {
-  if (plan.parts == 0) return loss_as<DT, 0, 4>(a, rows, s);
-  const int64_t runs = plan.parts > 1 ? plan.part / Wide<DT>::E : runs_of(a.logits.vocab, DT);
-  if (runs <= kShort) return loss_as<DT, 8, 7>(a, rows, s);
-  if (runs <= kMiddle) return loss_as<DT, 16, 5>(a, rows, s);
-  return loss_as<DT, 25, 4>(a, rows, s);
+  if (plan.parts == 0) return whole_as<DT, kThreads, 0, 0, 4>(a, rows, s);
+  // the shortest parts of a row of more than kLong runs have half as many
+  if (plan.parts > 1)
+    return plan.part / Wide<DT>::E <= kMiddle ? parts_as<DT, 16, 5>(a, rows, s) : parts_as<DT, 25, 4>(a, rows, s);
+  const int64_t runs = runs_of(a.logits.vocab, DT);
+  if (runs <= kShort) return whole_as<DT, kThreads, 8, 0, 7>(a, rows, s);
+  if (runs <= kMiddle) return whole_as<DT, kThreads, 16, 0, 5>(a, rows, s);
+  if (runs <= kLong) return whole_as<DT, kThreads, 25, 0, 4>(a, rows, s);
+  if (runs <= kWide) return whole_as<DT, 2 * kThreads, 25, 0, 4>(a, rows, s);
+  return whole_as<DT, 2 * kThreads, 25, kKept, 4>(a, rows, s);
 }
 
 template <int DT>
@@ -517,7 +533,7 @@ Args arguments(const Logits& logits, const int64_t* tokens, const float* values,
 }  // namespace distill
 
 size_t distill_workspace(int64_t rows, int64_t vocab, int dtype, int with_grad) {
-  const int parts = distill::forward_plan(rows, vocab, dtype).parts;
+  const int parts = distill::forward_plan(rows, vocab, dtype, with_grad).parts;
   // the parts' sums, and the row statistics that a gradient after the join reads
   return parts > 1 ? static_cast<size_t>(rows) * 4 * (4 * parts + (with_grad ? distill::kStats : 0)) : 0;
 }
@@ -541,7 +557,7 @@ int launch_distill(const vocab::Logits& logits, int dtype, int64_t rows, const i
                    int64_t k, double temperature, int tail, float* losses, float* stats, const float* loss_grad,
                    void* grad, void* workspace, hipStream_t s) {
   using namespace distill;
-  const Plan plan = forward_plan(rows, logits.vocab, dtype);
+  const Plan plan = forward_plan(rows, logits.vocab, dtype, grad != nullptr);
   Args a = arguments(logits, tokens, values, k, temperature, tail);
   a.losses = losses;
   a.stats = stats;

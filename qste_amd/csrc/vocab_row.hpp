@@ -96,24 +96,26 @@ struct Wide {
 // All threads make the same calls, so f may hold barriers; without a head the
 // calls go up through the columns by thread and then by call.
 //
-// With HELD > 0 the columns are loaded once, HELD 16-byte runs a thread, and
-// stay in registers for every pass (up to THREADS * HELD runs); with HELD = 0
-// each pass reads them again.
-template <int DT, int THREADS, int HELD>
+// With HELD > 0 the columns are loaded once and stay for every pass: HELD
+// 16-byte runs a thread in registers and KEPT more in LDS (up to THREADS *
+// (HELD + KEPT) runs; a thread reads back what it wrote).  With HELD = 0 each
+// pass reads them again.
+template <int DT, int THREADS, int HELD, int KEPT = 0>
 struct Row {
   using W = Wide<DT>;
   using T = typename W::T;
   static constexpr int E = W::E;
-  static constexpr int kStep = THREADS * E;
+  static constexpr int kStep = THREADS * E, kWaves = THREADS / kWave;
   static constexpr bool kHeld = HELD > 0;
   static constexpr bool kTight = HELD > 16;  // few registers are left
   const T* p;
   int count, head, whole;  // whole: the columns in runs
   uint4 held[HELD > 0 ? HELD : 1];
+  uint4* kept;  // [KEPT, THREADS]
   float last;
 
-  __device__ __forceinline__ Row(const T* columns, int n, int before = 0, bool once = false)
-      : p(columns), count(n), head(min(before, n)), whole((n - min(before, n)) / E * E) {
+  __device__ __forceinline__ Row(const T* columns, int n, int before = 0, bool once = false, uint4* lds = nullptr)
+      : p(columns), count(n), head(min(before, n)), whole((n - min(before, n)) / E * E), kept(lds) {
     if constexpr (HELD > 0) {
       if (once)
         hold<true>();
@@ -124,18 +126,30 @@ struct Row {
     }
   }
 
+  // the i-th run of this thread
+  template <bool ONCE>
+  __device__ __forceinline__ uint4 run(int i) const {
+    const T* at = p + head + i * kStep + static_cast<int>(threadIdx.x) * E;
+    uint4 c = W::none();
+    if ((i + 1) * kStep <= whole)
+      c = W::template load<ONCE>(at);
+    else if (i * kStep + static_cast<int>(threadIdx.x) * E < whole)
+      c = W::template load<ONCE>(at);
+    return c;
+  }
+
+  // what goes to LDS is asked for first and written while most of the rest is on its way
   template <bool ONCE>
   __device__ __forceinline__ void hold() {
-    const T* runs = p + head;
-    const int mine = static_cast<int>(threadIdx.x) * E;
+    uint4 passing[KEPT > 0 ? KEPT : 1];
 #pragma unroll
-    for (int i = 0; i < HELD; ++i) {
-      held[i] = W::none();
-      if ((i + 1) * kStep <= whole)
-        held[i] = W::template load<ONCE>(runs + i * kStep + mine);
-      else if (i * kStep + mine < whole)
-        held[i] = W::template load<ONCE>(runs + i * kStep + mine);
-    }
+    for (int i = 0; i < KEPT; ++i) passing[i] = run<ONCE>(HELD + i);
+#pragma unroll
+    for (int i = 0; i < HELD - KEPT; ++i) held[i] = run<ONCE>(i);
+#pragma unroll
+    for (int i = 0; i < KEPT; ++i) kept[i * THREADS + threadIdx.x] = passing[i];
+#pragma unroll
+    for (int i = HELD - KEPT; i < HELD; ++i) held[i] = run<ONCE>(i);
   }
 
   // this thread's column outside the runs
@@ -154,11 +168,14 @@ struct Row {
       // a pass works its columns out anew: carried from pass to pass they would take a register for each run
       asm volatile("" : "+v"(mine));
 #pragma unroll
-      for (int i = 0; i < HELD; ++i) {
+      for (int i = 0; i < HELD + KEPT; ++i) {
         if (i * kStep < whole) {
           const int first = i * kStep + mine;
           float x[E];
-          W::unpack(held[i], x);
+          if constexpr (KEPT > 0)
+            W::unpack(i < HELD ? held[i < HELD ? i : 0] : kept[(i - HELD) * THREADS + threadIdx.x], x);
+          else
+            W::unpack(held[i], x);
           f(first < end ? first : count, x);
         }
       }

@@ -294,7 +294,9 @@ def test_broadcast_weights():
 @pytest.mark.parametrize("tail", [False, True])
 @pytest.mark.parametrize("dtype,rows,vocab", [(torch.bfloat16, 1, 1_700_003), (torch.float32, 2, 900_001),
                                               (torch.float16, 300, 32776), (torch.bfloat16, 60, 51200),
-                                              (torch.bfloat16, 60, 51208)])
+                                              (torch.bfloat16, 60, 51208), (torch.bfloat16, 40, 102407),
+                                              (torch.bfloat16, 160, 131079), (torch.float32, 170, 65537),
+                                              (torch.float16, 165, 110001), (torch.bfloat16, 170, 131080)])
 def test_long_rows(dtype, rows, vocab, tail):
     """Past what registers hold in one workgroup, and past what they hold in parts."""
 
