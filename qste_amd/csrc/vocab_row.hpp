@@ -10,8 +10,17 @@
 namespace qste {
 namespace vocab {
 
+// two values to an fp16 pair; a product before it may be rounded once, to fp16
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t f32x2_to_f16x2(float lo, float hi) {
+  f16x2_t v;
+  v[0] = static_cast<_Float16>(lo);
+  v[1] = static_cast<_Float16>(hi);
+  return __builtin_bit_cast(uint32_t, v);
+}
+
 constexpr int64_t kMaxVocab = int64_t{1} << 30;  // columns are ints
-constexpr float kLog2e = 1.44269504088896340736f;
+constexpr double kLog2e = 1.4426950408889634074;
 constexpr float kLn2 = 0.69314718055994530942f;
 
 // Rows of logits: row r is at (r / inner) * outer_stride + (r % inner) *
@@ -75,7 +84,7 @@ struct Wide {
       else if constexpr (DT == QSTE_BF16)
         v[i] = f32x2_to_bf16x2(x[2 * i], x[2 * i + 1]);
       else
-        v[i] = f32_to_f16(x[2 * i]) | static_cast<uint32_t>(f32_to_f16(x[2 * i + 1])) << 16;
+        v[i] = f32x2_to_f16x2(x[2 * i], x[2 * i + 1]);
     }
     if constexpr (ONCE)
       __builtin_nontemporal_store(v, reinterpret_cast<V*>(p));
@@ -107,7 +116,6 @@ struct Row {
   static constexpr int E = W::E;
   static constexpr int kStep = THREADS * E, kWaves = THREADS / kWave;
   static constexpr bool kHeld = HELD > 0;
-  static constexpr bool kTight = HELD > 16;  // few registers are left
   const T* p;
   int count, head, whole;  // whole: the columns in runs
   uint4 held[HELD > 0 ? HELD : 1];
@@ -252,15 +260,14 @@ __device__ __forceinline__ int before_line(const typename Elem<DT>::T* out) {
 // the 16-byte runs that a row of `vocab` columns has
 inline int64_t runs_of(int64_t vocab, int dtype) { return vocab / (dtype == QSTE_F32 ? 4 : 8); }
 
-// Zeros in the columns [from, to) of a row of gradients, from = 0 or a multiple of
-// 16-byte accesses past it.
+// Zeros in n columns of a row of gradients
 template <int DT, int THREADS>
-__device__ __forceinline__ void zero_row(typename Elem<DT>::T* out, int from, int to) {
+__device__ __forceinline__ void zero_row(typename Elem<DT>::T* out, int n) {
   using W = Wide<DT>;
   const float zeros[W::E] = {}, zero[1] = {};
-  const int whole = from + (to - from) / W::E * W::E;
-  for (int i = from + static_cast<int>(threadIdx.x) * W::E; i < whole; i += THREADS * W::E) W::store(out + i, zeros);
-  for (int i = whole + static_cast<int>(threadIdx.x); i < to; i += THREADS) W::store(out + i, zero);
+  const int whole = n / W::E * W::E;
+  for (int i = static_cast<int>(threadIdx.x) * W::E; i < whole; i += THREADS * W::E) W::store(out + i, zeros);
+  for (int i = whole + static_cast<int>(threadIdx.x); i < n; i += THREADS) W::store(out + i, zero);
 }
 
 // Reductions over a wave in data-parallel moves: lanes 1, 2, 4 and 8 apart
@@ -288,25 +295,13 @@ __device__ __forceinline__ float fold_sum(float v) {
   return wave_fold(v, 0.0f, [](float a, float b) { return a + b; });
 }
 
-template <int THREADS>
-__device__ __forceinline__ float block_max(float v, float* scratch) {
-  v = fold_max(v);
-  __syncthreads();
-  if ((threadIdx.x & (kWave - 1)) == 0) scratch[threadIdx.x / kWave] = v;
-  __syncthreads();
-  float best = scratch[0];
-#pragma unroll
-  for (int w = 1; w < THREADS / kWave; ++w) best = fmaxf(best, scratch[w]);
-  return best;
-}
-
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
   asm("v_max3_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c));
   return d;
 }
 
-// The largest of m and x (NaN where x holds a signalling one, else the numbers')
+// The largest of m and x, passing over NaN (a signalling one may come out)
 template <int N>
 __device__ __forceinline__ float max_of(float m, const float (&x)[N]) {
   if constexpr (N == 1) {
