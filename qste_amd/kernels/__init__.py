@@ -977,6 +977,51 @@ def _row_weights(weights: Tensor | None, shape, what: str) -> Tensor | None:
     return _f32(weights)
 
 
+# The forwards below come in two layers: the checks, which also say how the rows
+# lie and bring tokens and weights to the types the library takes, and the call.
+# An autograd node keeps what the checks made and makes its backward's call
+# without them (they are half of a small call's time on the host).
+
+
+def _check_scores(logits: Tensor, tokens: Tensor | None, top: int, temperature: float):
+    """(rows, layout, tokens int64 or None, top, temperature)"""
+
+    _require_gpu(logits, tokens)
+    _dtype_code(logits)
+    rows, layout = _logit_rows(logits)
+    top, most = int(top), min(MAX_TOP, layout[4])
+    if not 0 <= top <= most:
+        raise ValueError(f"top must lie in 0 .. {most}, got {top}")
+    tokens_i64 = None if tokens is None else _row_tokens(tokens, logits.shape[:-1], "tokens")
+    return rows, layout, tokens_i64, top, _temperature(temperature)
+
+
+def _call_scores(rows: Tensor, layout, tokens: Tensor | None, top: int, temperature: float, want_stats: bool):
+    shape, device, code = rows.shape[:-1], rows.device, _DTYPES[rows.dtype]
+    entropy = torch.empty(shape, dtype=torch.float32, device=device)
+    logprobs = None if tokens is None else torch.empty_like(entropy)
+    top_logprobs = torch.empty(*shape, top, dtype=torch.float32, device=device) if top else None
+    top_tokens = torch.empty(*shape, top, dtype=torch.int64, device=device) if top else None
+    stats = torch.empty(*shape, 2, dtype=torch.float32, device=device) if want_stats else None
+    lib = _lib.load()
+    nbytes = lib.qste_token_logprobs_workspace_bytes(entropy.numel(), layout[4], code, top)
+    work = _workspace(nbytes, device) if nbytes else None
+    _lib.check(lib.qste_token_logprobs(
+        rows.data_ptr(), code, *layout, _ptr(tokens), temperature, top, _ptr(logprobs), entropy.data_ptr(),
+        _ptr(top_logprobs), _ptr(top_tokens), _ptr(stats), _ptr(work), nbytes, _stream(device)), "token_logprobs")
+    return logprobs, entropy, top_logprobs, top_tokens, stats
+
+
+def _call_scores_backward(rows: Tensor, layout, tokens: Tensor | None, temperature: float, logprob_grad: Tensor | None,
+                          entropy_grad: Tensor | None, entropy: Tensor, stats: Tensor) -> Tensor:
+    grad = torch.empty(rows.shape, dtype=rows.dtype, device=rows.device)
+    _lib.check(_lib.load().qste_token_logprobs_backward(
+        rows.data_ptr(), _DTYPES[rows.dtype], *layout, _ptr(tokens), temperature, _ptr(logprob_grad),
+        _ptr(entropy_grad), entropy.data_ptr(), stats.data_ptr(), grad.data_ptr(), _stream(rows.device)),
+        "token_logprobs_backward")
+    return grad
+
+
 def token_logprobs_forward(logits: Tensor, tokens: Tensor | None, *, top: int = 0, temperature: float = 1.0,
                            want_stats: bool = False):
     """``(logprobs, entropy, top_logprobs, top_tokens, stats)`` of the rows of logits.
@@ -988,25 +1033,7 @@ def token_logprobs_forward(logits: Tensor, tokens: Tensor | None, *, top: int = 
     ``top_tokens`` (int64) are fp32.
     """
 
-    device = _require_gpu(logits, tokens)
-    code = _dtype_code(logits)
-    rows, layout = _logit_rows(logits)
-    shape, vocab, top, temperature = logits.shape[:-1], layout[4], int(top), _temperature(temperature)
-    if not 0 <= top <= min(MAX_TOP, vocab):
-        raise ValueError(f"top must lie in 0 .. {min(MAX_TOP, vocab)}, got {top}")
-    tokens_i64 = None if tokens is None else _row_tokens(tokens, shape, "tokens")
-    entropy = torch.empty(shape, dtype=torch.float32, device=device)
-    logprobs = None if tokens is None else torch.empty_like(entropy)
-    top_logprobs = torch.empty(*shape, top, dtype=torch.float32, device=device) if top else None
-    top_tokens = torch.empty(*shape, top, dtype=torch.int64, device=device) if top else None
-    stats = torch.empty(*shape, 2, dtype=torch.float32, device=device) if want_stats else None
-    lib = _lib.load()
-    nbytes = lib.qste_token_logprobs_workspace_bytes(entropy.numel(), vocab, code, top)
-    work = _workspace(nbytes, device) if nbytes else None
-    _lib.check(lib.qste_token_logprobs(
-        _ptr(rows), code, *layout, _ptr(tokens_i64), temperature, top, _ptr(logprobs), _ptr(entropy),
-        _ptr(top_logprobs), _ptr(top_tokens), _ptr(stats), _ptr(work), nbytes, _stream(device)), "token_logprobs")
-    return logprobs, entropy, top_logprobs, top_tokens, stats
+    return _call_scores(*_check_scores(logits, tokens, top, temperature), want_stats)
 
 
 def token_logprobs_backward(logits: Tensor, tokens: Tensor | None, logprob_grad: Tensor | None,
@@ -1015,30 +1042,54 @@ def token_logprobs_backward(logits: Tensor, tokens: Tensor | None, logprob_grad:
     """The logits' gradient, contiguous in their dtype, for gradients [...] of the
     log probabilities and the entropies (None: zeros)."""
 
-    device = _require_gpu(logits, tokens, logprob_grad, entropy_grad, entropy, stats)
-    code = _dtype_code(logits)
+    _require_gpu(logits, tokens, logprob_grad, entropy_grad, entropy, stats)
+    rows, layout, tokens_i64, _, temperature = _check_scores(logits, tokens, 0, temperature)
+    shape = logits.shape[:-1]
+    return _call_scores_backward(
+        rows, layout, tokens_i64, temperature, _row_weights(logprob_grad, shape, "logprob_grad"),
+        _row_weights(entropy_grad, shape, "entropy_grad"), _row_weights(entropy, shape, "entropy"),
+        _row_weights(stats, (*shape, 2), "stats"))
+
+
+def _check_distill(logits: Tensor, top_tokens: Tensor, top_logprobs: Tensor, temperature: float, tail: bool):
+    """(rows, layout, tokens int64, log probabilities fp32, temperature, tail)"""
+
+    _require_gpu(logits, top_tokens, top_logprobs)
+    _dtype_code(logits)
     rows, layout = _logit_rows(logits)
-    shape, temperature = logits.shape[:-1], _temperature(temperature)
-    tokens_i64 = None if tokens is None else _row_tokens(tokens, shape, "tokens")
-    g = _row_weights(logprob_grad, shape, "logprob_grad")
-    h = _row_weights(entropy_grad, shape, "entropy_grad")
-    entropy_f32 = _row_weights(entropy, shape, "entropy")
-    stats_f32 = _row_weights(stats, (*shape, 2), "stats")
-    grad = torch.empty(logits.shape, dtype=logits.dtype, device=device)
-    _lib.check(_lib.load().qste_token_logprobs_backward(
-        _ptr(rows), code, *layout, _ptr(tokens_i64), temperature, _ptr(g), _ptr(h), _ptr(entropy_f32),
-        _ptr(stats_f32), _ptr(grad), _stream(device)), "token_logprobs_backward")
-    return grad
-
-
-def _teacher(logits: Tensor, top_tokens: Tensor, top_logprobs: Tensor) -> tuple[Tensor, Tensor]:
     if top_tokens.dim() != logits.dim() or not 1 <= top_tokens.shape[-1] <= MAX_ENTRIES:
         raise ValueError(f"top_tokens need the logits' leading dimensions and 1 to {MAX_ENTRIES} entries, "
                          f"got {tuple(top_tokens.shape)}")
     if not top_logprobs.dtype.is_floating_point:
         raise TypeError(f"top_logprobs must be floating point, got {top_logprobs.dtype}")
     shape = (*logits.shape[:-1], top_tokens.shape[-1])
-    return (_row_tokens(top_tokens, shape, "top_tokens"), _row_weights(top_logprobs, shape, "top_logprobs"))
+    return (rows, layout, _row_tokens(top_tokens, shape, "top_tokens"),
+            _row_weights(top_logprobs, shape, "top_logprobs"), _temperature(temperature), int(tail))
+
+
+def _call_distill(rows: Tensor, layout, tokens: Tensor, values: Tensor, temperature: float, tail: int,
+                  weights: Tensor | None, want_stats: bool):
+    shape, device, code = rows.shape[:-1], rows.device, _DTYPES[rows.dtype]
+    losses = torch.empty(shape, dtype=torch.float32, device=device)
+    stats = torch.empty(*shape, DISTILL_STATS, dtype=torch.float32, device=device) if want_stats else None
+    grad = torch.empty(rows.shape, dtype=rows.dtype, device=device) if weights is not None else None
+    lib = _lib.load()
+    nbytes = lib.qste_distill_workspace_bytes(losses.numel(), layout[4], code, int(grad is not None))
+    work = _workspace(nbytes, device) if nbytes else None
+    _lib.check(lib.qste_distill(
+        rows.data_ptr(), code, *layout, tokens.data_ptr(), values.data_ptr(), tokens.shape[-1], temperature, tail,
+        losses.data_ptr(), _ptr(stats), _ptr(weights), _ptr(grad), _ptr(work), nbytes, _stream(device)), "distill")
+    return losses, stats, grad
+
+
+def _call_distill_backward(rows: Tensor, layout, tokens: Tensor, values: Tensor, temperature: float, tail: int,
+                           weights: Tensor, stats: Tensor) -> Tensor:
+    grad = torch.empty(rows.shape, dtype=rows.dtype, device=rows.device)
+    _lib.check(_lib.load().qste_distill_backward(
+        rows.data_ptr(), _DTYPES[rows.dtype], *layout, tokens.data_ptr(), values.data_ptr(), tokens.shape[-1],
+        temperature, tail, stats.data_ptr(), weights.data_ptr(), grad.data_ptr(), _stream(rows.device)),
+        "distill_backward")
+    return grad
 
 
 def distill_forward(logits: Tensor, top_tokens: Tensor, top_logprobs: Tensor, *, temperature: float = 1.0,
@@ -1048,37 +1099,18 @@ def distill_forward(logits: Tensor, top_tokens: Tensor, top_logprobs: Tensor, *,
     ``distill_backward`` reads, if asked for; and with ``loss_grad`` [...] the
     logits' gradient for these weights, from the same pass, else None."""
 
-    device = _require_gpu(logits, top_tokens, top_logprobs, loss_grad)
-    code = _dtype_code(logits)
-    rows, layout = _logit_rows(logits)
-    shape, temperature = logits.shape[:-1], _temperature(temperature)
-    tokens_i64, values = _teacher(logits, top_tokens, top_logprobs)
-    weights = _row_weights(loss_grad, shape, "loss_grad")
-    losses = torch.empty(shape, dtype=torch.float32, device=device)
-    stats = torch.empty(*shape, DISTILL_STATS, dtype=torch.float32, device=device) if want_stats else None
-    grad = torch.empty(logits.shape, dtype=logits.dtype, device=device) if weights is not None else None
-    lib = _lib.load()
-    nbytes = lib.qste_distill_workspace_bytes(losses.numel(), layout[4], code, int(grad is not None))
-    work = _workspace(nbytes, device) if nbytes else None
-    _lib.check(lib.qste_distill(
-        _ptr(rows), code, *layout, _ptr(tokens_i64), _ptr(values), tokens_i64.shape[-1], temperature, int(tail),
-        _ptr(losses), _ptr(stats), _ptr(weights), _ptr(grad), _ptr(work), nbytes, _stream(device)), "distill")
-    return losses, stats, grad
+    checked = _check_distill(logits, top_tokens, top_logprobs, temperature, tail)
+    if loss_grad is not None:
+        _require_gpu(logits, loss_grad)
+    return _call_distill(*checked, _row_weights(loss_grad, logits.shape[:-1], "loss_grad"), want_stats)
 
 
 def distill_backward(logits: Tensor, top_tokens: Tensor, top_logprobs: Tensor, loss_grad: Tensor, stats: Tensor, *,
                      temperature: float = 1.0, tail: bool = False) -> Tensor:
     """The logits' gradient, contiguous in their dtype, for the weights ``loss_grad`` [...]."""
 
-    device = _require_gpu(logits, top_tokens, top_logprobs, loss_grad, stats)
-    code = _dtype_code(logits)
-    rows, layout = _logit_rows(logits)
-    shape, temperature = logits.shape[:-1], _temperature(temperature)
-    tokens_i64, values = _teacher(logits, top_tokens, top_logprobs)
-    weights = _row_weights(loss_grad, shape, "loss_grad")
-    stats_f32 = _row_weights(stats, (*shape, DISTILL_STATS), "stats")
-    grad = torch.empty(logits.shape, dtype=logits.dtype, device=device)
-    _lib.check(_lib.load().qste_distill_backward(
-        _ptr(rows), code, *layout, _ptr(tokens_i64), _ptr(values), tokens_i64.shape[-1], temperature, int(tail),
-        _ptr(stats_f32), _ptr(weights), _ptr(grad), _stream(device)), "distill_backward")
-    return grad
+    checked = _check_distill(logits, top_tokens, top_logprobs, temperature, tail)
+    _require_gpu(logits, loss_grad, stats)
+    shape = logits.shape[:-1]
+    return _call_distill_backward(*checked, _row_weights(loss_grad, shape, "loss_grad"),
+                                  _row_weights(stats, (*shape, DISTILL_STATS), "stats"))

@@ -38,12 +38,12 @@ class TokenLogprobsFn(Function):
     maxima and sums, and the entropies."""
 
     @staticmethod
-    def forward(ctx, logits, tokens, top: int, temperature: float):
+    def forward(ctx, logits, tokens, top, temperature):
         ctx.set_materialize_grads(False)
-        logprobs, entropy, top_logprobs, top_tokens, stats = kernels.token_logprobs_forward(
-            logits, tokens, top=top, temperature=temperature, want_stats=True)
-        ctx.save_for_backward(logits, tokens, entropy, stats)
-        ctx.temperature = temperature
+        checked = kernels._check_scores(logits, tokens, top, temperature)
+        logprobs, entropy, top_logprobs, top_tokens, stats = kernels._call_scores(*checked, True)
+        rows, ctx.layout, tokens_i64, _, ctx.temperature = checked
+        ctx.save_for_backward(rows, tokens_i64, entropy, stats)
         if top_tokens is not None:
             ctx.mark_non_differentiable(top_logprobs, top_tokens)
         return logprobs, entropy, top_logprobs, top_tokens
@@ -53,10 +53,11 @@ class TokenLogprobsFn(Function):
     def backward(ctx, logprob_grad, entropy_grad, *_):
         if logprob_grad is None and entropy_grad is None:
             return None, None, None, None
-        logits, tokens, entropy, stats = ctx.saved_tensors
-        grad = kernels.token_logprobs_backward(logits, tokens, logprob_grad, entropy_grad, entropy, stats,
-                                               temperature=ctx.temperature)
-        return grad, None, None, None
+        rows, tokens, entropy, stats = ctx.saved_tensors
+        g = None if logprob_grad is None else logprob_grad.contiguous()
+        h = None if entropy_grad is None else entropy_grad.contiguous()
+        return (kernels._call_scores_backward(rows, ctx.layout, tokens, ctx.temperature, g, h, entropy, stats),
+                None, None, None)
 
 
 def token_logprobs(logits: Tensor, tokens: Optional[Tensor] = None, *, top: int = 0,
@@ -73,7 +74,7 @@ def token_logprobs(logits: Tensor, tokens: Optional[Tensor] = None, *, top: int 
     """
 
     if torch.is_grad_enabled() and logits.requires_grad:
-        return TokenScores(*TokenLogprobsFn.apply(logits, tokens, int(top), float(temperature)))
+        return TokenScores(*TokenLogprobsFn.apply(logits, tokens, top, temperature))
     return TokenScores(*kernels.token_logprobs_forward(logits, tokens, top=top, temperature=temperature)[:4])
 
 
@@ -82,20 +83,19 @@ class DistillationFn(Function):
     teacher's entries and six floats a row."""
 
     @staticmethod
-    def forward(ctx, logits, top_tokens, top_logprobs, temperature: float, tail: bool):
-        losses, stats, _ = kernels.distill_forward(logits, top_tokens, top_logprobs, temperature=temperature, tail=tail,
-                                                   want_stats=True)
-        ctx.save_for_backward(logits, top_tokens, top_logprobs, stats)
-        ctx.temperature, ctx.tail = temperature, tail
+    def forward(ctx, logits, top_tokens, top_logprobs, temperature, tail):
+        checked = kernels._check_distill(logits, top_tokens, top_logprobs, temperature, tail)
+        losses, stats, _ = kernels._call_distill(*checked, None, True)
+        rows, ctx.layout, tokens_i64, values, ctx.temperature, ctx.tail = checked
+        ctx.save_for_backward(rows, tokens_i64, values, stats)
         return losses
 
     @staticmethod
     @once_differentiable
     def backward(ctx, loss_grad):
-        logits, top_tokens, top_logprobs, stats = ctx.saved_tensors
-        grad = kernels.distill_backward(logits, top_tokens, top_logprobs, loss_grad, stats,
-                                        temperature=ctx.temperature, tail=ctx.tail)
-        return grad, None, None, None, None
+        rows, tokens, values, stats = ctx.saved_tensors
+        return (kernels._call_distill_backward(rows, ctx.layout, tokens, values, ctx.temperature, ctx.tail,
+                                               loss_grad.contiguous(), stats), None, None, None, None)
 
 
 def _constant(top_logprobs: Tensor) -> None:
@@ -119,7 +119,7 @@ def distillation_loss(logits: Tensor, top_tokens: Tensor, top_logprobs: Tensor, 
 
     _constant(top_logprobs)
     if torch.is_grad_enabled() and logits.requires_grad:
-        return DistillationFn.apply(logits, top_tokens, top_logprobs, float(temperature), bool(tail))
+        return DistillationFn.apply(logits, top_tokens, top_logprobs, temperature, tail)
     return kernels.distill_forward(logits, top_tokens, top_logprobs, temperature=temperature, tail=tail)[0]
 
 
