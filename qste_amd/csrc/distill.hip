@@ -24,7 +24,8 @@ using namespace vocab;
 
 constexpr int kThreads = 256;
 constexpr int kMaxParts = 32;
-// columns whose membership in the list is held in LDS at a time, one bit each
+// columns of a row that is read again whose membership in the list is held in
+// LDS at a time, one bit each
 constexpr int kSpan = 1 << 17;
 constexpr int kSingles = 128;  // more than a Row's columns outside its runs
 constexpr int kStats = QSTE_DISTILL_STATS;
@@ -57,8 +58,11 @@ struct Teacher {
 };
 
 // The row's entries in LDS, k of each: its tokens (-1: none) and ln q; then the
-// bits of the listed columns, by their place in a Row (columns before the runs come
-// after the others).
+// bits of the listed columns: those in a Row's runs in their order, room for as
+// many as it can hold, and then its single columns by thread.  A thread's bits
+// of a 16-bit run are one byte at a place known ahead: with places counted in
+// columns, up to the row's own count, a pass took 107 us where it takes 102
+// (4096 rows of 50257), 103 / 95 (2048 of 131072 in parts).
 struct Entries {
   int* token;
   float* log_q;
@@ -67,10 +71,11 @@ struct Entries {
       : token(reinterpret_cast<int*>(lds)), log_q(reinterpret_cast<float*>(lds) + k), listed(lds + 2 * k) {}
 };
 
-inline size_t entries_bytes(int64_t k, int64_t columns) {
-  const int64_t span = columns < kSpan + kSingles ? columns : kSpan + kSingles;
-  return static_cast<size_t>(k * 8 + (span + 63) / 64 * 8);  // whole pairs of words
-}
+constexpr size_t entries_bytes(int k, int columns) { return static_cast<size_t>(k) * 8 + columns / 8; }
+
+// the bits that a Row's list takes
+template <class R>
+constexpr int kBits = (R::kHeld ? R::kRuns * R::E : kSpan) + kSingles;
 
 // exp(v) to 1e-11: the mass of a list is near 1, and what it leaves of 1 has to
 // be right to its own size, which sums of fp32 exponentials are not.  2^(n + f)
@@ -132,20 +137,27 @@ __device__ __forceinline__ Teacher load_entries(const Args& a, int64_t r, const 
   return out;
 }
 
-// By one wave: the bits of the listed columns whose places lie in [from, to),
-// of a view of `count` columns that begins at column `begin` and has `head` before
-// its runs.  Returns whether a token is there twice.
-__device__ __forceinline__ bool mark_listed(const Args& a, const Entries& t, int begin, int count, int head, int from,
-                                            int to) {
+// By one wave: the bits of the listed columns, of the runs in [from, to) columns
+// past the head and, with `singles`, of the single ones; the view begins at
+// column `begin`.  Returns whether a token is there twice.
+template <class R>
+__device__ __forceinline__ bool mark_listed(const Args& a, const R& row, const Entries& t, int begin, int from, int to,
+                                            bool singles) {
   const int lane = threadIdx.x & (kWave - 1);
-  for (int i = 2 * lane; i < (to - from + 31) / 32; i += 2 * kWave) t.listed[i] = t.listed[i + 1] = 0;
+  for (int i = 2 * lane; i < kBits<R> / 32; i += 2 * kWave) t.listed[i] = t.listed[i + 1] = 0;
   __builtin_amdgcn_wave_barrier();
   bool twice = false;
   for (int k = lane; k < a.k; k += kWave) {
     const int column = t.token[k] - begin;
-    if (t.token[k] < 0 || column < 0 || column >= count) continue;
-    const int at = column - head + (column < head ? count : 0) - from;
-    if (at < 0 || at >= to - from) continue;
+    if (t.token[k] < 0 || column < 0 || column >= row.count) continue;
+    int at = column - row.head;
+    if (at >= 0 && at < row.whole) {
+      if (at < from || at >= to) continue;
+      at -= from;
+    } else {
+      if (!singles) continue;
+      at = kBits<R> - kSingles + (at < 0 ? column : column - row.whole);
+    }
     const uint32_t bit = 1u << (at & 31);
     twice |= (atomicOr(&t.listed[at >> 5], bit) & bit) != 0;
   }
@@ -153,23 +165,29 @@ __device__ __forceinline__ bool mark_listed(const Args& a, const Entries& t, int
 }
 
 // A thread's sums of the exponentials over the columns, all and outside the
-// list; `from` and the bits as in mark_listed.
+// list, for the runs (and single columns) that mark_listed marked
 template <class R>
 __device__ __forceinline__ void sums(const Args& a, const R& row, const Entries& t, int from, int to,
                                      const Exponent& ex, float& sum, float& outside) {
   if (!a.tail) {
-    row.each(from, to, [&](int, auto& x) {
+    row.each(from, to, [&](int, auto& x, int) {
       constexpr int N = sizeof(x) / sizeof(x[0]);
 #pragma unroll
       for (int j = 0; j < N; ++j) sum += ex.of(ex.power(x[j]));
     });
     return;
   }
-  row.each(from, to, [&](int first, auto& x) {
+  const int tid = threadIdx.x;
+  const uint8_t* bytes = reinterpret_cast<const uint8_t*>(t.listed);
+  row.each(from, to, [&](int, auto& x, int slot) {
     constexpr int N = sizeof(x) / sizeof(x[0]);
-    const int at = first - row.head + (N == 1 && first < row.head ? row.count : 0) - from;
-    uint32_t bits = first < row.count && at >= 0 && at < to - from ? t.listed[at >> 5] >> (at & 31) : 0;
-    bits &= (1u << N) - 1;
+    uint32_t bits;
+    if constexpr (N == 8)
+      bits = bytes[slot * R::kThreads + tid];
+    else if constexpr (N == 4)
+      bits = bytes[(slot * R::kThreads + tid) / 2] >> (tid & 1) * 4 & 15;
+    else
+      bits = tid < kSingles ? t.listed[(kBits<R> - kSingles + tid) / 32] >> (tid & 31) & 1 : 0;
     float all = 0.0f;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
@@ -179,8 +197,9 @@ __device__ __forceinline__ void sums(const Args& a, const R& row, const Entries&
     sum += all;
     if (__any(bits)) {  // few waves' runs hold a listed column
       all = 0.0f;
+      const int kept = ~bits;
 #pragma unroll
-      for (int j = 0; j < N; ++j) all += bits >> j & 1 ? 0.0f : x[j];
+      for (int j = 0; j < N; ++j) all += __int_as_float(__float_as_int(x[j]) & (kept << (31 - j) >> 31));
     }
     outside += all;
   });
@@ -200,11 +219,11 @@ __device__ __forceinline__ void reduce(const Args& a, int64_t r, const First& fi
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   if (wave == 0) {
     Teacher teacher = load_entries(a, r, first, t);
-    if (R::kHeld) teacher.repeated = mark_listed(a, t, begin, row.count, row.head, 0, row.count);
+    if (R::kHeld) teacher.repeated = mark_listed(a, row, t, begin, 0, row.whole, true);
     if (lane == 0) sh.teacher = teacher;
   }
   m = -INFINITY;
-  row.each([&](int, auto& x) { m = max_of(m, x); });
+  row.each([&](int, auto& x, int) { m = max_of(m, x); });
   m = fold_max(m);
   if (lane == 0) sh.maxima[wave] = m;
   __syncthreads();
@@ -216,13 +235,13 @@ __device__ __forceinline__ void reduce(const Args& a, int64_t r, const First& fi
   if constexpr (R::kHeld) {
     sums(a, row, t, 0, row.count, ex, sum, outside);
   } else {
-    int to = 0;
-    for (int from = 0; to < row.count; from += kSpan) {
-      to = row.count - from <= kSpan + kSingles ? row.count : from + kSpan;  // the single columns in the last span
+    bool end = false;
+    for (int from = 0; !end; from += kSpan) {
+      end = row.whole - from <= kSpan;  // the single columns in the last span
       __syncthreads();
-      if (wave == 0 && mark_listed(a, t, begin, row.count, row.head, from, to) && lane == 0) sh.teacher.repeated = 1;
+      if (wave == 0 && mark_listed(a, row, t, begin, from, from + kSpan, end) && lane == 0) sh.teacher.repeated = 1;
       __syncthreads();
-      sums(a, row, t, from, to, ex, sum, outside);
+      sums(a, row, t, from, end ? row.count : from + kSpan, ex, sum, outside);
     }
   }
   sum = fold_sum(sum);
@@ -327,9 +346,9 @@ __device__ __forceinline__ void write_listed(const Args& a, const Entries& t, bo
 // Bound by reading the logits, and with the gradient by writing it: the row
 // stays in registers from its one read to the gradient.  The first wave reads
 // the entries while all waves' loads are on their way; by itself before the
-// row this took 163 us where it takes 107, the loss of 4096 rows of 50257 bf16
-// logits against 64 tokens and the tail (3.9 TB/s; a plain read reaches 6.2.
-// Without the tail 97: its sum takes the rest).  With the gradient 161 us (5.1
+// row this took 163 us where it takes 102, the loss of 4096 rows of 50257 bf16
+// logits against 64 tokens and the tail (4.0 TB/s; a plain read reaches 6.2.
+// Without the tail 97: its sum takes the rest).  With the gradient 159 us (5.2
 // TB/s; a copy reaches 4.9).
 // ---------------------------------------------------------------------------
 
@@ -494,7 +513,7 @@ Plan forward_plan(int64_t rows, int64_t vocab, int dtype, bool with_grad) {
 
 template <int DT, int THREADS, int HELD, int KEPT, int WAVES_A_SIMD>
 int whole_as(const Args& a, int64_t rows, hipStream_t s) {
-  const size_t lds = entries_bytes(a.k, a.logits.vocab) + static_cast<size_t>(KEPT) * THREADS * 16;
+  const size_t lds = entries_bytes(a.k, kBits<Row<DT, THREADS, HELD, KEPT>>) + static_cast<size_t>(KEPT) * THREADS * 16;
   forward_kernel<DT, THREADS, HELD, KEPT, WAVES_A_SIMD><<<static_cast<unsigned>(rows), THREADS, lds, s>>>(a);
   return static_cast<int>(hipGetLastError());
 }
@@ -502,7 +521,7 @@ int whole_as(const Args& a, int64_t rows, hipStream_t s) {
 template <int DT, int HELD, int WAVES_A_SIMD>
 int parts_as(const Args& a, int64_t rows, hipStream_t s) {
   part_kernel<DT, HELD, WAVES_A_SIMD>
-      <<<static_cast<unsigned>(rows * a.parts), kThreads, entries_bytes(a.k, a.part + Wide<DT>::E), s>>>(a);
+      <<<static_cast<unsigned>(rows * a.parts), kThreads, entries_bytes(a.k, kBits<Row<DT, kThreads, HELD>>), s>>>(a);
   if (int rc = static_cast<int>(hipGetLastError())) return rc;
   join_kernel<DT><<<static_cast<unsigned>(rows), kWave, entries_bytes(a.k, 0), s>>>(a);
   return static_cast<int>(hipGetLastError());

@@ -78,7 +78,7 @@ __device__ uint32_t kth_key(const R& row, int k, int* scratch) {
   for (int bit = BITS - 1; bit >= 0; --bit) {
     const uint32_t at_least = found | 1u << bit;
     int n = 0;
-    row.each([&](int first, auto& x) {
+    row.each([&](int first, auto& x, int) {
       constexpr int N = sizeof(x) / sizeof(x[0]);
       if (first < row.count)
 #pragma unroll
@@ -165,7 +165,7 @@ __device__ __forceinline__ void collect_many(const R& row, int from, float edge,
     __syncthreads();
     if (threadIdx.x == 0) c.count = 0;
     __syncthreads();
-    row.each([&](int first, auto& x) {
+    row.each([&](int first, auto& x, int) {
       constexpr int N = sizeof(x) / sizeof(x[0]);
       if (first < row.count && !nan_edge)
 #pragma unroll
@@ -188,8 +188,9 @@ __device__ __forceinline__ void collect_many(const R& row, int from, float edge,
 // ---------------------------------------------------------------------------
 // forward: one workgroup a row, or one for each part of it and one that joins them
 //
-// Bound by reading the logits: about eleven VALU slots an element (four of them
-// the exponential) against the read's time.  A row stays in registers from its
+// Bound by reading the logits and by the vector instructions alike: 12.5 an
+// element (the exponential takes the time of four), which keep the SIMDs busy
+// for 0.89 of the time.  A row stays in registers from its
 // one read over both passes, the maximum and the sums; four workgroups of 256
 // threads on a CU read, reduce and list at the same time.  4092 rows of 50257
 // bf16 logits 74 us (5.5 TB/s of the 6.2 that a plain read reaches), 8184 rows
@@ -259,7 +260,7 @@ __global__ __launch_bounds__(kThreads, WAVES_A_SIMD) void forward_kernel(Args a)
   const R row(columns, to - from, 0, a.logits.once);
   const int top = min(a.top, row.count);
   float lane_max = -INFINITY;
-  row.each([&](int, auto& x) { lane_max = max_of(lane_max, x); });
+  row.each([&](int, auto& x, int) { lane_max = max_of(lane_max, x); });
 
   // the maximum, and an edge that `top` values reach
   const int whole_waves = min(kWaves, row.count / (kWave * R::E));
@@ -286,7 +287,7 @@ __global__ __launch_bounds__(kThreads, WAVES_A_SIMD) void forward_kernel(Args a)
 
   const Exponent ex(m, a.scale);
   float sum = 0.0f, moment = 0.0f;
-  row.each([&](int first, auto& x) {
+  row.each([&](int first, auto& x, int) {
     constexpr int N = sizeof(x) / sizeof(x[0]);
     if (top > 0 && !(max_of(-INFINITY, x) < least)) {
       if (first < row.count) {

@@ -98,9 +98,10 @@ struct Wide {
   }
 };
 
-// A workgroup's view of one row, or of a part of one: `each` calls f(first, x)
-// for every run of E columns (x: their values; -inf and first >= count where a
-// thread has none) and once more for the columns that no run has, one a thread:
+// A workgroup's view of one row, or of a part of one: `each` calls f(first, x,
+// slot) for every run of E columns (x: their values; -inf and first >= count
+// where a thread has none; slot: the call's number, run slot * THREADS + thread)
+// and once more, with slot -1, for the columns that no run has, one a thread:
 // the `head` columns before the first run and the fewer than E after the last.
 // All threads make the same calls, so f may hold barriers; without a head the
 // calls go up through the columns by thread and then by call.
@@ -114,8 +115,9 @@ struct Row {
   using W = Wide<DT>;
   using T = typename W::T;
   static constexpr int E = W::E;
-  static constexpr int kStep = THREADS * E, kWaves = THREADS / kWave;
+  static constexpr int kThreads = THREADS, kStep = THREADS * E, kWaves = THREADS / kWave;
   static constexpr bool kHeld = HELD > 0;
+  static constexpr int kRuns = THREADS * (HELD + KEPT);  // that it holds
   const T* p;
   int count, head, whole;  // whole: the columns in runs
   uint4 held[HELD > 0 ? HELD : 1];
@@ -184,7 +186,7 @@ struct Row {
             W::unpack(i < HELD ? held[i < HELD ? i : 0] : kept[(i - HELD) * THREADS + threadIdx.x], x);
           else
             W::unpack(held[i], x);
-          f(first < end ? first : count, x);
+          f(first < end ? first : count, x, i);
         }
       }
     } else {
@@ -192,7 +194,7 @@ struct Row {
         const int first = at + mine;
         float x[E];
         W::unpack(first < end ? W::load(p + first) : W::none(), x);
-        f(first < end ? first : count, x);
+        f(first < end ? first : count, x, (at - from) / kStep);
       }
     }
     if (to >= count && whole < count) {
@@ -202,7 +204,7 @@ struct Row {
         x[0] = last;
       else
         x[0] = at < count ? Elem<DT>::load(p, at) : -INFINITY;
-      f(at < count ? at : count, x);
+      f(at < count ? at : count, x, -1);
     }
   }
   template <class F>
@@ -216,20 +218,20 @@ struct Row {
     static_assert(HELD == 0, "a row in registers has all its runs at hand");
     bool more = true;
     for (int at = 0; at < whole && more; at += kStep)
-      each(at, at + kStep < whole ? at + kStep : whole, [&](int first, auto& x) { more = f(first, x); });
-    if (more) each(whole, count, f);
+      each(at, at + kStep < whole ? at + kStep : whole, [&](int first, auto& x, int) { more = f(first, x); });
+    if (more) each(whole, count, [&](int first, auto& x, int) { f(first, x); });
   }
 
   // f(first, x) leaves in x what goes to `out`, a row of its own
   template <class F>
   __device__ __forceinline__ void map(T* out, bool once, F&& f) const {
     if (once)
-      each([&](int first, auto& x) {
+      each([&](int first, auto& x, int) {
         f(first, x);
         if (first < count) W::template store<true>(out + first, x);
       });
     else
-      each([&](int first, auto& x) {
+      each([&](int first, auto& x, int) {
         f(first, x);
         if (first < count) W::template store<false>(out + first, x);
       });
