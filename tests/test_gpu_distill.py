@@ -306,6 +306,23 @@ def test_long_rows(dtype, rows, vocab, tail):
     check(random_logits((rows, vocab), dtype, 16), tokens, values, tail=tail)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,vocab,k", [(5, 90, 90), (5, 2053, 1024), (4, 12291, 300), (4, 20013, 200), (3, 45003, 1024),
+                                          (2, 131075, 1024), (161, 120003, 1024), (1, 530003, 600)])
+def test_lists_at_the_ends(rows, vocab, k, dtype):
+    """Entries side by side at a row's first and last columns, in every run's place and
+    beside the runs; the widest lists on each way that a row is held."""
+
+    print(f"ends {rows} x {vocab}, {k} entries, {dtype}", flush=True)
+    _, values = random_teacher((rows,), vocab, k, 17)
+    g = torch.Generator().manual_seed(vocab)
+    ends = torch.cat([torch.arange(k // 2), torch.arange(vocab - (k + 1) // 2, vocab)])
+    tokens = torch.stack([ends[torch.randperm(k, generator=g)] for _ in range(rows)])
+    tokens[0, :k // 3] = -1
+    # with all of a vocabulary listed there is no tail
+    check(random_logits((rows, vocab), dtype, 17), tokens.to(DEV), values, tail=k < vocab)
+
+
 def test_rows_far_apart():
     """Offsets past 32 bits in the logits and in the gradient."""
 
