@@ -17,7 +17,7 @@ namespace scores {
 using namespace vocab;
 
 constexpr int kThreads = 256;
-constexpr int kWaves = kThreads / kWave;
+constexpr int kMostWaves = 8;
 constexpr int kCandidates = 1024, kRuns = 384;  // values and runs that a workgroup keeps as candidates for the list
 constexpr int kMaxParts = 32;
 
@@ -43,7 +43,7 @@ struct Args {
 
 struct Candidates {
   int count, runs;
-  int scan[kWaves];
+  int scan[kMostWaves];
   int first[kRuns];
   float run[kRuns][8];
   uint64_t entry[kCandidates];  // key above ~column: larger is better, and no two are equal
@@ -59,6 +59,7 @@ __device__ __forceinline__ void push(Candidates& c, float x, int column) {
 }
 
 // The sum of the threads' v
+template <int WAVES>
 __device__ __forceinline__ int block_count(int v, int* scratch) {
   v = wave_sum(v);
   __syncthreads();
@@ -66,7 +67,7 @@ __device__ __forceinline__ int block_count(int v, int* scratch) {
   __syncthreads();
   int total = 0;
 #pragma unroll
-  for (int w = 0; w < kThreads / kWave; ++w) total += scratch[w];
+  for (int w = 0; w < WAVES; ++w) total += scratch[w];
   return total;
 }
 
@@ -84,7 +85,7 @@ __device__ uint32_t kth_key(const R& row, int k, int* scratch) {
 #pragma unroll
         for (int j = 0; j < N; ++j) n += (key_of(x[j]) >> (32 - BITS)) >= at_least;
     });
-    if (block_count(n, scratch) >= k) found = at_least;
+    if (block_count<R::kWaves>(n, scratch) >= k) found = at_least;
   }
   return found;
 }
@@ -135,7 +136,7 @@ __device__ __forceinline__ void add_equals(const R& row, int from, float edge, b
     if (lane == kWave - 1) c.scan[wave] = upto;
     __syncthreads();
     int at = have + upto - mine, total = 0;
-    for (int w = 0; w < kWaves; ++w) {
+    for (int w = 0; w < R::kWaves; ++w) {
       if (w < wave) at += c.scan[w];
       total += c.scan[w];
     }
@@ -190,23 +191,24 @@ __device__ __forceinline__ void collect_many(const R& row, int from, float edge,
 //
 // Bound by reading the logits and by the vector instructions alike: 10.3 an
 // element, 13.6 with 64 tokens to list, keep the SIMDs busy for 0.86 and 0.92 of
-// the time.  A row stays in registers from its one read over both passes,
-// the maximum and the sums; four workgroups of 256 threads on a CU read, reduce
-// and list at the same time.  4092 rows of 50257 bf16 logits 74 us (5.5 TB/s of
-// the 6.2 that a plain read reaches), 8184 rows with 64 tokens listed 174 us
-// (4.7 TB/s).  512 or 1024 threads a row, which leave fewer rows on a CU to read
-// while another reduces, took 86 and 101 us
-// where this took 77.
+// the time.  A row stays in registers from its one read over both passes, the
+// maximum and the sums; four workgroups of 256 threads on a CU read, reduce and
+// list at the same time.  4092 rows of 50257 bf16 logits 74 us (5.5 TB/s of the
+// 6.2 that a plain read reaches), 8184 rows with 64 tokens listed 172 us (4.8
+// TB/s).  512 or 1024 threads a row, which leave fewer rows on a CU to read while
+// another reduces, took 86 and 101 us where this took 77.  Few rows are bound by
+// the chain of steps in each; there 512 threads are ahead (kFew).
 // ---------------------------------------------------------------------------
 
 // A row that is not to be scored
+template <int THREADS>
 __device__ __forceinline__ void unscored(const Args& a, int64_t r) {
   if (threadIdx.x == 0) {
     a.logprobs[r] = 0.0f;
     a.entropy[r] = 0.0f;
     if (a.stats) reinterpret_cast<float2*>(a.stats)[r] = make_float2(0.0f, 1.0f);
   }
-  for (int i = threadIdx.x; i < a.top; i += kThreads) {
+  for (int i = threadIdx.x; i < a.top; i += THREADS) {
     a.top_logprobs[r * a.top + i] = -INFINITY;
     a.top_tokens[r * a.top + i] = -1;
   }
@@ -239,10 +241,11 @@ __device__ __forceinline__ void write_top(const Args& a, int64_t r, int rank, ui
   a.top_tokens[r * a.top + rank] = static_cast<int64_t>(~static_cast<uint32_t>(entry));
 }
 
-template <int DT, int HELD, int WAVES_A_SIMD, bool SPLIT>
-__global__ __launch_bounds__(kThreads, WAVES_A_SIMD) void forward_kernel(Args a) {
+template <int DT, int THREADS, int HELD, int WAVES_A_SIMD, bool SPLIT>
+__global__ __launch_bounds__(THREADS, WAVES_A_SIMD) void forward_kernel(Args a) {
   constexpr int BITS = kKeyBits<DT>;
-  using R = Row<DT, kThreads, HELD>;
+  using R = Row<DT, THREADS, HELD>;
+  constexpr int kWaves = R::kWaves;
   __shared__ float maxima[kWaves], sums[kWaves], moments[kWaves];
   __shared__ uint32_t bounds[kWaves];
   __shared__ Candidates c;
@@ -251,7 +254,7 @@ __global__ __launch_bounds__(kThreads, WAVES_A_SIMD) void forward_kernel(Args a)
   const int part = SPLIT ? blockIdx.x % static_cast<uint32_t>(a.parts) : 0;
   const int64_t token = a.tokens ? a.tokens[r] : 0;
   if (token < 0) {
-    if (!SPLIT) unscored(a, r);
+    if (!SPLIT) unscored<THREADS>(a, r);
     return;
   }
   const int from = SPLIT ? part * a.part : 0;
@@ -335,22 +338,23 @@ __global__ __launch_bounds__(kThreads, WAVES_A_SIMD) void forward_kernel(Args a)
 
   const int runs = c.runs;
   if (runs <= kRuns) {
-    for (int i = tid; i < runs; i += kThreads) {
-      const int first = c.first[i];
-#pragma unroll
-      for (int j = 0; j < R::E; ++j)
-        if (!(c.run[i][j] < least)) push(c, c.run[i][j], from + first + j);
+    // a thread a value: a thread a run, its values in turn, took 6.1 us where this takes 5.2 (40 rows of 4099 bf16
+    // logits, top 5) and 19.7 where this takes 17.7 (4096 rows, top 20)
+    for (int i = tid; i < runs * R::E; i += THREADS) {
+      const int at = i / R::E, j = i % R::E;
+      const float z = c.run[at][j];
+      if (!(z < least)) push(c, z, from + c.first[at] + j);
     }
     __syncthreads();
   }
-  const Row<DT, kThreads, 0> again(columns, to - from);
+  const Row<DT, THREADS, 0> again(columns, to - from);
   int n = c.count;
   if (runs > kRuns || n > kCandidates || sum != sum)  // a run's maximum passes over NaN
     collect_many<DT>(again, from, edge, top, c);
   else if (n < top)
     add_equals(again, from, -INFINITY, false, n, top, c);
   n = c.count;
-  for (int i = tid; i < n; i += kThreads) {
+  for (int i = tid; i < n; i += THREADS) {
     const uint64_t mine = c.entry[i];
     int rank = 0;
     for (int j = 0; j < n; ++j) rank += c.entry[j] > mine;
@@ -361,7 +365,7 @@ __global__ __launch_bounds__(kThreads, WAVES_A_SIMD) void forward_kernel(Args a)
       write_top(a, r, rank, mine, m, sum, log_sum);
   }
   if constexpr (SPLIT)
-    for (int i = top + tid; i < a.top; i += kThreads) a.part_entries[slot * a.top + i] = 0;
+    for (int i = top + tid; i < a.top; i += THREADS) a.part_entries[slot * a.top + i] = 0;
 }
 
 // The parts of a row as one: their sums against the common maximum, and the
@@ -379,7 +383,7 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Args a) {
   const int64_t r = blockIdx.x;
   const int64_t token = a.tokens ? a.tokens[r] : 0;
   if (token < 0) {
-    unscored(a, r);
+    unscored<kThreads>(a, r);
     return;
   }
   int* ranks = reinterpret_cast<int*>(lists + n);
@@ -444,15 +448,21 @@ struct Plan {
 // kShort runs, bring in more workgroups for few rows: 131072 bf16 logits a row,
 // top 20, in 3 / in 8 parts: 1 row 14.3 / 12.4 us, 128 21.2 / 18.7, 600 44.3 /
 // 40.8; but 2048 107 / 111, and with many tokens to list the join decides (16
-// rows of 131072 fp32 logits, top 128, in 6 / in 16: 28 / 36).  A row that one
-// workgroup holds is left whole: cutting 40 rows of 50257 gained 14.3 -> 12.3
-// us on the GPU, less than the second launch takes on the host.
+// rows of 131072 fp32 logits, top 128, in 6 / in 16: 28 / 36).
+//
+// Up to kFew rows, two workgroups to a CU, have 512 threads each if they have
+// more than kShort runs, and rows of up to kWide runs stay whole.  256 threads /
+// 512: 50257 bf16 logits, top 20, 1 row 10.9 / 9.5 us, 128 14.3 / 12.8, 512 20.0 /
+// 18.8, but 1024 31.6 / 33.3; 700 rows of 32003 17.6 / 19.3; 16384 columns, kShort
+// runs, 256 rows 7.5 / 7.8.  65536 logits, top 20, in parts / whole: 1 row 10.6 /
+// 10.8 and a launch less, 128 14.9 / 12.9, 512 24.3 / 22.2.
 constexpr int kShort = kThreads * 8, kMiddle = kThreads * 16, kLong = kThreads * 25;
-constexpr int64_t kGroups = 4800, kListed = 1024;
+constexpr int kWide = 2 * kThreads * 16;
+constexpr int64_t kFew = 512, kGroups = 4800, kListed = 1024;
 
 Plan forward_plan(int64_t rows, int64_t vocab, int dtype, int64_t top) {
   const int64_t runs = runs_of(vocab, dtype), e = dtype == QSTE_F32 ? 4 : 8;
-  if (runs <= kLong) return {1, 0};
+  if (runs <= kLong || (runs <= kWide && rows <= kFew)) return {1, 0};
   int64_t parts = (runs + kLong - 1) / kLong;
   const int64_t more = (runs + kShort - 1) / kShort;
   if (more <= kMaxParts && rows * more <= kGroups && more * top <= kListed) parts = more;
@@ -461,17 +471,17 @@ Plan forward_plan(int64_t rows, int64_t vocab, int dtype, int64_t top) {
   return {static_cast<int>(parts), static_cast<int>((runs + parts - 1) / parts * e)};
 }
 
-template <int DT, int HELD, int WAVES_A_SIMD>
+template <int DT, int THREADS, int HELD, int WAVES_A_SIMD>
 int forward_as(const Args& a, int64_t rows, hipStream_t s) {
-  if constexpr (HELD > 0) {
+  if constexpr (HELD > 0 && THREADS == kThreads) {
     if (a.parts > 1) {
-      forward_kernel<DT, HELD, WAVES_A_SIMD, true><<<static_cast<unsigned>(rows * a.parts), kThreads, 0, s>>>(a);
+      forward_kernel<DT, THREADS, HELD, WAVES_A_SIMD, true><<<static_cast<unsigned>(rows * a.parts), kThreads, 0, s>>>(a);
       if (int rc = static_cast<int>(hipGetLastError())) return rc;
       join_kernel<DT><<<static_cast<unsigned>(rows), kThreads, static_cast<size_t>(a.parts) * a.top * 16, s>>>(a);
       return static_cast<int>(hipGetLastError());
     }
   }
-  forward_kernel<DT, HELD, WAVES_A_SIMD, false><<<static_cast<unsigned>(rows), kThreads, 0, s>>>(a);
+  forward_kernel<DT, THREADS, HELD, WAVES_A_SIMD, false><<<static_cast<unsigned>(rows), THREADS, 0, s>>>(a);
   return static_cast<int>(hipGetLastError());
 }
 
@@ -479,11 +489,12 @@ template <int DT>
 int forward(Args a, int64_t rows, const Plan& plan, hipStream_t s) {
   a.parts = plan.parts ? plan.parts : 1;
   a.part = plan.part;
-  if (plan.parts == 0) return forward_as<DT, 0, 4>(a, rows, s);
+  if (plan.parts == 0) return forward_as<DT, kThreads, 0, 4>(a, rows, s);
   const int64_t runs = plan.parts > 1 ? plan.part / (DT == QSTE_F32 ? 4 : 8) : runs_of(a.logits.vocab, DT);
-  if (runs <= kShort) return forward_as<DT, 8, 7>(a, rows, s);
-  if (runs <= kMiddle) return forward_as<DT, 16, 5>(a, rows, s);
-  return forward_as<DT, 25, 4>(a, rows, s);
+  if (plan.parts == 1 && runs > kShort && rows <= kFew) return forward_as<DT, 2 * kThreads, 16, 4>(a, rows, s);
+  if (runs <= kShort) return forward_as<DT, kThreads, 8, 7>(a, rows, s);
+  if (runs <= kMiddle) return forward_as<DT, kThreads, 16, 5>(a, rows, s);
+  return forward_as<DT, kThreads, 25, 4>(a, rows, s);
 }
 
 // ---------------------------------------------------------------------------

@@ -287,6 +287,24 @@ def test_many_long_rows(rows, vocab):
     check(logits, tokens, top=7)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,bytes_a_row", [(512, 32776), (512, 64006), (513, 64006), (512, 102400), (513, 102400),
+                                              (512, 131086), (513, 131086), (512, 131088)])
+def test_rows_around_the_wide_workgroups(rows, bytes_a_row, dtype):
+    """Both sides of what a workgroup of more threads takes: by the number of rows, and by their length."""
+
+    vocab = bytes_a_row // dtype.itemsize
+    print(f"wide {rows} x {vocab} {dtype}", flush=True)
+    logits = random_logits((rows, vocab), dtype, rows)
+    logits[1] = torch.arange(vocab, device=DEV).float() / vocab
+    logits[2, 5:] = -math.inf
+    logits[3] = 1.5
+    logits[4] = -math.inf
+    tokens = random_tokens((rows,), vocab, rows)
+    tokens[5] = -1
+    check(logits, tokens, top=30)
+
+
 def test_rows_far_apart():
     """Offsets past 32 bits, in elements and in bytes."""
 
