@@ -372,7 +372,10 @@ __global__ __launch_bounds__(THREADS, WAVES_A_SIMD) void forward_kernel(Args a) 
 // best of their lists.  With r = ceil(top / parts), r entries of every part are
 // at or above the least of the parts' r-th, so only what is not below that
 // stays.  An entry's rank is its own place and, by a search in each other
-// list, how many there are larger.
+// list, how many there are larger.  A few entries are each compared with all:
+// 40 rows of 131072 fp32 logits, top 5 of 16 parts, 16.6 -> 14.5 us in all; but
+// 2048 rows of 131072 bf16 logits, top 64 of 3 parts, 117 -> 122.
+constexpr int kDirect = 128;
 template <int DT>
 __global__ __launch_bounds__(kThreads) void join_kernel(Args a) {
   extern __shared__ uint64_t lists[];  // [parts, top], then a rank and a place of those that stay for each
@@ -395,7 +398,7 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Args a) {
     stay = 0;
   }
   __syncthreads();
-  if (k > 0 && tid < a.parts)
+  if (n > kDirect && tid < a.parts)
     atomicMin(&edge, static_cast<unsigned long long>(lists[tid * k + (k + a.parts - 1) / a.parts - 1]));
   float m = -INFINITY;
   for (int p = 0; p < a.parts; ++p) m = fmaxf(m, stats[3 * p]);
@@ -409,6 +412,14 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Args a) {
   }
   const float log_sum = scored<DT>(a, r, token, m, sum, moment);
   if (k == 0) return;
+  if (n <= kDirect) {
+    const uint64_t mine = tid < n ? lists[tid] : 0;
+    if (mine == 0) return;
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += lists[j] > mine;
+    if (rank < k) write_top(a, r, rank, mine, m, sum, log_sum);
+    return;
+  }
   __syncthreads();
   for (int i = tid; i < n; i += kThreads) {
     if (lists[i] == 0 || lists[i] < edge) continue;

@@ -305,6 +305,22 @@ def test_rows_around_the_wide_workgroups(rows, bytes_a_row, dtype):
     check(logits, tokens, top=30)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("top", [1, 4, 8, 9, 16, 17])
+def test_short_lists_of_parts(top, dtype):
+    """Both sides of how the lists of a row's parts become one."""
+
+    vocab = 131079
+    logits = random_logits((7, vocab), dtype, top)
+    logits[1] = torch.arange(vocab, device=DEV).float() / vocab
+    logits[2, 5:] = -math.inf
+    logits[3] = 1.5
+    logits[4] = -math.inf
+    logits[5, ::9001] = 60.0  # as the largest, some in every part
+    check(logits, random_tokens((7,), vocab, top), top=top)
+    check(logits, torch.full((7,), -1, device=DEV), top=top)
+
+
 def test_rows_far_apart():
     """Offsets past 32 bits, in elements and in bytes."""
 
