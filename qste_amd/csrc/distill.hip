@@ -485,16 +485,24 @@ __global__ __launch_bounds__(kThreads) void backward_kernel(Args a) {
 
 // Up to 25 runs a thread stay in registers with four waves on a SIMD, so a row
 // of up to kLong runs has one workgroup of 256 threads, four to a CU.  The
-// gradient wants a longer row held too: 512 threads hold up to kWide runs, two
-// workgroups to a CU, and with seven more a thread in LDS (56 KiB and the
-// list's bits: two still fit) kWidest.  Against three launches that read the
+// gradient wants a longer row held too: 512 threads hold up to kFewWide runs
+// with 16 a thread, kWide with 25, two workgroups to a CU, and with seven more a
+// thread in LDS (56 KiB and the list's bits: two still fit) kWidest.  Against three launches that read the
 // row twice (in parts, the join, the gradient): 2046 rows of 50257 fp32 logits
-// 209 -> 166 us, 2048 of 65536 bf16 149 -> 119, 8192 of 131072 1072 -> 821;
+// 209 -> 166 us, 2048 of 65536 bf16 149 -> 112 (119 with 25 runs a thread), 8192 of 131072 1072 -> 821;
 // rows of kWidest gain from about 160 of them (128: 31 / 34 us, 200: 41 / 36).
 // The loss alone reads a row once in any case, faster in parts.
+//
+// Few rows are bound by the chain of steps in each: up to kFew, two workgroups
+// to a CU, have 512 threads if they have more than kShort runs, and are whole up
+// to kFewWide, with 64 entries and the tail.  In 256 threads / 512: 1 row of
+// 50257 bf16 logits 10.9 / 8.8 us, 512 rows 19.4 / 17.0, with the gradient 27.4 /
+// 24.6; but 700 rows of 32003 24.4 / 27.3.  65536 logits in parts / whole: 1 row 10.6 / 10.0, 512 rows
+// 22.9 / 20.1.
 constexpr int kShort = kThreads * 8, kMiddle = kThreads * 16, kLong = kThreads * 25;
 constexpr int kKept = 7, kWide = 2 * kThreads * 25, kWidest = 2 * kThreads * (25 + kKept);
-constexpr int64_t kWidestRows = 160;
+constexpr int kFewWide = 2 * kThreads * 16;
+constexpr int64_t kFew = 512, kWidestRows = 160;
 
 struct Plan {
   // parts a row, columns a part (the last has the rest); 0 parts: one workgroup
@@ -504,7 +512,7 @@ struct Plan {
 
 Plan forward_plan(int64_t rows, int64_t vocab, int dtype, bool with_grad) {
   const int64_t runs = runs_of(vocab, dtype), e = dtype == QSTE_F32 ? 4 : 8;
-  if (runs <= kLong || (with_grad && (runs <= kWide || (runs <= kWidest && rows >= kWidestRows)))) return {1, 0};
+  if (runs <= kLong || (runs <= kFewWide && rows <= kFew) || (with_grad && (runs <= kWide || (runs <= kWidest && rows >= kWidestRows)))) return {1, 0};
   const int64_t parts = (runs + kLong - 1) / kLong;
   if (parts > kMaxParts) return {0, 0};
   // runs > parts * parts: no part is empty
@@ -535,6 +543,7 @@ int loss(const Args& a, const Plan& plan, int64_t rows, hipStream_t s) {
     return plan.part / Wide<DT>::E <= kMiddle ? parts_as<DT, 16, 5>(a, rows, s) : parts_as<DT, 25, 4>(a, rows, s);
   const int64_t runs = runs_of(a.logits.vocab, DT);
   if (runs <= kShort) return whole_as<DT, kThreads, 8, 0, 7>(a, rows, s);
+  if (runs <= kFewWide && (rows <= kFew || runs > kLong)) return whole_as<DT, 2 * kThreads, 16, 0, 4>(a, rows, s);
   if (runs <= kMiddle) return whole_as<DT, kThreads, 16, 0, 5>(a, rows, s);
   if (runs <= kLong) return whole_as<DT, kThreads, 25, 0, 4>(a, rows, s);
   if (runs <= kWide) return whole_as<DT, 2 * kThreads, 25, 0, 4>(a, rows, s);

@@ -457,8 +457,8 @@ struct Plan {
 // 126 of 128 registers), so a row has up to kLong runs in one workgroup, or is
 // cut into parts of as many.  Where it is cut in any case, shorter parts, of
 // kShort runs, bring in more workgroups for few rows: 131072 bf16 logits a row,
-// top 20, in 3 / in 8 parts: 1 row 14.3 / 12.4 us, 128 21.2 / 18.7, 600 44.3 /
-// 40.8; but 2048 107 / 111, and with many tokens to list the join decides (16
+// top 20, in 3 / in 8 parts: 1 row 14.5 / 11.1 us, 128 21.4 / 18.7, 600 44.9 /
+// 40.4; but 2048 104 / 110, and with many tokens to list the join decides (16
 // rows of 131072 fp32 logits, top 128, in 6 / in 16: 28 / 36).
 //
 // Up to kFew rows, two workgroups to a CU, have 512 threads each if they have

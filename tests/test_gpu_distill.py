@@ -323,6 +323,22 @@ def test_lists_at_the_ends(rows, vocab, k, dtype):
     check(random_logits((rows, vocab), dtype, 17), tokens.to(DEV), values, tail=k < vocab)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,bytes_a_row", [(512, 32784), (512, 64006), (513, 64006), (513, 102400), (512, 131086),
+                                              (513, 131086), (512, 131088)])
+def test_rows_around_the_wide_workgroups(rows, bytes_a_row, dtype):
+    """Both sides of what a workgroup of more threads takes: by the number of rows, and by their length."""
+
+    vocab = bytes_a_row // dtype.itemsize
+    print(f"wide {rows} x {vocab} {dtype}", flush=True)
+    tokens, values = random_teacher((rows,), vocab, 50, 18)
+    tokens[3, 10:] = -1
+    tokens[4] = -1
+    logits = random_logits((rows, vocab), dtype, 18)
+    logits[5, 1000:] = -math.inf
+    check(logits, tokens, values, tail=rows % 2 == 0)
+
+
 def test_rows_far_apart():
     """Offsets past 32 bits in the logits and in the gradient."""
 
