@@ -487,18 +487,19 @@ __global__ __launch_bounds__(kThreads) void backward_kernel(Args a) {
 // of up to kLong runs has one workgroup of 256 threads, four to a CU.  The
 // gradient wants a longer row held too: 512 threads hold up to kFewWide runs
 // with 16 a thread, kWide with 25, two workgroups to a CU, and with seven more a
-// thread in LDS (56 KiB and the list's bits: two still fit) kWidest.  Against three launches that read the
-// row twice (in parts, the join, the gradient): 2046 rows of 50257 fp32 logits
-// 209 -> 166 us, 2048 of 65536 bf16 149 -> 112 (119 with 25 runs a thread), 8192 of 131072 1072 -> 821;
-// rows of kWidest gain from about 160 of them (128: 31 / 34 us, 200: 41 / 36).
-// The loss alone reads a row once in any case, faster in parts.
+// thread in LDS (56 KiB and the list's bits: two still fit) kWidest.  Against
+// three launches that read the row twice (in parts, the join, the gradient):
+// 2046 rows of 50257 fp32 logits 209 -> 166 us, 2048 of 65536 bf16 149 -> 112
+// (119 with 25 runs a thread), 8192 of 131072 1072 -> 821; rows of kWidest gain
+// from about 160 of them (128: 31 / 34 us, 200: 41 / 36).  The loss alone reads
+// a row once in any case, faster in parts.
 //
 // Few rows are bound by the chain of steps in each: up to kFew, two workgroups
 // to a CU, have 512 threads if they have more than kShort runs, and are whole up
-// to kFewWide, with 64 entries and the tail.  In 256 threads / 512: 1 row of
+// to kFewWide.  With 64 entries and the tail, in 256 threads / 512: 1 row of
 // 50257 bf16 logits 10.9 / 8.8 us, 512 rows 19.4 / 17.0, with the gradient 27.4 /
-// 24.6; but 700 rows of 32003 24.4 / 27.3.  65536 logits in parts / whole: 1 row 10.6 / 10.0, 512 rows
-// 22.9 / 20.1.
+// 24.6; but 700 rows of 32003 24.4 / 27.3.  65536 logits in parts / whole: 1 row
+// 10.6 / 10.0, 512 rows 22.9 / 20.1.
 constexpr int kShort = kThreads * 8, kMiddle = kThreads * 16, kLong = kThreads * 25;
 constexpr int kKept = 7, kWide = 2 * kThreads * 25, kWidest = 2 * kThreads * (25 + kKept);
 constexpr int kFewWide = 2 * kThreads * 16;
