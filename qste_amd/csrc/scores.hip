@@ -190,7 +190,7 @@ __device__ __forceinline__ void collect_many(const R& row, int from, float edge,
 // forward: one workgroup a row, or one for each part of it and one that joins them
 //
 // Bound by reading the logits and by the vector instructions alike: 10.3 an
-// element, 13.6 with 64 tokens to list, keep the SIMDs busy for 0.86 and 0.92 of
+// element, 13.6 with 64 tokens to list, keep the SIMDs busy for 0.87 and 0.95 of
 // the time.  A row stays in registers from its one read over both passes, the
 // maximum and the sums; four workgroups of 256 threads on a CU read, reduce and
 // list at the same time.  4092 rows of 50257 bf16 logits 74 us (5.5 TB/s of the
