@@ -3,7 +3,7 @@
 Both work on a model's logits, ``[..., vocab]`` in fp32, fp16 or bf16 on the GPU,
 in any layout whose columns are adjacent (``logits[:, :-1]`` is read in place).
 Softmax, sums and losses are fp32; a gradient is rounded once, to the
-logits' dtype.  The kernels are ``csrc/scores.hip`` and ``csrc/distill.hip``; the
+logits' dtype.  Forward-mode differentiation is refused.  The kernels are ``csrc/scores.hip`` and ``csrc/distill.hip``; the
 reference ends at the logits and has no counterparts.
 
     with torch.no_grad():                    # the teacher, and what it thinks likely
@@ -18,7 +18,7 @@ from typing import NamedTuple, Optional
 
 import torch
 from torch import Tensor
-from torch.autograd import Function
+from torch.autograd import Function, forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import kernels
@@ -60,6 +60,16 @@ class TokenLogprobsFn(Function):
                 None, None, None)
 
 
+def _no_tangent(what: str, *tensors: Tensor) -> None:
+    """Refuses forward-mode differentiation.  A dual tensor need not have
+    ``requires_grad``, so it can reach the kernels' calls, which would take its
+    values and lose its tangent."""
+
+    for t in tensors:
+        if forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{what} has no forward-mode derivative")
+
+
 def token_logprobs(logits: Tensor, tokens: Optional[Tensor] = None, *, top: int = 0,
                    temperature: float = 1.0) -> TokenScores:
     """Log probabilities of ``tokens`` under ``softmax(logits / temperature)``, each
@@ -73,6 +83,7 @@ def token_logprobs(logits: Tensor, tokens: Optional[Tensor] = None, *, top: int 
     log probabilities carry no gradient.
     """
 
+    _no_tangent("token_logprobs", logits)
     if torch.is_grad_enabled() and logits.requires_grad:
         return TokenScores(*TokenLogprobsFn.apply(logits, tokens, top, temperature))
     return TokenScores(*kernels.token_logprobs_forward(logits, tokens, top=top, temperature=temperature)[:4])
@@ -117,6 +128,7 @@ def distillation_loss(logits: Tensor, top_tokens: Tensor, top_logprobs: Tensor, 
     token is no entry; a position with none has the loss 0 and no gradient.
     """
 
+    _no_tangent("distillation_loss", logits, top_logprobs)
     _constant(top_logprobs)
     if torch.is_grad_enabled() and logits.requires_grad:
         return DistillationFn.apply(logits, top_tokens, top_logprobs, temperature, tail)
@@ -136,9 +148,11 @@ def distillation_loss_and_grad(logits: Tensor, top_tokens: Tensor, top_logprobs:
     Positions of weight 0 get zeros, whatever their logits hold.
     """
 
+    _no_tangent("distillation_loss_and_grad", logits, top_logprobs)
     _constant(top_logprobs)
     shape = logits.shape[:-1]
     if isinstance(loss_grad, Tensor):
+        _no_tangent("distillation_loss_and_grad", loss_grad)
         weights = loss_grad if loss_grad.shape == shape else loss_grad.expand(shape)
     else:
         weights = torch.full(shape, float(loss_grad), dtype=torch.float32, device=logits.device)
