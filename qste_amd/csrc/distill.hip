@@ -354,7 +354,7 @@ __device__ __forceinline__ void write_listed(const Args& a, const Entries& t, bo
 
 template <int DT, int THREADS, int HELD, int KEPT, int WAVES_A_SIMD>
 __global__ __launch_bounds__(THREADS, WAVES_A_SIMD) void forward_kernel(Args a) {
-  extern __shared__ uint32_t lds[];
+  extern __shared__ __align__(16) uint32_t lds[];  // kept runs first: 16-byte accesses
   __shared__ Shared sh;
   using R = Row<DT, THREADS, HELD, KEPT>;
   const int64_t r = blockIdx.x;
@@ -397,7 +397,7 @@ __global__ __launch_bounds__(THREADS, WAVES_A_SIMD) void forward_kernel(Args a) 
 
 template <int DT, int HELD, int WAVES_A_SIMD>
 __global__ __launch_bounds__(kThreads, WAVES_A_SIMD) void part_kernel(Args a) {
-  extern __shared__ uint32_t lds[];
+  extern __shared__ __align__(16) uint32_t lds[];
   __shared__ Shared sh;
   using R = Row<DT, kThreads, HELD>;
   const int64_t r = blockIdx.x / static_cast<uint32_t>(a.parts);
@@ -416,7 +416,7 @@ __global__ __launch_bounds__(kThreads, WAVES_A_SIMD) void part_kernel(Args a) {
 // one wave a row
 template <int DT>
 __global__ __launch_bounds__(kWave) void join_kernel(Args a) {
-  extern __shared__ uint32_t lds[];
+  extern __shared__ __align__(16) uint32_t lds[];
   const int64_t r = blockIdx.x;
   const Entries t(lds, a.k);
   const float4* parts = reinterpret_cast<const float4*>(a.part_stats) + r * a.parts;
@@ -450,7 +450,7 @@ constexpr int kBackRuns = 4;  // 16-byte accesses a thread makes
 
 template <int DT>
 __global__ __launch_bounds__(kThreads) void backward_kernel(Args a) {
-  extern __shared__ uint32_t lds[];
+  extern __shared__ __align__(16) uint32_t lds[];
   using R = Row<DT, kThreads, kBackRuns>;
   const int64_t r = blockIdx.x / static_cast<uint32_t>(a.parts);
   const int part = blockIdx.x % static_cast<uint32_t>(a.parts), vocab = a.logits.vocab;
