@@ -515,7 +515,8 @@ int qste_token_logprobs(const void* logits, int dtype, int64_t outer, int64_t in
  * logits' gradient (g ([j = token] - p_j) - h p_j (ln p_j + entropy)) /
  * temperature for g = logprob_grad[row] and h = entropy_grad[row] (fp32; NULL
  * is zeros), with the forward's entropy and stats.  Zeros where nothing
- * flows back (g = h = 0, a row that is not scored, a row of only -inf). */
+ * flows back (g = h = 0, a row that is not scored, a row of only -inf); NaN
+ * in a row whose token is >= vocab, unless its g is 0. */
 int qste_token_logprobs_backward(const void* logits, int dtype, int64_t outer, int64_t inner, int64_t outer_stride,
                                  int64_t inner_stride, int64_t vocab, const int64_t* tokens, double temperature,
                                  const float* logprob_grad, const float* entropy_grad, const float* entropy,

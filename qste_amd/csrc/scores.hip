@@ -551,7 +551,7 @@ __global__ __launch_bounds__(kThreads) void backward_kernel(BackArgs a, int part
     return;
   }
   const R row(a.logits.row<typename R::T>(r) + from, to - from, part == 0 ? head : 0, a.logits.once);
-  if (token >= vocab) g = NAN;
+  if (token >= vocab && g != 0.0f) g = NAN;  // the log probability is NaN; the entropy knows no token
   const Exponent ex(m, a.scale);
   // dz = e (flat + slope power), from p = e / S and ln p = ln2 power - ln S
   const float per = -a.inverse / sum;

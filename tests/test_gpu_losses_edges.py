@@ -1,0 +1,71 @@
+"""Token scores and distillation at the ends of what they accept.
+
+Bounds as in test_gpu_scores.py and test_gpu_distill.py: a log probability is within LOG = 4e-5 (the sums' chain of
+additions) and 1e-6 of itself (its three roundings).
+"""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+LOG = 4e-5
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+@pytest.fixture(autouse=True)
+def _gpu():
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    from qste_amd import kernels
+
+    assert kernels.native_available(), kernels.status()
+
+
+def near(got, want, bound):
+    got, want = got.detach().cpu().double(), want.cpu().double()
+    assert got.shape == want.shape
+    same = (got == want) | (got.isnan() & want.isnan())
+    off = torch.where(same, 0.0, (got - want).abs()).nan_to_num(nan=math.inf)
+    bound = torch.as_tensor(bound).double().cpu().nan_to_num(nan=0.0, posinf=0.0)
+    assert bool((off <= bound).all()), (float(off.max()), float((off - bound).max()))
+
+
+# ---------------------------------------------------------------------------
+# a token past the vocabulary
+# ---------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("weighted", [False, True])
+def test_entropy_gradient_beside_a_token_outside(weighted, dtype):
+    """The entropy does not depend on the token: its gradient is the formula's, unless a NaN log probability has a
+    weight."""
+
+    import qste_amd as qste
+
+    vocab = 3001
+    g = torch.Generator(device=DEV).manual_seed(5)
+    logits = (torch.randn(3, vocab, generator=g, device=DEV) * 2).to(dtype).requires_grad_(True)
+    tokens = torch.tensor([7, vocab, 1 << 40], device=DEV)
+    s = qste.nn.token_logprobs(logits, tokens)
+    h = torch.tensor([0.5, -1.0, 2.0], device=DEV)
+    if weighted:
+        grad, = torch.autograd.grad((s.logprobs, s.entropy), logits, (torch.zeros(3, device=DEV), h))
+    else:
+        grad, = torch.autograd.grad(s.entropy, logits, h)
+    lnp = torch.log_softmax(logits.detach().cpu().double(), 1)
+    p = lnp.exp()
+    entropy = -(p * lnp).sum(1, keepdim=True)
+    want = -h.cpu().double()[:, None] * p * (lnp + entropy)
+    size = h.cpu().double().abs()[:, None] * p * (lnp.abs() + entropy)
+    rounding = {torch.float32: 2.0 ** -23, torch.float16: 2.0 ** -10, torch.bfloat16: 2.0 ** -8}[dtype]
+    near(grad, want, rounding * want.abs() + LOG * size + (2.0 ** -24 if dtype == torch.float16 else 1e-37))
+    s = qste.nn.token_logprobs(logits, tokens)
+    grad, = torch.autograd.grad(s.logprobs, logits, torch.tensor([1.0, 0.0, 1.0], device=DEV))
+    assert grad[0].isfinite().all() and not grad[1].any() and grad[2].isnan().all()
