@@ -285,7 +285,10 @@ __device__ __forceinline__ Coefficients coefficients(const Args& a, const Teache
   return {weight, weight - rest / p_rest, rest * (logf(rest) - logf(p_rest))};
 }
 
-// The row's loss and statistics, by one wave
+// The row's loss and statistics, by one wave.  A log probability can be past
+// fp32 (at a temperature below 1, logits near its ends) where the loss, T times
+// a difference of logits, is not: in `far` are halves of such differences, beside
+// which the rest of their terms is nothing.
 template <int DT>
 __device__ __forceinline__ void write_loss(const Args& a, int64_t r, const Entries& t, const Teacher& teacher, float m,
                                            float sum, const Coefficients& co) {
@@ -293,18 +296,24 @@ __device__ __forceinline__ void write_loss(const Args& a, int64_t r, const Entri
   const int lane = threadIdx.x & (kWave - 1);
   const T* row = a.logits.row<T>(r);
   const float log_sum = logf(sum);
-  float loss = 0.0f;
+  float loss = 0.0f, far = 0.0f;
   if (sum != 0.0f)
     for (int k = lane; k < a.k; k += kWave) {
       const int at = t.token[k];
       const float log_q = t.log_q[k], q = expf(log_q);
-      if (at >= 0 && q != 0.0f) loss += q * (log_q - ((Elem<DT>::load(row, at) - m) * a.inverse - log_sum));
+      if (at < 0 || q == 0.0f) continue;
+      const float z = Elem<DT>::load(row, at), scaled = scaled_difference(z, m, a.inverse);
+      if (scaled == -INFINITY && z > -INFINITY && m < INFINITY)
+        far += q * (m * 0.5f - z * 0.5f);
+      else
+        loss += q * (log_q - (scaled - log_sum));
     }
   loss = fold_sum(loss);
+  far = fold_sum(far);
   if (lane == 0) {
     loss += co.rest_loss;
     if (sum == 0.0f) loss = teacher.mass == 0.0f ? 0.0f : teacher.mass != teacher.mass ? teacher.mass : INFINITY;
-    a.losses[r] = loss * a.temperature * a.temperature;
+    a.losses[r] = loss * a.temperature * a.temperature + far * (2.0f * a.temperature);
     set_stats(a, r, m, sum == 0.0f ? 1.0f : sum,
               {co.weight, co.other, teacher.shift, teacher.repeated ? 1.0f : 0.0f});
   }

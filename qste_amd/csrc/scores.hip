@@ -224,7 +224,7 @@ __device__ __forceinline__ float scored(const Args& a, int64_t r, int64_t token,
       if (token >= a.logits.vocab)
         lp = NAN;
       else if (sum != 0.0f)
-        lp = (Elem<DT>::load(a.logits.row<typename Elem<DT>::T>(r), token) - m) * a.inverse - log_sum;
+        lp = scaled_difference(Elem<DT>::load(a.logits.row<typename Elem<DT>::T>(r), token), m, a.inverse) - log_sum;
       a.logprobs[r] = lp;
     }
     const float h = sum == 0.0f ? 0.0f : log_sum - kLn2 * (moment / sum);
@@ -237,7 +237,7 @@ __device__ __forceinline__ float scored(const Args& a, int64_t r, int64_t token,
 __device__ __forceinline__ void write_top(const Args& a, int64_t r, int rank, uint64_t entry, float m, float sum,
                                           float log_sum) {
   const float x = value_of(static_cast<uint32_t>(entry >> 32));
-  a.top_logprobs[r * a.top + rank] = sum == 0.0f ? -INFINITY : (x - m) * a.inverse - log_sum;
+  a.top_logprobs[r * a.top + rank] = sum == 0.0f ? -INFINITY : scaled_difference(x, m, a.inverse) - log_sum;
   a.top_tokens[r * a.top + rank] = static_cast<int64_t>(~static_cast<uint32_t>(entry));
 }
 

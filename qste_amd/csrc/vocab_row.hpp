@@ -317,9 +317,9 @@ __device__ __forceinline__ float max_of(float m, const float (&x)[N]) {
 
 // The exponentials of a row, 2^((z - m) c) with m the row's maximum and c =
 // log2(e) / temperature.  The difference is formed before the scale: it is
-// exact near m, so the maximum's weight is exactly 1, and neither a logit near
-// the end of fp32 nor a small temperature can leave the range (one
-// multiply-add of z c - m c would save an operation and lose both).
+// exact near m, so the maximum's weight is exactly 1, and where it passes the
+// end of fp32 the exponential is 0, as it would be (one multiply-add of z c - m
+// c would save an operation and lose both).
 struct Exponent {
   float m, c;
 
@@ -328,6 +328,12 @@ struct Exponent {
   __device__ __forceinline__ float power(float z) const { return (z - m) * c; }
   __device__ __forceinline__ static float of(float power) { return __builtin_amdgcn_exp2f(power); }
 };
+
+// (z - m) / temperature by its inverse, for single values: the halves' difference
+// is in fp32's range for any two logits, and the same bits times two where that is
+__device__ __forceinline__ float scaled_difference(float z, float m, float inverse) {
+  return (z * 0.5f - m * 0.5f) * (inverse * 2.0f);
+}
 
 // Values in their order as unsigned integers: -0 equals 0, every NaN is one
 // and the largest.

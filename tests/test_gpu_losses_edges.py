@@ -69,3 +69,62 @@ def test_entropy_gradient_beside_a_token_outside(weighted, dtype):
     s = qste.nn.token_logprobs(logits, tokens)
     grad, = torch.autograd.grad(s.logprobs, logits, torch.tensor([1.0, 0.0, 1.0], device=DEV))
     assert grad[0].isfinite().all() and not grad[1].any() and grad[2].isnan().all()
+
+
+# ---------------------------------------------------------------------------
+# logits further apart than fp32's largest number
+# ---------------------------------------------------------------------------
+
+
+def far_apart(vocab, dtype):
+    """Three rows of logits, two tokens of each further below its largest than fp32 reaches."""
+
+    logits = torch.full((3, vocab), -1e38, device=DEV)
+    logits[0, 3] = 3e38
+    logits[1, 2:6] = 3.3e38
+    logits[1, 8] = -3.3e38
+    logits[2, 0] = torch.finfo(dtype).max
+    logits[2, 7] = torch.finfo(dtype).min
+    return logits.to(dtype), torch.tensor([[4, 5], [8, 0], [7, 8]], device=DEV)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("temperature", [2.5, 50.0, 1e20])
+@pytest.mark.parametrize("vocab", [9, 5000, 60000, 150001])
+def test_log_probabilities_of_differences_past_fp32(vocab, temperature, dtype):
+    """Finite at a temperature that brings the differences back."""
+
+    import qste_amd as qste
+
+    logits, tokens = far_apart(vocab, dtype)
+    z = logits.cpu().double()
+    lnp = torch.log_softmax(z / temperature, 1)
+    got = qste.nn.token_logprobs(logits, tokens[:, 0], top=9, temperature=temperature)
+    want = lnp.gather(1, tokens.cpu())[:, 0]
+    assert got.logprobs.isfinite().all()
+    near(got.logprobs, want, LOG + 1e-6 * want.abs())
+    places = torch.sort(z, dim=1, descending=True, stable=True).indices[:, :9]
+    assert torch.equal(got.top_tokens.cpu(), places)
+    want = lnp.gather(1, places)
+    near(got.top_logprobs, want, LOG + 1e-6 * want.abs())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("temperature", [0.01, 0.25, 50.0])
+@pytest.mark.parametrize("vocab", [9, 5000, 60000, 150001])
+def test_losses_of_differences_past_fp32(vocab, temperature, dtype):
+    """About temperature times a difference: finite where that fits, though the log probabilities in it do not."""
+
+    import qste_amd as qste
+
+    logits, tokens = far_apart(vocab, dtype)
+    values = torch.tensor([0.75, 0.25], device=DEV).log().expand(3, 2)
+    lnp = torch.log_softmax(logits.cpu().double() / temperature, 1).gather(1, tokens.cpu())
+    q = torch.tensor([0.75, 0.25]).double()
+    want = temperature ** 2 * (q * (q.log() - lnp)).sum(1)
+    want = torch.where(want > torch.finfo(torch.float32).max, math.inf, want)
+    assert want.isfinite().all() if temperature < 1 else want.isinf().all()
+    losses, grad = qste.nn.distillation_loss_and_grad(logits, tokens, values, temperature=temperature)
+    near(losses, want, 2e-6 * want)
+    near(qste.nn.distillation_loss(logits, tokens, values, temperature=temperature), want, 2e-6 * want)
+    assert grad.isfinite().all()
