@@ -312,7 +312,7 @@ __device__ __forceinline__ void write_loss(const Args& a, int64_t r, const Entri
   far = fold_sum(far);
   if (lane == 0) {
     loss += co.rest_loss;
-    if (sum == 0.0f) loss = teacher.mass == 0.0f ? 0.0f : teacher.mass != teacher.mass ? teacher.mass : INFINITY;
+    if (sum == 0.0f) loss = teacher.mass != teacher.mass ? teacher.mass : INFINITY;
     a.losses[r] = loss * a.temperature * a.temperature + far * (2.0f * a.temperature);
     set_stats(a, r, m, sum == 0.0f ? 1.0f : sum,
               {co.weight, co.other, teacher.shift, teacher.repeated ? 1.0f : 0.0f});

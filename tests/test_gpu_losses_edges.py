@@ -128,3 +128,29 @@ def test_losses_of_differences_past_fp32(vocab, temperature, dtype):
     near(losses, want, 2e-6 * want)
     near(qste.nn.distillation_loss(logits, tokens, values, temperature=temperature), want, 2e-6 * want)
     assert grad.isfinite().all()
+
+
+# ---------------------------------------------------------------------------
+# a student and a list without mass
+# ---------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("vocab", [700, 60000, 150001])
+def test_a_masked_student_against_a_list_without_mass(vocab):
+    """With the tail all of the teacher's mass is outside the list: entries there are, and a row of only -inf has an
+    infinite loss as with any others; without the tail it is a row without entries of mass."""
+
+    import qste_amd as qste
+
+    logits = torch.full((3, vocab), -math.inf, device=DEV)
+    logits[2] = 0.0
+    tokens = torch.tensor([[4, 5], [-1, -1], [4, 5]], device=DEV)
+    values = torch.full((3, 2), -math.inf, device=DEV)
+    for tail, first in ((True, math.inf), (False, 0.0)):
+        losses, grad = qste.nn.distillation_loss_and_grad(logits, tokens, values, tail=tail)
+        alone = qste.nn.distillation_loss(logits, tokens, values, tail=tail)
+        for got in (losses, alone):
+            assert got[0] == first and got[1] == 0
+            # a flat student has all but 2 / vocab of its mass outside the list
+            near(got[2:], torch.tensor([-math.log1p(-2 / vocab) if tail else 0.0]), LOG)
+        assert not grad[:2].any() and grad.isfinite().all()
