@@ -485,8 +485,8 @@ int qste_embedding_backward(const int64_t* ids, int64_t count, const void* grad,
 
 /* ---- scores of tokens, distillation from a teacher's top tokens ---------- */
 
-/* Rows of logits, in the four entry points below: outer * inner rows of
- * `vocab` columns (at most 2^30), row (o, i) starting at element o *
+/* Rows of logits, in the four entry points below: outer * inner rows (less
+ * than 2^31) of `vocab` columns (at most 2^30), row (o, i) starting at element o *
  * outer_stride + i * inner_stride of `logits` (any element: no alignment past
  * the type's own; strides may be 0 or negative), its columns one element apart.  Everything per row is
  * contiguous, row o * inner + i at that index.  z is a row of logits over

@@ -32,6 +32,7 @@ constexpr int kStats = QSTE_DISTILL_STATS;
 
 struct Args {
   Logits logits;
+  int64_t first_row;  // of this launch
   const int64_t* tokens;  // [rows, k]
   const float* values;    // [rows, k]
   int k, tail;
@@ -366,7 +367,7 @@ __global__ __launch_bounds__(THREADS, WAVES_A_SIMD) void forward_kernel(Args a) 
   extern __shared__ __align__(16) uint32_t lds[];  // kept runs first: 16-byte accesses
   __shared__ Shared sh;
   using R = Row<DT, THREADS, HELD, KEPT>;
-  const int64_t r = blockIdx.x;
+  const int64_t r = a.first_row + blockIdx.x;
   const int vocab = a.logits.vocab;
   const Entries t(lds + KEPT * THREADS * 4, a.k);
   typename R::T* out = static_cast<typename R::T*>(a.grad) + r * vocab;
@@ -409,7 +410,7 @@ __global__ __launch_bounds__(kThreads, WAVES_A_SIMD) void part_kernel(Args a) {
   extern __shared__ __align__(16) uint32_t lds[];
   __shared__ Shared sh;
   using R = Row<DT, kThreads, HELD>;
-  const int64_t r = blockIdx.x / static_cast<uint32_t>(a.parts);
+  const int64_t r = a.first_row + blockIdx.x / static_cast<uint32_t>(a.parts);
   const int part = blockIdx.x % static_cast<uint32_t>(a.parts);
   const int from = part * a.part, to = part < a.parts - 1 ? from + a.part : a.logits.vocab;
   const Entries t(lds, a.k);
@@ -426,7 +427,7 @@ __global__ __launch_bounds__(kThreads, WAVES_A_SIMD) void part_kernel(Args a) {
 template <int DT>
 __global__ __launch_bounds__(kWave) void join_kernel(Args a) {
   extern __shared__ __align__(16) uint32_t lds[];
-  const int64_t r = blockIdx.x;
+  const int64_t r = a.first_row + blockIdx.x;
   const Entries t(lds, a.k);
   const float4* parts = reinterpret_cast<const float4*>(a.part_stats) + r * a.parts;
   Teacher teacher = load_entries(a, r, load_first(a, r), t);
@@ -461,7 +462,7 @@ template <int DT>
 __global__ __launch_bounds__(kThreads) void backward_kernel(Args a) {
   extern __shared__ __align__(16) uint32_t lds[];
   using R = Row<DT, kThreads, kBackRuns>;
-  const int64_t r = blockIdx.x / static_cast<uint32_t>(a.parts);
+  const int64_t r = a.first_row + blockIdx.x / static_cast<uint32_t>(a.parts);
   const int part = blockIdx.x % static_cast<uint32_t>(a.parts), vocab = a.logits.vocab;
   typename R::T* out = static_cast<typename R::T*>(a.grad) + r * vocab;
   // parts begin at whole lines of the gradient, but for the first
@@ -530,19 +531,26 @@ Plan forward_plan(int64_t rows, int64_t vocab, int dtype, bool with_grad) {
 }
 
 template <int DT, int THREADS, int HELD, int KEPT, int WAVES_A_SIMD>
-int whole_as(const Args& a, int64_t rows, hipStream_t s) {
+int whole_as(Args a, int64_t rows, hipStream_t s) {
   const size_t lds = entries_bytes(a.k, kBits<Row<DT, THREADS, HELD, KEPT>>) + static_cast<size_t>(KEPT) * THREADS * 16;
-  forward_kernel<DT, THREADS, HELD, KEPT, WAVES_A_SIMD><<<static_cast<unsigned>(rows), THREADS, lds, s>>>(a);
-  return static_cast<int>(hipGetLastError());
+  return launch_rows(rows, 1, THREADS, [&](int64_t first, unsigned blocks) {
+    a.first_row = first;
+    forward_kernel<DT, THREADS, HELD, KEPT, WAVES_A_SIMD><<<blocks, THREADS, lds, s>>>(a);
+  });
 }
 
 template <int DT, int HELD, int WAVES_A_SIMD>
-int parts_as(const Args& a, int64_t rows, hipStream_t s) {
-  part_kernel<DT, HELD, WAVES_A_SIMD>
-      <<<static_cast<unsigned>(rows * a.parts), kThreads, entries_bytes(a.k, kBits<Row<DT, kThreads, HELD>>), s>>>(a);
-  if (int rc = static_cast<int>(hipGetLastError())) return rc;
-  join_kernel<DT><<<static_cast<unsigned>(rows), kWave, entries_bytes(a.k, 0), s>>>(a);
-  return static_cast<int>(hipGetLastError());
+int parts_as(Args a, int64_t rows, hipStream_t s) {
+  const size_t lds = entries_bytes(a.k, kBits<Row<DT, kThreads, HELD>>);
+  const int rc = launch_rows(rows, a.parts, kThreads, [&](int64_t first, unsigned blocks) {
+    a.first_row = first;
+    part_kernel<DT, HELD, WAVES_A_SIMD><<<blocks, kThreads, lds, s>>>(a);
+  });
+  if (rc) return rc;
+  return launch_rows(rows, 1, kWave, [&](int64_t first, unsigned blocks) {
+    a.first_row = first;
+    join_kernel<DT><<<blocks, kWave, entries_bytes(a.k, 0), s>>>(a);
+  });
 }
 
 template <int DT>
@@ -564,9 +572,10 @@ template <int DT>
 int backward(Args a, int64_t rows, hipStream_t s) {
   a.part = kThreads * kBackRuns * Wide<DT>::E;
   a.parts = ceil_div(a.logits.vocab, a.part);
-  if (rows * a.parts > INT32_MAX) return QSTE_E_SHAPE;
-  backward_kernel<DT><<<static_cast<unsigned>(rows * a.parts), kThreads, entries_bytes(a.k, 0), s>>>(a);
-  return static_cast<int>(hipGetLastError());
+  return launch_rows(rows, a.parts, kThreads, [&](int64_t first, unsigned blocks) {
+    a.first_row = first;
+    backward_kernel<DT><<<blocks, kThreads, entries_bytes(a.k, 0), s>>>(a);
+  });
 }
 
 Args arguments(const Logits& logits, const int64_t* tokens, const float* values, int64_t k, double temperature,
@@ -616,7 +625,6 @@ int launch_distill(const vocab::Logits& logits, int dtype, int64_t rows, const i
   a.stats = stats;
   a.loss_grad = loss_grad;
   if (plan.parts > 1) {
-    if (rows * plan.parts > INT32_MAX) return QSTE_E_SHAPE;
     a.parts = plan.parts;
     a.part = plan.part;
     a.part_stats = static_cast<float*>(workspace);

@@ -23,6 +23,7 @@ constexpr int kMaxParts = 32;
 
 struct Args {
   Logits logits;
+  int64_t first_row;  // of this launch
   const int64_t* tokens;
   float scale, inverse;  // log2(e) / temperature and 1 / temperature
   int top;
@@ -250,7 +251,7 @@ __global__ __launch_bounds__(THREADS, WAVES_A_SIMD) void forward_kernel(Args a) 
   __shared__ uint32_t bounds[kWaves];
   __shared__ Candidates c;
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
-  const int64_t r = SPLIT ? blockIdx.x / static_cast<uint32_t>(a.parts) : blockIdx.x;
+  const int64_t r = a.first_row + (SPLIT ? blockIdx.x / static_cast<uint32_t>(a.parts) : blockIdx.x);
   const int part = SPLIT ? blockIdx.x % static_cast<uint32_t>(a.parts) : 0;
   const int64_t token = a.tokens ? a.tokens[r] : 0;
   if (token < 0) {
@@ -383,7 +384,7 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Args a) {
   __shared__ unsigned long long edge;
   __shared__ int stay;
   const int tid = threadIdx.x, k = a.top, n = a.parts * k;
-  const int64_t r = blockIdx.x;
+  const int64_t r = a.first_row + blockIdx.x;
   const int64_t token = a.tokens ? a.tokens[r] : 0;
   if (token < 0) {
     unscored<kThreads>(a, r);
@@ -483,17 +484,24 @@ Plan forward_plan(int64_t rows, int64_t vocab, int dtype, int64_t top) {
 }
 
 template <int DT, int THREADS, int HELD, int WAVES_A_SIMD>
-int forward_as(const Args& a, int64_t rows, hipStream_t s) {
+int forward_as(Args a, int64_t rows, hipStream_t s) {
   if constexpr (HELD > 0 && THREADS == kThreads) {
     if (a.parts > 1) {
-      forward_kernel<DT, THREADS, HELD, WAVES_A_SIMD, true><<<static_cast<unsigned>(rows * a.parts), kThreads, 0, s>>>(a);
-      if (int rc = static_cast<int>(hipGetLastError())) return rc;
-      join_kernel<DT><<<static_cast<unsigned>(rows), kThreads, static_cast<size_t>(a.parts) * a.top * 16, s>>>(a);
-      return static_cast<int>(hipGetLastError());
+      const int rc = launch_rows(rows, a.parts, kThreads, [&](int64_t first, unsigned blocks) {
+        a.first_row = first;
+        forward_kernel<DT, THREADS, HELD, WAVES_A_SIMD, true><<<blocks, kThreads, 0, s>>>(a);
+      });
+      if (rc) return rc;
+      return launch_rows(rows, 1, kThreads, [&](int64_t first, unsigned blocks) {
+        a.first_row = first;
+        join_kernel<DT><<<blocks, kThreads, static_cast<size_t>(a.parts) * a.top * 16, s>>>(a);
+      });
     }
   }
-  forward_kernel<DT, THREADS, HELD, WAVES_A_SIMD, false><<<static_cast<unsigned>(rows), THREADS, 0, s>>>(a);
-  return static_cast<int>(hipGetLastError());
+  return launch_rows(rows, 1, THREADS, [&](int64_t first, unsigned blocks) {
+    a.first_row = first;
+    forward_kernel<DT, THREADS, HELD, WAVES_A_SIMD, false><<<blocks, THREADS, 0, s>>>(a);
+  });
 }
 
 template <int DT>
@@ -521,6 +529,7 @@ constexpr int kBackRuns = 4;  // 16-byte accesses a thread makes
 
 struct BackArgs {
   Logits logits;
+  int64_t first_row;  // of this launch
   const int64_t* tokens;
   float scale, inverse;
   const float* logprob_grad;
@@ -535,7 +544,7 @@ __global__ __launch_bounds__(kThreads) void backward_kernel(BackArgs a, int part
   using W = Wide<DT>;
   using R = Row<DT, kThreads, kBackRuns>;
   constexpr int kPart = kThreads * kBackRuns * W::E;
-  const int64_t r = blockIdx.x / static_cast<uint32_t>(parts);
+  const int64_t r = a.first_row + blockIdx.x / static_cast<uint32_t>(parts);
   const int part = blockIdx.x % static_cast<uint32_t>(parts), vocab = a.logits.vocab;
   typename R::T* out = static_cast<typename R::T*>(a.grad) + r * vocab;
   // parts begin at whole lines of the gradient, but for the first
@@ -581,10 +590,9 @@ int launch_token_logprobs(const vocab::Logits& logits, int dtype, int64_t rows, 
                           int64_t* top_tokens, float* stats, void* workspace, hipStream_t s) {
   using namespace scores;
   const Plan plan = forward_plan(rows, logits.vocab, dtype, top);
-  if (rows * (plan.parts > 1 ? plan.parts : 1) > INT32_MAX) return QSTE_E_SHAPE;
   uint64_t* entries = plan.parts > 1 ? static_cast<uint64_t*>(workspace) : nullptr;
   float* part_stats = plan.parts > 1 ? reinterpret_cast<float*>(entries + rows * plan.parts * top) : nullptr;
-  const Args a{logits, tokens, static_cast<float>(kLog2e / temperature),
+  const Args a{logits, 0, tokens, static_cast<float>(kLog2e / temperature),
                static_cast<float>(1.0 / temperature), static_cast<int>(top), logprobs, entropy, top_logprobs,
                top_tokens, stats, 1, 0, part_stats, entries};
   switch (dtype) {
@@ -598,20 +606,19 @@ int launch_token_logprobs_backward(const vocab::Logits& logits, int dtype, int64
                                    double temperature, const float* logprob_grad, const float* entropy_grad,
                                    const float* entropy, const float* stats, void* grad, hipStream_t s) {
   using namespace scores;
-  const BackArgs a{logits, tokens, static_cast<float>(kLog2e / temperature),
+  BackArgs a{logits, 0, tokens, static_cast<float>(kLog2e / temperature),
                    static_cast<float>(1.0 / temperature), logprob_grad, entropy_grad, entropy, stats, grad};
   const int part = kThreads * kBackRuns * (dtype == QSTE_F32 ? 4 : 8);
   const int parts = ceil_div(logits.vocab, part);
-  const int64_t blocks = rows * parts;
-  if (blocks > INT32_MAX) return QSTE_E_SHAPE;
-  const dim3 grid(static_cast<unsigned>(blocks));
-  if (dtype == QSTE_F32)
-    backward_kernel<QSTE_F32><<<grid, kThreads, 0, s>>>(a, parts);
-  else if (dtype == QSTE_F16)
-    backward_kernel<QSTE_F16><<<grid, kThreads, 0, s>>>(a, parts);
-  else
-    backward_kernel<QSTE_BF16><<<grid, kThreads, 0, s>>>(a, parts);
-  return static_cast<int>(hipGetLastError());
+  return launch_rows(rows, parts, kThreads, [&](int64_t first, unsigned blocks) {
+    a.first_row = first;
+    if (dtype == QSTE_F32)
+      backward_kernel<QSTE_F32><<<blocks, kThreads, 0, s>>>(a, parts);
+    else if (dtype == QSTE_F16)
+      backward_kernel<QSTE_F16><<<blocks, kThreads, 0, s>>>(a, parts);
+    else
+      backward_kernel<QSTE_BF16><<<blocks, kThreads, 0, s>>>(a, parts);
+  });
 }
 
 }  // namespace qste

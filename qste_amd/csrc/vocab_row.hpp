@@ -259,6 +259,18 @@ __device__ __forceinline__ int before_line(const typename Elem<DT>::T* out) {
   return static_cast<int>((128 - reinterpret_cast<uintptr_t>(out) % 128) % 128) / size;
 }
 
+// A grid has less than 2^32 threads: `launch(first, blocks)` for as many rows at a
+// time as fit, from row `first` on, with `groups` workgroups of `threads` for each
+template <class F>
+int launch_rows(int64_t rows, int64_t groups, int threads, F&& launch) {
+  const int64_t most = UINT32_MAX / threads / groups;
+  for (int64_t first = 0; first < rows; first += most) {
+    launch(first, static_cast<unsigned>((rows - first < most ? rows - first : most) * groups));
+    if (int rc = static_cast<int>(hipGetLastError())) return rc;
+  }
+  return 0;
+}
+
 // the 16-byte runs that a row of `vocab` columns has
 inline int64_t runs_of(int64_t vocab, int dtype) { return vocab / (dtype == QSTE_F32 ? 4 : 8); }
 

@@ -154,3 +154,88 @@ def test_a_masked_student_against_a_list_without_mass(vocab):
             # a flat student has all but 2 / vocab of its mass outside the list
             near(got[2:], torch.tensor([-math.log1p(-2 / vocab) if tail else 0.0]), LOG)
         assert not grad[:2].any() and grad.isfinite().all()
+
+
+# ---------------------------------------------------------------------------
+# more rows than one launch has workgroups for (2^32 threads of 256 a row)
+# ---------------------------------------------------------------------------
+
+
+def repeated(rows, want, got):
+    """Every ``len(want)`` rows of ``got`` are ``want``."""
+
+    n = len(want)
+    whole = rows // n * n
+    assert torch.equal(got[:whole].view(rows // n, n, *want.shape[1:]), want.expand(rows // n, *want.shape))
+    assert torch.equal(got[whole:], want[: rows - whole])
+
+
+@pytest.mark.parametrize("rows", [(1 << 24) - 1, 1 << 24, (1 << 24) + 21])
+def test_scores_of_many_rows(rows):
+    """Every row as the same ones alone, in both directions."""
+
+    import qste_amd as qste
+
+    n, vocab = 11, 8
+    g = torch.Generator(device=DEV).manual_seed(1)
+    base = torch.randn(n, vocab, generator=g, device=DEV, dtype=torch.bfloat16)
+    marks = torch.randint(-1, vocab, (n,), generator=g, device=DEV)
+    logits = base.repeat(-(-rows // n), 1)[:rows].requires_grad_(True)
+    tokens = marks.repeat(-(-rows // n))[:rows]
+    print(f"scores of {rows} rows", flush=True)
+    few = base.clone().requires_grad_(True)
+    want, got = (qste.nn.token_logprobs(x, t, top=2) for x, t in ((few, marks), (logits, tokens)))
+    for a, b in zip(want, got):
+        repeated(rows, a.detach(), b.detach())
+    ones = torch.ones(rows, device=DEV)
+    want, = torch.autograd.grad((want.logprobs, want.entropy), few, (ones[:n], ones[:n]))
+    got, = torch.autograd.grad((got.logprobs, got.entropy), logits, (ones, ones))
+    repeated(rows, want, got)
+
+
+@pytest.mark.parametrize("rows", [(1 << 24) - 1, 1 << 24, (1 << 24) + 21])
+def test_distillation_of_many_rows(rows):
+    import qste_amd as qste
+
+    n, vocab = 11, 8
+    g = torch.Generator(device=DEV).manual_seed(2)
+    base = torch.randn(n, vocab, generator=g, device=DEV, dtype=torch.bfloat16)
+    entries = torch.stack([torch.arange(n, device=DEV) % 5, torch.arange(n, device=DEV) % 3 + 5], 1)
+    entries[4] = -1
+    values = torch.log_softmax(torch.randn(n, 2, generator=g, device=DEV), 1) - 0.1
+    logits = base.repeat(-(-rows // n), 1)[:rows].requires_grad_(True)
+    tokens, mass = (t.repeat(-(-rows // n), 1)[:rows] for t in (entries, values))
+    print(f"distillation of {rows} rows", flush=True)
+    few = base.clone().requires_grad_(True)
+    want = qste.nn.distillation_loss(few, entries, values, tail=True)
+    got = qste.nn.distillation_loss(logits, tokens, mass, tail=True)
+    repeated(rows, want.detach(), got.detach())
+    ones = torch.ones(rows, device=DEV)
+    a, = torch.autograd.grad(want, few, ones[:n])
+    b, = torch.autograd.grad(got, logits, ones)
+    repeated(rows, a, b)
+    losses, grad = qste.nn.distillation_loss_and_grad(logits.detach(), tokens, mass, tail=True)
+    # a row's sums are ordered by where its gradient lies in a line of 128 bytes: as alone in the same eight places
+    want, a = qste.nn.distillation_loss_and_grad(*(t.repeat(8, 1) for t in (base, entries, values)), tail=True)
+    repeated(rows, want, losses)
+    repeated(rows, a, grad)
+
+
+def test_many_rows_in_parts():
+    """Two parts a row, one physical row read for all: the parts pass the limit before the rows do."""
+
+    import qste_amd as qste
+
+    rows, vocab = (1 << 23) + 5, 51208
+    g = torch.Generator(device=DEV).manual_seed(3)
+    row = torch.randn(vocab, generator=g, device=DEV, dtype=torch.bfloat16)
+    tokens = torch.arange(rows, device=DEV) % 997 - 1
+    print(f"parts of {rows} rows", flush=True)
+    want = qste.nn.token_logprobs(row.expand(997 + 512, vocab), tokens[: 997 + 512], top=1)
+    got = qste.nn.token_logprobs(row.expand(rows, vocab), tokens, top=1)
+    for a, b in zip(want, got):
+        repeated(rows, a[:997], b)
+    values = torch.zeros(rows, 1, device=DEV)
+    want = qste.nn.distillation_loss(row.expand(997 + 512, vocab), tokens[: 997 + 512, None], values[: 997 + 512])
+    got = qste.nn.distillation_loss(row.expand(rows, vocab), tokens[:, None], values)
+    repeated(rows, want[:997], got)
