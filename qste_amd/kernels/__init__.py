@@ -961,7 +961,7 @@ def _row_tokens(tokens: Tensor, shape, what: str) -> Tensor:
     if tokens.shape != shape:
         raise ValueError(f"{what} have shape {tuple(tokens.shape)}, expected {tuple(shape)}")
     if tokens.dtype != torch.int64:
-        if tokens.dtype not in (torch.int32, torch.int16, torch.uint8):
+        if tokens.dtype not in (torch.int32, torch.int16, torch.int8, torch.uint8):
             raise TypeError(f"{what} must be integers, got {tokens.dtype}")
         tokens = tokens.to(torch.int64)
     return tokens.contiguous()
