@@ -524,8 +524,9 @@ int qste_token_logprobs_backward(const void* logits, int dtype, int64_t outer, i
 
 /* Distillation from a teacher's top tokens.  Per row the teacher's log
  * probabilities top_logprobs fp32 [rows, k] of top_tokens int64 [rows, k] (k 1
- * .. QSTE_MAX_ENTRIES; a negative token is no entry, a token listed twice
- * counts with the sum), taken at the same temperature.
+ * .. QSTE_MAX_ENTRIES; a negative token is no entry), taken at the same
+ * temperature.  A token listed twice has a term for each entry in the loss; its
+ * q in the gradient is their sum.
  *   tail = 0: q = softmax(top_logprobs), q_r = 0
  *   tail = 1: q = exp(top_logprobs), q_r = max(0, 1 - sum q) against the
  *             student's mass p_r outside the list (left out when p_r < 2^-100)
@@ -533,9 +534,10 @@ int qste_token_logprobs_backward(const void* logits, int dtype, int64_t outer, i
  * A row without entries (tail = 0: without one of mass) has the loss 0 and no
  * gradient, whatever its logits hold; one with a token >= vocab a NaN loss and
  * gradient; one of only -inf logits the loss inf and no gradient.  stats fp32
- * [rows, QSTE_DISTILL_STATS], or NULL, is what qste_distill_backward reads.  With grad ([rows, vocab] in dtype, 16-byte
- * aligned; NULL: the loss alone) the logits' gradient for the row weights
- * loss_grad fp32 [rows] is written by the same pass:
+ * [rows, QSTE_DISTILL_STATS], or NULL, is what qste_distill_backward reads.
+ * With grad ([rows, vocab] in dtype, 16-byte aligned; NULL: the loss alone) the
+ * logits' gradient for the row weights loss_grad fp32 [rows] is written by the
+ * same pass:
  *   loss_grad temperature (s p - q) for a listed token, loss_grad temperature
  *   p (s - q_r / p_r) for another, s = sum q + q_r; zeros where loss_grad is 0.
  * Needs qste_distill_workspace_bytes(outer * inner, vocab, dtype, grad != NULL)

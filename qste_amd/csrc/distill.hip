@@ -12,9 +12,10 @@
 //   dz_j = g T (s p_j - q_j) for a listed token, g T p_j (s - q_r / p_r) for any
 //          other; s = sum q + q_r
 // Terms with q = 0 are 0; a tail in which the student has no mass (p_r below
-// 2^-100, where q_r / p_r nears the end of fp32) is left out (q_r = 0).  p_r is
-// summed over the tokens outside the list, not taken as what the listed ones
-// leave of 1: a trained student leaves little.
+// 2^-100, where q_r / p_r nears the end of fp32) is left out (q_r = 0); against
+// a row of only -inf the loss of any entry is infinite.  p_r is summed over the
+// tokens outside the list, not taken as what the listed ones leave of 1: a
+// trained student leaves little.
 #include "vocab_row.hpp"
 
 namespace qste {
@@ -122,8 +123,7 @@ __device__ __forceinline__ Teacher load_entries(const Args& a, int64_t r, const 
   top = a.tail ? 0.0f : fold_max(top);
   if (top == -INFINITY) top = 0.0f;
   double total = 0.0;
-  // not unrolled: a second entry's registers would push those of a long row into memory (4096 rows of 50257 bf16
-  // logits: the loss 120 us, 106 so)
+  // unrolled, the loss of 4096 rows of 50257 bf16 logits took 120 us where it took 106 so
 #pragma unroll 1
   for (int k = lane; k < a.k; k += kWave) total += exp_exactly(t.log_q[k] - top);
   total = wave_sum(total);
@@ -166,7 +166,9 @@ __device__ __forceinline__ bool mark_listed(const Args& a, const R& row, const E
 }
 
 // A thread's sums of the exponentials over the columns, all and outside the
-// list, for the runs (and single columns) that mark_listed marked
+// list, for the runs (and single columns) that mark_listed marked.  The two
+// branches' last additions to `sum` and `outside` are merged by the compiler
+// behind an address, so both are in scratch memory: see the forward kernel.
 template <class R>
 __device__ __forceinline__ void sums(const Args& a, const R& row, const Entries& t, int from, int to,
                                      const Exponent& ex, float& sum, float& outside) {
@@ -353,13 +355,20 @@ __device__ __forceinline__ void write_listed(const Args& a, const Entries& t, bo
 // ---------------------------------------------------------------------------
 // the loss, and with `grad` the gradient too: one workgroup a row
 //
-// Bound by reading the logits, and with the gradient by writing it: the row
-// stays in registers from its one read to the gradient.  The first wave reads
-// the entries while all waves' loads are on their way; by itself before the
-// row this took 163 us where it takes 102, the loss of 4096 rows of 50257 bf16
-// logits against 64 tokens and the tail (4.0 TB/s; a plain read reaches 6.2.
-// Without the tail 97: its sum takes the rest).  With the gradient 159 us (5.2
-// TB/s; a copy reaches 4.9).
+// Bound by reading the logits, and with the gradient by writing it: the row is
+// held from its one read to the gradient.  The first wave reads the entries
+// while all waves' loads are on their way; by itself before the row this took
+// 163 us where it takes 102, the loss of 4096 rows of 50257 bf16 logits against
+// 64 tokens and the tail (4.0 TB/s; a plain read reaches 6.2.  Without the tail
+// 97: its sum takes the rest).  With the gradient 159 us (5.2 TB/s; a copy
+// reaches 4.9).
+//
+// Not all that a thread has is in registers.  Its two sums are 12 bytes of
+// scratch in every instance and in the parts' kernel, stored once a run; with 25
+// runs a thread some registers are spilled too: 16 bytes in all for 16-bit rows
+// in 256 threads, 32 in 512, 44 (fp32) and 60 with runs in LDS as well.  How much
+// of the 102 us that is has not been measured; the token scores' kernel, which
+// has no scratch, takes 74 for such rows.
 // ---------------------------------------------------------------------------
 
 template <int DT, int THREADS, int HELD, int KEPT, int WAVES_A_SIMD>
@@ -493,11 +502,12 @@ __global__ __launch_bounds__(kThreads) void backward_kernel(Args a) {
   write_listed<DT, kThreads>(a, t, st[5] != 0.0f, r, ex, per_p * weight, per_q, from, to);
 }
 
-// Up to 25 runs a thread stay in registers with four waves on a SIMD, so a row
-// of up to kLong runs has one workgroup of 256 threads, four to a CU.  The
-// gradient wants a longer row held too: 512 threads hold up to kFewWide runs
-// with 16 a thread, kWide with 25, two workgroups to a CU, and with seven more a
-// thread in LDS (56 KiB and the list's bits: two still fit) kWidest.  Against
+// Up to 25 runs a thread are held with four waves on a SIMD (with a few
+// registers spilled), so a row of up to kLong runs has one workgroup of 256
+// threads, four to a CU.  The gradient wants a longer row held too: 512 threads
+// hold up to kFewWide runs with 16 a thread, kWide with 25, two workgroups to a
+// CU, and with seven more a thread in LDS (56 KiB and the list's bits: two still
+// fit) kWidest.  Against
 // three launches that read the row twice (in parts, the join, the gradient):
 // 2046 rows of 50257 fp32 logits 209 -> 166 us, 2048 of 65536 bf16 149 -> 112
 // (119 with 25 runs a thread), 8192 of 131072 1072 -> 821; rows of kWidest gain
@@ -523,7 +533,8 @@ struct Plan {
 
 Plan forward_plan(int64_t rows, int64_t vocab, int dtype, bool with_grad) {
   const int64_t runs = runs_of(vocab, dtype), e = dtype == QSTE_F32 ? 4 : 8;
-  if (runs <= kLong || (runs <= kFewWide && rows <= kFew) || (with_grad && (runs <= kWide || (runs <= kWidest && rows >= kWidestRows)))) return {1, 0};
+  const bool held_for_grad = runs <= kWide || (runs <= kWidest && rows >= kWidestRows);
+  if (runs <= kLong || (runs <= kFewWide && rows <= kFew) || (with_grad && held_for_grad)) return {1, 0};
   const int64_t parts = (runs + kLong - 1) / kLong;
   if (parts > kMaxParts) return {0, 0};
   // runs > parts * parts: no part is empty

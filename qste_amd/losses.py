@@ -3,8 +3,9 @@
 Both work on a model's logits, ``[..., vocab]`` in fp32, fp16 or bf16 on the GPU,
 in any layout whose columns are adjacent (``logits[:, :-1]`` is read in place).
 Softmax, sums and losses are fp32; a gradient is rounded once, to the
-logits' dtype.  Forward-mode differentiation is refused.  The kernels are ``csrc/scores.hip`` and ``csrc/distill.hip``; the
-reference ends at the logits and has no counterparts.
+logits' dtype.  Forward-mode differentiation is refused.  The kernels are
+``csrc/scores.hip`` and ``csrc/distill.hip``; the reference ends at the logits and
+has no counterparts.
 
     with torch.no_grad():                    # the teacher, and what it thinks likely
         scores = qste.nn.token_logprobs(teacher(ids), top=64)
@@ -78,7 +79,8 @@ def token_logprobs(logits: Tensor, tokens: Optional[Tensor] = None, *, top: int 
     ``tokens`` are integers of the logits' leading shape, or None.  A negative
     token marks a position that is not scored (padding): logprob and entropy
     0, top tokens -1 with -inf, no gradient, its logits not read.  A token past
-    the vocabulary gives NaN.  Equal logits are listed by the lowest token; ``top`` is
+    the vocabulary gives a NaN log probability, and NaN where a gradient flows back
+    through it.  Equal logits are listed by the lowest token; ``top`` is
     at most 128.  Differentiable in ``logprobs`` and ``entropy``; the top
     log probabilities carry no gradient.
     """
@@ -125,7 +127,9 @@ def distillation_loss(logits: Tensor, top_tokens: Tensor, top_logprobs: Tensor, 
     ``tail`` the teacher is renormalised over its list (any logits, already over the
     temperature, will do); with it the mass that the list leaves is one more
     outcome, set against all the student's mass outside the list.  A negative
-    token is no entry; a position with none has the loss 0 and no gradient.
+    token is no entry; a position with none has the loss 0 and no gradient.  A
+    token listed twice has a term for each entry in the loss, and their sum as its
+    probability in the gradient.
     """
 
     _no_tangent("distillation_loss", logits, top_logprobs)
@@ -145,7 +149,8 @@ def distillation_loss_and_grad(logits: Tensor, top_tokens: Tensor, top_logprobs:
         losses, grad = distillation_loss_and_grad(logits, top_tokens, top_logprobs, loss_grad=mask / mask.sum())
         logits.backward(grad)
 
-    Positions of weight 0 get zeros, whatever their logits hold.
+    Positions of weight 0 get zeros, whatever their logits hold.  Neither result
+    carries a graph, also where ``logits`` or ``loss_grad`` require gradients.
     """
 
     _no_tangent("distillation_loss_and_grad", logits, top_logprobs)
