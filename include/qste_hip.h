@@ -427,6 +427,75 @@ int qste_swiglu_backward_sums_into(const void* grad, const void* gate, const voi
                                    const float* offset_gate, const float* offset_up, float* sums, int64_t rows,
                                    int64_t cols, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- 8-bit blocks -------------------------------------------------------- */
+
+/* x [rows, cols] in `dtype` as 8-bit blocks: 32 consecutive columns of a row
+ * (the last block of a row may be shorter) share codes[row][block], uint8
+ * [rows, ceil(cols / 32)], the biased fp32 exponent of their largest magnitude
+ * but at least 7; payload int8 [rows, cols] holds clamp(rint(x * 2^(133 -
+ * code)), -127, 127).  An infinity or a NaN makes the block's code 255 and its
+ * payload 0.  No counterpart in the reference. */
+int qste_quantize_blocks(const void* x, int dtype, int8_t* payload, uint8_t* codes, int64_t rows, int64_t cols,
+                         void* stream);
+
+/* What blocks stand for, payload * 2^(code - 133), rounded to `dtype` (exact for
+ * the dtype they were made from); NaN for code 255.  No counterpart in the
+ * reference. */
+int qste_dequantize_blocks(const int8_t* payload, const uint8_t* codes, void* x, int dtype, int64_t rows, int64_t cols,
+                           void* stream);
+
+/* qste_swiglu_forward that also writes gate and up as 8-bit blocks
+ * (qste_quantize_blocks of them), which is what the two entries below read.  No
+ * counterpart in the reference (see qste_swiglu_forward). */
+int qste_swiglu_forward_blocks(const void* gate, const void* up, int dtype, void* out, uint8_t* packed, float* offset,
+                               float* scale, int8_t* gate_payload, uint8_t* gate_codes, int8_t* up_payload,
+                               uint8_t* up_codes, int64_t rows, int64_t cols, void* stream);
+
+/* qste_swiglu_backward with the gate and up that 8-bit blocks stand for. */
+int qste_swiglu_backward_blocks(const void* grad, int dtype, const int8_t* gate_payload, const uint8_t* gate_codes,
+                                const int8_t* up_payload, const uint8_t* up_codes, void* grad_gate, void* grad_up,
+                                int64_t rows, int64_t cols, void* stream);
+
+/* qste_swiglu_backward_sums with the gate and up that 8-bit blocks stand for.
+ * ld: elements between the gradients' rows, cols, or with 16-bit dtypes and cols
+ * a multiple of 8 any larger multiple of 8 (both gradients side by side in one
+ * [rows, 2 cols] tensor: grad_up = grad_gate + cols, ld = 2 cols).  The same
+ * workspace as that entry. */
+int qste_swiglu_backward_blocks_sums(const void* grad, int dtype, const int8_t* gate_payload,
+                                     const uint8_t* gate_codes, const int8_t* up_payload, const uint8_t* up_codes,
+                                     void* grad_gate, void* grad_up, int64_t ld, const float* offset_gate,
+                                     const float* offset_up, float* sums, int64_t rows, int64_t cols, void* workspace,
+                                     size_t workspace_bytes, void* stream);
+
+/* ---- the gated feed-forward block ----------------------------------------- */
+
+/* out [m, rows] = silu(g) * u with g = (x . sign(gate)^T) * gate_scale +
+ * gate_bias and u likewise of up: two binary layers of one input x [m, cols] and
+ * the gate between them, g and u rounded to `dtype` and the gate as
+ * qste_swiglu_forward rounds it.  Signs are packed [rows, ceil(cols / 8)],
+ * scales fp32 [rows], biases fp32 [rows] or NULL.
+ * What a backward needs is written where asked for: g and u as they are
+ * (gate_out and up_out, both or neither) and as 8-bit blocks (the four blocks'
+ * pointers, all or none).
+ * One launch (two where K is cut into ranges) up to 64 rows of bf16 / fp16 and 21
+ * of fp32 with nothing kept, and on the 16-bit tiles where cols is a multiple
+ * of 64 and rows of 8; elsewhere the two products (qste_packed_linear_affine_ws)
+ * and the gate one after the other, with g and u in the workspace.  Sums are
+ * fp32, in an order that may differ from the two products' called alone: g and u
+ * may then differ by an ulp.  x, the signs, out, gate_out and up_out start at
+ * 16-byte steps and payloads at 8-byte steps (QSTE_E_ALIGN otherwise).
+ * keep: bit 0 for gate_out and up_out, bit 1 for the blocks.  No counterpart in
+ * the reference. */
+size_t qste_gated_workspace_bytes(int64_t m, int64_t rows, int64_t cols, int dtype, int keep);
+int qste_gated(const void* x, int dtype, const uint8_t* gate, const float* gate_scale, const float* gate_bias,
+               const uint8_t* up, const float* up_scale, const float* up_bias, void* out, void* gate_out, void* up_out,
+               int8_t* gate_payload, uint8_t* gate_codes, int8_t* up_payload, uint8_t* up_codes, int64_t m,
+               int64_t rows, int64_t cols, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Which way qste_gated takes: 0 the products one after the other, 1 the kernel for
+ * few rows, 2 the tiles (a query, for tests and tuning). */
+int qste_gated_route(int64_t m, int64_t rows, int64_t cols, int dtype, int keep);
+
 /* ---- the learned row scale (src/qste/surface.py:84-85) ------------------- */
 
 /* scale = clamp(exp(log_scale), lo, hi) over n rows, and exp_value = the

@@ -1,6 +1,7 @@
 // extern "C" entry points declared in include/qste_hip.h: argument checks,
 // workspace carving and kernel dispatch.  Nothing here allocates or
 // synchronizes; every launch goes on the caller's stream.
+#include "blocks.hpp"
 #include "common.hpp"
 #include "prep.hpp"
 #include "vocab_row.hpp"
@@ -71,6 +72,25 @@ int launch_row_scale(const void*, int, void*, void*, int64_t, float, float, hipS
 size_t swiglu_backward_sums_workspace(int64_t, int64_t);
 int launch_swiglu_backward_sums(const void*, const void*, const void*, int, void*, void*, const float*, const float*,
                                 int64_t, int64_t, float*, float*, hipStream_t, int64_t);
+int launch_quantize_blocks(const void*, int, int8_t*, uint8_t*, int64_t, int64_t, hipStream_t);
+int launch_dequantize_blocks(const int8_t*, const uint8_t*, void*, int, int64_t, int64_t, hipStream_t);
+int launch_swiglu_forward_blocks(const void*, const void*, int, void*, uint8_t*, float*, float*, int8_t*, uint8_t*,
+                                 int8_t*, uint8_t*, int64_t, int64_t, hipStream_t);
+int launch_swiglu_backward_blocks(const void*, int, const int8_t*, const uint8_t*, const int8_t*, const uint8_t*, void*,
+                                  void*, int64_t, int64_t, hipStream_t);
+int launch_swiglu_backward_blocks_sums(const void*, int, const int8_t*, const uint8_t*, const int8_t*, const uint8_t*,
+                                       void*, void*, const float*, const float*, int64_t, int64_t, float*, float*,
+                                       hipStream_t, int64_t);
+double gemv_gated_us(int64_t, int64_t, int64_t, int);
+size_t gemv_gated_workspace(int64_t, int64_t, int64_t, int);
+int gemv_gated(const void*, int, const uint8_t*, const float*, const float*, const uint8_t*, const float*,
+               const float*, void*, int64_t, int64_t, int64_t, void*, hipStream_t);
+bool mfma_gated_ok(int64_t, int64_t, int64_t, int);
+double mfma_gated_us(int64_t, int64_t, int64_t);
+size_t mfma_gated_workspace(int64_t, int64_t, int64_t);
+int mfma_gated(const void*, int, const uint8_t*, const float*, const float*, const uint8_t*, const float*,
+               const float*, void*, void*, void*, const blocks::Blocks&, const blocks::Blocks&, int64_t, int64_t,
+               int64_t, void*, hipStream_t);
 int launch_step_finish(float* const*, const int64_t*, int, const int64_t* const*, int, float, float, int64_t*,
                        hipStream_t);
 int launch_row_scale_backward(const void*, const void*, int, void*, int64_t, float, float, hipStream_t);
@@ -719,6 +739,149 @@ int qste_swiglu_backward_sums_into(const void* grad, const void* gate, const voi
   uint16_t* out = static_cast<uint16_t*>(grads);
   return launch_swiglu_backward_sums(grad, gate, up, dtype, out, out + cols, offset_gate, offset_up, rows, cols, sums,
                                      static_cast<float*>(workspace), s, 2 * cols);
+}
+
+int qste_quantize_blocks(const void* x, int dtype, int8_t* payload, uint8_t* codes, int64_t rows, int64_t cols,
+                         void* stream) {
+  if (!dtype_ok(dtype)) return QSTE_E_DTYPE;
+  if (rows < 0 || cols < 0) return QSTE_E_SHAPE;
+  if (rows * cols == 0) return 0;
+  if (!x || !payload || !codes) return QSTE_E_NULL;
+  return launch_quantize_blocks(x, dtype, payload, codes, rows, cols, as_stream(stream));
+}
+
+int qste_dequantize_blocks(const int8_t* payload, const uint8_t* codes, void* x, int dtype, int64_t rows, int64_t cols,
+                           void* stream) {
+  if (!dtype_ok(dtype)) return QSTE_E_DTYPE;
+  if (rows < 0 || cols < 0) return QSTE_E_SHAPE;
+  if (rows * cols == 0) return 0;
+  if (!x || !payload || !codes) return QSTE_E_NULL;
+  return launch_dequantize_blocks(payload, codes, x, dtype, rows, cols, as_stream(stream));
+}
+
+int qste_swiglu_forward_blocks(const void* gate, const void* up, int dtype, void* out, uint8_t* packed, float* offset,
+                               float* scale, int8_t* gate_payload, uint8_t* gate_codes, int8_t* up_payload,
+                               uint8_t* up_codes, int64_t rows, int64_t cols, void* stream) {
+  if (!dtype_ok(dtype)) return QSTE_E_DTYPE;
+  if (rows < 0 || cols < 0) return QSTE_E_SHAPE;
+  if (rows * cols == 0) return 0;
+  if (!gate || !up || !out || !gate_payload || !gate_codes || !up_payload || !up_codes) return QSTE_E_NULL;
+  if (packed && (!offset || !scale)) return QSTE_E_NULL;
+  return launch_swiglu_forward_blocks(gate, up, dtype, out, packed, offset, scale, gate_payload, gate_codes, up_payload,
+                                      up_codes, rows, cols, as_stream(stream));
+}
+
+int qste_swiglu_backward_blocks(const void* grad, int dtype, const int8_t* gate_payload, const uint8_t* gate_codes,
+                                const int8_t* up_payload, const uint8_t* up_codes, void* grad_gate, void* grad_up,
+                                int64_t rows, int64_t cols, void* stream) {
+  if (!dtype_ok(dtype)) return QSTE_E_DTYPE;
+  if (rows < 0 || cols < 0) return QSTE_E_SHAPE;
+  if (rows * cols == 0) return 0;
+  if (!grad || !gate_payload || !gate_codes || !up_payload || !up_codes || !grad_gate || !grad_up) return QSTE_E_NULL;
+  return launch_swiglu_backward_blocks(grad, dtype, gate_payload, gate_codes, up_payload, up_codes, grad_gate, grad_up,
+                                       rows, cols, as_stream(stream));
+}
+
+int qste_swiglu_backward_blocks_sums(const void* grad, int dtype, const int8_t* gate_payload,
+                                     const uint8_t* gate_codes, const int8_t* up_payload, const uint8_t* up_codes,
+                                     void* grad_gate, void* grad_up, int64_t ld, const float* offset_gate,
+                                     const float* offset_up, float* sums, int64_t rows, int64_t cols, void* workspace,
+                                     size_t workspace_bytes, void* stream) {
+  if (!dtype_ok(dtype)) return QSTE_E_DTYPE;
+  if (rows < 0 || cols < 0 || ld < cols) return QSTE_E_SHAPE;
+  if (cols == 0) return 0;
+  if (!sums) return QSTE_E_NULL;
+  hipStream_t s = as_stream(stream);
+  if (rows == 0) return fill_zero(sums, 2 * cols, s);
+  if (!grad || !gate_payload || !gate_codes || !up_payload || !up_codes || !grad_gate || !grad_up || !offset_gate ||
+      !offset_up)
+    return QSTE_E_NULL;
+  if (!workspace || workspace_bytes < swiglu_backward_sums_workspace(rows, cols)) return QSTE_E_WORKSPACE;
+  return launch_swiglu_backward_blocks_sums(grad, dtype, gate_payload, gate_codes, up_payload, up_codes, grad_gate,
+                                            grad_up, offset_gate, offset_up, rows, cols, sums,
+                                            static_cast<float*>(workspace), s, ld);
+}
+
+namespace {
+
+enum GatedRoute { kOneByOne = 0, kSkinny = 1, kTiles = 2 };
+
+// How a gated block runs.  Few rows with nothing kept take the kernel for them
+// where its estimate is the lower one; what neither that nor the tiles take runs
+// layer by layer.
+GatedRoute gated_route(int64_t m, int64_t rows, int64_t cols, int dtype, int keep) {
+  if (m <= 0 || rows <= 0 || cols <= 0) return kOneByOne;
+  const double skinny = keep ? -1.0 : gemv_gated_us(m, rows, cols, dtype);
+  if (mfma_gated_ok(m, rows, cols, dtype)) {
+    const double tiles = mfma_gated_us(m <= 16 ? m : (m + 15) / 16 * 16, rows, cols);
+    return skinny >= 0.0 && skinny < tiles ? kSkinny : kTiles;
+  }
+  return skinny >= 0.0 ? kSkinny : kOneByOne;
+}
+
+bool aligned_to(const void* p, uintptr_t step) { return (reinterpret_cast<uintptr_t>(p) & (step - 1)) == 0; }
+
+}  // namespace
+
+int qste_gated_route(int64_t m, int64_t rows, int64_t cols, int dtype, int keep) {
+  return dtype_ok(dtype) ? gated_route(m, rows, cols, dtype, keep) : QSTE_E_DTYPE;
+}
+
+size_t qste_gated_workspace_bytes(int64_t m, int64_t rows, int64_t cols, int dtype, int keep) {
+  if (!dtype_ok(dtype) || m <= 0 || rows <= 0 || cols <= 0) return 0;
+  switch (gated_route(m, rows, cols, dtype, keep)) {
+    case kSkinny: return gemv_gated_workspace(m, rows, cols, dtype);
+    case kTiles: return mfma_gated_workspace(m, rows, cols);
+    default:
+      return (keep & 1 ? 0 : 2 * align_up(static_cast<size_t>(m * rows) * elem_bytes(dtype))) +
+             qste_packed_linear_affine_workspace_bytes(m, rows, cols, dtype);
+  }
+}
+
+int qste_gated(const void* x, int dtype, const uint8_t* gate, const float* gate_scale, const float* gate_bias,
+               const uint8_t* up, const float* up_scale, const float* up_bias, void* out, void* gate_out, void* up_out,
+               int8_t* gate_payload, uint8_t* gate_codes, int8_t* up_payload, uint8_t* up_codes, int64_t m,
+               int64_t rows, int64_t cols, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!dtype_ok(dtype)) return QSTE_E_DTYPE;
+  if (m < 0 || rows < 0 || cols < 0) return QSTE_E_SHAPE;
+  if (m * rows == 0) return 0;
+  if (!out || !gate_scale || !up_scale || (cols > 0 && (!x || !gate || !up))) return QSTE_E_NULL;
+  const bool blocks8 = gate_payload || gate_codes || up_payload || up_codes;
+  if (!gate_out != !up_out || (blocks8 && !(gate_payload && gate_codes && up_payload && up_codes))) return QSTE_E_NULL;
+  if (!aligned_to(x, 16) || !aligned_to(gate, 16) || !aligned_to(up, 16) || !aligned_to(out, 16) ||
+      !aligned_to(gate_out, 16) || !aligned_to(up_out, 16) || !aligned_to(gate_payload, 8) || !aligned_to(up_payload, 8))
+    return QSTE_E_ALIGN;
+  const int keep = (gate_out ? 1 : 0) | (blocks8 ? 2 : 0);
+  const size_t need = qste_gated_workspace_bytes(m, rows, cols, dtype, keep);
+  if (need && (!workspace || workspace_bytes < need)) return QSTE_E_WORKSPACE;
+  if (need && !aligned_to(workspace, 16)) return QSTE_E_ALIGN;
+  hipStream_t s = as_stream(stream);
+  switch (gated_route(m, rows, cols, dtype, keep)) {
+    case kSkinny:
+      return gemv_gated(x, dtype, gate, gate_scale, gate_bias, up, up_scale, up_bias, out, m, rows, cols, workspace, s);
+    case kTiles:
+      return mfma_gated(x, dtype, gate, gate_scale, gate_bias, up, up_scale, up_bias, out, gate_out, up_out,
+                        blocks::Blocks{gate_payload, gate_codes}, blocks::Blocks{up_payload, up_codes}, m, rows, cols,
+                        workspace, s);
+    default: break;
+  }
+  char* ws = static_cast<char*>(workspace);
+  const size_t hidden = align_up(static_cast<size_t>(m * rows) * elem_bytes(dtype));
+  size_t left = workspace_bytes;
+  if (!gate_out) {
+    gate_out = ws;
+    up_out = ws + hidden;
+    ws += 2 * hidden;
+    left -= 2 * hidden;
+  }
+  int rc = qste_packed_linear_affine_ws(x, dtype, gate, gate_scale, gate_bias, gate_out, m, rows, cols, ws, left, stream);
+  if (rc) return rc;
+  rc = qste_packed_linear_affine_ws(x, dtype, up, up_scale, up_bias, up_out, m, rows, cols, ws, left, stream);
+  if (rc) return rc;
+  if (blocks8)
+    return launch_swiglu_forward_blocks(gate_out, up_out, dtype, out, nullptr, nullptr, nullptr, gate_payload,
+                                        gate_codes, up_payload, up_codes, m, rows, s);
+  return launch_swiglu_forward(gate_out, up_out, dtype, out, nullptr, nullptr, nullptr, m, rows, s);
 }
 
 size_t qste_coordinate_update_workspace_bytes(int64_t rows, int64_t cols, int64_t block_size) {

@@ -1,0 +1,176 @@
+// 8-bit blocks: 32 values along a row share a power of two.
+//
+// For a block with largest magnitude a, code = max(biased exponent of a, 7) as
+// one byte and each value is kept as the int8 q = clamp(rint(x 2^(133 -
+// code)), -127, 127); it reads back as q 2^(code - 133).  (The Open Compute
+// Project's microscaling format MXINT8, with the smallest exponents held at 7 so
+// that a step is a normal number.)  A block that holds an infinity or a NaN has
+// code 255, q = 0, and reads back as NaN throughout.
+//
+// Why a power of two: nothing but q is rounded (x 2^k and q 2^k are exact in
+// fp32, and a value read back is exact in bf16, and in fp16 where it came from
+// fp16), a step costs a byte and no division.  The error is at most half a step,
+// 2^(code - 134), or 2^-7 of the block's largest value, and up to a step for
+// magnitudes past 127.5 / 128 of the next power of two, which are clamped: a
+// larger step for the whole block would cost all the others a bit.  A block of
+// 32 keeps a large value's step from its neighbours at one byte in 33.
+#pragma once
+
+#include "common.hpp"
+
+namespace qste {
+namespace blocks {
+
+constexpr int kBlock = 32;
+constexpr uint32_t kLeastCode = 7, kBadCode = 255;
+
+inline int64_t blocks_of(int64_t cols) { return (cols + kBlock - 1) / kBlock; }
+
+// the code of a block from the bits of its largest magnitude (a NaN's are the largest of all)
+__device__ __forceinline__ uint32_t code_of(uint32_t magnitude) {
+  const uint32_t e = magnitude >> 23;
+  return e > kLeastCode ? e : kLeastCode;
+}
+
+// 2^(133 - code); 0 for a bad block
+__device__ __forceinline__ float to_steps(uint32_t code) {
+  return __uint_as_float(code == kBadCode ? 0u : (260u - code) << 23);
+}
+
+// a step, 2^(code - 133); NaN for a bad block
+__device__ __forceinline__ float step_of(uint32_t code) {
+  return __uint_as_float(code == kBadCode ? 0x7FC00000u : (code - 6u) << 23);
+}
+
+// rint(x * to) within +-127, in the low byte of what is returned: added to 1.5 *
+// 2^23 a product rounds to a whole number, to the nearest even, whose low bits
+// are the sum's.  A bad block's are zeros: x * 0 is NaN there for the values that
+// make it bad, and the clamp takes NaN to one of its ends, so that is asked first.
+__device__ __forceinline__ uint32_t steps(float x, float to) {
+  constexpr float kMagic = 12582912.0f;
+  const float t = __builtin_amdgcn_fmed3f(fmaf(x, to, kMagic), kMagic - 127.0f, kMagic + 127.0f);
+  return to == 0.0f ? 0u : __float_as_uint(t);
+}
+
+// four low bytes to a word
+__device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  const uint32_t lo = __builtin_amdgcn_perm(b, a, 0x0C0C0400u), hi = __builtin_amdgcn_perm(d, c, 0x04000C0Cu);
+  return lo | hi;
+}
+
+// the magnitude bits of the largest of a thread's eight values
+__device__ __forceinline__ uint32_t largest(const float (&x)[8]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t u = __float_as_uint(x[i]) & 0x7FFFFFFFu;
+    m = m > u ? m : u;
+  }
+  return m;
+}
+
+// the largest over the four lanes 4j .. 4j + 3, which hold a block of 32 together
+__device__ __forceinline__ uint32_t over_four(uint32_t m) {
+  uint32_t o = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(m), 0xB1, 0xF, 0xF, false));
+  m = m > o ? m : o;  // quad_perm 1,0,3,2
+  o = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(m), 0x4E, 0xF, 0xF, false));
+  return m > o ? m : o;  // quad_perm 2,3,0,1
+}
+
+// Eight values of a block that four lanes hold: their bytes, and the block's
+// code.  All four lanes make the call, with zeros past the row's end.
+__device__ __forceinline__ uint2 quantize8(const float (&x)[8], uint32_t& code) {
+  code = code_of(over_four(largest(x)));
+  const float to = to_steps(code);
+  return make_uint2(pack4(steps(x[0], to), steps(x[1], to), steps(x[2], to), steps(x[3], to)),
+                    pack4(steps(x[4], to), steps(x[5], to), steps(x[6], to), steps(x[7], to)));
+}
+
+__device__ __forceinline__ void dequantize8(uint2 q, uint32_t code, float (&x)[8]) {
+  const float step = step_of(code);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t w = (i < 4 ? q.x : q.y) ^ 0x80808080u;
+    x[i] = (static_cast<float>((w >> (8 * (i & 3))) & 0xFFu) - 128.0f) * step;
+  }
+}
+
+__device__ __forceinline__ float dequantize1(int8_t q, uint32_t code) { return static_cast<float>(q) * step_of(code); }
+
+// Eight values of an element type at 16-byte aligned p.
+template <int DT>
+__device__ __forceinline__ void load8(const typename Elem<DT>::T* p, float (&x)[8]) {
+  const uint4 a = *reinterpret_cast<const uint4*>(p);
+  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+  if constexpr (DT == QSTE_F32) {
+    const uint4 b = *reinterpret_cast<const uint4*>(p + 4);
+    const uint32_t v[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[i] = __uint_as_float(w[i]);
+      x[4 + i] = __uint_as_float(v[i]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = DT == QSTE_BF16 ? __uint_as_float(w[i] << 16) : f16_to_f32(static_cast<uint16_t>(w[i]));
+      x[2 * i + 1] = DT == QSTE_BF16 ? __uint_as_float(w[i] & 0xFFFF0000u) : f16_to_f32(static_cast<uint16_t>(w[i] >> 16));
+    }
+  }
+}
+
+template <int DT>
+__device__ __forceinline__ void store8(typename Elem<DT>::T* p, const float (&x)[8]) {
+  if constexpr (DT == QSTE_F32) {
+    *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+    *reinterpret_cast<float4*>(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
+  } else {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (DT == QSTE_BF16)
+        w[i] = f32x2_to_bf16x2(x[2 * i], x[2 * i + 1]);
+      else
+        w[i] = static_cast<uint32_t>(f32_to_f16(x[2 * i])) | (static_cast<uint32_t>(f32_to_f16(x[2 * i + 1])) << 16);
+    }
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+// A tensor in blocks: int8 [rows, cols] and a code for every block of a row.
+struct Blocks {
+  int8_t* q;
+  uint8_t* codes;
+};
+
+// Work is handed out by quarters of blocks, eight values to a thread: quarter j
+// (of rows * per_row * 4, per_row the blocks of a row) as its row and first
+// column.  With cols a multiple of 32 the quarters lie end to end.
+struct Quarter {
+  int64_t row, block;  // block: its index in the codes
+  int col;
+  __device__ __forceinline__ Quarter(int64_t j, int64_t cols, int64_t per_row) {
+    block = j >> 2;
+    if (cols % kBlock == 0) {
+      row = 0;  // one long row
+      col = 0;
+      at_ = 8 * j;
+      whole_ = true;
+    } else {
+      // 32-bit where it reaches: a 64-bit division is several times as long
+      row = (block >> 32) == 0 ? static_cast<int64_t>(static_cast<uint32_t>(block) / static_cast<uint32_t>(per_row)) : block / per_row;
+      col = static_cast<int>((block - row * per_row) * kBlock + 8 * (j & 3));
+      at_ = row * cols + col;
+      whole_ = col < cols;
+    }
+  }
+  __device__ __forceinline__ int64_t at() const { return at_; }     // its first value in the tensor
+  __device__ __forceinline__ bool there() const { return whole_; }  // false past the row's end
+
+ private:
+  int64_t at_;
+  bool whole_;
+};
+
+}  // namespace blocks
+}  // namespace qste

@@ -25,7 +25,9 @@
 #include <mutex>
 #include <vector>
 
+#include "blocks.hpp"
 #include "common.hpp"
+#include "swiglu.hpp"
 
 namespace qste {
 namespace mfma {
@@ -46,7 +48,8 @@ enum { B_BITS_ALONG_K = 0, B_BITS_ALONG_N = 1, B_BITS_ALONG_K_SCALED = 2 };
 // forward's scale and bias, stored as fp32 (the fp32 products, whose dense
 // operand arrives as three bf16 limbs along K).  EPI_EVIDENCE_F32: the
 // evidence of such an operand.  Both undo the limbs' power of two per row.
-enum { EPI_FORWARD = 0, EPI_PLAIN = 1, EPI_EVIDENCE = 2, EPI_PARTIAL = 3, EPI_FORWARD_F32 = 4, EPI_EVIDENCE_F32 = 5 };
+// EPI_GATED: two forwards of one input, g and u, that end in silu(g) * u (PairParams).
+enum { EPI_FORWARD = 0, EPI_PLAIN = 1, EPI_EVIDENCE = 2, EPI_PARTIAL = 3, EPI_FORWARD_F32 = 4, EPI_EVIDENCE_F32 = 5, EPI_GATED = 6 };
 
 struct Params {
   const uint16_t* a;     // bf16 dense operand (x or dy)
@@ -68,6 +71,19 @@ struct Params {
   int64_t w_pb;          // evidence: bytes per row of w_bits
   float* gs_partial;     // evidence: [WAVES_N * tiles_n][M]
   const int* m_top;      // limbs: the largest exponent of row m's operands (limb_shift)
+};
+
+// The gated block: `bits`, n_scale and n_bias are the gate layer's, these the up
+// layer's; N counts features.  A wave's 64 columns are 32 features of the gate
+// and the same 32 of up, so that a lane's two accumulator columns are g and u of
+// one element and the gate needs no exchange between waves.
+struct PairParams : Params {
+  const uint8_t* bits_up;
+  const float* up_scale;
+  const float* up_bias;
+  // kept for the backward where not null: g and u as they are, or as 8-bit blocks
+  uint16_t *gate, *up;
+  blocks::Blocks gate8, up8;
 };
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void* base, int64_t bytes) {
@@ -259,16 +275,97 @@ constexpr int A_STAGE_K = (BK / 2) * APK;    // bytes
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
 
+// The end of a gated block's tile: g and u from the accumulators (scale, bias,
+// rounded to the type, as the two layers alone give them), through LDS EPR rows
+// at a time, so that a lane holds eight features of g and of u of one row;
+// h = silu(g) u and what the backward keeps leave from there in 16-byte (8-bit:
+// 8-byte) pieces, 64 (32) bytes of a row by four lanes, which are a block of 32.
+// N is a multiple of 8: a piece lies inside the row or outside.
+template <int DT, int MBN>
+__device__ __forceinline__ void gated_epilogue(const PairParams& p, f32x16 (&acc)[MBN][NBN], int64_t m0, int64_t n0,
+                                               int wave, int lane, uint8_t* stg) {
+  const int l32 = lane & 31, kg = lane >> 5;
+  const bool odd = l32 & 1;
+  float sc[2], bi[2];
+  {
+    const int64_t col = n0 + 32 * wave + l32;
+    const bool in = col < p.N;
+    sc[0] = in ? p.n_scale[col] : 0.0f;
+    sc[1] = in ? p.up_scale[col] : 0.0f;
+    bi[0] = in && p.n_bias ? p.n_bias[col] : 0.0f;
+    bi[1] = in && p.up_bias ? p.up_bias[col] : 0.0f;
+  }
+  const int piece = lane & 3;
+  const int64_t gcol = n0 + 32 * wave + 8 * piece;
+  const int64_t per_row = (p.N + blocks::kBlock - 1) / blocks::kBlock;
+  uint16_t* h = static_cast<uint16_t*>(p.out);
+#pragma unroll
+  for (int mb = 0; mb < MBN; ++mb) {
+#pragma unroll
+    for (int half = 0; half < 32 / EPR; ++half) {
+#pragma unroll
+      for (int nb = 0; nb < 2; ++nb) {
+#pragma unroll
+        for (int r = (EPR / 2) * half; r < (EPR / 2) * (half + 1); r += 2) {
+          const float v0 = acc[mb][nb][r] * sc[nb] + bi[nb], v1 = acc[mb][nb][r + 1] * sc[nb] + bi[nb];
+          // lanes l, l ^ 1 trade one value per row pair, as in the forward's epilogue
+          const float send = odd ? v0 : v1;
+          const float recv = __int_as_float(
+              __builtin_amdgcn_update_dpp(0, __float_as_int(send), 0xB1, 0xF, 0xF, false));  // quad_perm 1,0,3,2
+          const uint32_t word = round16x2<DT>(odd ? recv : v0, odd ? v1 : recv);
+          const int row = 8 * (r >> 2) + 4 * kg + (r & 3) + (odd ? 1 : 0) - EPR * half;
+          *reinterpret_cast<uint32_t*>(stg + row * EPL + 2 * (32 * nb + (l32 & ~1))) = word;
+        }
+      }
+      const int row = lane >> 2;
+      const int64_t grow = m0 + 32 * mb + EPR * half + row;
+      const bool there = grow < p.M && gcol < p.N;
+      float g[8], u[8], v[8];
+      const uint16_t* at = reinterpret_cast<const uint16_t*>(stg + row * EPL + 16 * piece);
+      blocks::load8<DT>(at, g);
+      blocks::load8<DT>(at + 32, u);
+      if (p.gate8.q) {
+        if (!there) {  // what lies past the row's end is no part of its last block
+#pragma unroll
+          for (int i = 0; i < 8; ++i) g[i] = u[i] = 0.0f;
+        }
+        uint32_t gc, uc;
+        const uint2 gq = blocks::quantize8(g, gc), uq = blocks::quantize8(u, uc);
+        if (there) {
+          *reinterpret_cast<uint2*>(p.gate8.q + grow * p.N + gcol) = gq;
+          *reinterpret_cast<uint2*>(p.up8.q + grow * p.N + gcol) = uq;
+          if (piece == 0) {
+            p.gate8.codes[grow * per_row + gcol / blocks::kBlock] = static_cast<uint8_t>(gc);
+            p.up8.codes[grow * per_row + gcol / blocks::kBlock] = static_cast<uint8_t>(uc);
+          }
+        }
+      }
+      if (!there) continue;
+      if (p.gate) {
+        *reinterpret_cast<uint4*>(p.gate + grow * p.N + gcol) = *reinterpret_cast<const uint4*>(at);
+        *reinterpret_cast<uint4*>(p.up + grow * p.N + gcol) = *reinterpret_cast<const uint4*>(at + 32);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = swiglu::forward_one<DT>(g[i], u[i]);
+      blocks::store8<DT>(h + grow * p.N + gcol, v);
+    }
+  }
+}
+
 // One output tile; the LDS stages are the caller's (one __shared__ array per
 // stage, so that the compiler tracks each stage's direct loads separately
 // and waits only where this code says).
 // TM: rows of the tile, 256, or 128 for A as rows of M and bits along K
 // (half_kernel below).
-template <int AKIND, int BKIND, int EPI, int DT, int TM = BM>
-__device__ __forceinline__ void wide_tile(const Params& p, int pid, uint8_t* A0, uint8_t* A1, uint8_t* A2,
+// P = PairParams: the gated block's pair of layers (bits along K, EPI_GATED or EPI_PARTIAL).
+template <int AKIND, int BKIND, int EPI, int DT, int TM = BM, class P = Params>
+__device__ __forceinline__ void wide_tile(const P& p, int pid, uint8_t* A0, uint8_t* A1, uint8_t* A2,
                                           uint8_t* A3, uint8_t* B0, uint8_t* B1, uint8_t* B2, uint8_t* B3,
                                           uint16_t* Sc) {
   static_assert(TM == BM || (AKIND == A_ROWS_M && BKIND != B_BITS_ALONG_N && EPI != EPI_PARTIAL), "half tiles");
+  constexpr bool PAIR = std::is_same<P, PairParams>::value;
+  static_assert(!PAIR || (AKIND == A_ROWS_M && BKIND == B_BITS_ALONG_K && NBN == 2), "pairs of layers");
+  constexpr int FN = PAIR ? BN / 2 : BN;   // the tile's columns of the output
   constexpr int NL = Loads<BKIND, TM>::value, NLA = Loads<BKIND, TM>::a;
   constexpr int WMR = TM, MBN = WMR / 32;  // rows and 32 x 32 blocks per wave across M
   constexpr int wm = 0;                    // every wave covers all the tile's rows
@@ -277,10 +374,10 @@ __device__ __forceinline__ void wide_tile(const Params& p, int pid, uint8_t* A0,
   const int wn = wave;
   const int l32 = lane & 31, kg = lane >> 5;
   const int tiles_m = static_cast<int>((p.M + TM - 1) / TM);
-  const int tiles_n = static_cast<int>((p.N + BN - 1) / BN);
+  const int tiles_n = static_cast<int>((p.N + FN - 1) / FN);
   int tm, tn;
   tile_of<AKIND == A_ROWS_K ? 1 : 2>(pid, tiles_m, tiles_n, tm, tn);
-  const int64_t m0 = static_cast<int64_t>(tm) * TM, n0 = static_cast<int64_t>(tn) * BN;
+  const int64_t m0 = static_cast<int64_t>(tm) * TM, n0 = static_cast<int64_t>(tn) * FN;
   const uint32_t one = one_pair<DT>();
   const int nk = static_cast<int>((p.K + BK - 1) / BK);  // K % BK != 0 only for A as rows of K
 
@@ -312,12 +409,18 @@ __device__ __forceinline__ void wide_tile(const Params& p, int pid, uint8_t* A0,
   // 64w+63 with 2 direct loads of 4 bytes per lane.
   // B along N: 64 k-rows x 32 bytes per stage; thread t loads the dwords
   // t and t + 256 (k-row d/8, bytes 4(d%8) ..) and one scale, k = t % 64.
-  __amdgpu_buffer_rsrc_t rb;
+  // Pairs: rows 64w .. + 31 are the gate's signs and the next 32 up's.
+  __amdgpu_buffer_rsrc_t rb, rb_up;
   uint32_t b_voff, b_step;
   __amdgpu_buffer_rsrc_t rs = rsrc(p.kscale, p.kscale ? p.K * 4 : 0);
   // bf16 scales are padded with zeros to a whole number of K steps
   const __amdgpu_buffer_rsrc_t rs16 = rsrc(p.kscale16, BKIND == B_BITS_ALONG_K_SCALED ? int64_t{nk} * BK * 2 : 0);
-  if (BKIND != B_BITS_ALONG_N) {
+  if constexpr (PAIR) {
+    rb = rsrc(p.bits + n0 * p.pb, (p.bit_rows - n0) * p.pb);
+    rb_up = rsrc(p.bits_up + n0 * p.pb, (p.bit_rows - n0) * p.pb);
+    b_voff = static_cast<uint32_t>((32 * wave + (lane >> 1)) * p.pb + 4 * (lane & 1));
+    b_step = 0;
+  } else if (BKIND != B_BITS_ALONG_N) {
     rb = rsrc(p.bits + n0 * p.pb, (p.bit_rows - n0) * p.pb);
     b_voff = static_cast<uint32_t>((64 * wave + (lane >> 1)) * p.pb + 4 * (lane & 1));
     b_step = static_cast<uint32_t>(32 * p.pb);
@@ -357,8 +460,8 @@ __device__ __forceinline__ void wide_tile(const Params& p, int pid, uint8_t* A0,
       const uint32_t kb = live ? static_cast<uint32_t>(it) * (BK / 8) : 0x80000000u;
 #pragma unroll
       for (int j = 0; j < 2; ++j)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_t*)(Bs + (64 * wave + 32 * j) * 8), 4, b_voff,
-                                                 static_cast<int>(j * b_step + kb), 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(PAIR && j == 1 ? rb_up : rb, (lds_t*)(Bs + (64 * wave + 32 * j) * 8), 4,
+                                                 b_voff, static_cast<int>(j * b_step + kb), 0, 0);
       if (BKIND == B_BITS_ALONG_K_SCALED) {
         // wave w brings the bf16 scales of k = 16w .. 16w+15, a pair per
         // lane (lanes 0..7: direct loads narrower than a dword still take a
@@ -694,6 +797,11 @@ __device__ __forceinline__ void wide_tile(const Params& p, int pid, uint8_t* A0,
     return;
   }
 
+  if constexpr (EPI == EPI_GATED) {
+    gated_epilogue<DT, MBN>(p, acc, m0, n0, wave, lane, (wave < 2 ? A0 : A1) + (wave & 1) * (EPR * EPL));
+    return;
+  }
+
   // Epilogue: (scale and bias,) round to bf16 and stage through LDS EPR rows
   // at a time so each row segment of the wave's WNC outputs leaves as
   // 16-byte stores of consecutive lanes.  Waves 0, 1 stage in A0 and waves
@@ -803,6 +911,22 @@ __global__ __launch_bounds__(THREADS, 2) void half_kernel(Params p) {
   using SZ = StageSizes<A_ROWS_M, BKIND>;
   QSTE_WIDE_STAGES(A_STAGE / 2, SZ::b, SZ::s)
   wide_tile<A_ROWS_M, BKIND, EPI, DT, BM / 2>(p, blockIdx.x, A0, A1, A2, A3, B0, B1, B2, B3, Sc);
+}
+
+// The gated block on whole and on half tiles: two layers' products of 128
+// features from one reading of x.
+template <int DT>
+__global__ __launch_bounds__(THREADS, 2) void gated_half_kernel(PairParams p) {
+  using SZ = StageSizes<A_ROWS_M, B_BITS_ALONG_K>;
+  QSTE_WIDE_STAGES(A_STAGE / 2, SZ::b, SZ::s)
+  wide_tile<A_ROWS_M, B_BITS_ALONG_K, EPI_GATED, DT, BM / 2>(p, blockIdx.x, A0, A1, A2, A3, B0, B1, B2, B3, Sc);
+}
+
+template <int DT>
+__global__ __launch_bounds__(THREADS, 1) void gated_wide_kernel(PairParams p) {
+  using SZ = StageSizes<A_ROWS_M, B_BITS_ALONG_K>;
+  QSTE_WIDE_STAGES(SZ::a, SZ::b, SZ::s)
+  wide_tile<A_ROWS_M, B_BITS_ALONG_K, EPI_GATED, DT>(p, blockIdx.x, A0, A1, A2, A3, B0, B1, B2, B3, Sc);
 }
 
 template <int AKIND, int BKIND, int EPI, int DT>
@@ -1033,6 +1157,76 @@ __global__ __launch_bounds__(THREADS) void forward_combine_kernel(const float* _
     }
   }
 }
+
+// The gated block's tiles over K ranges, slabs as product_split_kernel leaves
+// them: row r of a slab holds 32 features of g, the same 32 of u, and so on.
+template <int DT>
+__global__ __launch_bounds__(THREADS, 1) void gated_split_kernel(PairParams p, int tiles, int ks_steps, float* partial) {
+  using SZ = StageSizes<A_ROWS_M, B_BITS_ALONG_K>;
+  QSTE_WIDE_STAGES(SZ::a, SZ::b, SZ::s)
+  const int w = static_cast<int>(blockIdx.x), i = w % tiles, j = w / tiles;
+  const int64_t k0 = static_cast<int64_t>(j) * ks_steps * BK;
+  PairParams q = p;
+  q.a = p.a + k0;
+  q.bits = p.bits + k0 / 8;
+  q.bits_up = p.bits_up + k0 / 8;
+  q.K = p.K - k0 < static_cast<int64_t>(ks_steps) * BK ? p.K - k0 : static_cast<int64_t>(ks_steps) * BK;
+  q.out = partial + static_cast<int64_t>(w) * (BM * BN);
+  wide_tile<A_ROWS_M, B_BITS_ALONG_K, EPI_PARTIAL, DT>(q, i, A0, A1, A2, A3, B0, B1, B2, B3, Sc);
+}
+
+// The ranges' sums in range order, then as gated_epilogue.  Workgroup (x, i):
+// rows 16x .. 16x + 15 of tile i, eight features a thread.
+template <int DT>
+__global__ __launch_bounds__(THREADS) void gated_combine_kernel(PairParams p, const float* __restrict__ partial,
+                                                                int tiles, int splits) {
+  const int tiles_m = static_cast<int>((p.M + BM - 1) / BM), tiles_n = static_cast<int>((p.N + BN / 2 - 1) / (BN / 2));
+  const int i = static_cast<int>(blockIdx.y), tid = static_cast<int>(threadIdx.x);
+  int tm, tn;
+  tile_of<2>(i, tiles_m, tiles_n, tm, tn);  // the tiles' mapping
+  const int lrow = static_cast<int>(blockIdx.x) * 16 + tid / 16, eight = tid % 16;
+  const int64_t row = static_cast<int64_t>(tm) * BM + lrow, col = static_cast<int64_t>(tn) * (BN / 2) + 8 * eight;
+  const bool there = row < p.M && col < p.N;  // N is a multiple of 8
+  float g[8] = {}, u[8] = {}, v[8];
+  if (there) {
+    const float* src = partial + static_cast<int64_t>(i) * (BM * BN) + lrow * BN + 64 * (eight / 4) + 8 * (eight % 4);
+    for (int j = 0; j < splits; ++j) {
+      const float* at = src + static_cast<int64_t>(j) * tiles * (BM * BN);
+#pragma unroll
+      for (int q = 0; q < 8; q += 4) {
+        const float4 a = *reinterpret_cast<const float4*>(at + q), b = *reinterpret_cast<const float4*>(at + 32 + q);
+        g[q] += a.x; g[q + 1] += a.y; g[q + 2] += a.z; g[q + 3] += a.w;
+        u[q] += b.x; u[q + 1] += b.y; u[q + 2] += b.z; u[q + 3] += b.w;
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      g[q] = Elem<DT>::round(g[q] * p.n_scale[col + q] + (p.n_bias ? p.n_bias[col + q] : 0.0f));
+      u[q] = Elem<DT>::round(u[q] * p.up_scale[col + q] + (p.up_bias ? p.up_bias[col + q] : 0.0f));
+    }
+  }
+  if (p.gate8.q) {
+    uint32_t gc, uc;
+    const uint2 gq = blocks::quantize8(g, gc), uq = blocks::quantize8(u, uc);
+    if (there) {
+      *reinterpret_cast<uint2*>(p.gate8.q + row * p.N + col) = gq;
+      *reinterpret_cast<uint2*>(p.up8.q + row * p.N + col) = uq;
+      if (eight % 4 == 0) {
+        const int64_t block = row * ((p.N + blocks::kBlock - 1) / blocks::kBlock) + col / blocks::kBlock;
+        p.gate8.codes[block] = static_cast<uint8_t>(gc);
+        p.up8.codes[block] = static_cast<uint8_t>(uc);
+      }
+    }
+  }
+  if (!there) return;
+  if (p.gate) {
+    blocks::store8<DT>(p.gate + row * p.N + col, g);
+    blocks::store8<DT>(p.up + row * p.N + col, u);
+  }
+#pragma unroll
+  for (int q = 0; q < 8; ++q) v[q] = swiglu::forward_one<DT>(g[q], u[q]);
+  blocks::store8<DT>(static_cast<uint16_t*>(p.out) + row * p.N + col, v);
+}
 #undef QSTE_WIDE_STAGES
 }  // namespace wide
 }  // namespace mfma
@@ -1250,6 +1444,70 @@ int mfma_linear_forward_split(const void* x, int dtype, const uint8_t* packed, c
   return dtype == QSTE_F16
              ? launch_split<mfma::B_BITS_ALONG_K, QSTE_F16, QSTE_F16>(p, sp, partial, stream)
              : launch_split<mfma::B_BITS_ALONG_K, QSTE_BF16, QSTE_BF16>(p, sp, partial, stream);
+}
+
+// The gated block on the tiles: two layers of `rows` features each are a product
+// of 2 * rows columns, in tiles of 128 features of both.
+static int64_t gated_columns(int64_t rows) { return (rows + 127) / 128 * 256; }
+
+// Whether it is for this path: what the tiles need, and features in whole eights.
+bool mfma_gated_ok(int64_t m, int64_t rows, int64_t cols, int dtype) {
+  return mfma_dtype(dtype) && m > 0 && rows > 0 && rows % 8 == 0 && cols > 0 && cols % 64 == 0 && fits32(m * cols * 2) &&
+         fits32((rows + 128) * (cols / 8));
+}
+
+static ProductPlan gated_plan(int64_t m, int64_t rows, int64_t cols) {
+  return product_plan(m, gated_columns(rows), static_cast<int>(cols / mfma::wide::BK), m > 16);
+}
+double mfma_gated_us(int64_t m, int64_t rows, int64_t cols) { return gated_plan(m, rows, cols).us; }
+size_t mfma_gated_workspace(int64_t m, int64_t rows, int64_t cols) {
+  return split_bytes(gated_plan(m, rows, cols).split, wide_grid(m, gated_columns(rows)));
+}
+
+template <int DT>
+static int launch_gated(const mfma::PairParams& p, const ProductPlan& plan, float* partial, hipStream_t stream) {
+  const int tiles = wide_grid(p.M, gated_columns(p.N));
+  if (plan.split.splits > 1) {
+    mfma::wide::gated_split_kernel<DT>
+        <<<tiles * plan.split.splits, mfma::wide::THREADS, 0, stream>>>(p, tiles, plan.split.ks_steps, partial);
+    const int rc = static_cast<int>(hipGetLastError());
+    if (rc) return rc;
+    const dim3 grid(mfma::wide::BM / 16, static_cast<unsigned>(tiles));
+    mfma::wide::gated_combine_kernel<DT>
+        <<<grid, mfma::wide::THREADS, 0, stream>>>(p, partial, tiles, plan.split.splits);
+  } else if (plan.half) {
+    const int64_t grid = (p.M + 127) / 128 * ((p.N + 127) / 128);
+    mfma::wide::gated_half_kernel<DT><<<static_cast<unsigned>(grid), mfma::wide::THREADS, 0, stream>>>(p);
+  } else {
+    mfma::wide::gated_wide_kernel<DT><<<tiles, mfma::wide::THREADS, 0, stream>>>(p);
+  }
+  return static_cast<int>(hipGetLastError());
+}
+
+// h [m, rows] = silu(g) * u of two layers; `gate`, `up` and the blocks as PairParams has
+// them.  Operands at 16-byte steps, mfma_gated_ok's sizes, mfma_gated_workspace of space.
+int mfma_gated(const void* x, int dtype, const uint8_t* gate_bits, const float* gate_scale, const float* gate_bias,
+               const uint8_t* up_bits, const float* up_scale, const float* up_bias, void* h, void* gate, void* up,
+               const blocks::Blocks& gate8, const blocks::Blocks& up8, int64_t m, int64_t rows, int64_t cols,
+               void* workspace, hipStream_t stream) {
+  mfma::PairParams p{};
+  p.a = static_cast<const uint16_t*>(x);
+  p.bits = gate_bits;
+  p.bits_up = up_bits;
+  p.out = h;
+  p.M = m; p.N = rows; p.K = cols;
+  p.lda = cols; p.pb = cols / 8;
+  p.a_rows = m; p.bit_rows = rows;
+  p.n_scale = gate_scale; p.n_bias = gate_bias;
+  p.up_scale = up_scale; p.up_bias = up_bias;
+  p.gate = static_cast<uint16_t*>(gate);
+  p.up = static_cast<uint16_t*>(up);
+  p.gate8 = gate8;
+  p.up8 = up8;
+  const ProductPlan plan = gated_plan(m, rows, cols);
+  float* partial = static_cast<float*>(workspace);
+  return dtype == QSTE_F16 ? launch_gated<QSTE_F16>(p, plan, partial, stream)
+                           : launch_gated<QSTE_BF16>(p, plan, partial, stream);
 }
 
 // The input gradient as a launch of its own, where its tiles are few: K cut

@@ -42,9 +42,16 @@
 // them in range order: every workgroup reads all of x's rows over its range,
 // so at many rows of x and few rows of weights x's traffic from L2 is what
 // splitting K saves.
+//
+// A gated block of few rows (silu(gate(x)) * up(x)) is the same kernel with its
+// blocks in pairs: the first half of a workgroup's are 16 rows each of the gate's
+// weights, the second half the same rows of up's, so that the gate is formed
+// where the waves' sums meet, and one launch with one reading of x takes the
+// place of three with two.
 #include <type_traits>
 
 #include "common.hpp"
+#include "swiglu.hpp"
 
 namespace qste {
 namespace gemv {
@@ -125,7 +132,11 @@ struct Args {
   int limbs;            // 1, or 3 (y in fp32, row m = rows 3m .. 3m + 2 of x)
   int splits;
   int chunks_per_split;
-  int64_t N, K;
+  int64_t N, K;         // N: rows of weights; of a gated block, features
+  // a gated block's second layer (bits, scale and bias are its first)
+  const uint8_t* bits_up;
+  const float* scale_up;
+  const float* bias_up;
 };
 
 // Four outputs n .. n + 3 of row m from their sums.
@@ -164,6 +175,21 @@ __device__ __forceinline__ void finish4(const Args& p, int64_t m, int64_t n, f32
   }
 }
 
+// The same for a gated block: silu(g) * u of the two layers' sums, each scaled,
+// given its bias and rounded as finish4 would.
+template <int OUT>
+__device__ __forceinline__ void finish_gated4(const Args& p, int64_t m, int64_t n, f32x4 g, f32x4 u, const float* gs,
+                                              const float* gb, const float* us, const float* ub, bool vec) {
+  const float ones[4] = {1.0f, 1.0f, 1.0f, 1.0f}, zeros[4] = {-0.0f, -0.0f, -0.0f, -0.0f};  // keep a zero's sign
+  f32x4 h;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float a = Elem<OUT>::round(g[j] * gs[j] + gb[j]), b = Elem<OUT>::round(u[j] * us[j] + ub[j]);
+    h[j] = swiglu::forward_one<OUT>(a, b);
+  }
+  finish4<OUT>(p, m, n, h, ones, zeros, vec);
+}
+
 // XR rows of x are staged (>= p.xr: 4 or a multiple of 16; rows past p.xr
 // are left as they are, their outputs are never stored), NBW blocks of 16
 // weight rows per workgroup.  STAGED: x arrives in four stages a chunk, as it
@@ -195,9 +221,11 @@ struct Cfg {
   static constexpr int D = RESIDENT ? 2 : NBW;
 };
 
-template <int DT, int XR, int NBW, bool STAGED>
+template <int DT, int XR, int NBW, bool STAGED, bool PAIR>
 __global__ __launch_bounds__(THREADS, 1) void skinny_kernel(Args p) {
   using C = Cfg<XR, NBW, STAGED>;
+  static_assert(!PAIR || NBW % 2 == 0, "a gated block's blocks come in pairs");
+  constexpr int FB = PAIR ? NBW / 2 : NBW;  // blocks of 16 outputs
   constexpr int MT = C::MT, JS = C::JS, D = C::D;
   __shared__ __attribute__((aligned(16))) uint8_t smem[C::bytes];
   __shared__ float epi[2][16 * NBW];
@@ -210,17 +238,18 @@ __global__ __launch_bounds__(THREADS, 1) void skinny_kernel(Args p) {
   // consecutive workgroups land on different XCDs: with the range as the
   // fastest index, an XCD's workgroups read few ranges of x
   const int range = static_cast<int>(blockIdx.x) % p.splits;
-  const int64_t n0 = static_cast<int64_t>(static_cast<int>(blockIdx.x) / p.splits) * (16 * NBW);
+  const int64_t n0 = static_cast<int64_t>(static_cast<int>(blockIdx.x) / p.splits) * (16 * FB);
   const int c_first = range * p.chunks_per_split;
   const int c_all = static_cast<int>((K + CHUNK_K - 1) / CHUNK_K);
   const int c_last = min(c_first + p.chunks_per_split, c_all);
 
   // rows past N read zero through the buffer bounds
   const __amdgpu_buffer_rsrc_t rb = rsrc(p.bits, p.N * pb);
+  const __amdgpu_buffer_rsrc_t rb_up = rsrc(PAIR ? p.bits_up : p.bits, p.N * pb);
   const __amdgpu_buffer_rsrc_t rx = rsrc(p.x, static_cast<int64_t>(p.xr) * K * 2);
   uint32_t boff[NBW];
 #pragma unroll
-  for (int b = 0; b < NBW; ++b) boff[b] = static_cast<uint32_t>((n0 + 16 * b + l16) * pb + 16 * q);
+  for (int b = 0; b < NBW; ++b) boff[b] = static_cast<uint32_t>((n0 + 16 * (b % FB) + l16) * pb + 16 * q);
 
   uint8_t* xs = smem + wave * C::x_bytes;
   auto issue_x = [&](int c, int stage, int buf = 0) {
@@ -276,7 +305,7 @@ __global__ __launch_bounds__(THREADS, 1) void skinny_kernel(Args p) {
   };
 
   u32x4 W[NBW];
-  auto issue_w1 = [&](int c, int b) { return ld128(rb, c < c_last ? boff[b] + 64u * static_cast<uint32_t>(c) : kOob); };
+  auto issue_w1 = [&](int c, int b) { return ld128(PAIR && b >= FB ? rb_up : rb, c < c_last ? boff[b] + 64u * static_cast<uint32_t>(c) : kOob); };
 
   f32x4 acc[NBW][MT];
 #pragma unroll
@@ -302,7 +331,15 @@ __global__ __launch_bounds__(THREADS, 1) void skinny_kernel(Args p) {
   }
   // the epilogue's row scale, bias and powers of two, fetched while the first loads fly
   float out_scale = 0.0f, out_bias = 0.0f;
-  if (tid < 16 * NBW && n0 + tid < p.N) {
+  if constexpr (PAIR) {
+    const bool up = tid >= 16 * FB;
+    const int64_t n = n0 + tid - (up ? 16 * FB : 0);
+    if (tid < 16 * NBW && n < p.N) {
+      const float* bias = up ? p.bias_up : p.bias;
+      out_scale = (up ? p.scale_up : p.scale)[n];
+      out_bias = bias ? bias[n] : 0.0f;
+    }
+  } else if (tid < 16 * NBW && n0 + tid < p.N) {
     out_scale = p.scale[n0 + tid];
     out_bias = p.bias ? p.bias[n0 + tid] : 0.0f;
   }
@@ -454,13 +491,14 @@ __global__ __launch_bounds__(THREADS, 1) void skinny_kernel(Args p) {
   };
   const bool full = (p.N & 3) == 0;
   if (p.splits > 1) {
-    float* part = p.partial + static_cast<int64_t>(range) * p.xr * p.N;
+    // (a gated block: the rows of the gate's sums, then those of up's)
+    float* part = p.partial + static_cast<int64_t>(range) * p.xr * p.N * (PAIR ? 2 : 1);
     for (int i = tid; i < NBW * p.xr * 4; i += THREADS) {
       const int g = i & 3, b = (i >> 2) % NBW, row = (i >> 2) / NBW;
-      const int64_t n = n0 + 16 * b + 4 * g;
+      const int64_t n = n0 + 16 * (b % FB) + 4 * g;
       if (n >= p.N) continue;
       const f32x4 v = total(b, row, g);
-      float* d = part + static_cast<int64_t>(row) * p.N + n;
+      float* d = part + static_cast<int64_t>(row + (PAIR && b >= FB ? p.xr : 0)) * p.N + n;
       if (full) {
         *reinterpret_cast<f32x4*>(d) = v;
       } else {
@@ -474,12 +512,29 @@ __global__ __launch_bounds__(THREADS, 1) void skinny_kernel(Args p) {
   const int rows = p.xr / p.limbs;
   const int align = p.limbs == 3 ? 15 : 7;
   const bool vec = full && (reinterpret_cast<uintptr_t>(p.y) & align) == 0;
-  for (int i = tid; i < NBW * rows * 4; i += THREADS) {
-    const int g = i & 3, b = (i >> 2) % NBW, m = (i >> 2) / NBW;
+  for (int i = tid; i < FB * rows * 4; i += THREADS) {
+    const int g = i & 3, b = (i >> 2) % FB, m = (i >> 2) / FB;
     const int64_t n = n0 + 16 * b + 4 * g;
     if (n >= p.N) continue;
     const float* sc = &epi[0][16 * b + 4 * g];
     const float* bi = &epi[1][16 * b + 4 * g];
+    if constexpr (PAIR) {
+      const float *us = sc + 16 * FB, *ub = bi + 16 * FB;
+      if constexpr (kLimbs) {
+        if (p.limbs == 3) {
+          auto limbs = [&](int block) {
+            f32x4 v = (total(block, 3 * m + 2, g) + total(block, 3 * m + 1, g)) + total(block, 3 * m, g);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = ldexpf(v[j], back[m]);
+            return v;
+          };
+          finish_gated4<QSTE_F32>(p, m, n, limbs(b), limbs(b + FB), sc, bi, us, ub, vec);
+          continue;
+        }
+      }
+      finish_gated4<DT>(p, m, n, total(b, m, g), total(b + FB, m, g), sc, bi, us, ub, vec);
+      continue;
+    }
     if constexpr (kLimbs) {
       if (p.limbs == 3) {
         f32x4 v = (total(b, 3 * m + 2, g) + total(b, 3 * m + 1, g)) + total(b, 3 * m, g);
@@ -495,7 +550,7 @@ __global__ __launch_bounds__(THREADS, 1) void skinny_kernel(Args p) {
 
 // splits > 1 (16-bit x): the range sums added in range order, then scale, bias
 // and one rounding; four outputs a thread.
-template <int DT>
+template <int DT, bool PAIR>
 __global__ __launch_bounds__(256) void combine_kernel(Args p) {
   const int64_t quads = (p.N + 3) / 4;
   const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
@@ -508,18 +563,32 @@ __global__ __launch_bounds__(256) void combine_kernel(Args p) {
     sc[j] = n + j < p.N ? p.scale[n + j] : 0.0f;
     bi[j] = n + j < p.N && p.bias ? p.bias[n + j] : 0.0f;
   }
-  f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int s = 0; s < p.splits; ++s) {
-    const float* d = p.partial + (static_cast<int64_t>(s) * p.xr + m) * p.N + n;
-    if (full) {
-      v += *reinterpret_cast<const f32x4*>(d);
-    } else {
+  auto sums = [&](int64_t first, int64_t range) {  // of row `first` of a range's `range` rows
+    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s = 0; s < p.splits; ++s) {
+      const float* d = p.partial + (static_cast<int64_t>(s) * range + first) * p.N + n;
+      if (full) {
+        v += *reinterpret_cast<const f32x4*>(d);
+      } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (n + j < p.N) v[j] += d[j];
+        for (int j = 0; j < 4; ++j)
+          if (n + j < p.N) v[j] += d[j];
+      }
     }
-  }
+    return v;
+  };
   const bool vec = full && (reinterpret_cast<uintptr_t>(p.y) & 7) == 0;
+  if constexpr (PAIR) {
+    float us[4], ub[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      us[j] = n + j < p.N ? p.scale_up[n + j] : 0.0f;
+      ub[j] = n + j < p.N && p.bias_up ? p.bias_up[n + j] : 0.0f;
+    }
+    finish_gated4<DT>(p, m, n, sums(m, 2 * p.xr), sums(p.xr + m, 2 * p.xr), sc, bi, us, ub, vec);
+    return;
+  }
+  const f32x4 v = sums(m, p.xr);
   finish4<DT>(p, m, n, v, sc, bi, vec);
 }
 
@@ -527,25 +596,27 @@ __global__ __launch_bounds__(256) void combine_kernel(Args p) {
 // image in LDS at the end have room for.
 constexpr int most_blocks(int xr) { return xr <= 32 ? 8 : (xr <= 48 ? 6 : 4); }
 
-template <int DT, int XR, bool STAGED, int NBW = 1>
+template <int DT, int XR, bool STAGED, bool PAIR, int NBW = PAIR ? 2 : 1>
 void launch_nbw(int nbw, const Args& p, hipStream_t stream) {
+  constexpr int next = PAIR ? 2 : 1;
   if constexpr (NBW < most_blocks(XR)) {
-    if (nbw > NBW) return launch_nbw<DT, XR, STAGED, NBW + 1>(nbw, p, stream);
+    if (nbw > NBW) return launch_nbw<DT, XR, STAGED, PAIR, NBW + next>(nbw, p, stream);
   }
-  const int groups = static_cast<int>((p.N + 16 * NBW - 1) / (16 * NBW));
-  skinny_kernel<DT, XR, NBW, STAGED><<<groups * p.splits, THREADS, 0, stream>>>(p);
+  constexpr int outputs = 16 * NBW / next;
+  const int groups = static_cast<int>((p.N + outputs - 1) / outputs);
+  skinny_kernel<DT, XR, NBW, STAGED, PAIR><<<groups * p.splits, THREADS, 0, stream>>>(p);
 }
 
-template <int DT>
+template <int DT, bool PAIR>
 void launch_xr(int nbw, const Args& p, hipStream_t stream) {
   if constexpr (DT == QSTE_BF16) {
-    if (p.limbs == 3 && p.xr <= 16) return launch_nbw<DT, 16, true>(nbw, p, stream);
+    if (p.limbs == 3 && p.xr <= 16) return launch_nbw<DT, 16, true, PAIR>(nbw, p, stream);
   }
-  if (p.xr <= 4) launch_nbw<DT, 4, false>(nbw, p, stream);
-  else if (p.xr <= 16) launch_nbw<DT, 16, false>(nbw, p, stream);
-  else if (p.xr <= 32) launch_nbw<DT, 32, true>(nbw, p, stream);
-  else if (p.xr <= 48) launch_nbw<DT, 48, true>(nbw, p, stream);
-  else launch_nbw<DT, 64, true>(nbw, p, stream);
+  if (p.xr <= 4) launch_nbw<DT, 4, false, PAIR>(nbw, p, stream);
+  else if (p.xr <= 16) launch_nbw<DT, 16, false, PAIR>(nbw, p, stream);
+  else if (p.xr <= 32) launch_nbw<DT, 32, true, PAIR>(nbw, p, stream);
+  else if (p.xr <= 48) launch_nbw<DT, 48, true, PAIR>(nbw, p, stream);
+  else launch_nbw<DT, 64, true, PAIR>(nbw, p, stream);
 }
 
 // Rows of x a launch takes: four tiles of 16, or 21 rows of three limbs.
@@ -627,14 +698,21 @@ int64_t x_rows(int dtype, int64_t m, int64_t rows, int64_t cols) {
   return (rows + 128) * (cols / 8) < (int64_t{1} << 31) && xr * cols * 2 < (int64_t{1} << 31) ? xr : 0;
 }
 
-template <int DT>
+template <int DT, bool PAIR = false>
 int run(const Args& p, const Plan& plan, hipStream_t stream) {
-  launch_xr<DT>(plan.nbw, p, stream);
+  launch_xr<DT, PAIR>(plan.nbw, p, stream);
   int rc = static_cast<int>(hipGetLastError());
   if (rc || p.splits == 1) return rc;
   const int64_t items = p.xr * ((p.N + 3) / 4);
-  combine_kernel<DT><<<static_cast<int>((items + 255) / 256), 256, 0, stream>>>(p);
+  combine_kernel<DT, PAIR><<<static_cast<int>((items + 255) / 256), 256, 0, stream>>>(p);
   return static_cast<int>(hipGetLastError());
+}
+
+// A gated block of two layers of `features`: the plan of one of twice the rows, with its blocks in pairs.
+Plan pair_plan(int64_t xr, int64_t features, int64_t cols, bool may_split) {
+  Plan plan = plan_of(xr, 2 * ((features + 15) / 16 * 16), cols, may_split);
+  plan.nbw += plan.nbw & 1;  // the most blocks a workgroup can have is even for every number of rows
+  return plan;
 }
 
 size_t up256(size_t v) { return (v + 255) & ~static_cast<size_t>(255); }
@@ -707,6 +785,61 @@ int gemv_linear_forward(const void* x, int dtype, const uint8_t* packed, const f
   }
   p.partial = reinterpret_cast<float*>(ws);
   return dtype == QSTE_F16 ? gemv::run<QSTE_F16>(p, plan, stream) : gemv::run<QSTE_BF16>(p, plan, stream);
+}
+
+// The gated block on this path: its time in us (negative when its sizes are not
+// for it), workspace, and the call.  fp32 rows' sums, and up to 16 rows' of 16
+// bits, are in an order of their own K alone, as the layers' are.
+double gemv_gated_us(int64_t m, int64_t features, int64_t cols, int dtype) {
+  const int64_t xr = gemv::x_rows(dtype, m, 2 * ((features + 15) / 16 * 16), cols);
+  if (xr == 0) return -1.0;
+  const bool fp32 = dtype == QSTE_F32;
+  const int64_t top = fp32 ? 3 * gemv::kRows32 : (xr + 15) / 16 * 16;
+  return gemv::estimate(top, gemv::pair_plan(top, features, cols, !fp32), 2 * features, fp32 || top > 16) +
+         (fp32 ? 2.7 : 0.0);
+}
+
+size_t gemv_gated_workspace(int64_t m, int64_t features, int64_t cols, int dtype) {
+  const int64_t xr = gemv::x_rows(dtype, m, 2 * ((features + 15) / 16 * 16), cols);
+  if (xr == 0) return 0;
+  if (dtype == QSTE_F32)
+    return gemv::up256(static_cast<size_t>(xr * cols) * 2) + gemv::up256(static_cast<size_t>(m) * sizeof(int));
+  const gemv::Plan plan = gemv::pair_plan(xr, features, cols, true);
+  return plan.splits > 1 ? static_cast<size_t>(plan.splits * xr * 2 * features) * sizeof(float) : 0;
+}
+
+// Operands at 16-byte steps, gemv_gated_workspace of space.
+int gemv_gated(const void* x, int dtype, const uint8_t* gate_bits, const float* gate_scale, const float* gate_bias,
+               const uint8_t* up_bits, const float* up_scale, const float* up_bias, void* h, int64_t m,
+               int64_t features, int64_t cols, void* workspace, hipStream_t stream) {
+  const bool fp32 = dtype == QSTE_F32;
+  gemv::Args p{};
+  p.xr = static_cast<int>(fp32 ? 3 * m : m);
+  const gemv::Plan plan = gemv::pair_plan(p.xr, features, cols, !fp32);
+  p.x = static_cast<const uint16_t*>(x);
+  p.bits = gate_bits;
+  p.scale = gate_scale;
+  p.bias = gate_bias;
+  p.bits_up = up_bits;
+  p.scale_up = up_scale;
+  p.bias_up = up_bias;
+  p.y = h;
+  p.limbs = fp32 ? 3 : 1;
+  p.splits = plan.splits;
+  p.chunks_per_split = plan.chunks_per_split;
+  p.N = features;
+  p.K = cols;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  if (fp32) {
+    uint16_t* xl = reinterpret_cast<uint16_t*>(ws);
+    int* top = reinterpret_cast<int*>(ws + gemv::up256(static_cast<size_t>(p.xr * cols) * 2));
+    const int rc = launch_limbs(static_cast<const float*>(x), m, cols, xl, top, stream);
+    if (rc) return rc;
+    p.x = xl;
+    p.top = top;
+  }
+  p.partial = reinterpret_cast<float*>(ws);
+  return dtype == QSTE_F16 ? gemv::run<QSTE_F16, true>(p, plan, stream) : gemv::run<QSTE_BF16, true>(p, plan, stream);
 }
 
 }  // namespace qste

@@ -22,8 +22,16 @@
 // The forward can also encode each row of h as the next layer's saved
 // activation (the one-bit affine encoding, encode.hpp), from the values it
 // already holds, so the down projection's forward need not read h again.
+//
+// With a checkpoint, what autograd keeps of g and u is 8 bits an element
+// (blocks.hpp): the forward writes them beside h from the values it holds, and
+// the backward takes the g and u that they stand for.  HBM-bound like the
+// rest: 16384 x 14336 in bf16 read and write 1.89 GB forward (1.41 without) and
+// 1.89 GB backward (2.35 without).
+#include "blocks.hpp"
 #include "common.hpp"
 #include "encode.hpp"
+#include "swiglu.hpp"
 
 namespace qste {
 namespace swiglu {
@@ -31,8 +39,6 @@ namespace swiglu {
 constexpr int kThreads = 256;
 constexpr int64_t kEncodeGroups = 1024;  // workgroups of the tabled encoding forward (4 per CU on 256 CUs)
 constexpr int64_t kTabRows = 4;          // rows per workgroup from which the table pays for itself
-
-__device__ __forceinline__ float silu_value(float x) { return x / (1.0f + expf(-x)); }
 
 // The two fp32 factors of dg, from the rounded da and the input g
 __device__ __forceinline__ void silu_grad_factors(float da, float x, float& ds, float& inner) {
@@ -47,13 +53,6 @@ __device__ __forceinline__ float silu_grad(float da, float x) {
   float ds, inner;
   silu_grad_factors(da, x, ds, inner);
   return ds * inner;
-}
-
-template <int DT>
-__device__ __forceinline__ float forward_one(float g, float u) {
-  using E = Elem<DT>;
-  const float a = E::round(silu_value(g));
-  return a * u;  // rounded by the caller's store
 }
 
 // Generic elementwise forward: any dtype, any alignment.
@@ -125,20 +124,46 @@ __device__ __forceinline__ uint4 forward_chunk_tab(const uint4& gc, const uint4&
   return make_uint4(out[0], out[1], out[2], out[3]);
 }
 
+// g and u as 8-bit blocks
+struct Pair {
+  blocks::Blocks gate, up;
+};
+
+// Chunk q of a row of g and of u (zeros past the row) to their blocks, the four
+// lanes of a block together.
+__device__ __forceinline__ void keep_chunk(const Pair& kept, const uint4& gc, const uint4& uc, int64_t row, int64_t q,
+                                           int64_t cols, int64_t stride) {
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    const uint4& c = which ? uc : gc;
+    const blocks::Blocks& to = which ? kept.up : kept.gate;
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = chunk_value(c, i);
+    uint32_t code;
+    const uint2 bytes = blocks::quantize8(x, code);
+    if (q < stride) {
+      *reinterpret_cast<uint2*>(to.q + row * cols + 8 * q) = bytes;
+      if ((q & 3) == 0) to.codes[row * ((stride + 3) / 4) + (q >> 2)] = static_cast<uint8_t>(code);
+    }
+  }
+}
+
 // bf16 rows of `stride` 8-value chunks (stride <= CH * kThreads); workgroup
 // b takes rows b, b + gridDim.x, ...: h is written and its row encoded from
 // the registers.  With TAB the rounded silu of tabulated gates comes from an
 // LDS table the workgroup fills once for all its rows (the exponential and
 // the correctly rounded division per entry, not per element); without, for
 // grids of about one row per workgroup, every element computes it.
-template <int CH, bool TAB>
+// With KEPT the 8-bit blocks of g and u are written too (`gate8`, `up8`).
+template <int CH, bool TAB, bool KEPT>
 __global__ __launch_bounds__(kThreads) void forward_encode_kernel(const uint16_t* __restrict__ g,
                                                                   const uint16_t* __restrict__ u,
                                                                   uint16_t* __restrict__ h,
                                                                   uint8_t* __restrict__ packed,
                                                                   float* __restrict__ offset,
                                                                   float* __restrict__ scale, int64_t rows,
-                                                                  int64_t cols, int64_t stride) {
+                                                                  int64_t cols, int64_t stride, Pair kept) {
   __shared__ double red[kThreads / kWave];
   __shared__ uint16_t tab_a[TAB ? kFwdEntries : 1];
   if (TAB) {
@@ -171,8 +196,38 @@ __global__ __launch_bounds__(kThreads) void forward_encode_kernel(const uint16_t
       v[k] = q >= stride ? make_uint4(0, 0, 0, 0)
                          : TAB ? forward_chunk_tab(gv[k], uv[k], tab_a) : forward_chunk(gv[k], uv[k]);
       if (q < stride) hr[q] = v[k];
+      if constexpr (KEPT) keep_chunk(kept, gv[k], uv[k], row, q, cols, stride);
     }
     encode_row_chunks<kThreads, CH>(v, packed + row * stride, offset + row, scale + row, cols, stride, red);
+  }
+}
+
+// The forward with a checkpoint: any dtype, a quarter of a block a thread.
+template <int DT>
+__global__ __launch_bounds__(kThreads) void forward_blocks_kernel(const typename Elem<DT>::T* __restrict__ g,
+                                                                  const typename Elem<DT>::T* __restrict__ u,
+                                                                  typename Elem<DT>::T* __restrict__ h, Pair kept,
+                                                                  int64_t cols, int64_t per_row, int64_t quarters) {
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kThreads;
+  for (int64_t j = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; j < quarters; j += step) {
+    const blocks::Quarter p(j, cols, per_row);
+    float gv[8] = {}, uv[8] = {}, hv[8];
+    if (p.there()) {
+      blocks::load8<DT>(g + p.at(), gv);
+      blocks::load8<DT>(u + p.at(), uv);
+    }
+    uint32_t gcode, ucode;
+    const uint2 gq = blocks::quantize8(gv, gcode), uq = blocks::quantize8(uv, ucode);
+    if ((j & 3) == 0) {
+      kept.gate.codes[p.block] = static_cast<uint8_t>(gcode);
+      kept.up.codes[p.block] = static_cast<uint8_t>(ucode);
+    }
+    if (!p.there()) continue;
+    *reinterpret_cast<uint2*>(kept.gate.q + p.at()) = gq;
+    *reinterpret_cast<uint2*>(kept.up.q + p.at()) = uq;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) hv[i] = forward_one<DT>(gv[i], uv[i]);
+    blocks::store8<DT>(h + p.at(), hv);
   }
 }
 
@@ -196,6 +251,44 @@ __global__ __launch_bounds__(kThreads) void backward_kernel(const typename Elem<
        i += static_cast<int64_t>(gridDim.x) * kThreads) {
     float a, b;
     backward_one<DT>(E::load(dh, i), E::load(g, i), E::load(u, i), a, b);
+    E::store(dg, i, a);
+    E::store(du, i, b);
+  }
+}
+
+// The backward of g and u kept in 8-bit blocks: a quarter of a block a thread.
+template <int DT>
+__global__ __launch_bounds__(kThreads) void backward_blocks_kernel(const typename Elem<DT>::T* __restrict__ dh,
+                                                                   Pair kept, typename Elem<DT>::T* __restrict__ dg,
+                                                                   typename Elem<DT>::T* __restrict__ du,
+                                                                   int64_t cols, int64_t per_row, int64_t quarters) {
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kThreads;
+  for (int64_t j = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; j < quarters; j += step) {
+    const blocks::Quarter p(j, cols, per_row);
+    if (!p.there()) continue;
+    float hv[8], gv[8], uv[8], a[8], b[8];
+    blocks::load8<DT>(dh + p.at(), hv);
+    blocks::dequantize8(*reinterpret_cast<const uint2*>(kept.gate.q + p.at()), kept.gate.codes[p.block], gv);
+    blocks::dequantize8(*reinterpret_cast<const uint2*>(kept.up.q + p.at()), kept.up.codes[p.block], uv);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) backward_one<DT>(hv[i], gv[i], uv[i], a[i], b[i]);
+    blocks::store8<DT>(dg + p.at(), a);
+    blocks::store8<DT>(du + p.at(), b);
+  }
+}
+
+// Any width and alignment: an element a thread.
+template <int DT>
+__global__ __launch_bounds__(kThreads) void backward_blocks_any_kernel(
+    const typename Elem<DT>::T* __restrict__ dh, Pair kept, typename Elem<DT>::T* __restrict__ dg,
+    typename Elem<DT>::T* __restrict__ du, int64_t cols, int64_t per_row, int64_t n) {
+  using E = Elem<DT>;
+  for (int64_t i = blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x; i < n;
+       i += static_cast<int64_t>(gridDim.x) * kThreads) {
+    const int64_t row = i / cols, block = row * per_row + (i - row * cols) / blocks::kBlock;
+    float a, b;
+    backward_one<DT>(E::load(dh, i), blocks::dequantize1(kept.gate.q[i], kept.gate.codes[block]),
+                     blocks::dequantize1(kept.up.q[i], kept.up.codes[block]), a, b);
     E::store(dg, i, a);
     E::store(du, i, b);
   }
@@ -300,11 +393,51 @@ __device__ __forceinline__ void backward_x8(const uint4& hc, const uint4& gc, co
   }
 }
 
+// Where the sums' backward finds eight values of g or u, columns c .. c + 7 of
+// row t: in a 16-bit tensor, or in 8-bit blocks (whose values are exact in the type).
 template <int DT>
+struct Plain {
+  const uint16_t* p;
+  struct Held {
+    uint4 v;
+  };
+  __device__ __forceinline__ Held load(int64_t t, int64_t c, int64_t cols) const {
+    return Held{*reinterpret_cast<const uint4*>(p + t * cols + c)};
+  }
+  __device__ __forceinline__ static uint4 values(const Held& h) { return h.v; }
+};
+
+template <int DT>
+struct Kept {
+  blocks::Blocks b;
+  struct Held {
+    uint2 q;
+    uint32_t code;
+  };
+  __device__ __forceinline__ Held load(int64_t t, int64_t c, int64_t cols) const {
+    return Held{*reinterpret_cast<const uint2*>(b.q + t * cols + c),
+                b.codes[t * ((cols + blocks::kBlock - 1) / blocks::kBlock) + c / blocks::kBlock]};
+  }
+  __device__ __forceinline__ static uint4 values(const Held& h) {
+    float x[8];
+    blocks::dequantize8(h.q, h.code, x);
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (DT == QSTE_BF16)
+        w[i] = f32x2_to_bf16x2(x[2 * i], x[2 * i + 1]);
+      else
+        w[i] = static_cast<uint32_t>(f32_to_f16(x[2 * i])) | (static_cast<uint32_t>(f32_to_f16(x[2 * i + 1])) << 16);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+};
+
+template <int DT, class SRC>
 __global__ __launch_bounds__(kSumThreads) void backward_sums_kernel(
-    const uint16_t* __restrict__ dh, const uint16_t* __restrict__ g, const uint16_t* __restrict__ u,
-    uint16_t* __restrict__ dg, uint16_t* __restrict__ du, const float* __restrict__ off_g,
-    const float* __restrict__ off_u, int64_t samples, int64_t cols, int64_t ldo, float* __restrict__ part) {
+    const uint16_t* __restrict__ dh, SRC g, SRC u, uint16_t* __restrict__ dg, uint16_t* __restrict__ du,
+    const float* __restrict__ off_g, const float* __restrict__ off_u, int64_t samples, int64_t cols, int64_t ldo,
+    float* __restrict__ part) {
   constexpr int UNROLL = 4;
   constexpr int kPad = 17;
   constexpr int kRed = kSumWaves * 64 * kPad;
@@ -345,24 +478,25 @@ __global__ __launch_bounds__(kSumThreads) void backward_sums_kernel(
   if (c < cols) {
     int64_t t = t0;
     for (; t + UNROLL <= t1; t += UNROLL) {
-      uint4 hq[UNROLL], gq[UNROLL], uq[UNROLL];
+      uint4 hq[UNROLL];
+      typename SRC::Held gq[UNROLL], uq[UNROLL];
       float og[UNROLL], ou[UNROLL];
 #pragma unroll
       for (int k = 0; k < UNROLL; ++k) {
         const int64_t at = (t + k) * cols + c;
         hq[k] = *reinterpret_cast<const uint4*>(dh + at);
-        gq[k] = *reinterpret_cast<const uint4*>(g + at);
-        uq[k] = *reinterpret_cast<const uint4*>(u + at);
+        gq[k] = g.load(t + k, c, cols);
+        uq[k] = u.load(t + k, c, cols);
         og[k] = off_g[t + k];
         ou[k] = off_u[t + k];
       }
 #pragma unroll
-      for (int k = 0; k < UNROLL; ++k) one(hq[k], gq[k], uq[k], t + k, og[k], ou[k]);
+      for (int k = 0; k < UNROLL; ++k) one(hq[k], SRC::values(gq[k]), SRC::values(uq[k]), t + k, og[k], ou[k]);
     }
     for (; t < t1; ++t) {
       const int64_t at = t * cols + c;
-      one(*reinterpret_cast<const uint4*>(dh + at), *reinterpret_cast<const uint4*>(g + at),
-          *reinterpret_cast<const uint4*>(u + at), t, off_g[t], off_u[t]);
+      one(*reinterpret_cast<const uint4*>(dh + at), SRC::values(g.load(t, c, cols)), SRC::values(u.load(t, c, cols)), t,
+          off_g[t], off_u[t]);
     }
   }
   __syncthreads();  // every wave is done with the tables
@@ -399,6 +533,30 @@ inline bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15
 
 int launch_pack_affine_rows(const void*, int, uint8_t*, float*, float*, int64_t, int64_t, hipStream_t);
 
+// The forward that encodes h, for bf16 rows of at most 8 * kThreads chunks.
+template <bool KEPT>
+static void launch_encode(bool tab, const void* g, const void* u, void* h, uint8_t* packed, float* offset,
+                          float* scale, int64_t rows, int64_t cols, const swiglu::Pair& kept, hipStream_t s) {
+  using namespace swiglu;
+  const int64_t stride = cols / 8;
+  const unsigned grid = static_cast<unsigned>(tab ? kEncodeGroups : rows);
+  const auto* gp = static_cast<const uint16_t*>(g);
+  const auto* up = static_cast<const uint16_t*>(u);
+  auto* hp = static_cast<uint16_t*>(h);
+  if (stride <= 2 * kThreads && tab)
+    forward_encode_kernel<2, true, KEPT>
+        <<<grid, kThreads, 0, s>>>(gp, up, hp, packed, offset, scale, rows, cols, stride, kept);
+  else if (stride <= 2 * kThreads)
+    forward_encode_kernel<2, false, KEPT>
+        <<<grid, kThreads, 0, s>>>(gp, up, hp, packed, offset, scale, rows, cols, stride, kept);
+  else if (tab)
+    forward_encode_kernel<8, true, KEPT>
+        <<<grid, kThreads, 0, s>>>(gp, up, hp, packed, offset, scale, rows, cols, stride, kept);
+  else
+    forward_encode_kernel<8, false, KEPT>
+        <<<grid, kThreads, 0, s>>>(gp, up, hp, packed, offset, scale, rows, cols, stride, kept);
+}
+
 int launch_swiglu_forward(const void* g, const void* u, int dtype, void* h, uint8_t* packed, float* offset,
                           float* scale, int64_t rows, int64_t cols, hipStream_t s) {
   using namespace swiglu;
@@ -410,22 +568,7 @@ int launch_swiglu_forward(const void* g, const void* u, int dtype, void* h, uint
     // with at least kTabRows rows per workgroup of kEncodeGroups, each fills
     // the table once for its rows; fewer rows take a workgroup per row
     const bool tab = rows >= kTabRows * kEncodeGroups;
-    const unsigned grid = static_cast<unsigned>(tab ? kEncodeGroups : rows);
-    const auto* gp = static_cast<const uint16_t*>(g);
-    const auto* upp = static_cast<const uint16_t*>(u);
-    auto* hp = static_cast<uint16_t*>(h);
-    if (stride <= 2 * kThreads && tab)
-      forward_encode_kernel<2, true>
-          <<<grid, kThreads, 0, s>>>(gp, upp, hp, packed, offset, scale, rows, cols, stride);
-    else if (stride <= 2 * kThreads)
-      forward_encode_kernel<2, false>
-          <<<grid, kThreads, 0, s>>>(gp, upp, hp, packed, offset, scale, rows, cols, stride);
-    else if (tab)
-      forward_encode_kernel<8, true>
-          <<<grid, kThreads, 0, s>>>(gp, upp, hp, packed, offset, scale, rows, cols, stride);
-    else
-      forward_encode_kernel<8, false>
-          <<<grid, kThreads, 0, s>>>(gp, upp, hp, packed, offset, scale, rows, cols, stride);
+    launch_encode<false>(tab, g, u, h, packed, offset, scale, rows, cols, Pair{}, s);
     return static_cast<int>(hipGetLastError());
   }
   if (vec) {
@@ -511,12 +654,12 @@ int launch_swiglu_backward_sums(const void* dh, const void* g, const void* u, in
     const dim3 grid(static_cast<unsigned>((cols + 511) / 512), static_cast<unsigned>(chunks));
     if (dtype == QSTE_BF16)
       backward_sums_kernel<QSTE_BF16><<<grid, kSumThreads, 0, s>>>(
-          static_cast<const uint16_t*>(dh), static_cast<const uint16_t*>(g), static_cast<const uint16_t*>(u),
-          static_cast<uint16_t*>(dg), static_cast<uint16_t*>(du), off_g, off_u, rows, cols, ld_out, part);
+          static_cast<const uint16_t*>(dh), Plain<QSTE_BF16>{static_cast<const uint16_t*>(g)},
+          Plain<QSTE_BF16>{static_cast<const uint16_t*>(u)}, static_cast<uint16_t*>(dg), static_cast<uint16_t*>(du), off_g, off_u, rows, cols, ld_out, part);
     else
       backward_sums_kernel<QSTE_F16><<<grid, kSumThreads, 0, s>>>(
-          static_cast<const uint16_t*>(dh), static_cast<const uint16_t*>(g), static_cast<const uint16_t*>(u),
-          static_cast<uint16_t*>(dg), static_cast<uint16_t*>(du), off_g, off_u, rows, cols, ld_out, part);
+          static_cast<const uint16_t*>(dh), Plain<QSTE_F16>{static_cast<const uint16_t*>(g)},
+          Plain<QSTE_F16>{static_cast<const uint16_t*>(u)}, static_cast<uint16_t*>(dg), static_cast<uint16_t*>(du), off_g, off_u, rows, cols, ld_out, part);
     const int rc = static_cast<int>(hipGetLastError());
     if (rc) return rc;
     return launch_sum_partials(part, chunks, 2 * cols, sums, s);
@@ -524,6 +667,112 @@ int launch_swiglu_backward_sums(const void* dh, const void* g, const void* u, in
   // any other dtype or layout: the plain pass, then the layers' own column
   // sums over what it wrote
   int rc = launch_swiglu_backward(dh, g, u, dtype, dg, du, rows * cols, s);
+  if (rc) return rc;
+  if ((rc = launch_colsums(dg, dtype, off_g, rows, cols, part, nullptr, sums, nullptr, s))) return rc;
+  return launch_colsums(du, dtype, off_u, rows, cols, part, nullptr, sums + cols, nullptr, s);
+}
+
+// ---------------------------------------------------------------------------
+// with g and u kept in 8-bit blocks
+// ---------------------------------------------------------------------------
+
+int launch_quantize_blocks(const void*, int, int8_t*, uint8_t*, int64_t, int64_t, hipStream_t);
+
+namespace swiglu {
+
+inline bool aligned8(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7) == 0; }
+inline bool kept_ok(const Pair& kept, int64_t cols) { return cols % 8 == 0 && aligned8(kept.gate.q) && aligned8(kept.up.q); }
+
+template <int DT>
+void run_forward_blocks(const void* g, const void* u, void* h, const Pair& kept, int64_t rows, int64_t cols,
+                        hipStream_t s) {
+  using T = typename Elem<DT>::T;
+  const int64_t per_row = blocks::blocks_of(cols), quarters = 4 * rows * per_row;
+  forward_blocks_kernel<DT><<<grid_of(quarters), kThreads, 0, s>>>(
+      static_cast<const T*>(g), static_cast<const T*>(u), static_cast<T*>(h), kept, cols, per_row, quarters);
+}
+
+template <int DT>
+void run_backward_blocks(const void* dh, const Pair& kept, void* dg, void* du, int64_t rows, int64_t cols,
+                         hipStream_t s) {
+  using T = typename Elem<DT>::T;
+  const int64_t per_row = blocks::blocks_of(cols), quarters = 4 * rows * per_row;
+  if (kept_ok(kept, cols) && aligned(dh) && aligned(dg) && aligned(du))
+    backward_blocks_kernel<DT><<<grid_of(quarters), kThreads, 0, s>>>(
+        static_cast<const T*>(dh), kept, static_cast<T*>(dg), static_cast<T*>(du), cols, per_row, quarters);
+  else
+    backward_blocks_any_kernel<DT><<<grid_of(rows * cols), kThreads, 0, s>>>(
+        static_cast<const T*>(dh), kept, static_cast<T*>(dg), static_cast<T*>(du), cols, per_row, rows * cols);
+}
+
+template <int DT>
+int run_backward_blocks_sums(const void* dh, const Pair& kept, void* dg, void* du, const float* off_g,
+                             const float* off_u, int64_t rows, int64_t cols, float* sums, float* part, hipStream_t s,
+                             int64_t ld_out) {
+  const int64_t chunks = (rows + kSumChunk - 1) / kSumChunk;
+  const dim3 grid(static_cast<unsigned>((cols + 511) / 512), static_cast<unsigned>(chunks));
+  backward_sums_kernel<DT><<<grid, kSumThreads, 0, s>>>(
+      static_cast<const uint16_t*>(dh), Kept<DT>{kept.gate}, Kept<DT>{kept.up}, static_cast<uint16_t*>(dg),
+      static_cast<uint16_t*>(du), off_g, off_u, rows, cols, ld_out, part);
+  const int rc = static_cast<int>(hipGetLastError());
+  return rc ? rc : launch_sum_partials(part, chunks, 2 * cols, sums, s);
+}
+
+}  // namespace swiglu
+
+int launch_swiglu_forward_blocks(const void* g, const void* u, int dtype, void* h, uint8_t* packed, float* offset,
+                                 float* scale, int8_t* gq, uint8_t* gcodes, int8_t* uq, uint8_t* ucodes, int64_t rows,
+                                 int64_t cols, hipStream_t s) {
+  using namespace swiglu;
+  const Pair kept{{gq, gcodes}, {uq, ucodes}};
+  if (!kept_ok(kept, cols) || !aligned(g) || !aligned(u) || !aligned(h)) {
+    // any width: the pass without a checkpoint, and the blocks from g and u
+    int rc = launch_swiglu_forward(g, u, dtype, h, packed, offset, scale, rows, cols, s);
+    if (rc) return rc;
+    if ((rc = launch_quantize_blocks(g, dtype, gq, gcodes, rows, cols, s))) return rc;
+    return launch_quantize_blocks(u, dtype, uq, ucodes, rows, cols, s);
+  }
+  if (packed && dtype == QSTE_BF16 && cols / 8 <= 8 * kThreads) {
+    launch_encode<true>(rows >= kTabRows * kEncodeGroups, g, u, h, packed, offset, scale, rows, cols, kept, s);
+    return static_cast<int>(hipGetLastError());
+  }
+  if (dtype == QSTE_F32) run_forward_blocks<QSTE_F32>(g, u, h, kept, rows, cols, s);
+  else if (dtype == QSTE_F16) run_forward_blocks<QSTE_F16>(g, u, h, kept, rows, cols, s);
+  else run_forward_blocks<QSTE_BF16>(g, u, h, kept, rows, cols, s);
+  const int rc = static_cast<int>(hipGetLastError());
+  if (rc || !packed) return rc;
+  return launch_pack_affine_rows(h, dtype, packed, offset, scale, rows, cols, s);
+}
+
+int launch_swiglu_backward_blocks(const void* dh, int dtype, const int8_t* gq, const uint8_t* gcodes, const int8_t* uq,
+                                  const uint8_t* ucodes, void* dg, void* du, int64_t rows, int64_t cols,
+                                  hipStream_t s) {
+  using namespace swiglu;
+  const Pair kept{{const_cast<int8_t*>(gq), const_cast<uint8_t*>(gcodes)},
+                  {const_cast<int8_t*>(uq), const_cast<uint8_t*>(ucodes)}};
+  if (dtype == QSTE_F32) run_backward_blocks<QSTE_F32>(dh, kept, dg, du, rows, cols, s);
+  else if (dtype == QSTE_F16) run_backward_blocks<QSTE_F16>(dh, kept, dg, du, rows, cols, s);
+  else run_backward_blocks<QSTE_BF16>(dh, kept, dg, du, rows, cols, s);
+  return static_cast<int>(hipGetLastError());
+}
+
+// sums and part as launch_swiglu_backward_sums has them
+int launch_swiglu_backward_blocks_sums(const void* dh, int dtype, const int8_t* gq, const uint8_t* gcodes,
+                                       const int8_t* uq, const uint8_t* ucodes, void* dg, void* du, const float* off_g,
+                                       const float* off_u, int64_t rows, int64_t cols, float* sums, float* part,
+                                       hipStream_t s, int64_t ld_out) {
+  using namespace swiglu;
+  const Pair kept{{const_cast<int8_t*>(gq), const_cast<uint8_t*>(gcodes)},
+                  {const_cast<int8_t*>(uq), const_cast<uint8_t*>(ucodes)}};
+  if ((dtype == QSTE_BF16 || dtype == QSTE_F16) && kept_ok(kept, cols) && aligned(dh) && aligned(dg) && aligned(du) &&
+      ld_out % 8 == 0)
+    return dtype == QSTE_BF16 ? run_backward_blocks_sums<QSTE_BF16>(dh, kept, dg, du, off_g, off_u, rows, cols, sums,
+                                                                   part, s, ld_out)
+                              : run_backward_blocks_sums<QSTE_F16>(dh, kept, dg, du, off_g, off_u, rows, cols, sums,
+                                                                  part, s, ld_out);
+  // outputs with a row pitch of their own are written by the 8-wide pass only
+  if (ld_out != cols) return QSTE_E_ALIGN;
+  int rc = launch_swiglu_backward_blocks(dh, dtype, gq, gcodes, uq, ucodes, dg, du, rows, cols, s);
   if (rc) return rc;
   if ((rc = launch_colsums(dg, dtype, off_g, rows, cols, part, nullptr, sums, nullptr, s))) return rc;
   return launch_colsums(du, dtype, off_u, rows, cols, part, nullptr, sums + cols, nullptr, s);

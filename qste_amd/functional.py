@@ -19,8 +19,10 @@ import weakref
 import torch
 from torch import Tensor
 from torch.autograd import Function
+from torch.autograd.function import once_differentiable
 
 from . import kernels
+from .losses import _no_tangent
 from .surface import Surface
 
 
@@ -177,18 +179,48 @@ class QSTEWeightFn(Function):
         return None, grad_scale.to(scale.dtype), None
 
 
+def _save_kept(ctx, gate: kernels.Blocks8, up: kernels.Blocks8, *more: Tensor) -> None:
+    """Saves gate's and up's 8-bit blocks, and ``more`` after them."""
+
+    ctx.kept_dtype = gate.dtype
+    ctx.save_for_backward(gate.payload, gate.codes, up.payload, up.codes, *more)
+
+
+def _kept(ctx, saved) -> tuple:
+    """g and u as a forward saved them: two tensors, or with a checkpoint the first four as two ``Blocks8``."""
+
+    if not ctx.checkpoint:
+        return saved[:2]
+    gate_payload, gate_codes, up_payload, up_codes = saved[:4]
+    return (kernels.Blocks8(gate_payload, gate_codes, ctx.kept_dtype),
+            kernels.Blocks8(up_payload, up_codes, ctx.kept_dtype))
+
+
+def _flat_blocks(b: kernels.Blocks8) -> kernels.Blocks8:
+    """Blocks of a tensor as those of its rows."""
+
+    return kernels.Blocks8(b.payload.reshape(-1, b.payload.shape[-1]), b.codes.reshape(-1, b.codes.shape[-1]), b.dtype)
+
+
 class SwiGLUFn(Function):
     """``silu(gate) * up`` in one kernel each way, rounded as torch's
     ``F.silu(gate) * up`` and its autograd round, keeping ``gate`` and ``up``
     for backward.  With ``encode`` the forward also encodes the output's rows
     for the binary layer that reads it next (a SwiGLU MLP's down
-    projection), which then does not read the output again to encode it."""
+    projection), which then does not read the output again to encode it.  With
+    ``checkpoint`` gate and up are kept in 8-bit blocks, and the gradients are
+    those at the values that the blocks stand for."""
 
     @staticmethod
-    def forward(ctx, gate, up, encode: bool):
+    def forward(ctx, gate, up, encode: bool, checkpoint: bool):
         forget_offers()
-        out, encoding = kernels.swiglu_forward(gate, up, encode=encode)
-        ctx.save_for_backward(gate, up)
+        ctx.checkpoint = checkpoint
+        if checkpoint:
+            out, encoding, *kept = kernels.swiglu_forward_blocks(gate, up, encode=encode)
+            _save_kept(ctx, *kept)
+        else:
+            out, encoding = kernels.swiglu_forward(gate, up, encode=encode)
+            ctx.save_for_backward(gate, up)
         if encoding is not None:
             packed, offset, scale = encoding
             remember_encoding(out, packed, kernels.stacked_pair(offset, scale))
@@ -205,20 +237,109 @@ class SwiGLUFn(Function):
     @staticmethod
     def backward(ctx, grad_output):
         forget_offers()
-        gate, up = ctx.saved_tensors
+        gate, up = _kept(ctx, ctx.saved_tensors)
         if ctx.auxes is None:
-            grad_gate, grad_up = kernels.swiglu_backward(grad_output.contiguous(), gate, up)
-            return grad_gate, grad_up, None
+            backward = kernels.swiglu_backward_blocks if ctx.checkpoint else kernels.swiglu_backward
+            grad_gate, grad_up = backward(grad_output.contiguous(), gate, up)
+            return grad_gate, grad_up, None, None
         # the gradients and, for the two layers' backward, their offset sums
         aux_g, aux_u = ctx.auxes
-        cols = gate.shape[-1]
-        grad_gate, grad_up, sums = kernels.swiglu_backward_sums(
-            grad_output.reshape(-1, cols), gate.reshape(-1, cols), up.reshape(-1, cols), aux_g[0], aux_u[0])
-        grad_gate, grad_up = grad_gate.view(gate.shape), grad_up.view(up.shape)
+        shape = grad_output.shape
+        flat = grad_output.reshape(-1, shape[-1])
+        if ctx.checkpoint:
+            grad_gate, grad_up, sums = kernels.swiglu_backward_blocks(
+                flat, _flat_blocks(gate), _flat_blocks(up), aux_g[0], aux_u[0])
+        else:
+            grad_gate, grad_up, sums = kernels.swiglu_backward_sums(
+                flat, gate.reshape(flat.shape), up.reshape(flat.shape), aux_g[0], aux_u[0])
+        grad_gate, grad_up = grad_gate.view(shape), grad_up.view(shape)
         _offer_offset_dot(grad_gate, aux_g, sums[0])
         _offer_offset_dot(grad_up, aux_u, sums[1])
         torch.autograd.Variable._execution_engine.queue_callback(forget_offers)
-        return grad_gate, grad_up, None
+        return grad_gate, grad_up, None, None
+
+
+def _cast(grad: Tensor | None, dtype: torch.dtype | None) -> Tensor | None:
+    return None if grad is None or dtype is None else grad.to(dtype)
+
+
+def _through_scale(grad_scale: Tensor, e: Tensor, surface: Surface) -> Tensor:
+    """The scale's gradient carried to the log-scale, as RowScaleFn does."""
+
+    return kernels.row_scale_backward(e, grad_scale.to(e.dtype), surface.cfg.scale_min, surface.cfg.scale_max)
+
+
+def _gate_up_backward(ctx, dh: list, kept: tuple, payload_x: Tensor, aux_x: Tensor, packed_g: Tensor, scale_g: Tensor,
+                      packed_u: Tensor, scale_u: Tensor, sg: Surface, su: Surface):
+    """The gate's backward and that of the two layers before it as one layer of 2
+    ffn rows, their evidence delivered: ``(dx, gate's and up's scale gradients and
+    bias gradients)``.  ``dh``: the gradient of h in a list, taken out of it so that it
+    is free during the product; ``kept``: g and u, as tensors or ``Blocks8``."""
+
+    d, ffn = sg.columns, sg.rows
+    backward = kernels.swiglu_backward_blocks if isinstance(kept[0], kernels.Blocks8) else kernels.swiglu_backward_sums
+    both, sums = backward(dh.pop(), *kept, aux_x[0], aux_x[0], side_by_side=True)
+    # gate and up as one layer of 2 ffn rows (copies of their signs and
+    # scales: the deliveries below may rewrite the signs)
+    packed_gu = torch.cat((packed_g, packed_u))
+    scale_gu = torch.cat((scale_g.detach().float(), scale_u.detach().float()))
+    bg, bu = ctx.bias_dtypes[:2]
+    need_bias = bg is not None or bu is not None
+    dx, ev_gu, gs_gu, gb_gu = kernels.linear_backward(
+        both, payload_x, aux_x[0], aux_x[1], packed_gu, scale_gu, d, need_bias=need_bias,
+        need_input=ctx.needs_input_grad[0], offset_dot=sums.reshape(-1))
+    del both
+    if dx is not None:
+        dx = dx.reshape(ctx.input_shape)
+    sg.consume_evidence(ev_gu[:ffn])
+    su.consume_evidence(ev_gu[ffn:])
+    gb_g, gb_u = (gb_gu[:ffn], gb_gu[ffn:]) if need_bias else (None, None)
+    return dx, gs_gu[:ffn], gs_gu[ffn:], gb_g, gb_u
+
+
+class GatedFn(Function):
+    """``silu(gate(x)) * up(x)`` of two binary layers as one autograd node.
+
+    The forward is one kernel over both layers' signs (``kernels.gated_forward``)
+    and x's encoding; what it keeps of g and u is them, or with ``checkpoint``
+    their 8-bit blocks.  The backward is the gate and up layers' part of
+    SwiGLUMLPFn's."""
+
+    @staticmethod
+    def forward(ctx, inputs, packed_g, log_g, bias_g, packed_u, log_u, bias_u, surfaces, checkpoint: bool,
+                grad_on: bool):
+        sg, su = surfaces
+        d = sg.columns
+        flat = inputs.reshape(-1, d)
+        scale_g, e_g = kernels.row_scale(log_g, sg.cfg.scale_min, sg.cfg.scale_max)
+        scale_u, e_u = kernels.row_scale(log_u, su.cfg.scale_min, su.cfg.scale_max)
+        keep = "" if not grad_on else "blocks" if checkpoint else "values"
+        h, g, u = kernels.gated_forward(flat, packed_g, scale_g, bias_g, packed_u, scale_u, bias_u, d, keep=keep)
+        if grad_on:
+            payload_x, aux_x = _encoding_of(inputs, flat, d)
+            more = (payload_x, aux_x, packed_g, scale_g, packed_u, scale_u, e_g, e_u)
+            if checkpoint:
+                _save_kept(ctx, g, u, *more)
+            else:
+                ctx.save_for_backward(g, u, *more)
+        ctx.checkpoint = checkpoint
+        ctx.surfaces = surfaces
+        ctx.input_shape = inputs.shape
+        ctx.bias_dtypes = tuple(None if b is None else b.dtype for b in (bias_g, bias_u))
+        return h.reshape(*inputs.shape[:-1], sg.rows)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_output):
+        forget_encodings()
+        saved = ctx.saved_tensors
+        payload_x, aux_x, packed_g, scale_g, packed_u, scale_u, e_g, e_u = saved[-8:]
+        sg, su = ctx.surfaces
+        dx, gs_g, gs_u, gb_g, gb_u = _gate_up_backward(ctx, [grad_output.reshape(-1, sg.rows)], _kept(ctx, saved),
+                                                       payload_x, aux_x, packed_g, scale_g, packed_u, scale_u, sg, su)
+        bg, bu = ctx.bias_dtypes
+        return (dx, None, _through_scale(gs_g, e_g, sg), _cast(gb_g, bg), None, _through_scale(gs_u, e_u, su),
+                _cast(gb_u, bu), None, None, None)
 
 
 class SwiGLUMLPFn(Function):
@@ -249,7 +370,7 @@ class SwiGLUMLPFn(Function):
 
     @staticmethod
     def forward(ctx, inputs, packed_g, log_g, bias_g, packed_u, log_u, bias_u, packed_d, log_d, bias_d,
-                surfaces, grad_on: bool):
+                surfaces, checkpoint: bool, grad_on: bool):
         sg, su, sd = surfaces
         d, ffn = sg.columns, sg.rows
         flat = inputs.reshape(-1, d)
@@ -257,17 +378,28 @@ class SwiGLUMLPFn(Function):
         # before the product that needs it, so the first product is queued
         # after one small launch rather than three
         scale_g, e_g = kernels.row_scale(log_g, sg.cfg.scale_min, sg.cfg.scale_max)
-        g = kernels.packed_linear_affine(flat, packed_g, scale_g, bias_g, d)
-        scale_u, e_u = kernels.row_scale(log_u, su.cfg.scale_min, su.cfg.scale_max)
-        u = kernels.packed_linear_affine(flat, packed_u, scale_u, bias_u, d)
-        h, enc = kernels.swiglu_forward(g, u, encode=grad_on)
+        checkpoint = checkpoint and grad_on
+        if checkpoint:
+            scale_u, e_u = kernels.row_scale(log_u, su.cfg.scale_min, su.cfg.scale_max)
+            h, g, u = kernels.gated_forward(flat, packed_g, scale_g, bias_g, packed_u, scale_u, bias_u, d, keep="blocks")
+            enc = kernels.pack_affine_rows(h)
+        else:
+            g = kernels.packed_linear_affine(flat, packed_g, scale_g, bias_g, d)
+            scale_u, e_u = kernels.row_scale(log_u, su.cfg.scale_min, su.cfg.scale_max)
+            u = kernels.packed_linear_affine(flat, packed_u, scale_u, bias_u, d)
+            h, enc = kernels.swiglu_forward(g, u, encode=grad_on)
         scale_d, e_d = kernels.row_scale(log_d, sd.cfg.scale_min, sd.cfg.scale_max)
         y = kernels.packed_linear_affine(h, packed_d, scale_d, bias_d, ffn)
         if grad_on:
             payload_x, aux_x = _encoding_of(inputs, flat, d)
             aux_h = kernels.stacked_pair(enc[1], enc[2])
-            ctx.save_for_backward(payload_x, aux_x, g, u, enc[0], aux_h, packed_g, scale_g, packed_u, scale_u,
-                                  packed_d, scale_d, e_g, e_u, e_d)
+            more = (payload_x, aux_x, enc[0], aux_h, packed_g, scale_g, packed_u, scale_u, packed_d, scale_d, e_g, e_u,
+                    e_d)
+            if checkpoint:
+                _save_kept(ctx, g, u, *more)
+            else:
+                ctx.save_for_backward(g, u, *more)
+        ctx.checkpoint = checkpoint
         ctx.surfaces = surfaces
         ctx.input_shape = inputs.shape
         ctx.bias_dtypes = tuple(None if b is None else b.dtype for b in (bias_g, bias_u, bias_d))
@@ -276,8 +408,10 @@ class SwiGLUMLPFn(Function):
     @staticmethod
     def backward(ctx, grad_output):
         forget_encodings()
-        (payload_x, aux_x, g, u, payload_h, aux_h, packed_g, scale_g, packed_u, scale_u, packed_d,
-         scale_d, e_g, e_u, e_d) = ctx.saved_tensors
+        saved = ctx.saved_tensors
+        kept = _kept(ctx, saved)
+        (payload_x, aux_x, payload_h, aux_h, packed_g, scale_g, packed_u, scale_u, packed_d, scale_d, e_g, e_u,
+         e_d) = saved[-13:]
         sg, su, sd = ctx.surfaces
         d, ffn = sg.columns, sg.rows
         bg, bu, bd = ctx.bias_dtypes
@@ -290,33 +424,12 @@ class SwiGLUMLPFn(Function):
             dy, payload_h, aux_h[0], aux_h[1], packed_d, scale_d.detach(), ffn, need_bias=bd is not None)
         sd.consume_evidence(ev_d)
         del ev_d
-        both, sums = kernels.swiglu_backward_sums(dh, g, u, aux_x[0], aux_x[0], side_by_side=True)
-        del dh
-        # gate and up as one layer of 2 ffn rows (copies of their signs and
-        # scales: the deliveries below may rewrite the signs)
-        packed_gu = torch.cat((packed_g, packed_u))
-        scale_gu = torch.cat((scale_g.detach().float(), scale_u.detach().float()))
-        need_bias = bg is not None or bu is not None
-        dx, ev_gu, gs_gu, gb_gu = kernels.linear_backward(
-            both, payload_x, aux_x[0], aux_x[1], packed_gu, scale_gu, d, need_bias=need_bias,
-            need_input=ctx.needs_input_grad[0], offset_dot=sums.reshape(-1))
-        del both
-        if dx is not None:
-            dx = dx.reshape(ctx.input_shape)
-        sg.consume_evidence(ev_gu[:ffn])
-        su.consume_evidence(ev_gu[ffn:])
-        gs_g, gs_u = gs_gu[:ffn], gs_gu[ffn:]
-        gb_g, gb_u = (gb_gu[:ffn], gb_gu[ffn:]) if need_bias else (None, None)
+        dh = [dh]
+        dx, gs_g, gs_u, gb_g, gb_u = _gate_up_backward(ctx, dh, kept, payload_x, aux_x, packed_g, scale_g, packed_u, scale_u,
+                                                       sg, su)
 
-        def cast(grad, dtype):
-            return None if grad is None or dtype is None else grad.to(dtype)
-
-        def through_scale(gs, e, surface):
-            # the scale's gradient carried to the log-scale, as RowScaleFn does
-            return kernels.row_scale_backward(e, gs.to(e.dtype), surface.cfg.scale_min, surface.cfg.scale_max)
-
-        return (dx, None, through_scale(gs_g, e_g, sg), cast(gb_g, bg), None, through_scale(gs_u, e_u, su),
-                cast(gb_u, bu), None, through_scale(gs_d, e_d, sd), cast(gb_d, bd), None, None)
+        return (dx, None, _through_scale(gs_g, e_g, sg), _cast(gb_g, bg), None, _through_scale(gs_u, e_u, su),
+                _cast(gb_u, bu), None, _through_scale(gs_d, e_d, sd), _cast(gb_d, bd), None, None, None)
 
 
 # log-scale dtypes the row-scale kernels take (surface.row_scale)
@@ -336,16 +449,34 @@ def swiglu_mlp_fusable(inputs: Tensor, gate, up, down) -> bool:
             and all(s.log_scale.is_cuda and s.log_scale.dtype in _SCALE_DTYPES for s in (sg, su, sd)))
 
 
-def swiglu(gate: Tensor, up: Tensor) -> Tensor:
+def gated_fusable(inputs: Tensor, gate, up) -> bool:
+    """Whether ``GatedFn`` takes this block: a bf16 or fp16 input on the GPU,
+    its columns a multiple of 64 and the layers' rows of 8."""
+
+    sg, su = gate.surface, up.surface
+    return (inputs.is_cuda and inputs.dtype in (torch.bfloat16, torch.float16) and inputs.dim() >= 1
+            and inputs.shape[-1] == sg.columns == su.columns and sg.rows == su.rows and sg.columns % 64 == 0
+            and sg.rows % 8 == 0 and inputs.numel() > 0
+            and all(s.log_scale.is_cuda and s.log_scale.dtype in _SCALE_DTYPES for s in (sg, su)))
+
+
+def swiglu(gate: Tensor, up: Tensor, *, checkpoint: bool = False) -> Tensor:
     """The SwiGLU gate ``F.silu(gate) * up`` (same values and gradients), fused.
 
     No counterpart in the reference; a SwiGLU MLP written
     ``down(swiglu(gate(x), up(x)))`` computes what
     ``down(F.silu(gate(x)) * up(x))`` computes, with two elementwise passes
     instead of five and the down projection's activation encoding produced
-    with its input."""
+    with its input.
 
-    return SwiGLUFn.apply(gate, up, torch.is_grad_enabled())
+    With ``checkpoint`` what is kept of gate and up for the backward are 8-bit
+    blocks of 32 columns, 33 bytes for 32 elements: the value is the same, the
+    gradients are those at the blocks' values (``nn.quantize_blocks``)."""
+
+    if checkpoint:
+        _no_tangent("swiglu with a checkpoint", gate, up)
+    grad_on = torch.is_grad_enabled()
+    return SwiGLUFn.apply(gate, up, grad_on, checkpoint and grad_on and (gate.requires_grad or up.requires_grad))
 
 
 def qste_weight(surface: Surface) -> Tensor:

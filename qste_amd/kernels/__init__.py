@@ -13,7 +13,9 @@ workspaces the C entry points ask for; the library itself never allocates.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
+from typing import NamedTuple
 
 import torch
 from torch import Tensor
@@ -32,13 +34,16 @@ __all__ = [
     "smooth_activation",
     "smooth_backward",
     "unpack_bits",
+    "Blocks8",
     "coordinate_update",
     "cuda_available",
+    "dequantize_blocks",
     "distill_backward",
     "distill_forward",
     "embedding_backward",
     "packed_embedding",
     "evidence_from_packed",
+    "gated_forward",
     "linear_backward",
     "native_available",
     "pack_affine_rows",
@@ -46,9 +51,12 @@ __all__ = [
     "packed_linear_affine",
     "packed_row_inner",
     "packed_transpose",
+    "quantize_blocks",
     "status",
     "swiglu_backward",
+    "swiglu_backward_blocks",
     "swiglu_forward",
+    "swiglu_forward_blocks",
     "token_logprobs_backward",
     "token_logprobs_forward",
     "unpack_rows",
@@ -791,6 +799,217 @@ def swiglu_backward_sums(grad: Tensor, gate: Tensor, up: Tensor, offset_gate: Te
         _ptr(sums), rows, cols, _ptr(work), work.numel(), _stream(device))
     _lib.check(code, "swiglu_backward_sums")
     return dg, du, sums
+
+
+# ---------------------------------------------------------------------------
+# 8-bit blocks, and the gated feed-forward block (no counterparts in the reference)
+# ---------------------------------------------------------------------------
+
+BLOCK = 32  # columns that share a power of two, as in csrc/blocks.hpp
+
+
+class Blocks8(NamedTuple):
+    """A tensor in 8-bit blocks: ``payload * 2 ** (codes - 133)``, a code for every
+    32 columns of a row (the last may have fewer)."""
+
+    payload: Tensor  # int8, the tensor's shape
+    codes: Tensor  # uint8 [..., ceil(columns / 32)]
+    dtype: torch.dtype  # the tensor's
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _device_of(device: torch.device):
+    """A context in which the library's launches go to ``device``: nothing where that is the current one."""
+
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _blocks_like(t: Tensor) -> Blocks8:
+    """Room for t's blocks."""
+
+    codes = torch.empty(*t.shape[:-1], -(-t.shape[-1] // BLOCK), dtype=torch.uint8, device=t.device)
+    return Blocks8(torch.empty(t.shape, dtype=torch.int8, device=t.device), codes, t.dtype)
+
+
+def _check_blocks(b: Blocks8, what: str) -> Blocks8:
+    payload, codes, dtype = b
+    if payload.dtype != torch.int8 or codes.dtype != torch.uint8:
+        raise TypeError(f"{what} need an int8 payload and uint8 codes, got {payload.dtype} and {codes.dtype}")
+    if dtype not in _DTYPES:
+        raise TypeError(f"unsupported dtype {dtype}; expected float32, float16 or bfloat16")
+    if payload.dim() == 0 or codes.shape != (*payload.shape[:-1], -(-payload.shape[-1] // BLOCK)):
+        raise ValueError(f"{what} with a payload of shape {tuple(payload.shape)} have codes of shape "
+                         f"{tuple(codes.shape)}")
+    return Blocks8(payload.contiguous(), codes.contiguous(), dtype)
+
+
+def _rows_of(t: Tensor) -> tuple[int, int]:
+    """(rows, columns) of a tensor over its last dimension."""
+
+    cols = int(t.shape[-1])
+    return (t.numel() // cols if cols else 0), cols
+
+
+def quantize_blocks(values: Tensor) -> Blocks8:
+    """``values`` (fp32, fp16 or bf16, any shape but a scalar's) in 8-bit blocks along the last dimension."""
+
+    device = _require_gpu(values)
+    code = _dtype_code(values)
+    if values.dim() == 0:
+        raise ValueError("quantize_blocks needs at least one dimension")
+    x = values.detach().contiguous()
+    out = _blocks_like(x)
+    with _device_of(device):
+        _lib.check(_lib.load().qste_quantize_blocks(_ptr(x), code, _ptr(out.payload), _ptr(out.codes), *_rows_of(x),
+                                                    _stream(device)), "quantize_blocks")
+    return out
+
+
+def dequantize_blocks(blocks: Blocks8, dtype: torch.dtype | None = None) -> Tensor:
+    """What ``blocks`` stand for, in their own dtype (exactly) or in ``dtype`` (rounded once)."""
+
+    payload, codes, own = _check_blocks(blocks, "blocks")
+    device = _require_gpu(payload, codes)
+    out = torch.empty(payload.shape, dtype=own if dtype is None else dtype, device=device)
+    code = _dtype_code(out)
+    with _device_of(device):
+        _lib.check(_lib.load().qste_dequantize_blocks(_ptr(payload), _ptr(codes), _ptr(out), code, *_rows_of(out),
+                                                      _stream(device)), "dequantize_blocks")
+    return out
+
+
+def swiglu_forward_blocks(gate: Tensor, up: Tensor, *, encode: bool = False):
+    """``swiglu_forward`` that also keeps gate and up in 8-bit blocks, from the
+    same pass.  Returns ``(out, encoding, gate blocks, up blocks)``."""
+
+    device = _require_gpu(gate, up)
+    if gate.shape != up.shape or gate.dtype != up.dtype:
+        raise ValueError("gate and up must have the same shape and dtype")
+    code = _dtype_code(gate)
+    if gate.dim() == 0:
+        raise ValueError("swiglu with a checkpoint needs at least one dimension")
+    g, u = _aligned(gate), _aligned(up)
+    rows, cols = _rows_of(g)
+    out, kept_g, kept_u = torch.empty_like(g), _blocks_like(g), _blocks_like(g)
+    packed = offset = scale = None
+    if encode:
+        packed = torch.empty(rows, _packed_width(cols), dtype=torch.uint8, device=device)
+        offset, scale = torch.empty(2, rows, dtype=torch.float32, device=device).unbind(0)
+    with _device_of(device):
+        _lib.check(_lib.load().qste_swiglu_forward_blocks(
+            _ptr(g), _ptr(u), code, _ptr(out), _ptr(packed), _ptr(offset), _ptr(scale), _ptr(kept_g.payload),
+            _ptr(kept_g.codes), _ptr(kept_u.payload), _ptr(kept_u.codes), rows, cols, _stream(device)),
+            "swiglu_forward_blocks")
+    return out, ((packed, offset, scale) if encode else None), kept_g, kept_u
+
+
+def swiglu_backward_blocks(grad: Tensor, gate: Blocks8, up: Blocks8, offset_gate: Tensor | None = None,
+                           offset_up: Tensor | None = None, *, side_by_side: bool = False):
+    """``swiglu_backward`` with the gate and up that 8-bit blocks stand for:
+    ``(grad_gate, grad_up)``; with offsets fp32 [rows] what ``swiglu_backward_sums``
+    returns (``side_by_side`` as there)."""
+
+    gate, up = _check_blocks(gate, "gate blocks"), _check_blocks(up, "up blocks")
+    device = _require_gpu(grad, gate.payload, gate.codes, up.payload, up.codes, offset_gate, offset_up)
+    if not (grad.shape == gate.payload.shape == up.payload.shape) or not (grad.dtype == gate.dtype == up.dtype):
+        raise ValueError("grad and the blocks of gate and up must have the same shape and dtype")
+    code = _dtype_code(grad)
+    dh = _aligned(grad)
+    rows, cols = _rows_of(dh)
+    kept = (_ptr(gate.payload), _ptr(gate.codes), _ptr(up.payload), _ptr(up.codes))
+    lib = _lib.load()
+    if offset_gate is None and offset_up is None:
+        if side_by_side:
+            raise ValueError("side_by_side needs the offsets")
+        dg, du = torch.empty_like(dh), torch.empty_like(dh)
+        with _device_of(device):
+            _lib.check(lib.qste_swiglu_backward_blocks(_ptr(dh), code, *kept, _ptr(dg), _ptr(du), rows, cols,
+                                                       _stream(device)), "swiglu_backward_blocks")
+        return dg, du
+    offs = []
+    for name, o in (("offset_gate", offset_gate), ("offset_up", offset_up)):
+        if o is None or o.dtype != torch.float32 or o.numel() != rows:
+            raise ValueError(f"{name} must be fp32 [rows]")
+        offs.append(o.contiguous())
+    if side_by_side and (dh.dtype == torch.float32 or cols % 8):
+        raise ValueError("side_by_side needs a 16-bit dtype and columns in whole eights")
+    sums = torch.empty(2, cols, dtype=torch.float32, device=device)
+    work = _workspace(lib.qste_swiglu_backward_sums_workspace_bytes(rows, cols), device)
+    if side_by_side:
+        both = torch.empty(rows, 2 * cols, dtype=dh.dtype, device=device)
+        at, ld = (_ptr(both), _ptr(both) + cols * dh.element_size()), 2 * cols
+    else:
+        dg, du = torch.empty_like(dh), torch.empty_like(dh)
+        at, ld = (_ptr(dg), _ptr(du)), cols
+    with _device_of(device):
+        _lib.check(lib.qste_swiglu_backward_blocks_sums(_ptr(dh), code, *kept, *at, ld, _ptr(offs[0]), _ptr(offs[1]),
+                                                        _ptr(sums), rows, cols, _ptr(work), work.numel(),
+                                                        _stream(device)), "swiglu_backward_blocks_sums")
+    return (both, sums) if side_by_side else (dg, du, sums)
+
+
+def _layer_vector(t: Tensor | None, rows: int, what: str) -> Tensor | None:
+    """A layer's scale or bias as contiguous fp32 [rows]."""
+
+    if t is None:
+        return None
+    if t.shape != (rows,):
+        raise ValueError(f"{what} has shape {tuple(t.shape)}, expected ({rows},)")
+    return t if t.dtype == torch.float32 and t.is_contiguous() else _f32(t)
+
+
+def gated_forward(inputs: Tensor, gate: Tensor, gate_scale: Tensor, gate_bias: Tensor | None, up: Tensor,
+                  up_scale: Tensor, up_bias: Tensor | None, columns: int, *, keep: str = ""):
+    """``silu(g) * u`` of two packed layers of one input, g and u being
+    ``packed_linear_affine`` of ``gate`` and ``up`` (packed signs [rows, ...]).
+
+    ``keep`` says what a backward is to find: "" nothing, "values" g and u, "blocks"
+    them in 8-bit blocks.  Returns ``(out, g, u)``, g and u tensors, ``Blocks8``
+    or None.
+    """
+
+    device = _require_gpu(inputs, gate, gate_scale, gate_bias, up, up_scale, up_bias)
+    code = _dtype_code(inputs)
+    columns = int(columns)
+    if inputs.dim() == 0 or inputs.shape[-1] != columns:
+        raise ValueError(f"inputs of shape {tuple(inputs.shape)} do not match {columns} columns")
+    if keep not in ("", "values", "blocks"):
+        raise ValueError(f"keep must be '', 'values' or 'blocks', got {keep!r}")
+    gate, up = _check_packed(gate, columns), _check_packed(up, columns)
+    rows = gate.shape[0]
+    if up.shape[0] != rows:
+        raise ValueError(f"gate has {rows} rows and up {up.shape[0]}")
+    gs, gb = _layer_vector(gate_scale, rows, "gate_scale"), _layer_vector(gate_bias, rows, "gate_bias")
+    us, ub = _layer_vector(up_scale, rows, "up_scale"), _layer_vector(up_bias, rows, "up_bias")
+    x, gate, up = _aligned(inputs), _aligned(gate), _aligned(up)
+    shape = (*inputs.shape[:-1], rows)
+    m = x.numel() // columns if columns else _leading(inputs)
+    out = torch.empty(shape, dtype=inputs.dtype, device=device)
+    g = u = None
+    values, blocks = (None, None), (None, None, None, None)
+    if keep == "values":
+        g, u = torch.empty_like(out), torch.empty_like(out)
+        values = (_ptr(g), _ptr(u))
+    elif keep == "blocks":
+        g, u = _blocks_like(out), _blocks_like(out)
+        blocks = (_ptr(g.payload), _ptr(g.codes), _ptr(u.payload), _ptr(u.codes))
+    lib = _lib.load()
+    nbytes = lib.qste_gated_workspace_bytes(m, rows, columns, code, {"": 0, "values": 1, "blocks": 2}[keep])
+    work = _workspace(nbytes, device) if nbytes else None
+    with _device_of(device):
+        _lib.check(lib.qste_gated(x.data_ptr(), code, gate.data_ptr(), gs.data_ptr(), _ptr(gb), up.data_ptr(),
+                                  us.data_ptr(), _ptr(ub), out.data_ptr(), *values, *blocks, m, rows, columns,
+                                  _ptr(work), nbytes, _stream(device)), "gated_forward")
+    return out, g, u
+
+
+def _leading(t: Tensor) -> int:
+    count = 1
+    for size in t.shape[:-1]:
+        count *= int(size)
+    return count
 
 
 def row_scale(log_scale: Tensor, lo: float, hi: float) -> tuple[Tensor, Tensor]:

@@ -26,7 +26,8 @@ from torch.autograd import Function
 
 from . import kernels
 from .functional import swiglu
-from .losses import TokenScores, distillation_loss, distillation_loss_and_grad, token_logprobs
+from .kernels import Blocks8, dequantize_blocks, quantize_blocks
+from .losses import TokenScores, _no_tangent, distillation_loss, distillation_loss_and_grad, token_logprobs
 
 # The originals, bound before ``packed_activations`` can patch them: the
 # wrappers call these for values the kernels do not produce, and a patched
@@ -72,7 +73,43 @@ def _take_activation_input(value: Tensor) -> Tensor | None:
     return value if getattr(value, "_qste_activation_input", False) else None
 
 
-def swiglu_mlp(inputs: Tensor, gate, up, down) -> Tensor:
+def gated(inputs: Tensor, gate, up, *, checkpoint: bool = False) -> Tensor:
+    """``swiglu(gate(inputs), up(inputs))``, the gated feed-forward block, of two
+    converted layers (QSTELinear) or two packed ones (PackedLinear, which carry no
+    gradient): both products, the activation and the product in one kernel.
+
+    No counterpart in the reference.  The values are those of the layers called
+    one by one up to the order of the fp32 sums.  With gradients it is one
+    autograd node, whose backward runs the two layers as one; evidence and
+    scale gradients go where the layers' own would.  ``checkpoint`` keeps gate and up
+    for the backward in 8-bit blocks (``quantize_blocks``) in place of 16 bits.  Sizes
+    that the one kernel does not take (columns that are no multiple of 64, rows that
+    are none of 8, fp32 past 21 rows) run layer by layer."""
+
+    from .functional import GatedFn, _autocast, gated_fusable
+
+    trained = [hasattr(layer, "surface") for layer in (gate, up)]
+    if all(trained):
+        x = _autocast(inputs)
+        _no_tangent("gated", x)
+        if not gated_fusable(x, gate, up):
+            return swiglu(gate(inputs), up(inputs), checkpoint=checkpoint)
+        surfaces = (gate.surface, up.surface)
+        for s in surfaces:
+            s.note_forward()
+        return GatedFn.apply(x, gate.surface.packed_sign, gate.surface.log_scale, gate.bias, up.surface.packed_sign,
+                             up.surface.log_scale, up.bias, surfaces, checkpoint, torch.is_grad_enabled())
+    if any(trained) or not (hasattr(gate, "packed_sign") and hasattr(up, "packed_sign")):
+        raise TypeError("gated takes two QSTELinear or two PackedLinear layers, got "
+                        f"{type(gate).__name__} and {type(up).__name__}")
+    if gate.in_features != up.in_features:
+        raise ValueError(f"gate takes {gate.in_features} columns and up {up.in_features}")
+    with torch.no_grad():
+        return kernels.gated_forward(inputs, gate.packed_sign, gate.scale, gate.bias, up.packed_sign, up.scale, up.bias,
+                                     gate.in_features)[0]
+
+
+def swiglu_mlp(inputs: Tensor, gate, up, down, *, checkpoint: bool = False) -> Tensor:
     """``down(swiglu(gate(inputs), up(inputs)))`` for three converted layers
     (QSTELinear: gate and up d -> ffn, down ffn -> d).
 
@@ -81,19 +118,22 @@ def swiglu_mlp(inputs: Tensor, gate, up, down) -> Tensor:
     bf16 inputs on the GPU with d and ffn multiples of 64 the whole MLP is
     one autograd node whose input gradient is one product over the gate and
     up layers, rounded once (``functional.SwiGLUMLPFn``).  Anything else is
-    the layer-by-layer composition."""
+    the layer-by-layer composition.  With ``checkpoint`` gate and up are one
+    kernel (``gated``), which keeps them for the backward in 8-bit blocks."""
 
     from .functional import SwiGLUMLPFn, _autocast, swiglu_mlp_fusable
 
     x = _autocast(inputs)
     if not swiglu_mlp_fusable(x, gate, up, down):
+        if checkpoint:
+            return down(gated(inputs, gate, up, checkpoint=True))
         return down(swiglu(gate(inputs), up(inputs)))
     surfaces = (gate.surface, up.surface, down.surface)
     for s in surfaces:
         s.note_forward()
     y = SwiGLUMLPFn.apply(x, gate.surface.packed_sign, gate.surface.log_scale, gate.bias, up.surface.packed_sign,
                           up.surface.log_scale, up.bias, down.surface.packed_sign, down.surface.log_scale, down.bias,
-                          surfaces, torch.is_grad_enabled())
+                          surfaces, checkpoint, torch.is_grad_enabled())
     return _mark_activation_input(y)
 
 
@@ -781,7 +821,7 @@ __all__ = [
     "CELU", "Dropout", "ELU", "EXACT_REPLACEMENTS", "GELU", "Hardsigmoid", "Hardswish", "Hardtanh",
     "LeakyReLU", "Mish", "REPLACEMENTS", "ReLU", "ReLU6", "SELU", "SMOOTH_REPLACEMENTS", "SiLU",
     "Sigmoid", "Softplus", "Tanh", "celu", "dropout", "elementwise", "elu", "gelu", "hardsigmoid", "swiglu", "swiglu_mlp",
-    "TokenScores", "distillation_loss", "distillation_loss_and_grad", "token_logprobs",
+    "Blocks8", "TokenScores", "dequantize_blocks", "gated", "quantize_blocks", "distillation_loss", "distillation_loss_and_grad", "token_logprobs",
     "hardswish", "hardtanh", "leaky_relu", "mish", "packed", "packed_activations", "relu",
     "relu6", "relu_square", "replace", "selu", "sigmoid", "silu", "softplus", "tanh",
 ]

@@ -1,0 +1,493 @@
+"""The gated feed-forward block in one kernel.
+
+Values: against the definition in 64 bits, with the bound that the roundings
+give, and bit for bit against the layers called one by one where the sums run
+in the same order.  The backward: bit for bit against the layers' own
+backward calls at the values that were kept, and against differences.
+"""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+@pytest.fixture(autouse=True)
+def _gpu():
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    from qste_amd import kernels
+
+    assert kernels.native_available(), kernels.status()
+
+
+def _bits(t):
+    return t.contiguous().view({1: torch.int8, 2: torch.int16, 4: torch.int32}[t.element_size()])
+
+
+def _operands(m, rows, cols, dtype, seed=0, bias=False):
+    g = torch.Generator(device=DEV).manual_seed(seed + m + 3 * rows + 7 * cols)
+    x = (torch.randn(m, cols, generator=g, device=DEV) + 0.1).to(dtype)
+    layers = []
+    for _ in range(2):
+        bits = torch.randint(0, 256, (rows, -(-cols // 8)), generator=g, device=DEV, dtype=torch.uint8)
+        if cols % 8:
+            bits[:, -1] &= (1 << (cols % 8)) - 1
+        scale = torch.rand(rows, generator=g, device=DEV) / math.sqrt(cols) + 0.2 / math.sqrt(cols)
+        layers += [bits, scale, torch.randn(rows, generator=g, device=DEV) * 0.1 if bias else None]
+    return x, layers
+
+
+def _route(m, rows, cols, dtype, keep=0):
+    from qste_amd.kernels import _lib
+
+    return _lib.load().qste_gated_route(m, rows, cols, CODES[dtype], keep)
+
+
+def _within_roundings(h, x, layers, dtype):
+    """Whether h is silu(g) u in 64 bits but for the roundings.
+
+    e: half a step of the type, relative.  A sum of K terms in fp32 is off by at most K 2^-24 times the sum of their
+    magnitudes, and scale and bias round twice more; g and u are then rounded (e).  silu's slope is at most 1.1; its
+    value is computed in fp32 (16 units of 2^-24 for the exponential and the division) and rounded (e), and so is the
+    product (e).  Subnormal fp16 values are rounded to 2^-25 at most."""
+
+    e, tiny = torch.finfo(dtype).eps / 2, (2.0 ** -24 if dtype == torch.float16 else 1e-36)
+    cols = x.shape[1]
+    place = torch.arange(cols, device=DEV)
+    values, errors = [], []
+    for bits, scale, bias in (layers[:3], layers[3:]):
+        sign = ((bits[:, place // 8].int() >> (place % 8)) & 1).double() * 2 - 1
+        y = x.double() @ sign.t() * scale.double()
+        if bias is not None:
+            y = y + bias.double()
+        size = x.double().abs().sum(1, keepdim=True) * scale.double()
+        errors.append((cols + 2) * 2.0 ** -24 * size + (2.0 ** -23 + e) * y.abs() + tiny)
+        values.append(y)
+    g, u = values
+    a = g * torch.sigmoid(g)
+    error_a = 1.1 * errors[0] + (16 * 2.0 ** -24 + e) * (a.abs() + 1.1 * errors[0]) + tiny
+    bound = error_a * (u.abs() + errors[1]) + a.abs() * errors[1]
+    bound = bound + e * ((a * u).abs() + bound) + tiny
+    return bool(((h.double() - a * u).abs() <= bound).all())
+
+
+# sizes of each way, with ends inside every unit: 16-row blocks, 512-column chunks, 128- and 256-row and
+# 128-feature tiles, K in ranges
+FEW = [(1, 16, 128), (1, 8, 256), (2, 24, 384), (3, 999, 128), (4, 4096, 1024), (5, 1000, 640), (7, 2816, 1024),
+       (16, 5480, 2048), (17, 136, 4096), (21, 512, 2048), (31, 640, 512), (33, 5480, 2048), (48, 1000, 8192),
+       (49, 77, 1024), (64, 256, 4096), (1, 14336, 4096)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("m,rows,cols", FEW)
+def test_few_rows(m, rows, cols, dtype):
+    from qste_amd import kernels
+
+    if dtype == torch.float32 and m > 21:
+        m = m % 21 + 1
+    print(f"gated {m} x {rows} x {cols} {dtype}", flush=True)
+    for bias in (False, True):
+        x, layers = _operands(m, rows, cols, dtype, bias=bias)
+        h, g, u = kernels.gated_forward(x, *layers, cols)
+        assert g is None and u is None and h.dtype == dtype and h.shape == (m, rows)
+        assert _within_roundings(h, x, layers, dtype)
+    again = kernels.gated_forward(x, *layers, cols)[0]
+    assert torch.equal(_bits(again), _bits(h))
+
+
+def test_few_rows_take_their_kernel():
+    assert _route(1, 14336, 4096, torch.bfloat16) == 1
+    assert _route(3, 999, 128, torch.float16) == 1 and _route(21, 512, 2048, torch.float32) == 1
+
+
+def test_a_row_is_the_same_beside_others():
+    """Up to 16 rows a row's bits do not depend on how many there are."""
+
+    from qste_amd import kernels
+
+    for dtype in (torch.bfloat16, torch.float32):
+        x, layers = _operands(16, 1000, 1024, dtype)
+        whole = kernels.gated_forward(x, *layers, 1024)[0]
+        for m in (1, 4, 5, 11):
+            part = kernels.gated_forward(x[:m], *layers, 1024)[0]
+            assert torch.equal(_bits(part), _bits(whole[:m]))
+
+
+TILES = [(65, 8, 64), (100, 1024, 4096), (128, 120, 64), (129, 136, 128), (250, 2048, 768), (300, 264, 1024),
+         (500, 8192, 2048), (513, 1000, 192), (2048, 4096, 1024), (2050, 16384, 256), (70, 4104, 8192)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,rows,cols", TILES)
+def test_tiles(m, rows, cols, dtype):
+    from qste_amd import kernels
+
+    print(f"gated {m} x {rows} x {cols} {dtype}", flush=True)
+    assert _route(m, rows, cols, dtype) == 2
+    x, layers = _operands(m, rows, cols, dtype, bias=rows % 16 == 8)
+    h = kernels.gated_forward(x, *layers, cols)[0]
+    assert _within_roundings(h, x, layers, dtype)
+    # what is kept changes nothing, and is what the values' blocks are
+    h1, g, u = kernels.gated_forward(x, *layers, cols, keep="values")
+    h2, g8, u8 = kernels.gated_forward(x, *layers, cols, keep="blocks")
+    assert torch.equal(_bits(h1), _bits(h)) and torch.equal(_bits(h2), _bits(h))
+    assert torch.equal(_bits(kernels.swiglu_forward(g, u)[0]), _bits(h))
+    for kept, t in ((g8, g), (u8, u)):
+        want = kernels.quantize_blocks(t)
+        assert torch.equal(kept.payload, want.payload) and torch.equal(kept.codes, want.codes)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,rows,cols", [(2048, 4096, 1024), (4096, 8192, 512), (8192, 1000, 256)])
+def test_the_same_bits_as_the_layers_one_by_one(m, rows, cols, dtype):
+    """Products whose K is not cut, alone or together, sum in one order."""
+
+    from qste_amd import kernels
+
+    x, layers = _operands(m, rows, cols, dtype, bias=True)
+    h, g, u = kernels.gated_forward(x, *layers, cols, keep="values")
+    want = [kernels.packed_linear_affine(x, *layer, cols) for layer in (layers[:3], layers[3:])]
+    assert torch.equal(_bits(g), _bits(want[0])) and torch.equal(_bits(u), _bits(want[1]))
+    assert torch.equal(_bits(h), _bits(kernels.swiglu_forward(*want)[0]))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("m,rows,cols", [(100, 63, 64), (70, 1000, 100), (3, 33, 65), (1, 1, 1), (80, 264, 7),
+                                         (30, 128, 256)])
+def test_sizes_that_go_layer_by_layer(m, rows, cols, dtype):
+    from qste_amd import kernels
+
+    x, layers = _operands(m, rows, cols, dtype, bias=True)
+    for keep in ("", "values", "blocks"):
+        h, g, u = kernels.gated_forward(x, *layers, cols, keep=keep)
+        assert _within_roundings(h, x, layers, dtype)
+        if keep == "values":
+            assert torch.equal(_bits(kernels.swiglu_forward(g, u)[0]), _bits(h))
+        if keep == "blocks":
+            assert g.payload.shape == h.shape
+
+
+def test_special_values():
+    """Infinities and NaN in a row stay in it and give what the layers one by one give.
+
+    Row 4 holds finite values whose sums pass the end of fp32: 3e38 - 3e38 + 3e38 + 3e38 is finite up to its third
+    term and infinite from its fourth on, 3e38 + 3e38 - 3e38 - 3e38 from its second, and with sums of either sign
+    in a tree inf - inf is NaN; which of them a sum meets is a matter of its order alone, which two layers in one
+    kernel need not share with two kernels.  What it gives is not compared, that it stays in its row is."""
+
+    from qste_amd import kernels
+
+    same = [0, 1, 2, 3, 5]
+    for m in (6, 300):
+        x, layers = _operands(m, 256, 512, torch.bfloat16)
+        clean = kernels.gated_forward(x, *layers, 512)[0]
+        x[1, 5], x[2, 7], x[4] = math.inf, math.nan, 3e38
+        h, g8, u8 = kernels.gated_forward(x, *layers, 512, keep="blocks")
+        want = [kernels.packed_linear_affine(x, *layer, 512) for layer in (layers[:3], layers[3:])]
+        plain = kernels.swiglu_forward(*want)[0]
+        assert torch.equal(torch.isnan(h[same]), torch.isnan(plain[same]))
+        assert torch.equal(torch.isinf(h[same]), torch.isinf(plain[same]))
+        assert bool((g8.codes[1] == 255).all()) and bool((u8.codes[2] == 255).all())
+        few = kernels.gated_forward(x, *layers, 512)[0]
+        assert torch.equal(torch.isnan(few[same]), torch.isnan(plain[same]))
+        for row in (0, 3, 5):
+            assert torch.equal(_bits(few[row]), _bits(clean[row]))
+
+
+def test_empty_and_shaped_inputs():
+    from qste_amd import kernels
+
+    x, layers = _operands(12, 64, 128, torch.bfloat16)
+    flat = kernels.gated_forward(x, *layers, 128)[0]
+    assert torch.equal(kernels.gated_forward(x.view(3, 4, 128), *layers, 128)[0], flat.view(3, 4, 64))
+    assert kernels.gated_forward(x[:0], *layers, 128)[0].shape == (0, 64)
+    wide = torch.zeros(12, 137, dtype=torch.bfloat16, device=DEV)
+    wide[:, 9:] = x
+    assert torch.equal(kernels.gated_forward(wide[:, 9:], *layers, 128)[0], flat)  # strided, off 16-byte steps
+    assert torch.equal(kernels.gated_forward(x[0], *layers, 128)[0], flat[0])
+
+
+def test_refusals():
+    from qste_amd import kernels
+
+    x, layers = _operands(4, 64, 128, torch.bfloat16)
+    bits, scale = layers[:2]
+    with pytest.raises(TypeError):
+        kernels.gated_forward(x.double(), *layers, 128)
+    with pytest.raises(ValueError, match="columns"):
+        kernels.gated_forward(x[:, :64], *layers, 128)
+    with pytest.raises(ValueError, match="rows"):
+        kernels.gated_forward(x, bits, scale, None, bits[:32], scale[:32], None, 128)
+    with pytest.raises(ValueError, match="scale"):
+        kernels.gated_forward(x, bits, scale[:3], None, bits, scale, None, 128)
+    with pytest.raises(ValueError, match="bias"):
+        kernels.gated_forward(x, bits, scale, scale[:3], bits, scale, None, 128)
+    with pytest.raises(ValueError, match="keep"):
+        kernels.gated_forward(x, *layers, 128, keep="all")
+
+
+# ---------------------------------------------------------------------------
+# layers
+# ---------------------------------------------------------------------------
+
+
+def _pair(rows, cols, seed, bias=False, dtype=torch.float32):
+    import qste_amd as qste
+
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    layers = []
+    for _ in range(2):
+        coordinate = torch.randint(-127, 128, (rows, cols), generator=g, device=DEV, dtype=torch.int8)
+        log_scale = torch.randn(rows, generator=g, device=DEV) * 0.1 - 0.5 * math.log(cols)
+        layer = qste.QSTELinear(qste.Surface.from_state(coordinate, log_scale),
+                                torch.randn(rows, generator=g, device=DEV) * 0.1 if bias else None).to(DEV)
+        layer.surface.log_scale.data = log_scale.to(dtype)
+        layer.evidence = []
+        layer.surface.route_evidence(lambda s, e, to=layer.evidence: to.append(e.clone()))
+        layers.append(layer)
+    return layers
+
+
+@pytest.mark.parametrize("checkpoint", [False, True])
+@pytest.mark.parametrize("dtype,bias", [(torch.bfloat16, False), (torch.float16, True)])
+@pytest.mark.parametrize("m,rows,cols", [(3, 64, 64), (250, 2048, 768), (300, 264, 128), (1030, 1000, 512)])
+def test_training_node(m, rows, cols, dtype, bias, checkpoint):
+    """Values and gradients are those of the kernels that the node stands for, at the g and u it kept."""
+
+    import qste_amd as qste
+    from qste_amd import kernels
+
+    print(f"gated node {m} x {rows} x {cols} {dtype} {checkpoint}", flush=True)
+    gate, up = _pair(rows, cols, m, bias, torch.bfloat16)
+    gen = torch.Generator(device=DEV).manual_seed(m)
+    x = (torch.randn(m, cols, generator=gen, device=DEV) + 0.1).to(dtype).requires_grad_()
+    grad = torch.randn(m, rows, generator=gen, device=DEV).to(dtype)
+    h = qste.nn.gated(x, gate, up, checkpoint=checkpoint)
+    h.backward(grad)
+    # piece by piece
+    flat = x.detach()
+    sides = [(layer.surface.packed_sign.detach(), layer.scale.detach(), layer.bias) for layer in (gate, up)]
+    operands = [t if t is None else t.detach() for side in sides for t in side]
+    want, g, u = kernels.gated_forward(flat, *operands, cols, keep="values")
+    assert torch.equal(_bits(h.detach()), _bits(want))
+    if checkpoint:
+        g, u = (kernels.dequantize_blocks(kernels.quantize_blocks(t)) for t in (g, u))
+    payload, offset, xscale = kernels.pack_affine_rows(flat)
+    both, sums = kernels.swiglu_backward_sums(grad, g, u, offset, offset, side_by_side=True)
+    dx, evidence, grad_scale, grad_bias = kernels.linear_backward(
+        both, payload, offset, xscale, torch.cat((sides[0][0], sides[1][0])),
+        torch.cat((sides[0][1].float(), sides[1][1].float())), cols, need_bias=bias, offset_dot=sums.reshape(-1))
+    assert torch.equal(_bits(x.grad), _bits(dx))
+    for i, layer in enumerate((gate, up)):
+        part = slice(i * rows, (i + 1) * rows)
+        assert len(layer.evidence) == 1 and torch.equal(layer.evidence[0], evidence[part])
+        scale = layer.scale
+        scale.backward(grad_scale[part].to(scale.dtype))
+    once = [layer.surface.log_scale.grad for layer in (gate, up)]
+    # both the node's gradient and scale's own have been added: twice one of them
+    gate.surface.log_scale.grad = up.surface.log_scale.grad = None
+    for i, layer in enumerate((gate, up)):
+        layer.scale.backward(grad_scale[i * rows:(i + 1) * rows].to(layer.scale.dtype))
+        assert torch.equal(once[i], 2 * layer.surface.log_scale.grad)
+        if bias:
+            assert torch.equal(layer.bias.grad, grad_bias[i * rows:(i + 1) * rows])
+
+
+def test_node_against_the_layers_one_by_one():
+    """Output, input gradient, evidence and scale gradients of the composition with the plain gate."""
+
+    import qste_amd as qste
+
+    gate, up = _pair(4096, 1024, 5)
+    x = (torch.randn(2048, 1024, device=DEV, generator=torch.Generator(device=DEV).manual_seed(1)) + 0.1).bfloat16()
+    grad = torch.randn(2048, 4096, device=DEV, generator=torch.Generator(device=DEV).manual_seed(2)).bfloat16()
+    results = []
+    for call in (lambda t: qste.nn.gated(t, gate, up), lambda t: qste.nn.swiglu(gate(t), up(t))):
+        t = x.clone().requires_grad_()
+        h = call(t)
+        h.backward(grad)
+        results.append((h.detach(), t.grad, gate.evidence.pop(), up.evidence.pop(), gate.surface.log_scale.grad,
+                        up.surface.log_scale.grad))
+        gate.surface.log_scale.grad = up.surface.log_scale.grad = None
+    one, other = results
+    assert torch.equal(_bits(one[0]), _bits(other[0]))
+    # the input gradient is rounded once rather than twice with a sum in between; the others may sum in another order
+    e = 2.0 ** -8
+    assert float((one[1].double() - other[1].double()).norm() / other[1].double().norm()) <= 2 * e
+    for a, b in zip(one[2:], other[2:]):
+        assert float((a - b).norm() / b.norm()) <= 1e-5
+
+
+def test_node_against_differences():
+    """The input gradient along a direction against differences of the definition in 64 bits.
+
+    dx is rounded to bf16, dg and du before it, and the row scales: each 2^-9 of a term at most, of random sign over
+    thousands of terms; the direction's sum is within 4 2^-9 of the terms' root sum of squares, far above the
+    difference's own error."""
+
+    import qste_amd as qste
+
+    m, rows, cols = 64, 512, 256
+    gate, up = _pair(rows, cols, 9, dtype=torch.bfloat16)
+    gen = torch.Generator(device=DEV).manual_seed(4)
+    x = torch.randn(m, cols, generator=gen, device=DEV).bfloat16().requires_grad_()
+    w = torch.randn(m, rows, generator=gen, device=DEV).bfloat16()
+    v = torch.randn(m, cols, generator=gen, device=DEV).double()
+    qste.nn.gated(x, gate, up).backward(w)
+    signs = [layer.surface.sign.double() * layer.scale.detach().double()[:, None] for layer in (gate, up)]
+
+    def value(t):
+        g, u = t @ signs[0].t(), t @ signs[1].t()
+        return (w.double() * g * torch.sigmoid(g) * u).sum()
+
+    step = 2.0 ** -14
+    slope = float((value(x.detach().double() + step * v) - value(x.detach().double() - step * v)) / (2 * step))
+    terms = x.grad.double() * v
+    assert abs(float(terms.sum()) - slope) <= 4 * 2.0 ** -9 * float(terms.norm()) * math.sqrt(8)
+
+
+def test_node_in_use():
+    """Frozen inputs, gradients turned off, autocast, a pair of one layer, a strided and a broadcast gradient, a second
+    backward through a kept graph, forward-mode refused."""
+
+    import qste_amd as qste
+
+    gate, up = _pair(128, 64, 3)
+    x = torch.randn(10, 64, device=DEV, generator=torch.Generator(device=DEV).manual_seed(1)).bfloat16()
+    with torch.no_grad():
+        plain = qste.nn.gated(x, gate, up, checkpoint=True)
+    assert not plain.requires_grad and gate.surface.ledger.open_uses == 0
+    h = qste.nn.gated(x, gate, up, checkpoint=True)  # x is no leaf that wants a gradient
+    assert torch.equal(h.detach(), plain)
+    h.sum().backward()  # a broadcast gradient
+    assert len(gate.evidence) == 1 and x.grad is None
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        assert torch.equal(qste.nn.gated(x.float(), gate, up).detach(), plain)
+    gate.surface.reset_tracking(), up.surface.reset_tracking()
+    gate.evidence.clear(), up.evidence.clear()
+    t = x.clone().requires_grad_()
+    h = qste.nn.gated(t, gate, up)
+    wide = torch.randn(128, 10, device=DEV).bfloat16()
+    h.backward(wide.t(), retain_graph=True)
+    first = t.grad.clone()
+    t.grad = None
+    h.backward(wide.t().contiguous())
+    assert torch.equal(t.grad, first)
+    gate.evidence.clear()
+    qste.nn.gated(x, gate, gate).sum().backward()  # one surface for both
+    assert len(gate.evidence) == 1
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        with pytest.raises(NotImplementedError):
+            qste.nn.gated(dual, gate, up)
+        with pytest.raises(NotImplementedError):
+            qste.nn.swiglu(dual, x, checkpoint=True)
+
+
+@pytest.mark.parametrize("dtype,cols,rows", [(torch.float32, 64, 128), (torch.bfloat16, 72, 128),
+                                             (torch.bfloat16, 64, 100)])
+def test_layers_that_the_node_does_not_take(dtype, cols, rows):
+    import qste_amd as qste
+
+    gate, up = _pair(rows, cols, 3)
+    x = torch.randn(10, cols, device=DEV, generator=torch.Generator(device=DEV).manual_seed(1)).to(dtype)
+    a, b = x.clone().requires_grad_(), x.clone().requires_grad_()
+    one = qste.nn.gated(a, gate, up)
+    one.sum().backward()  # (evidence is delivered when every forward has had its backward)
+    evidence = gate.evidence.pop()
+    other = qste.nn.swiglu(gate(b), up(b))
+    other.sum().backward()
+    assert torch.equal(one, other)
+    assert torch.equal(a.grad, b.grad) and torch.equal(evidence, gate.evidence.pop())
+    qste.nn.gated(a, gate, up, checkpoint=True).sum().backward()
+    assert len(gate.evidence) == 1
+
+
+def test_packed_layers():
+    """As a model is served: exported layers, one token and many."""
+
+    import qste_amd as qste
+
+    for m, dtype in ((1, torch.bfloat16), (9, torch.float32), (200, torch.float16), (30, torch.float32)):
+        x, layers = _operands(m, 1000, 256, dtype, bias=True)
+        gate, up = qste.PackedLinear(*layers[:2], 256, layers[2]), qste.PackedLinear(*layers[3:5], 256, layers[5])
+        h = qste.nn.gated(x.requires_grad_(), gate, up)
+        assert not h.requires_grad and _within_roundings(h, x.detach(), layers, dtype)
+
+
+def test_mlp_with_a_checkpoint():
+    """swiglu_mlp with its gate and up kept in 8 bits: the output of the MLP without, gradients near its, and the steps
+    that the coordinates take inside backward from them; a run of everything together."""
+
+    import qste_amd as qste
+
+    class MLP(torch.nn.Module):
+        def __init__(self, checkpoint):
+            super().__init__()
+            gen = torch.Generator().manual_seed(0)
+            self.gate, self.up = torch.nn.Linear(256, 640, bias=False), torch.nn.Linear(256, 640, bias=False)
+            self.down = torch.nn.Linear(640, 256, bias=False)
+            for p in self.parameters():
+                p.data.copy_(torch.randn(p.shape, generator=gen) * 0.05)
+            self.checkpoint = checkpoint
+
+        def forward(self, x):
+            return qste.nn.swiglu_mlp(x, self.gate, self.up, self.down, checkpoint=self.checkpoint)
+
+    runs = []
+    for checkpoint in (False, True):
+        model = MLP(checkpoint)
+        qste.convert(model, include=["*"])
+        model.to(DEV)
+        coords = qste.QSTEOptimizer(model)
+        before = [s.coordinate.detach().clone() for s in qste.surfaces(model)]
+        x = torch.randn(128, 256, device=DEV, generator=torch.Generator(device=DEV).manual_seed(1)).bfloat16().requires_grad_()
+        w = torch.randn(128, 256, device=DEV, generator=torch.Generator(device=DEV).manual_seed(2)).bfloat16()
+        y = model(x)
+        y.backward(w)
+        coords.step()
+        moved = [float((s.coordinate.detach() != b).float().mean()) for s, b in zip(qste.surfaces(model), before)]
+        runs.append((y.detach(), x.grad, moved))
+    (y0, dx0, moved0), (y1, dx1, moved1) = runs
+    assert float((y1.double() - y0.double()).norm() / y0.double().norm()) <= 2.0 ** -8
+    # a kept value is off by up to a 128th of its block's largest, uniformly: about 1% of the gradient
+    assert float((dx1.double() - dx0.double()).norm() / dx0.double().norm()) <= 0.05
+    assert all(a > 0 and b > 0 for a, b in zip(moved0, moved1))
+
+
+def test_streams_and_graphs():
+    """On a side stream, and captured with two ways in one graph and replayed with eager work in between."""
+
+    from qste_amd import kernels
+
+    small, layers = _operands(3, 640, 512, torch.bfloat16)
+    large = _operands(90, 640, 512, torch.bfloat16, seed=1)[0]  # K in ranges, with a workspace
+    want = [kernels.gated_forward(t, *layers, 512)[0] for t in (small, large)]
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        got = [kernels.gated_forward(t, *layers, 512)[0] for t in (small, large)]
+    stream.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = [kernels.gated_forward(t, *layers, 512)[0] for t in (small, large)]
+        kept = kernels.gated_forward(large, *layers, 512, keep="blocks")
+    for seed in (5, 6, 7):
+        gen = torch.Generator(device=DEV).manual_seed(seed)
+        for t in (small, large):
+            t.copy_(torch.randn(t.shape, generator=gen, device=DEV))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = [kernels.gated_forward(t, *layers, 512)[0] for t in (small, large)]
+        assert all(torch.equal(a, b) for a, b in zip(captured, want))
+        eager = kernels.gated_forward(large, *layers, 512, keep="blocks")
+        assert torch.equal(kept[0], eager[0]) and torch.equal(kept[1].payload, eager[1].payload)
