@@ -451,16 +451,20 @@ int qste_swiglu_forward_blocks(const void* gate, const void* up, int dtype, void
                                float* scale, int8_t* gate_payload, uint8_t* gate_codes, int8_t* up_payload,
                                uint8_t* up_codes, int64_t rows, int64_t cols, void* stream);
 
-/* qste_swiglu_backward with the gate and up that 8-bit blocks stand for. */
+/* The gradients of silu(gate) * up at the gate and up that 8-bit blocks stand for,
+ * in fp32 and rounded once (qste_swiglu_backward rounds on the way as torch's
+ * operators do). */
 int qste_swiglu_backward_blocks(const void* grad, int dtype, const int8_t* gate_payload, const uint8_t* gate_codes,
                                 const int8_t* up_payload, const uint8_t* up_codes, void* grad_gate, void* grad_up,
                                 int64_t rows, int64_t cols, void* stream);
 
-/* qste_swiglu_backward_sums with the gate and up that 8-bit blocks stand for.
+/* qste_swiglu_backward_blocks that also sums its outputs against the offsets, as
+ * qste_swiglu_backward_sums does (in an order of its own, and before dg and du are
+ * rounded).
  * ld: elements between the gradients' rows, cols, or with 16-bit dtypes and cols
  * a multiple of 8 any larger multiple of 8 (both gradients side by side in one
- * [rows, 2 cols] tensor: grad_up = grad_gate + cols, ld = 2 cols).  The same
- * workspace as that entry. */
+ * [rows, 2 cols] tensor: grad_up = grad_gate + cols, ld = 2 cols). */
+size_t qste_swiglu_backward_blocks_sums_workspace_bytes(int64_t rows, int64_t cols);
 int qste_swiglu_backward_blocks_sums(const void* grad, int dtype, const int8_t* gate_payload,
                                      const uint8_t* gate_codes, const int8_t* up_payload, const uint8_t* up_codes,
                                      void* grad_gate, void* grad_up, int64_t ld, const float* offset_gate,

@@ -78,6 +78,7 @@ int launch_swiglu_forward_blocks(const void*, const void*, int, void*, uint8_t*,
                                  int8_t*, uint8_t*, int64_t, int64_t, hipStream_t);
 int launch_swiglu_backward_blocks(const void*, int, const int8_t*, const uint8_t*, const int8_t*, const uint8_t*, void*,
                                   void*, int64_t, int64_t, hipStream_t);
+size_t swiglu_backward_blocks_sums_workspace(int64_t, int64_t);
 int launch_swiglu_backward_blocks_sums(const void*, int, const int8_t*, const uint8_t*, const int8_t*, const uint8_t*,
                                        void*, void*, const float*, const float*, int64_t, int64_t, float*, float*,
                                        hipStream_t, int64_t);
@@ -782,6 +783,11 @@ int qste_swiglu_backward_blocks(const void* grad, int dtype, const int8_t* gate_
                                        rows, cols, as_stream(stream));
 }
 
+size_t qste_swiglu_backward_blocks_sums_workspace_bytes(int64_t rows, int64_t cols) {
+  if (rows <= 0 || cols <= 0) return 0;
+  return swiglu_backward_blocks_sums_workspace(rows, cols);
+}
+
 int qste_swiglu_backward_blocks_sums(const void* grad, int dtype, const int8_t* gate_payload,
                                      const uint8_t* gate_codes, const int8_t* up_payload, const uint8_t* up_codes,
                                      void* grad_gate, void* grad_up, int64_t ld, const float* offset_gate,
@@ -796,7 +802,7 @@ int qste_swiglu_backward_blocks_sums(const void* grad, int dtype, const int8_t* 
   if (!grad || !gate_payload || !gate_codes || !up_payload || !up_codes || !grad_gate || !grad_up || !offset_gate ||
       !offset_up)
     return QSTE_E_NULL;
-  if (!workspace || workspace_bytes < swiglu_backward_sums_workspace(rows, cols)) return QSTE_E_WORKSPACE;
+  if (!workspace || workspace_bytes < swiglu_backward_blocks_sums_workspace(rows, cols)) return QSTE_E_WORKSPACE;
   return launch_swiglu_backward_blocks_sums(grad, dtype, gate_payload, gate_codes, up_payload, up_codes, grad_gate,
                                             grad_up, offset_gate, offset_up, rows, cols, sums,
                                             static_cast<float*>(workspace), s, ld);

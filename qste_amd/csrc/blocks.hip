@@ -16,8 +16,7 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(const typename Elem<
   // whole blocks at a time: four lanes go on or stop together (quarters is a multiple of four)
   for (int64_t j = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; j < quarters; j += step) {
     const Quarter p(j, cols, per_row);
-    float v[8] = {};
-    if (p.there()) load8<DT>(x + p.at(), v);
+    const Eight<DT> v = p.there() ? Eight<DT>::load(x + p.at()) : Eight<DT>::zeros();
     uint32_t code;
     const uint2 q = quantize8(v, code);
     if (p.there()) *reinterpret_cast<uint2*>(out.q + p.at()) = q;
@@ -54,7 +53,7 @@ __global__ __launch_bounds__(kThreads) void quantize_any_kernel(const typename E
       m = m > other ? m : other;
     }
     const uint32_t code = code_of(m);
-    if (col < cols) out.q[row * cols + col] = static_cast<int8_t>(steps(v, to_steps(code)));
+    if (col < cols) out.q[row * cols + col] = static_cast<int8_t>(steps(v, to_steps(code)) & unless_bad(code));
     if (lane == 0) out.codes[b] = static_cast<uint8_t>(code);
   }
 }

@@ -44,29 +44,17 @@ __device__ __forceinline__ float step_of(uint32_t code) {
 
 // rint(x * to) within +-127, in the low byte of what is returned: added to 1.5 *
 // 2^23 a product rounds to a whole number, to the nearest even, whose low bits
-// are the sum's.  A bad block's are zeros: x * 0 is NaN there for the values that
-// make it bad, and the clamp takes NaN to one of its ends, so that is asked first.
+// are the sum's.  Of a bad block the caller takes zeros.
 __device__ __forceinline__ uint32_t steps(float x, float to) {
   constexpr float kMagic = 12582912.0f;
-  const float t = __builtin_amdgcn_fmed3f(fmaf(x, to, kMagic), kMagic - 127.0f, kMagic + 127.0f);
-  return to == 0.0f ? 0u : __float_as_uint(t);
+  return __float_as_uint(__builtin_amdgcn_fmed3f(fmaf(x, to, kMagic), kMagic - 127.0f, kMagic + 127.0f));
 }
+__device__ __forceinline__ uint32_t unless_bad(uint32_t code) { return code == kBadCode ? 0u : 0xFFFFFFFFu; }
 
 // four low bytes to a word
 __device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   const uint32_t lo = __builtin_amdgcn_perm(b, a, 0x0C0C0400u), hi = __builtin_amdgcn_perm(d, c, 0x04000C0Cu);
   return lo | hi;
-}
-
-// the magnitude bits of the largest of a thread's eight values
-__device__ __forceinline__ uint32_t largest(const float (&x)[8]) {
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t u = __float_as_uint(x[i]) & 0x7FFFFFFFu;
-    m = m > u ? m : u;
-  }
-  return m;
 }
 
 // the largest over the four lanes 4j .. 4j + 3, which hold a block of 32 together
@@ -77,13 +65,69 @@ __device__ __forceinline__ uint32_t over_four(uint32_t m) {
   return m > o ? m : o;  // quad_perm 2,3,0,1
 }
 
+// Eight values of an element type as they lie in memory.
+template <int DT>
+struct Eight {
+  uint32_t w[DT == QSTE_F32 ? 8 : 4];
+
+  __device__ __forceinline__ static Eight zeros() { return Eight{}; }
+  // from 16-byte aligned p
+  __device__ __forceinline__ static Eight load(const typename Elem<DT>::T* p) {
+    Eight e;
+    const uint4 a = *reinterpret_cast<const uint4*>(p);
+    e.w[0] = a.x; e.w[1] = a.y; e.w[2] = a.z; e.w[3] = a.w;
+    if constexpr (DT == QSTE_F32) {
+      const uint4 b = *reinterpret_cast<const uint4*>(p + 4);
+      e.w[4] = b.x; e.w[5] = b.y; e.w[6] = b.z; e.w[7] = b.w;
+    }
+    return e;
+  }
+  __device__ __forceinline__ static Eight of(const uint4& a) {
+    Eight e;
+    e.w[0] = a.x; e.w[1] = a.y; e.w[2] = a.z; e.w[3] = a.w;
+    return e;
+  }
+  __device__ __forceinline__ void values(float (&x)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (DT == QSTE_F32)
+        x[i] = __uint_as_float(w[i]);
+      else if constexpr (DT == QSTE_BF16)
+        x[i] = __uint_as_float(i & 1 ? w[i / 2] & 0xFFFF0000u : w[i / 2] << 16);
+      else
+        x[i] = f16_to_f32(static_cast<uint16_t>(i & 1 ? w[i / 2] >> 16 : w[i / 2]));
+    }
+  }
+  // The magnitude bits, as an fp32 value's, of the largest: 16-bit magnitudes
+  // order as their values do (a NaN above all), two to an instruction.
+  __device__ __forceinline__ uint32_t largest() const {
+    if constexpr (DT == QSTE_F32) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) m = m > (w[i] & 0x7FFFFFFFu) ? m : w[i] & 0x7FFFFFFFu;
+      return m;
+    } else {
+      typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+      u16x2 m = __builtin_bit_cast(u16x2, w[0] & 0x7FFF7FFFu);
+#pragma unroll
+      for (int i = 1; i < 4; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, w[i] & 0x7FFF7FFFu));
+      const uint32_t top = m.x > m.y ? m.x : m.y;
+      return DT == QSTE_BF16 ? top << 16 : __float_as_uint(f16_to_f32(static_cast<uint16_t>(top)));
+    }
+  }
+};
+
 // Eight values of a block that four lanes hold: their bytes, and the block's
 // code.  All four lanes make the call, with zeros past the row's end.
-__device__ __forceinline__ uint2 quantize8(const float (&x)[8], uint32_t& code) {
-  code = code_of(over_four(largest(x)));
+template <int DT>
+__device__ __forceinline__ uint2 quantize8(const Eight<DT>& e, uint32_t& code) {
+  code = code_of(over_four(e.largest()));
   const float to = to_steps(code);
-  return make_uint2(pack4(steps(x[0], to), steps(x[1], to), steps(x[2], to), steps(x[3], to)),
-                    pack4(steps(x[4], to), steps(x[5], to), steps(x[6], to), steps(x[7], to)));
+  const uint32_t mask = unless_bad(code);
+  float x[8];
+  e.values(x);
+  return make_uint2(pack4(steps(x[0], to), steps(x[1], to), steps(x[2], to), steps(x[3], to)) & mask,
+                    pack4(steps(x[4], to), steps(x[5], to), steps(x[6], to), steps(x[7], to)) & mask);
 }
 
 __device__ __forceinline__ void dequantize8(uint2 q, uint32_t code, float (&x)[8]) {
@@ -97,44 +141,28 @@ __device__ __forceinline__ void dequantize8(uint2 q, uint32_t code, float (&x)[8
 
 __device__ __forceinline__ float dequantize1(int8_t q, uint32_t code) { return static_cast<float>(q) * step_of(code); }
 
-// Eight values of an element type at 16-byte aligned p.
+// eight values rounded to an element type
 template <int DT>
-__device__ __forceinline__ void load8(const typename Elem<DT>::T* p, float (&x)[8]) {
-  const uint4 a = *reinterpret_cast<const uint4*>(p);
-  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-  if constexpr (DT == QSTE_F32) {
-    const uint4 b = *reinterpret_cast<const uint4*>(p + 4);
-    const uint32_t v[4] = {b.x, b.y, b.z, b.w};
+__device__ __forceinline__ Eight<DT> rounded(const float (&x)[8]) {
+  Eight<DT> e;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[i] = __uint_as_float(w[i]);
-      x[4 + i] = __uint_as_float(v[i]);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[2 * i] = DT == QSTE_BF16 ? __uint_as_float(w[i] << 16) : f16_to_f32(static_cast<uint16_t>(w[i]));
-      x[2 * i + 1] = DT == QSTE_BF16 ? __uint_as_float(w[i] & 0xFFFF0000u) : f16_to_f32(static_cast<uint16_t>(w[i] >> 16));
-    }
+  for (int i = 0; i < (DT == QSTE_F32 ? 8 : 4); ++i) {
+    if constexpr (DT == QSTE_F32)
+      e.w[i] = __float_as_uint(x[i]);
+    else if constexpr (DT == QSTE_BF16)
+      e.w[i] = f32x2_to_bf16x2(x[2 * i], x[2 * i + 1]);
+    else
+      e.w[i] = static_cast<uint32_t>(f32_to_f16(x[2 * i])) | (static_cast<uint32_t>(f32_to_f16(x[2 * i + 1])) << 16);
   }
+  return e;
 }
 
+// to 16-byte aligned p
 template <int DT>
 __device__ __forceinline__ void store8(typename Elem<DT>::T* p, const float (&x)[8]) {
-  if constexpr (DT == QSTE_F32) {
-    *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
-    *reinterpret_cast<float4*>(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
-  } else {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (DT == QSTE_BF16)
-        w[i] = f32x2_to_bf16x2(x[2 * i], x[2 * i + 1]);
-      else
-        w[i] = static_cast<uint32_t>(f32_to_f16(x[2 * i])) | (static_cast<uint32_t>(f32_to_f16(x[2 * i + 1])) << 16);
-    }
-    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-  }
+  const Eight<DT> e = rounded<DT>(x);
+  *reinterpret_cast<uint4*>(p) = make_uint4(e.w[0], e.w[1], e.w[2], e.w[3]);
+  if constexpr (DT == QSTE_F32) *reinterpret_cast<uint4*>(p + 4) = make_uint4(e.w[4], e.w[5], e.w[6], e.w[7]);
 }
 
 // A tensor in blocks: int8 [rows, cols] and a code for every block of a row.

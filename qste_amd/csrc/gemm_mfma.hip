@@ -320,17 +320,12 @@ __device__ __forceinline__ void gated_epilogue(const PairParams& p, f32x16 (&acc
       const int row = lane >> 2;
       const int64_t grow = m0 + 32 * mb + EPR * half + row;
       const bool there = grow < p.M && gcol < p.N;
-      float g[8], u[8], v[8];
       const uint16_t* at = reinterpret_cast<const uint16_t*>(stg + row * EPL + 16 * piece);
-      blocks::load8<DT>(at, g);
-      blocks::load8<DT>(at + 32, u);
+      blocks::Eight<DT> g8 = blocks::Eight<DT>::load(at), u8 = blocks::Eight<DT>::load(at + 32);
       if (p.gate8.q) {
-        if (!there) {  // what lies past the row's end is no part of its last block
-#pragma unroll
-          for (int i = 0; i < 8; ++i) g[i] = u[i] = 0.0f;
-        }
+        if (!there) g8 = u8 = blocks::Eight<DT>::zeros();  // what lies past the row's end is no part of its last block
         uint32_t gc, uc;
-        const uint2 gq = blocks::quantize8(g, gc), uq = blocks::quantize8(u, uc);
+        const uint2 gq = blocks::quantize8(g8, gc), uq = blocks::quantize8(u8, uc);
         if (there) {
           *reinterpret_cast<uint2*>(p.gate8.q + grow * p.N + gcol) = gq;
           *reinterpret_cast<uint2*>(p.up8.q + grow * p.N + gcol) = uq;
@@ -345,6 +340,9 @@ __device__ __forceinline__ void gated_epilogue(const PairParams& p, f32x16 (&acc
         *reinterpret_cast<uint4*>(p.gate + grow * p.N + gcol) = *reinterpret_cast<const uint4*>(at);
         *reinterpret_cast<uint4*>(p.up + grow * p.N + gcol) = *reinterpret_cast<const uint4*>(at + 32);
       }
+      float g[8], u[8], v[8];
+      g8.values(g);
+      u8.values(u);
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = swiglu::forward_one<DT>(g[i], u[i]);
       blocks::store8<DT>(h + grow * p.N + gcol, v);
@@ -1207,7 +1205,7 @@ __global__ __launch_bounds__(THREADS) void gated_combine_kernel(PairParams p, co
   }
   if (p.gate8.q) {
     uint32_t gc, uc;
-    const uint2 gq = blocks::quantize8(g, gc), uq = blocks::quantize8(u, uc);
+    const uint2 gq = blocks::quantize8(blocks::rounded<DT>(g), gc), uq = blocks::quantize8(blocks::rounded<DT>(u), uc);
     if (there) {
       *reinterpret_cast<uint2*>(p.gate8.q + row * p.N + col) = gq;
       *reinterpret_cast<uint2*>(p.up8.q + row * p.N + col) = uq;

@@ -137,11 +137,8 @@ __device__ __forceinline__ void keep_chunk(const Pair& kept, const uint4& gc, co
   for (int which = 0; which < 2; ++which) {
     const uint4& c = which ? uc : gc;
     const blocks::Blocks& to = which ? kept.up : kept.gate;
-    float x[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = chunk_value(c, i);
     uint32_t code;
-    const uint2 bytes = blocks::quantize8(x, code);
+    const uint2 bytes = blocks::quantize8(blocks::Eight<QSTE_BF16>::of(c), code);
     if (q < stride) {
       *reinterpret_cast<uint2*>(to.q + row * cols + 8 * q) = bytes;
       if ((q & 3) == 0) to.codes[row * ((stride + 3) / 4) + (q >> 2)] = static_cast<uint8_t>(code);
@@ -211,13 +208,10 @@ __global__ __launch_bounds__(kThreads) void forward_blocks_kernel(const typename
   const int64_t step = static_cast<int64_t>(gridDim.x) * kThreads;
   for (int64_t j = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; j < quarters; j += step) {
     const blocks::Quarter p(j, cols, per_row);
-    float gv[8] = {}, uv[8] = {}, hv[8];
-    if (p.there()) {
-      blocks::load8<DT>(g + p.at(), gv);
-      blocks::load8<DT>(u + p.at(), uv);
-    }
+    using E8 = blocks::Eight<DT>;
+    const E8 g8 = p.there() ? E8::load(g + p.at()) : E8::zeros(), u8 = p.there() ? E8::load(u + p.at()) : E8::zeros();
     uint32_t gcode, ucode;
-    const uint2 gq = blocks::quantize8(gv, gcode), uq = blocks::quantize8(uv, ucode);
+    const uint2 gq = blocks::quantize8(g8, gcode), uq = blocks::quantize8(u8, ucode);
     if ((j & 3) == 0) {
       kept.gate.codes[p.block] = static_cast<uint8_t>(gcode);
       kept.up.codes[p.block] = static_cast<uint8_t>(ucode);
@@ -225,6 +219,9 @@ __global__ __launch_bounds__(kThreads) void forward_blocks_kernel(const typename
     if (!p.there()) continue;
     *reinterpret_cast<uint2*>(kept.gate.q + p.at()) = gq;
     *reinterpret_cast<uint2*>(kept.up.q + p.at()) = uq;
+    float gv[8], uv[8], hv[8];
+    g8.values(gv);
+    u8.values(uv);
 #pragma unroll
     for (int i = 0; i < 8; ++i) hv[i] = forward_one<DT>(gv[i], uv[i]);
     blocks::store8<DT>(h + p.at(), hv);
@@ -256,7 +253,36 @@ __global__ __launch_bounds__(kThreads) void backward_kernel(const typename Elem<
   }
 }
 
-// The backward of g and u kept in 8-bit blocks: a quarter of a block a thread.
+// The backward at the g and u that 8-bit blocks stand for: du = dh g s and dg =
+// dh u s (1 + g (1 - s)), s = 1 / (1 + e^-g), each rounded once.  (Without blocks a
+// and da are rounded on the way, as torch's operators do; there is no chain of
+// operators here to agree with.)  16-bit results leave room for the hardware's
+// exponential and reciprocal, within 2^-20 for |g| < 16; fp32 takes full ones.
+template <int DT>
+__device__ __forceinline__ void backward_at(float dh, float g, float u, float& dg, float& du) {
+  float s;
+  if constexpr (DT == QSTE_F32)
+    s = 1.0f / (1.0f + expf(-g));
+  else
+    s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -1.44269504088896340736f));
+  const float a = g * s;
+  du = dh * a;
+  dg = (dh * u) * (s * (1.0f + (g - a)));
+}
+
+// eight columns' gradients from their quarter of a block
+template <int DT>
+__device__ __forceinline__ void backward_quarter(const blocks::Eight<DT>& dh, uint2 gq, uint32_t gcode, uint2 uq,
+                                                 uint32_t ucode, float (&dg)[8], float (&du)[8]) {
+  float h[8], g[8], u[8];
+  dh.values(h);
+  blocks::dequantize8(gq, gcode, g);
+  blocks::dequantize8(uq, ucode, u);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) backward_at<DT>(h[i], g[i], u[i], dg[i], du[i]);
+}
+
+// a quarter of a block a thread
 template <int DT>
 __global__ __launch_bounds__(kThreads) void backward_blocks_kernel(const typename Elem<DT>::T* __restrict__ dh,
                                                                    Pair kept, typename Elem<DT>::T* __restrict__ dg,
@@ -266,14 +292,78 @@ __global__ __launch_bounds__(kThreads) void backward_blocks_kernel(const typenam
   for (int64_t j = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; j < quarters; j += step) {
     const blocks::Quarter p(j, cols, per_row);
     if (!p.there()) continue;
-    float hv[8], gv[8], uv[8], a[8], b[8];
-    blocks::load8<DT>(dh + p.at(), hv);
-    blocks::dequantize8(*reinterpret_cast<const uint2*>(kept.gate.q + p.at()), kept.gate.codes[p.block], gv);
-    blocks::dequantize8(*reinterpret_cast<const uint2*>(kept.up.q + p.at()), kept.up.codes[p.block], uv);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) backward_one<DT>(hv[i], gv[i], uv[i], a[i], b[i]);
+    float a[8], b[8];
+    backward_quarter<DT>(blocks::Eight<DT>::load(dh + p.at()), *reinterpret_cast<const uint2*>(kept.gate.q + p.at()),
+                         kept.gate.codes[p.block], *reinterpret_cast<const uint2*>(kept.up.q + p.at()),
+                         kept.up.codes[p.block], a, b);
     blocks::store8<DT>(dg + p.at(), a);
     blocks::store8<DT>(du + p.at(), b);
+  }
+}
+
+// The same with the sums over the rows of dg off_g and of du off_u, for the two
+// binary layers that made g and u: a workgroup takes 512 columns, eight a lane,
+// of `chunk` rows, each wave every fourth of them; its waves' sums meet in LDS in
+// wave order, and the chunks' [chunk][2][cols] are added in their order by
+// sum_partials_kernel.
+template <int DT>
+__global__ __launch_bounds__(kThreads) void backward_blocks_sums_kernel(
+    const uint16_t* __restrict__ dh, Pair kept, uint16_t* __restrict__ dg, uint16_t* __restrict__ du,
+    const float* __restrict__ off_g, const float* __restrict__ off_u, int64_t rows, int64_t cols, int64_t per_row,
+    int64_t ld, int chunk, float* __restrict__ part) {
+  constexpr int kWaves = kThreads / kWave;
+  __shared__ float red[kWaves][2][512];
+  const int lane = static_cast<int>(threadIdx.x) % kWave, wave = static_cast<int>(threadIdx.x) / kWave;
+  const int64_t base = static_cast<int64_t>(blockIdx.x) * 512, c = base + 8 * lane, block = c / blocks::kBlock;
+  const int64_t first = static_cast<int64_t>(blockIdx.y) * chunk;
+  const int64_t last = first + chunk < rows ? first + chunk : rows;
+  struct Held {
+    blocks::Eight<DT> dh;
+    uint2 gq, uq;
+    uint32_t gcode, ucode;
+    float og, ou;
+  };
+  auto load = [&](int64_t t) {
+    const int64_t at = t * cols + c;
+    return Held{blocks::Eight<DT>::load(dh + at), *reinterpret_cast<const uint2*>(kept.gate.q + at),
+                *reinterpret_cast<const uint2*>(kept.up.q + at), kept.gate.codes[t * per_row + block],
+                kept.up.codes[t * per_row + block], off_g[t], off_u[t]};
+  };
+  float sg[8] = {}, su[8] = {};
+  auto take = [&](int64_t t, const Held& r) {
+    float a[8], b[8];
+    backward_quarter<DT>(r.dh, r.gq, r.gcode, r.uq, r.ucode, a, b);
+    blocks::store8<DT>(dg + t * ld + c, a);
+    blocks::store8<DT>(du + t * ld + c, b);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      sg[i] = fmaf(a[i], r.og, sg[i]);
+      su[i] = fmaf(b[i], r.ou, su[i]);
+    }
+  };
+  if (c < cols) {
+    int64_t t = first + wave;
+    for (; t + 3 * kWaves < last; t += 4 * kWaves) {  // four rows' loads in flight
+      Held r[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) r[k] = load(t + k * kWaves);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) take(t + k * kWaves, r[k]);
+    }
+    for (; t < last; t += kWaves) take(t, load(t));
+  }
+#pragma unroll
+  for (int i = 0; i < 8; i += 4) {
+    *reinterpret_cast<float4*>(&red[wave][0][8 * lane + i]) = make_float4(sg[i], sg[i + 1], sg[i + 2], sg[i + 3]);
+    *reinterpret_cast<float4*>(&red[wave][1][8 * lane + i]) = make_float4(su[i], su[i + 1], su[i + 2], su[i + 3]);
+  }
+  __syncthreads();
+  for (int j = static_cast<int>(threadIdx.x); j < 2 * 512; j += kThreads) {
+    const int which = j / 512, cc = j % 512;
+    float sum = red[0][which][cc];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) sum += red[w][which][cc];
+    if (base + cc < cols) part[(static_cast<int64_t>(blockIdx.y) * 2 + which) * cols + base + cc] = sum;
   }
 }
 
@@ -287,7 +377,7 @@ __global__ __launch_bounds__(kThreads) void backward_blocks_any_kernel(
        i += static_cast<int64_t>(gridDim.x) * kThreads) {
     const int64_t row = i / cols, block = row * per_row + (i - row * cols) / blocks::kBlock;
     float a, b;
-    backward_one<DT>(E::load(dh, i), blocks::dequantize1(kept.gate.q[i], kept.gate.codes[block]),
+    backward_at<DT>(E::load(dh, i), blocks::dequantize1(kept.gate.q[i], kept.gate.codes[block]),
                      blocks::dequantize1(kept.up.q[i], kept.up.codes[block]), a, b);
     E::store(dg, i, a);
     E::store(du, i, b);
@@ -393,51 +483,11 @@ __device__ __forceinline__ void backward_x8(const uint4& hc, const uint4& gc, co
   }
 }
 
-// Where the sums' backward finds eight values of g or u, columns c .. c + 7 of
-// row t: in a 16-bit tensor, or in 8-bit blocks (whose values are exact in the type).
 template <int DT>
-struct Plain {
-  const uint16_t* p;
-  struct Held {
-    uint4 v;
-  };
-  __device__ __forceinline__ Held load(int64_t t, int64_t c, int64_t cols) const {
-    return Held{*reinterpret_cast<const uint4*>(p + t * cols + c)};
-  }
-  __device__ __forceinline__ static uint4 values(const Held& h) { return h.v; }
-};
-
-template <int DT>
-struct Kept {
-  blocks::Blocks b;
-  struct Held {
-    uint2 q;
-    uint32_t code;
-  };
-  __device__ __forceinline__ Held load(int64_t t, int64_t c, int64_t cols) const {
-    return Held{*reinterpret_cast<const uint2*>(b.q + t * cols + c),
-                b.codes[t * ((cols + blocks::kBlock - 1) / blocks::kBlock) + c / blocks::kBlock]};
-  }
-  __device__ __forceinline__ static uint4 values(const Held& h) {
-    float x[8];
-    blocks::dequantize8(h.q, h.code, x);
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (DT == QSTE_BF16)
-        w[i] = f32x2_to_bf16x2(x[2 * i], x[2 * i + 1]);
-      else
-        w[i] = static_cast<uint32_t>(f32_to_f16(x[2 * i])) | (static_cast<uint32_t>(f32_to_f16(x[2 * i + 1])) << 16);
-    }
-    return make_uint4(w[0], w[1], w[2], w[3]);
-  }
-};
-
-template <int DT, class SRC>
 __global__ __launch_bounds__(kSumThreads) void backward_sums_kernel(
-    const uint16_t* __restrict__ dh, SRC g, SRC u, uint16_t* __restrict__ dg, uint16_t* __restrict__ du,
-    const float* __restrict__ off_g, const float* __restrict__ off_u, int64_t samples, int64_t cols, int64_t ldo,
-    float* __restrict__ part) {
+    const uint16_t* __restrict__ dh, const uint16_t* __restrict__ g, const uint16_t* __restrict__ u,
+    uint16_t* __restrict__ dg, uint16_t* __restrict__ du, const float* __restrict__ off_g,
+    const float* __restrict__ off_u, int64_t samples, int64_t cols, int64_t ldo, float* __restrict__ part) {
   constexpr int UNROLL = 4;
   constexpr int kPad = 17;
   constexpr int kRed = kSumWaves * 64 * kPad;
@@ -478,25 +528,24 @@ __global__ __launch_bounds__(kSumThreads) void backward_sums_kernel(
   if (c < cols) {
     int64_t t = t0;
     for (; t + UNROLL <= t1; t += UNROLL) {
-      uint4 hq[UNROLL];
-      typename SRC::Held gq[UNROLL], uq[UNROLL];
+      uint4 hq[UNROLL], gq[UNROLL], uq[UNROLL];
       float og[UNROLL], ou[UNROLL];
 #pragma unroll
       for (int k = 0; k < UNROLL; ++k) {
         const int64_t at = (t + k) * cols + c;
         hq[k] = *reinterpret_cast<const uint4*>(dh + at);
-        gq[k] = g.load(t + k, c, cols);
-        uq[k] = u.load(t + k, c, cols);
+        gq[k] = *reinterpret_cast<const uint4*>(g + at);
+        uq[k] = *reinterpret_cast<const uint4*>(u + at);
         og[k] = off_g[t + k];
         ou[k] = off_u[t + k];
       }
 #pragma unroll
-      for (int k = 0; k < UNROLL; ++k) one(hq[k], SRC::values(gq[k]), SRC::values(uq[k]), t + k, og[k], ou[k]);
+      for (int k = 0; k < UNROLL; ++k) one(hq[k], gq[k], uq[k], t + k, og[k], ou[k]);
     }
     for (; t < t1; ++t) {
       const int64_t at = t * cols + c;
-      one(*reinterpret_cast<const uint4*>(dh + at), SRC::values(g.load(t, c, cols)), SRC::values(u.load(t, c, cols)), t,
-          off_g[t], off_u[t]);
+      one(*reinterpret_cast<const uint4*>(dh + at), *reinterpret_cast<const uint4*>(g + at),
+          *reinterpret_cast<const uint4*>(u + at), t, off_g[t], off_u[t]);
     }
   }
   __syncthreads();  // every wave is done with the tables
@@ -654,12 +703,12 @@ int launch_swiglu_backward_sums(const void* dh, const void* g, const void* u, in
     const dim3 grid(static_cast<unsigned>((cols + 511) / 512), static_cast<unsigned>(chunks));
     if (dtype == QSTE_BF16)
       backward_sums_kernel<QSTE_BF16><<<grid, kSumThreads, 0, s>>>(
-          static_cast<const uint16_t*>(dh), Plain<QSTE_BF16>{static_cast<const uint16_t*>(g)},
-          Plain<QSTE_BF16>{static_cast<const uint16_t*>(u)}, static_cast<uint16_t*>(dg), static_cast<uint16_t*>(du), off_g, off_u, rows, cols, ld_out, part);
+          static_cast<const uint16_t*>(dh), static_cast<const uint16_t*>(g), static_cast<const uint16_t*>(u),
+          static_cast<uint16_t*>(dg), static_cast<uint16_t*>(du), off_g, off_u, rows, cols, ld_out, part);
     else
       backward_sums_kernel<QSTE_F16><<<grid, kSumThreads, 0, s>>>(
-          static_cast<const uint16_t*>(dh), Plain<QSTE_F16>{static_cast<const uint16_t*>(g)},
-          Plain<QSTE_F16>{static_cast<const uint16_t*>(u)}, static_cast<uint16_t*>(dg), static_cast<uint16_t*>(du), off_g, off_u, rows, cols, ld_out, part);
+          static_cast<const uint16_t*>(dh), static_cast<const uint16_t*>(g), static_cast<const uint16_t*>(u),
+          static_cast<uint16_t*>(dg), static_cast<uint16_t*>(du), off_g, off_u, rows, cols, ld_out, part);
     const int rc = static_cast<int>(hipGetLastError());
     if (rc) return rc;
     return launch_sum_partials(part, chunks, 2 * cols, sums, s);
@@ -705,15 +754,27 @@ void run_backward_blocks(const void* dh, const Pair& kept, void* dg, void* du, i
         static_cast<const T*>(dh), kept, static_cast<T*>(dg), static_cast<T*>(du), cols, per_row, rows * cols);
 }
 
+// Rows of a chunk: as many as leave two workgroups a CU, from 16 (four a wave)
+// to 256 (the chunks' sums are then under 1% of the bytes).  us for chunks of 256
+// rows / of the rule's: 250 x 2048 61 / 8, 4096 x 4096 58 / 32, 8192 x 14336 the same.
+inline int chunk_of(int64_t rows, int64_t cols) {
+  const int64_t groups = (cols + 511) / 512;
+  int chunk = 16;
+  while (chunk < 256 && (rows + 2 * chunk - 1) / (2 * chunk) * groups >= 512) chunk *= 2;
+  while ((rows + chunk - 1) / chunk > 65535) chunk *= 2;  // what a grid's second dimension holds
+  return chunk;
+}
+
 template <int DT>
 int run_backward_blocks_sums(const void* dh, const Pair& kept, void* dg, void* du, const float* off_g,
                              const float* off_u, int64_t rows, int64_t cols, float* sums, float* part, hipStream_t s,
                              int64_t ld_out) {
-  const int64_t chunks = (rows + kSumChunk - 1) / kSumChunk;
+  const int chunk = chunk_of(rows, cols);
+  const int64_t chunks = (rows + chunk - 1) / chunk;
   const dim3 grid(static_cast<unsigned>((cols + 511) / 512), static_cast<unsigned>(chunks));
-  backward_sums_kernel<DT><<<grid, kSumThreads, 0, s>>>(
-      static_cast<const uint16_t*>(dh), Kept<DT>{kept.gate}, Kept<DT>{kept.up}, static_cast<uint16_t*>(dg),
-      static_cast<uint16_t*>(du), off_g, off_u, rows, cols, ld_out, part);
+  backward_blocks_sums_kernel<DT><<<grid, kThreads, 0, s>>>(
+      static_cast<const uint16_t*>(dh), kept, static_cast<uint16_t*>(dg), static_cast<uint16_t*>(du), off_g, off_u, rows,
+      cols, blocks::blocks_of(cols), ld_out, chunk, part);
   const int rc = static_cast<int>(hipGetLastError());
   return rc ? rc : launch_sum_partials(part, chunks, 2 * cols, sums, s);
 }
@@ -756,7 +817,13 @@ int launch_swiglu_backward_blocks(const void* dh, int dtype, const int8_t* gq, c
   return static_cast<int>(hipGetLastError());
 }
 
-// sums and part as launch_swiglu_backward_sums has them
+size_t swiglu_backward_blocks_sums_workspace(int64_t rows, int64_t cols) {
+  // (the chunks of other dtypes and layouts are swiglu_backward_sums_workspace's, of 256 rows)
+  const int64_t chunk = swiglu::chunk_of(rows, cols), chunks = (rows + chunk - 1) / chunk;
+  return static_cast<size_t>(chunks * 2 * cols) * sizeof(float);
+}
+
+// sums as launch_swiglu_backward_sums has them; part: swiglu_backward_blocks_sums_workspace of space
 int launch_swiglu_backward_blocks_sums(const void* dh, int dtype, const int8_t* gq, const uint8_t* gcodes,
                                        const int8_t* uq, const uint8_t* ucodes, void* dg, void* du, const float* off_g,
                                        const float* off_u, int64_t rows, int64_t cols, float* sums, float* part,

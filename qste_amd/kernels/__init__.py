@@ -907,9 +907,9 @@ def swiglu_forward_blocks(gate: Tensor, up: Tensor, *, encode: bool = False):
 
 def swiglu_backward_blocks(grad: Tensor, gate: Blocks8, up: Blocks8, offset_gate: Tensor | None = None,
                            offset_up: Tensor | None = None, *, side_by_side: bool = False):
-    """``swiglu_backward`` with the gate and up that 8-bit blocks stand for:
-    ``(grad_gate, grad_up)``; with offsets fp32 [rows] what ``swiglu_backward_sums``
-    returns (``side_by_side`` as there)."""
+    """The gradients of ``silu(gate) * up`` at the gate and up that 8-bit blocks stand
+    for, ``(grad_gate, grad_up)``, rounded once; with offsets fp32 [rows] also their
+    sums, laid out as ``swiglu_backward_sums`` does (``side_by_side`` as there)."""
 
     gate, up = _check_blocks(gate, "gate blocks"), _check_blocks(up, "up blocks")
     device = _require_gpu(grad, gate.payload, gate.codes, up.payload, up.codes, offset_gate, offset_up)
@@ -936,7 +936,7 @@ def swiglu_backward_blocks(grad: Tensor, gate: Blocks8, up: Blocks8, offset_gate
     if side_by_side and (dh.dtype == torch.float32 or cols % 8):
         raise ValueError("side_by_side needs a 16-bit dtype and columns in whole eights")
     sums = torch.empty(2, cols, dtype=torch.float32, device=device)
-    work = _workspace(lib.qste_swiglu_backward_sums_workspace_bytes(rows, cols), device)
+    work = _workspace(lib.qste_swiglu_backward_blocks_sums_workspace_bytes(rows, cols), device)
     if side_by_side:
         both = torch.empty(rows, 2 * cols, dtype=dh.dtype, device=device)
         at, ld = (_ptr(both), _ptr(both) + cols * dh.element_size()), 2 * cols

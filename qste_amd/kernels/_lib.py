@@ -80,6 +80,7 @@ SIGNATURES = {
     "qste_dequantize_blocks": (_int, [_vp, _vp, _vp, _int, _i64, _i64, _vp]),
     "qste_swiglu_forward_blocks": (_int, [_vp, _vp, _int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp]),
     "qste_swiglu_backward_blocks": (_int, [_vp, _int, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp]),
+    "qste_swiglu_backward_blocks_sums_workspace_bytes": (_sz, [_i64, _i64]),
     "qste_swiglu_backward_blocks_sums": (_int, [_vp, _int, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _i64,
                                                 _i64, _vp, _sz, _vp]),
     "qste_gated_workspace_bytes": (_sz, [_i64, _i64, _i64, _int, _int]),

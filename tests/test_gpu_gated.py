@@ -278,10 +278,11 @@ def test_training_node(m, rows, cols, dtype, bias, checkpoint):
     operands = [t if t is None else t.detach() for side in sides for t in side]
     want, g, u = kernels.gated_forward(flat, *operands, cols, keep="values")
     assert torch.equal(_bits(h.detach()), _bits(want))
-    if checkpoint:
-        g, u = (kernels.dequantize_blocks(kernels.quantize_blocks(t)) for t in (g, u))
     payload, offset, xscale = kernels.pack_affine_rows(flat)
-    both, sums = kernels.swiglu_backward_sums(grad, g, u, offset, offset, side_by_side=True)
+    if checkpoint:
+        g, u = kernels.quantize_blocks(g), kernels.quantize_blocks(u)
+    backward = kernels.swiglu_backward_blocks if checkpoint else kernels.swiglu_backward_sums
+    both, sums = backward(grad, g, u, offset, offset, side_by_side=True)
     dx, evidence, grad_scale, grad_bias = kernels.linear_backward(
         both, payload, offset, xscale, torch.cat((sides[0][0], sides[1][0])),
         torch.cat((sides[0][1].float(), sides[1][1].float())), cols, need_bias=bias, offset_dot=sums.reshape(-1))
