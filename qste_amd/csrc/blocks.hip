@@ -19,7 +19,7 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(const typename Elem<
     const Eight<DT> v = p.there() ? Eight<DT>::load(x + p.at()) : Eight<DT>::zeros();
     uint32_t code;
     const uint2 q = quantize8(v, code);
-    if (p.there()) *reinterpret_cast<uint2*>(out.q + p.at()) = q;
+    if (p.there()) store_bytes(out.q + p.at(), q);
     if ((j & 3) == 0) out.codes[p.block] = static_cast<uint8_t>(code);
   }
 }

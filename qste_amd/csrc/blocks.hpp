@@ -157,12 +157,34 @@ __device__ __forceinline__ Eight<DT> rounded(const float (&x)[8]) {
   return e;
 }
 
+// Whether a pass that writes `bytes` stores them without keeping their lines: more
+// than the 256 MiB last-level cache would only push each other out of it.
+inline bool streamed(double bytes) { return bytes > 268435456.0; }
+
+typedef unsigned int Words4 __attribute__((ext_vector_type(4)));
+typedef unsigned int Words2 __attribute__((ext_vector_type(2)));
+
+template <bool ONCE>
+__device__ __forceinline__ void store16(void* p, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  if constexpr (ONCE)
+    __builtin_nontemporal_store(Words4{a, b, c, d}, static_cast<Words4*>(p));
+  else
+    *static_cast<Words4*>(p) = Words4{a, b, c, d};
+}
+template <bool ONCE = false>
+__device__ __forceinline__ void store_bytes(int8_t* p, uint2 q) {
+  if constexpr (ONCE)
+    __builtin_nontemporal_store(Words2{q.x, q.y}, reinterpret_cast<Words2*>(p));
+  else
+    *reinterpret_cast<Words2*>(p) = Words2{q.x, q.y};
+}
+
 // to 16-byte aligned p
-template <int DT>
+template <int DT, bool ONCE = false>
 __device__ __forceinline__ void store8(typename Elem<DT>::T* p, const float (&x)[8]) {
   const Eight<DT> e = rounded<DT>(x);
-  *reinterpret_cast<uint4*>(p) = make_uint4(e.w[0], e.w[1], e.w[2], e.w[3]);
-  if constexpr (DT == QSTE_F32) *reinterpret_cast<uint4*>(p + 4) = make_uint4(e.w[4], e.w[5], e.w[6], e.w[7]);
+  store16<ONCE>(p, e.w[0], e.w[1], e.w[2], e.w[3]);
+  if constexpr (DT == QSTE_F32) store16<ONCE>(p + 4, e.w[4], e.w[5], e.w[6], e.w[7]);
 }
 
 // A tensor in blocks: int8 [rows, cols] and a code for every block of a row.

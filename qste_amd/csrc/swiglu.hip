@@ -129,8 +129,15 @@ struct Pair {
   blocks::Blocks gate, up;
 };
 
+// ONCE, here and below: what is written is stored without keeping its lines
+// (blocks::streamed).  us, kept / streamed, 16384 x 14336 in bf16: the forward with
+// blocks 404 / 393, with the encoding too 414 / 400, the backward 399 / 381, with the sums 380 / 372; 4096 x
+// 4096, whose gradients the next product finds in the cache, 30.6 / 31.3 with the
+// sums.
+
 // Chunk q of a row of g and of u (zeros past the row) to their blocks, the four
 // lanes of a block together.
+template <bool ONCE>
 __device__ __forceinline__ void keep_chunk(const Pair& kept, const uint4& gc, const uint4& uc, int64_t row, int64_t q,
                                            int64_t cols, int64_t stride) {
 #pragma unroll
@@ -140,7 +147,7 @@ __device__ __forceinline__ void keep_chunk(const Pair& kept, const uint4& gc, co
     uint32_t code;
     const uint2 bytes = blocks::quantize8(blocks::Eight<QSTE_BF16>::of(c), code);
     if (q < stride) {
-      *reinterpret_cast<uint2*>(to.q + row * cols + 8 * q) = bytes;
+      blocks::store_bytes<ONCE>(to.q + row * cols + 8 * q, bytes);
       if ((q & 3) == 0) to.codes[row * ((stride + 3) / 4) + (q >> 2)] = static_cast<uint8_t>(code);
     }
   }
@@ -152,9 +159,11 @@ __device__ __forceinline__ void keep_chunk(const Pair& kept, const uint4& gc, co
 // LDS table the workgroup fills once for all its rows (the exponential and
 // the correctly rounded division per entry, not per element); without, for
 // grids of about one row per workgroup, every element computes it.
-// With KEPT the 8-bit blocks of g and u are written too (`gate8`, `up8`).
-template <int CH, bool TAB, bool KEPT>
-__global__ __launch_bounds__(kThreads) void forward_encode_kernel(const uint16_t* __restrict__ g,
+// With KEPT the 8-bit blocks of g and u are written too; its registers are held to
+// the four workgroups a CU that the tabled grid is made for (16384 x 14336: 485 ->
+// 414 us, three at a time before).
+template <int CH, bool TAB, bool KEPT, bool ONCE>
+__global__ __launch_bounds__(kThreads, KEPT ? 4 : 1) void forward_encode_kernel(const uint16_t* __restrict__ g,
                                                                   const uint16_t* __restrict__ u,
                                                                   uint16_t* __restrict__ h,
                                                                   uint8_t* __restrict__ packed,
@@ -180,27 +189,35 @@ __global__ __launch_bounds__(kThreads) void forward_encode_kernel(const uint16_t
     const uint4* gr = reinterpret_cast<const uint4*>(g + row * cols);
     const uint4* ur = reinterpret_cast<const uint4*>(u + row * cols);
     uint4* hr = reinterpret_cast<uint4*>(h + row * cols);
-    uint4 gv[CH], uv[CH], v[CH];
+    uint4 v[CH];
+    // with KEPT two of a row's chunks at a time: all at once they do not fit the
+    // registers that four workgroups a CU leave
+    constexpr int AT = KEPT && CH > 4 ? 2 : CH;
 #pragma unroll
-    for (int k = 0; k < CH; ++k) {
-      const int64_t q = t + static_cast<int64_t>(k) * kThreads;
-      gv[k] = q < stride ? gr[q] : make_uint4(0, 0, 0, 0);
-      uv[k] = q < stride ? ur[q] : make_uint4(0, 0, 0, 0);
-    }
+    for (int k0 = 0; k0 < CH; k0 += AT) {
+      uint4 gv[AT], uv[AT];
 #pragma unroll
-    for (int k = 0; k < CH; ++k) {
-      const int64_t q = t + static_cast<int64_t>(k) * kThreads;
-      v[k] = q >= stride ? make_uint4(0, 0, 0, 0)
-                         : TAB ? forward_chunk_tab(gv[k], uv[k], tab_a) : forward_chunk(gv[k], uv[k]);
-      if (q < stride) hr[q] = v[k];
-      if constexpr (KEPT) keep_chunk(kept, gv[k], uv[k], row, q, cols, stride);
+      for (int k = 0; k < AT; ++k) {
+        const int64_t q = t + static_cast<int64_t>(k0 + k) * kThreads;
+        gv[k] = q < stride ? gr[q] : make_uint4(0, 0, 0, 0);
+        uv[k] = q < stride ? ur[q] : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int k = 0; k < AT; ++k) {
+        const int64_t q = t + static_cast<int64_t>(k0 + k) * kThreads;
+        v[k0 + k] = q >= stride ? make_uint4(0, 0, 0, 0)
+                                : TAB ? forward_chunk_tab(gv[k], uv[k], tab_a) : forward_chunk(gv[k], uv[k]);
+        if (q < stride) hr[q] = v[k0 + k];
+        if constexpr (KEPT) keep_chunk<ONCE>(kept, gv[k], uv[k], row, q, cols, stride);
+      }
+      if constexpr (AT < CH) __builtin_amdgcn_sched_barrier(0);
     }
     encode_row_chunks<kThreads, CH>(v, packed + row * stride, offset + row, scale + row, cols, stride, red);
   }
 }
 
 // The forward with a checkpoint: any dtype, a quarter of a block a thread.
-template <int DT>
+template <int DT, bool ONCE>
 __global__ __launch_bounds__(kThreads) void forward_blocks_kernel(const typename Elem<DT>::T* __restrict__ g,
                                                                   const typename Elem<DT>::T* __restrict__ u,
                                                                   typename Elem<DT>::T* __restrict__ h, Pair kept,
@@ -217,14 +234,14 @@ __global__ __launch_bounds__(kThreads) void forward_blocks_kernel(const typename
       kept.up.codes[p.block] = static_cast<uint8_t>(ucode);
     }
     if (!p.there()) continue;
-    *reinterpret_cast<uint2*>(kept.gate.q + p.at()) = gq;
-    *reinterpret_cast<uint2*>(kept.up.q + p.at()) = uq;
+    blocks::store_bytes<ONCE>(kept.gate.q + p.at(), gq);
+    blocks::store_bytes<ONCE>(kept.up.q + p.at(), uq);
     float gv[8], uv[8], hv[8];
     g8.values(gv);
     u8.values(uv);
 #pragma unroll
     for (int i = 0; i < 8; ++i) hv[i] = forward_one<DT>(gv[i], uv[i]);
-    blocks::store8<DT>(h + p.at(), hv);
+    blocks::store8<DT, ONCE>(h + p.at(), hv);
   }
 }
 
@@ -283,7 +300,7 @@ __device__ __forceinline__ void backward_quarter(const blocks::Eight<DT>& dh, ui
 }
 
 // a quarter of a block a thread
-template <int DT>
+template <int DT, bool ONCE>
 __global__ __launch_bounds__(kThreads) void backward_blocks_kernel(const typename Elem<DT>::T* __restrict__ dh,
                                                                    Pair kept, typename Elem<DT>::T* __restrict__ dg,
                                                                    typename Elem<DT>::T* __restrict__ du,
@@ -296,8 +313,8 @@ __global__ __launch_bounds__(kThreads) void backward_blocks_kernel(const typenam
     backward_quarter<DT>(blocks::Eight<DT>::load(dh + p.at()), *reinterpret_cast<const uint2*>(kept.gate.q + p.at()),
                          kept.gate.codes[p.block], *reinterpret_cast<const uint2*>(kept.up.q + p.at()),
                          kept.up.codes[p.block], a, b);
-    blocks::store8<DT>(dg + p.at(), a);
-    blocks::store8<DT>(du + p.at(), b);
+    blocks::store8<DT, ONCE>(dg + p.at(), a);
+    blocks::store8<DT, ONCE>(du + p.at(), b);
   }
 }
 
@@ -306,7 +323,7 @@ __global__ __launch_bounds__(kThreads) void backward_blocks_kernel(const typenam
 // of `chunk` rows, each wave every fourth of them; its waves' sums meet in LDS in
 // wave order, and the chunks' [chunk][2][cols] are added in their order by
 // sum_partials_kernel.
-template <int DT>
+template <int DT, bool ONCE>
 __global__ __launch_bounds__(kThreads) void backward_blocks_sums_kernel(
     const uint16_t* __restrict__ dh, Pair kept, uint16_t* __restrict__ dg, uint16_t* __restrict__ du,
     const float* __restrict__ off_g, const float* __restrict__ off_u, int64_t rows, int64_t cols, int64_t per_row,
@@ -333,8 +350,8 @@ __global__ __launch_bounds__(kThreads) void backward_blocks_sums_kernel(
   auto take = [&](int64_t t, const Held& r) {
     float a[8], b[8];
     backward_quarter<DT>(r.dh, r.gq, r.gcode, r.uq, r.ucode, a, b);
-    blocks::store8<DT>(dg + t * ld + c, a);
-    blocks::store8<DT>(du + t * ld + c, b);
+    blocks::store8<DT, ONCE>(dg + t * ld + c, a);
+    blocks::store8<DT, ONCE>(du + t * ld + c, b);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       sg[i] = fmaf(a[i], r.og, sg[i]);
@@ -583,7 +600,7 @@ inline bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15
 int launch_pack_affine_rows(const void*, int, uint8_t*, float*, float*, int64_t, int64_t, hipStream_t);
 
 // The forward that encodes h, for bf16 rows of at most 8 * kThreads chunks.
-template <bool KEPT>
+template <bool KEPT, bool ONCE>
 static void launch_encode(bool tab, const void* g, const void* u, void* h, uint8_t* packed, float* offset,
                           float* scale, int64_t rows, int64_t cols, const swiglu::Pair& kept, hipStream_t s) {
   using namespace swiglu;
@@ -593,16 +610,16 @@ static void launch_encode(bool tab, const void* g, const void* u, void* h, uint8
   const auto* up = static_cast<const uint16_t*>(u);
   auto* hp = static_cast<uint16_t*>(h);
   if (stride <= 2 * kThreads && tab)
-    forward_encode_kernel<2, true, KEPT>
+    forward_encode_kernel<2, true, KEPT, ONCE>
         <<<grid, kThreads, 0, s>>>(gp, up, hp, packed, offset, scale, rows, cols, stride, kept);
   else if (stride <= 2 * kThreads)
-    forward_encode_kernel<2, false, KEPT>
+    forward_encode_kernel<2, false, KEPT, ONCE>
         <<<grid, kThreads, 0, s>>>(gp, up, hp, packed, offset, scale, rows, cols, stride, kept);
   else if (tab)
-    forward_encode_kernel<8, true, KEPT>
+    forward_encode_kernel<8, true, KEPT, ONCE>
         <<<grid, kThreads, 0, s>>>(gp, up, hp, packed, offset, scale, rows, cols, stride, kept);
   else
-    forward_encode_kernel<8, false, KEPT>
+    forward_encode_kernel<8, false, KEPT, ONCE>
         <<<grid, kThreads, 0, s>>>(gp, up, hp, packed, offset, scale, rows, cols, stride, kept);
 }
 
@@ -617,7 +634,7 @@ int launch_swiglu_forward(const void* g, const void* u, int dtype, void* h, uint
     // with at least kTabRows rows per workgroup of kEncodeGroups, each fills
     // the table once for its rows; fewer rows take a workgroup per row
     const bool tab = rows >= kTabRows * kEncodeGroups;
-    launch_encode<false>(tab, g, u, h, packed, offset, scale, rows, cols, Pair{}, s);
+    launch_encode<false, false>(tab, g, u, h, packed, offset, scale, rows, cols, Pair{}, s);
     return static_cast<int>(hipGetLastError());
   }
   if (vec) {
@@ -730,6 +747,14 @@ int launch_quantize_blocks(const void*, int, int8_t*, uint8_t*, int64_t, int64_t
 namespace swiglu {
 
 inline bool aligned8(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7) == 0; }
+// whether the forward, which writes h and two bytes an element, and the backward,
+// which writes two tensors, stream them
+inline bool forward_once(int64_t rows, int64_t cols, int dtype) {
+  return blocks::streamed(static_cast<double>(rows) * cols * (dtype == QSTE_F32 ? 6 : 4));
+}
+inline bool backward_once(int64_t rows, int64_t cols, int dtype) {
+  return blocks::streamed(static_cast<double>(rows) * cols * (dtype == QSTE_F32 ? 8 : 4));
+}
 inline bool kept_ok(const Pair& kept, int64_t cols) { return cols % 8 == 0 && aligned8(kept.gate.q) && aligned8(kept.up.q); }
 
 template <int DT>
@@ -737,8 +762,9 @@ void run_forward_blocks(const void* g, const void* u, void* h, const Pair& kept,
                         hipStream_t s) {
   using T = typename Elem<DT>::T;
   const int64_t per_row = blocks::blocks_of(cols), quarters = 4 * rows * per_row;
-  forward_blocks_kernel<DT><<<grid_of(quarters), kThreads, 0, s>>>(
-      static_cast<const T*>(g), static_cast<const T*>(u), static_cast<T*>(h), kept, cols, per_row, quarters);
+  auto* kernel = forward_once(rows, cols, DT) ? forward_blocks_kernel<DT, true> : forward_blocks_kernel<DT, false>;
+  kernel<<<grid_of(quarters), kThreads, 0, s>>>(static_cast<const T*>(g), static_cast<const T*>(u), static_cast<T*>(h),
+                                                kept, cols, per_row, quarters);
 }
 
 template <int DT>
@@ -746,17 +772,20 @@ void run_backward_blocks(const void* dh, const Pair& kept, void* dg, void* du, i
                          hipStream_t s) {
   using T = typename Elem<DT>::T;
   const int64_t per_row = blocks::blocks_of(cols), quarters = 4 * rows * per_row;
-  if (kept_ok(kept, cols) && aligned(dh) && aligned(dg) && aligned(du))
-    backward_blocks_kernel<DT><<<grid_of(quarters), kThreads, 0, s>>>(
-        static_cast<const T*>(dh), kept, static_cast<T*>(dg), static_cast<T*>(du), cols, per_row, quarters);
-  else
+  if (kept_ok(kept, cols) && aligned(dh) && aligned(dg) && aligned(du)) {
+    auto* kernel = backward_once(rows, cols, DT) ? backward_blocks_kernel<DT, true> : backward_blocks_kernel<DT, false>;
+    kernel<<<grid_of(quarters), kThreads, 0, s>>>(static_cast<const T*>(dh), kept, static_cast<T*>(dg),
+                                                  static_cast<T*>(du), cols, per_row, quarters);
+  } else {
     backward_blocks_any_kernel<DT><<<grid_of(rows * cols), kThreads, 0, s>>>(
         static_cast<const T*>(dh), kept, static_cast<T*>(dg), static_cast<T*>(du), cols, per_row, rows * cols);
+  }
 }
 
 // Rows of a chunk: as many as leave two workgroups a CU, from 16 (four a wave)
-// to 256 (the chunks' sums are then under 1% of the bytes).  us for chunks of 256
-// rows / of the rule's: 250 x 2048 61 / 8, 4096 x 4096 58 / 32, 8192 x 14336 the same.
+// to 256 (the chunks' sums are then under 1% of the bytes).  us a call, chunks of
+// 256 rows / of the rule's: 250 x 2048 34.6 / 19.0, 4096 x 4096 42 / 31, 8192 x 14336
+// the same.
 inline int chunk_of(int64_t rows, int64_t cols) {
   const int64_t groups = (cols + 511) / 512;
   int chunk = 16;
@@ -772,7 +801,9 @@ int run_backward_blocks_sums(const void* dh, const Pair& kept, void* dg, void* d
   const int chunk = chunk_of(rows, cols);
   const int64_t chunks = (rows + chunk - 1) / chunk;
   const dim3 grid(static_cast<unsigned>((cols + 511) / 512), static_cast<unsigned>(chunks));
-  backward_blocks_sums_kernel<DT><<<grid, kThreads, 0, s>>>(
+  auto* kernel =
+      backward_once(rows, cols, DT) ? backward_blocks_sums_kernel<DT, true> : backward_blocks_sums_kernel<DT, false>;
+  kernel<<<grid, kThreads, 0, s>>>(
       static_cast<const uint16_t*>(dh), kept, static_cast<uint16_t*>(dg), static_cast<uint16_t*>(du), off_g, off_u, rows,
       cols, blocks::blocks_of(cols), ld_out, chunk, part);
   const int rc = static_cast<int>(hipGetLastError());
@@ -794,7 +825,11 @@ int launch_swiglu_forward_blocks(const void* g, const void* u, int dtype, void* 
     return launch_quantize_blocks(u, dtype, uq, ucodes, rows, cols, s);
   }
   if (packed && dtype == QSTE_BF16 && cols / 8 <= 8 * kThreads) {
-    launch_encode<true>(rows >= kTabRows * kEncodeGroups, g, u, h, packed, offset, scale, rows, cols, kept, s);
+    const bool tab = rows >= kTabRows * kEncodeGroups;
+    if (forward_once(rows, cols, dtype))
+      launch_encode<true, true>(tab, g, u, h, packed, offset, scale, rows, cols, kept, s);
+    else
+      launch_encode<true, false>(tab, g, u, h, packed, offset, scale, rows, cols, kept, s);
     return static_cast<int>(hipGetLastError());
   }
   if (dtype == QSTE_F32) run_forward_blocks<QSTE_F32>(g, u, h, kept, rows, cols, s);
