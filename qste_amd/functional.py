@@ -269,32 +269,60 @@ def _through_scale(grad_scale: Tensor, e: Tensor, surface: Surface) -> Tensor:
     return kernels.row_scale_backward(e, grad_scale.to(e.dtype), surface.cfg.scale_min, surface.cfg.scale_max)
 
 
-def _gate_up_backward(ctx, dh: list, kept: tuple, payload_x: Tensor, aux_x: Tensor, packed_g: Tensor, scale_g: Tensor,
-                      packed_u: Tensor, scale_u: Tensor, sg: Surface, su: Surface):
+def _gate_up_backward(ctx, dh: list, kept: tuple, payload_x: Tensor, aux_x: Tensor, packed_g: Tensor, packed_u: Tensor,
+                      scale_gu: Tensor, sg: Surface, su: Surface):
     """The gate's backward and that of the two layers before it as one layer of 2
-    ffn rows, their evidence delivered: ``(dx, gate's and up's scale gradients and
-    bias gradients)``.  ``dh``: the gradient of h in a list, taken out of it so that it
-    is free during the product; ``kept``: g and u, as tensors or ``Blocks8``."""
+    ffn rows, their evidence delivered: ``(dx, scale gradients [2 ffn], bias
+    gradients [2 ffn] or None)``.  ``dh``: the gradient of h in a list, taken out of it
+    so that it is free during the product; ``kept``: g and u, as tensors or ``Blocks8``;
+    ``scale_gu``: both layers' scales, fp32."""
 
     d, ffn = sg.columns, sg.rows
     backward = kernels.swiglu_backward_blocks if isinstance(kept[0], kernels.Blocks8) else kernels.swiglu_backward_sums
     both, sums = backward(dh.pop(), *kept, aux_x[0], aux_x[0], side_by_side=True)
-    # gate and up as one layer of 2 ffn rows (copies of their signs and
-    # scales: the deliveries below may rewrite the signs)
+    # (a copy of their signs: the deliveries below may rewrite them)
     packed_gu = torch.cat((packed_g, packed_u))
-    scale_gu = torch.cat((scale_g.detach().float(), scale_u.detach().float()))
-    bg, bu = ctx.bias_dtypes[:2]
-    need_bias = bg is not None or bu is not None
     dx, ev_gu, gs_gu, gb_gu = kernels.linear_backward(
-        both, payload_x, aux_x[0], aux_x[1], packed_gu, scale_gu, d, need_bias=need_bias,
-        need_input=ctx.needs_input_grad[0], offset_dot=sums.reshape(-1))
+        both, payload_x, aux_x[0], aux_x[1], packed_gu, scale_gu, d,
+        need_bias=any(b is not None for b in ctx.bias_dtypes[:2]), need_input=ctx.needs_input_grad[0],
+        offset_dot=sums.reshape(-1))
     del both
     if dx is not None:
         dx = dx.reshape(ctx.input_shape)
     sg.consume_evidence(ev_gu[:ffn])
     su.consume_evidence(ev_gu[ffn:])
-    gb_g, gb_u = (gb_gu[:ffn], gb_gu[ffn:]) if need_bias else (None, None)
-    return dx, gs_gu[:ffn], gs_gu[ffn:], gb_g, gb_u
+    return dx, gs_gu, gb_gu
+
+
+def _halves(t: Tensor | None, rows: int) -> tuple:
+    """A tensor of two layers' rows as the gate's and up's."""
+
+    return (None, None) if t is None else (t[:rows], t[rows:])
+
+
+def _two_scales(log_g: Tensor, log_u: Tensor, sg: Surface, su: Surface) -> tuple[Tensor, Tensor, Tensor | None]:
+    """Both layers' scales (fp32 [2 ffn]) and their exponentials: one tensor and
+    None, or, where the log-scales' dtypes differ, one each."""
+
+    ffn, (g, u) = sg.rows, (sg.cfg, su.cfg)
+    if log_g.dtype != log_u.dtype:
+        scale_g, e_g = kernels.row_scale(log_g, g.scale_min, g.scale_max)
+        scale_u, e_u = kernels.row_scale(log_u, u.scale_min, u.scale_max)
+        return torch.cat((scale_g.float(), scale_u.float())), e_g, e_u
+    scale, e = (torch.empty(2 * ffn, dtype=log_g.dtype, device=log_g.device) for _ in range(2))
+    kernels.row_scale(log_g, g.scale_min, g.scale_max, (scale[:ffn], e[:ffn]))
+    kernels.row_scale(log_u, u.scale_min, u.scale_max, (scale[ffn:], e[ffn:]))
+    return scale.float(), e, None
+
+
+def _through_two_scales(grad: Tensor, e: Tensor, e_u: Tensor | None, sg: Surface, su: Surface) -> tuple[Tensor, Tensor]:
+    """``_through_scale`` of both layers, of what ``_two_scales`` returned; one launch where their bounds agree."""
+
+    ffn = sg.rows
+    if e_u is None and (sg.cfg.scale_min, sg.cfg.scale_max) == (su.cfg.scale_min, su.cfg.scale_max):
+        return _halves(_through_scale(grad, e, sg), ffn)
+    e_g, e_u = (e[:ffn], e[ffn:]) if e_u is None else (e, e_u)
+    return _through_scale(grad[:ffn], e_g, sg), _through_scale(grad[ffn:], e_u, su)
 
 
 class GatedFn(Function):
@@ -309,15 +337,15 @@ class GatedFn(Function):
     def forward(ctx, inputs, packed_g, log_g, bias_g, packed_u, log_u, bias_u, surfaces, checkpoint: bool,
                 grad_on: bool):
         sg, su = surfaces
-        d = sg.columns
+        d, ffn = sg.columns, sg.rows
         flat = inputs.reshape(-1, d)
-        scale_g, e_g = kernels.row_scale(log_g, sg.cfg.scale_min, sg.cfg.scale_max)
-        scale_u, e_u = kernels.row_scale(log_u, su.cfg.scale_min, su.cfg.scale_max)
+        scale_gu, e, e_u = _two_scales(log_g, log_u, sg, su)
         keep = "" if not grad_on else "blocks" if checkpoint else "values"
-        h, g, u = kernels.gated_forward(flat, packed_g, scale_g, bias_g, packed_u, scale_u, bias_u, d, keep=keep)
+        h, g, u = kernels.gated_forward(flat, packed_g, scale_gu[:ffn], bias_g, packed_u, scale_gu[ffn:], bias_u, d,
+                                        keep=keep)
         if grad_on:
             payload_x, aux_x = _encoding_of(inputs, flat, d)
-            more = (payload_x, aux_x, packed_g, scale_g, packed_u, scale_u, e_g, e_u)
+            more = (payload_x, aux_x, packed_g, packed_u, scale_gu, e, e_u)
             if checkpoint:
                 _save_kept(ctx, g, u, *more)
             else:
@@ -326,20 +354,21 @@ class GatedFn(Function):
         ctx.surfaces = surfaces
         ctx.input_shape = inputs.shape
         ctx.bias_dtypes = tuple(None if b is None else b.dtype for b in (bias_g, bias_u))
-        return h.reshape(*inputs.shape[:-1], sg.rows)
+        return h.reshape(*inputs.shape[:-1], ffn)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_output):
         forget_encodings()
         saved = ctx.saved_tensors
-        payload_x, aux_x, packed_g, scale_g, packed_u, scale_u, e_g, e_u = saved[-8:]
+        payload_x, aux_x, packed_g, packed_u, scale_gu, e, e_u = saved[-7:]
         sg, su = ctx.surfaces
-        dx, gs_g, gs_u, gb_g, gb_u = _gate_up_backward(ctx, [grad_output.reshape(-1, sg.rows)], _kept(ctx, saved),
-                                                       payload_x, aux_x, packed_g, scale_g, packed_u, scale_u, sg, su)
+        dx, gs_gu, gb_gu = _gate_up_backward(ctx, [grad_output.reshape(-1, sg.rows)], _kept(ctx, saved), payload_x,
+                                             aux_x, packed_g, packed_u, scale_gu, sg, su)
+        log_g, log_u = _through_two_scales(gs_gu, e, e_u, sg, su)
+        gb_g, gb_u = _halves(gb_gu, sg.rows)
         bg, bu = ctx.bias_dtypes
-        return (dx, None, _through_scale(gs_g, e_g, sg), _cast(gb_g, bg), None, _through_scale(gs_u, e_u, su),
-                _cast(gb_u, bu), None, None, None)
+        return dx, None, log_g, _cast(gb_g, bg), None, log_u, _cast(gb_u, bu), None, None, None
 
 
 class SwiGLUMLPFn(Function):
@@ -425,8 +454,9 @@ class SwiGLUMLPFn(Function):
         sd.consume_evidence(ev_d)
         del ev_d
         dh = [dh]
-        dx, gs_g, gs_u, gb_g, gb_u = _gate_up_backward(ctx, dh, kept, payload_x, aux_x, packed_g, scale_g, packed_u, scale_u,
-                                                       sg, su)
+        scale_gu = torch.cat((scale_g.detach().float(), scale_u.detach().float()))
+        dx, gs_gu, gb_gu = _gate_up_backward(ctx, dh, kept, payload_x, aux_x, packed_g, packed_u, scale_gu, sg, su)
+        (gs_g, gs_u), (gb_g, gb_u) = _halves(gs_gu, ffn), _halves(gb_gu, ffn)
 
         return (dx, None, _through_scale(gs_g, e_g, sg), _cast(gb_g, bg), None, _through_scale(gs_u, e_u, su),
                 _cast(gb_u, bu), None, _through_scale(gs_d, e_d, sd), _cast(gb_d, bd), None, None, None)

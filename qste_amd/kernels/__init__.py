@@ -1012,14 +1012,18 @@ def _leading(t: Tensor) -> int:
     return count
 
 
-def row_scale(log_scale: Tensor, lo: float, hi: float) -> tuple[Tensor, Tensor]:
+def row_scale(log_scale: Tensor, lo: float, hi: float,
+              out: tuple[Tensor, Tensor] | None = None) -> tuple[Tensor, Tensor]:
     """``(clamp(exp(log_scale), lo, hi), exp(log_scale))`` in log_scale's
     dtype (fp32, fp16 or bf16), one launch (surface.py:84-85), rounded as
-    torch's ``exp().clamp()`` on that dtype."""
+    torch's ``exp().clamp()`` on that dtype; in ``out``, two contiguous tensors of
+    that shape and dtype, if given."""
 
     device = _require_gpu(log_scale)
     ls = log_scale.detach().contiguous()
-    scale, e = torch.empty_like(ls), torch.empty_like(ls)
+    scale, e = (torch.empty_like(ls), torch.empty_like(ls)) if out is None else out
+    if out is not None and not all(t.shape == ls.shape and t.dtype == ls.dtype and t.is_contiguous() for t in out):
+        raise ValueError("row_scale's outputs must be contiguous and of log_scale's shape and dtype")
     code = _lib.load().qste_row_scale(_ptr(ls), _dtype_code(ls), _ptr(scale), _ptr(e), ls.numel(), float(lo),
                                       float(hi), _stream(device))
     _lib.check(code, "row_scale")

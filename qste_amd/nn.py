@@ -86,27 +86,31 @@ def gated(inputs: Tensor, gate, up, *, checkpoint: bool = False) -> Tensor:
     that the one kernel does not take (columns that are no multiple of 64, rows that
     are none of 8, fp32 past 21 rows) run layer by layer."""
 
-    from .functional import GatedFn, _autocast, gated_fusable
-
-    trained = [hasattr(layer, "surface") for layer in (gate, up)]
-    if all(trained):
-        x = _autocast(inputs)
-        _no_tangent("gated", x)
-        if not gated_fusable(x, gate, up):
-            return swiglu(gate(inputs), up(inputs), checkpoint=checkpoint)
-        surfaces = (gate.surface, up.surface)
-        for s in surfaces:
-            s.note_forward()
-        return GatedFn.apply(x, gate.surface.packed_sign, gate.surface.log_scale, gate.bias, up.surface.packed_sign,
-                             up.surface.log_scale, up.bias, surfaces, checkpoint, torch.is_grad_enabled())
-    if any(trained) or not (hasattr(gate, "packed_sign") and hasattr(up, "packed_sign")):
+    # a module's buffers and parts by their dicts: attributes of modules are looked up in Python, half a microsecond each
+    try:
+        served, trained = gate._buffers, "surface" in gate._modules and "surface" in up._modules
+        other = up._buffers
+    except AttributeError:
+        served, other, trained = {}, {}, False
+    if "packed_sign" in served and "packed_sign" in other:
+        if gate.in_features != up.in_features:
+            raise ValueError(f"gate takes {gate.in_features} columns and up {up.in_features}")
+        return kernels.gated_forward(inputs.detach(), served["packed_sign"], served["scale"], served["bias"],
+                                     other["packed_sign"], other["scale"], other["bias"], gate.in_features)[0]
+    if not trained:
         raise TypeError("gated takes two QSTELinear or two PackedLinear layers, got "
                         f"{type(gate).__name__} and {type(up).__name__}")
-    if gate.in_features != up.in_features:
-        raise ValueError(f"gate takes {gate.in_features} columns and up {up.in_features}")
-    with torch.no_grad():
-        return kernels.gated_forward(inputs, gate.packed_sign, gate.scale, gate.bias, up.packed_sign, up.scale, up.bias,
-                                     gate.in_features)[0]
+    from .functional import GatedFn, _autocast, gated_fusable
+
+    x = _autocast(inputs)
+    _no_tangent("gated", x)
+    if not gated_fusable(x, gate, up):
+        return swiglu(gate(inputs), up(inputs), checkpoint=checkpoint)
+    surfaces = (gate.surface, up.surface)
+    for s in surfaces:
+        s.note_forward()
+    return GatedFn.apply(x, gate.surface.packed_sign, gate.surface.log_scale, gate.bias, up.surface.packed_sign,
+                         up.surface.log_scale, up.bias, surfaces, checkpoint, torch.is_grad_enabled())
 
 
 def swiglu_mlp(inputs: Tensor, gate, up, down, *, checkpoint: bool = False) -> Tensor:
