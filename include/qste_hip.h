@@ -475,8 +475,8 @@ int qste_swiglu_backward_blocks_sums(const void* grad, int dtype, const int8_t* 
 
 /* out [m, rows] = silu(g) * u with g = (x . sign(gate)^T) * gate_scale +
  * gate_bias and u likewise of up: two binary layers of one input x [m, cols] and
- * the gate between them, g and u rounded to `dtype` and the gate as
- * qste_swiglu_forward rounds it.  Signs are packed [rows, ceil(cols / 8)],
+ * the gate between them, g and u rounded to `dtype` and their gate once more.
+ * Signs are packed [rows, ceil(cols / 8)],
  * scales fp32 [rows], biases fp32 [rows] or NULL.
  * What a backward needs is written where asked for: g and u as they are
  * (gate_out and up_out, both or neither) and as 8-bit blocks (the four blocks'
@@ -484,7 +484,8 @@ int qste_swiglu_backward_blocks_sums(const void* grad, int dtype, const int8_t* 
  * One launch (two where K is cut into ranges) up to 64 rows of bf16 / fp16 and 21
  * of fp32 with nothing kept, and on the 16-bit tiles where cols is a multiple
  * of 64 and rows of 8; elsewhere the two products (qste_packed_linear_affine_ws)
- * and the gate one after the other, with g and u in the workspace.  Sums are
+ * and qste_swiglu_forward (which rounds silu(g) too) one after the other, with g and
+ * u in the workspace.  Sums are
  * fp32, in an order that may differ from the two products' called alone: g and u
  * may then differ by an ulp.  x, the signs, out, gate_out and up_out start at
  * 16-byte steps and payloads at 8-byte steps (QSTE_E_ALIGN otherwise).

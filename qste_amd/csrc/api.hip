@@ -834,7 +834,7 @@ int qste_gated_route(int64_t m, int64_t rows, int64_t cols, int dtype, int keep)
 }
 
 size_t qste_gated_workspace_bytes(int64_t m, int64_t rows, int64_t cols, int dtype, int keep) {
-  if (!dtype_ok(dtype) || m <= 0 || rows <= 0 || cols <= 0) return 0;
+  if (!dtype_ok(dtype) || m <= 0 || rows <= 0 || cols < 0) return 0;
   switch (gated_route(m, rows, cols, dtype, keep)) {
     case kSkinny: return gemv_gated_workspace(m, rows, cols, dtype);
     case kTiles: return mfma_gated_workspace(m, rows, cols);

@@ -344,8 +344,9 @@ __device__ __forceinline__ void gated_epilogue(const PairParams& p, f32x16 (&acc
       g8.values(g);
       u8.values(u);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = swiglu::forward_one<DT>(g[i], u[i]);
-      blocks::store8<DT>(h + grow * p.N + gcol, v);
+      for (int i = 0; i < 8; ++i) v[i] = swiglu::gated_one<DT>(g[i], u[i]);
+      // streaming, as the forward's: 500 x 8192 over 2048 29.6 -> 28.6 us, large sizes within noise
+      blocks::store8<DT, true>(h + grow * p.N + gcol, v);
     }
   }
 }
@@ -1222,7 +1223,7 @@ __global__ __launch_bounds__(THREADS) void gated_combine_kernel(PairParams p, co
     blocks::store8<DT>(p.up + row * p.N + col, u);
   }
 #pragma unroll
-  for (int q = 0; q < 8; ++q) v[q] = swiglu::forward_one<DT>(g[q], u[q]);
+  for (int q = 0; q < 8; ++q) v[q] = swiglu::gated_one<DT>(g[q], u[q]);
   blocks::store8<DT>(static_cast<uint16_t*>(p.out) + row * p.N + col, v);
 }
 #undef QSTE_WIDE_STAGES

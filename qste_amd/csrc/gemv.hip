@@ -185,7 +185,7 @@ __device__ __forceinline__ void finish_gated4(const Args& p, int64_t m, int64_t 
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const float a = Elem<OUT>::round(g[j] * gs[j] + gb[j]), b = Elem<OUT>::round(u[j] * us[j] + ub[j]);
-    h[j] = swiglu::forward_one<OUT>(a, b);
+    h[j] = swiglu::gated_one<OUT>(a, b);
   }
   finish4<OUT>(p, m, n, h, ones, zeros, vec);
 }

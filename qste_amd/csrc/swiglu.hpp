@@ -1,5 +1,5 @@
-// silu(g) * u for one element, rounded as torch's operators round it: shared by
-// the gate's own passes and the products that end in it, so all give the same bits.
+// silu(g) * u for one element: as torch's operators round it (the gate's own
+// passes), and in one (the products that end in it).
 #pragma once
 
 #include "common.hpp"
@@ -14,6 +14,18 @@ __device__ __forceinline__ float forward_one(float g, float u) {
   using E = Elem<DT>;
   const float a = E::round(silu_value(g));
   return a * u;  // rounded by the caller's store
+}
+
+// silu(g) u before its only rounding, to the type.  16-bit types leave room for
+// the hardware's exponential and reciprocal: within 2^-24 (|g| + 10) of the
+// value, and a third of the instructions (the tiles' 8190 x 14336 over 4096: 1373 ->
+// 1261 us).
+template <int DT>
+__device__ __forceinline__ float gated_one(float g, float u) {
+  if constexpr (DT == QSTE_F32)
+    return silu_value(g) * u;
+  else
+    return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -1.44269504088896340736f)) * u;
 }
 
 }  // namespace swiglu

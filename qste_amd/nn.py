@@ -78,8 +78,9 @@ def gated(inputs: Tensor, gate, up, *, checkpoint: bool = False) -> Tensor:
     converted layers (QSTELinear) or two packed ones (PackedLinear, which carry no
     gradient): both products, the activation and the product in one kernel.
 
-    No counterpart in the reference.  The values are those of the layers called
-    one by one up to the order of the fp32 sums.  With gradients it is one
+    No counterpart in the reference.  gate's and up's values are those of the
+    layers called one by one up to the order of the fp32 sums; their gate is rounded
+    once, where the operators one by one round silu's value too.  With gradients it is one
     autograd node, whose backward runs the two layers as one; evidence and
     scale gradients go where the layers' own would.  ``checkpoint`` keeps gate and up
     for the backward in 8-bit blocks (``quantize_blocks``) in place of 16 bits.  Sizes
@@ -88,11 +89,11 @@ def gated(inputs: Tensor, gate, up, *, checkpoint: bool = False) -> Tensor:
 
     # a module's buffers and parts by their dicts: attributes of modules are looked up in Python, half a microsecond each
     try:
-        served, trained = gate._buffers, "surface" in gate._modules and "surface" in up._modules
-        other = up._buffers
+        served, other = gate._buffers, up._buffers
+        trained = all("surface" in m._modules and "bias" in m._parameters for m in (gate, up))
     except AttributeError:
         served, other, trained = {}, {}, False
-    if "packed_sign" in served and "packed_sign" in other:
+    if "packed_sign" in served and "packed_sign" in other and "bias" in served and "bias" in other:
         if gate.in_features != up.in_features:
             raise ValueError(f"gate takes {gate.in_features} columns and up {up.in_features}")
         return kernels.gated_forward(inputs.detach(), served["packed_sign"], served["scale"], served["bias"],

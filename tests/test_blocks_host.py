@@ -47,6 +47,10 @@ def test_layers_that_are_no_pair():
     other = qste.PackedLinear(packed, scale, 60, None)
     with pytest.raises(TypeError, match="two QSTELinear or two PackedLinear"):
         qste.nn.gated(torch.zeros(2, 64), layer, torch.nn.Linear(64, 8))
+    with pytest.raises(TypeError, match="two QSTELinear or two PackedLinear"):
+        qste.nn.gated(torch.zeros(2, 64), layer, qste.PackedEmbedding(packed, scale, 64))
+    with pytest.raises(TypeError, match="two QSTELinear or two PackedLinear"):
+        qste.nn.gated(torch.zeros(2, 64), layer, lambda x: x)
     with pytest.raises(ValueError, match="columns"):
         qste.nn.gated(torch.zeros(2, 64), layer, other)
 

@@ -1,8 +1,8 @@
 """The gated feed-forward block in one kernel.
 
 Values: against the definition in 64 bits, with the bound that the roundings
-give, and bit for bit against the layers called one by one where the sums run
-in the same order.  The backward: bit for bit against the layers' own
+give; gate's and up's bit for bit against the layers called one by one where
+the sums run in the same order.  The backward: bit for bit against the layers' own
 backward calls at the values that were kept, and against differences.
 """
 
@@ -40,7 +40,7 @@ def _operands(m, rows, cols, dtype, seed=0, bias=False):
         bits = torch.randint(0, 256, (rows, -(-cols // 8)), generator=g, device=DEV, dtype=torch.uint8)
         if cols % 8:
             bits[:, -1] &= (1 << (cols % 8)) - 1
-        scale = torch.rand(rows, generator=g, device=DEV) / math.sqrt(cols) + 0.2 / math.sqrt(cols)
+        scale = (torch.rand(rows, generator=g, device=DEV) + 0.2) / math.sqrt(max(cols, 1))
         layers += [bits, scale, torch.randn(rows, generator=g, device=DEV) * 0.1 if bias else None]
     return x, layers
 
@@ -77,6 +77,18 @@ def _within_roundings(h, x, layers, dtype):
     bound = error_a * (u.abs() + errors[1]) + a.abs() * errors[1]
     bound = bound + e * ((a * u).abs() + bound) + tiny
     return bool(((h.double() - a * u).abs() <= bound).all())
+
+
+def _gate_of(h, g, u):
+    """Whether h is silu(g) u at these g and u, rounded once.
+
+    In units of 2^-24, relative: |g| for the exponential's argument, two each for it and the reciprocal, one each for an
+    addition and three products, 10 in all; then half a step of the type, or of its least one."""
+
+    e, tiny = torch.finfo(h.dtype).eps / 2, (2.0 ** -25 if h.dtype == torch.float16 else 1e-37)
+    want = g.double() * torch.sigmoid(g.double()) * u.double()
+    off = 2.0 ** -24 * (g.double().abs() + 10) * want.abs()
+    return bool(((h.double() - want).abs() <= off + e * (want.abs() + off) + tiny).all())
 
 
 # sizes of each way, with ends inside every unit: 16-row blocks, 512-column chunks, 128- and 256-row and
@@ -139,7 +151,7 @@ def test_tiles(m, rows, cols, dtype):
     h1, g, u = kernels.gated_forward(x, *layers, cols, keep="values")
     h2, g8, u8 = kernels.gated_forward(x, *layers, cols, keep="blocks")
     assert torch.equal(_bits(h1), _bits(h)) and torch.equal(_bits(h2), _bits(h))
-    assert torch.equal(_bits(kernels.swiglu_forward(g, u)[0]), _bits(h))
+    assert _gate_of(h, g, u)
     for kept, t in ((g8, g), (u8, u)):
         want = kernels.quantize_blocks(t)
         assert torch.equal(kept.payload, want.payload) and torch.equal(kept.codes, want.codes)
@@ -156,12 +168,12 @@ def test_the_same_bits_as_the_layers_one_by_one(m, rows, cols, dtype):
     h, g, u = kernels.gated_forward(x, *layers, cols, keep="values")
     want = [kernels.packed_linear_affine(x, *layer, cols) for layer in (layers[:3], layers[3:])]
     assert torch.equal(_bits(g), _bits(want[0])) and torch.equal(_bits(u), _bits(want[1]))
-    assert torch.equal(_bits(h), _bits(kernels.swiglu_forward(*want)[0]))
+    assert _gate_of(h, g, u)
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("m,rows,cols", [(100, 63, 64), (70, 1000, 100), (3, 33, 65), (1, 1, 1), (80, 264, 7),
-                                         (30, 128, 256)])
+                                         (30, 128, 256), (5, 24, 0)])
 def test_sizes_that_go_layer_by_layer(m, rows, cols, dtype):
     from qste_amd import kernels
 
@@ -169,7 +181,7 @@ def test_sizes_that_go_layer_by_layer(m, rows, cols, dtype):
     for keep in ("", "values", "blocks"):
         h, g, u = kernels.gated_forward(x, *layers, cols, keep=keep)
         assert _within_roundings(h, x, layers, dtype)
-        if keep == "values":
+        if keep == "values" and _route(m, rows, cols, dtype, 1) == 0:
             assert torch.equal(_bits(kernels.swiglu_forward(g, u)[0]), _bits(h))
         if keep == "blocks":
             assert g.payload.shape == h.shape
@@ -319,9 +331,10 @@ def test_node_against_the_layers_one_by_one():
                         up.surface.log_scale.grad))
         gate.surface.log_scale.grad = up.surface.log_scale.grad = None
     one, other = results
-    assert torch.equal(_bits(one[0]), _bits(other[0]))
-    # the input gradient is rounded once rather than twice with a sum in between; the others may sum in another order
+    # the output is rounded once and not twice; the input gradient once rather than twice with a sum in between; the
+    # others may sum in another order
     e = 2.0 ** -8
+    assert float((one[0].double() - other[0].double()).norm() / other[0].double().norm()) <= 2 * e
     assert float((one[1].double() - other[1].double()).norm() / other[1].double().norm()) <= 2 * e
     for a, b in zip(one[2:], other[2:]):
         assert float((a - b).norm() / b.norm()) <= 1e-5
