@@ -220,6 +220,17 @@ int qste_linear_backward_offset_dot(const void* dy, int dtype, const uint8_t* pa
                                     int64_t samples, int64_t rows, int64_t cols, void* workspace,
                                     size_t workspace_bytes, void* stream);
 
+/* qste_linear_backward_offset_dot (without a bias gradient) whose evidence
+ * takes `dy_evidence` in place of `dy`: the caller has folded into it what is lost
+ * where x_scale is rounded to the operands' type, dy * (x_scale / rounded(x_scale))
+ * (qste_gated_backward writes it so), and one rounding an element is left of two.
+ * bf16 or fp16.  No counterpart in the reference. */
+size_t qste_linear_backward_operands_workspace_bytes(int64_t samples, int64_t rows, int64_t cols, int dtype);
+int qste_linear_backward_operands(const void* dy, const void* dy_evidence, int dtype, const uint8_t* packed_x,
+                                  const float* x_scale, const uint8_t* packed_w, const float* scale, void* dx,
+                                  float* evidence, float* grad_scale, const float* offset_dot, int64_t samples,
+                                  int64_t rows, int64_t cols, void* workspace, size_t workspace_bytes, void* stream);
+
 /* One fused QSTE coordinate step on one surface
  * (qste.kernels.coordinate_update, loader.py:329-368; spec
  * fallback.py:158-242): factored second moment, global RMS clip, block
@@ -496,6 +507,22 @@ int qste_gated(const void* x, int dtype, const uint8_t* gate, const float* gate_
                const uint8_t* up, const float* up_scale, const float* up_bias, void* out, void* gate_out, void* up_out,
                int8_t* gate_payload, uint8_t* gate_codes, int8_t* up_payload, uint8_t* up_codes, int64_t m,
                int64_t rows, int64_t cols, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The first half of a gated block's backward, from out's gradient [rows, cols]
+ * (rows: samples, cols: the block's features) and what qste_gated kept, gate and up
+ * or their blocks (the other NULL): dg and du, the gradients of g and u, side by side in
+ * grads [rows, 2 cols], the operands of the two layers' evidence in evidence_grads
+ * [rows, 2 cols] (qste_linear_backward_operands' dy and dy_evidence, with the layers'
+ * signs and scales concatenated), and sums fp32 [4][cols] over the rows: of dg *
+ * x_offset and du * x_offset (its offset_dot), of dg and of du (bias gradients).
+ * x_offset and x_scale fp32 [rows] are the saved encoding of the layers' input.
+ * bf16 or fp16, cols a multiple of 8, tensors at 16-byte steps.  No counterpart in
+ * the reference. */
+size_t qste_gated_backward_workspace_bytes(int64_t rows, int64_t cols);
+int qste_gated_backward(const void* grad, int dtype, const void* gate, const void* up, const int8_t* gate_payload,
+                        const uint8_t* gate_codes, const int8_t* up_payload, const uint8_t* up_codes, void* grads,
+                        void* evidence_grads, const float* x_offset, const float* x_scale, float* sums, int64_t rows,
+                        int64_t cols, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Which way qste_gated takes: 0 the products one after the other, 1 the kernel for
  * few rows, 2 the tiles (a query, for tests and tuning). */

@@ -1,6 +1,8 @@
 // extern "C" entry points declared in include/qste_hip.h: argument checks,
 // workspace carving and kernel dispatch.  Nothing here allocates or
 // synchronizes; every launch goes on the caller's stream.
+#include <initializer_list>
+
 #include "blocks.hpp"
 #include "common.hpp"
 #include "prep.hpp"
@@ -52,7 +54,7 @@ int mfma_evidence_t(const void*, int64_t, int, const uint8_t*, int64_t, const ui
 int64_t mfma_evidence_tiles(int64_t cols);
 bool mfma_backward_ok(const void*, int64_t, int, int64_t, int64_t, int64_t);
 EvidencePlan mfma_evidence_plan(int64_t, int64_t, int64_t, bool);
-int mfma_backward_pair(const void*, int64_t, int, const uint8_t*, int64_t, const uint16_t*, float*, const uint8_t*,
+int mfma_backward_pair(const void*, const void*, int64_t, int, const uint8_t*, int64_t, const uint16_t*, float*, const uint8_t*,
                        int64_t, const uint16_t*, const uint8_t*, int64_t, void*, int64_t, int64_t, int64_t,
                        const float*, const float*, float*, const EvidencePlan&, float*, hipStream_t);
 int launch_pad_rows(const void*, void*, int64_t, int64_t, int64_t, hipStream_t);
@@ -82,6 +84,9 @@ size_t swiglu_backward_blocks_sums_workspace(int64_t, int64_t);
 int launch_swiglu_backward_blocks_sums(const void*, int, const int8_t*, const uint8_t*, const int8_t*, const uint8_t*,
                                        void*, void*, const float*, const float*, int64_t, int64_t, float*, float*,
                                        hipStream_t, int64_t);
+size_t gated_backward_workspace(int64_t, int64_t);
+int launch_gated_backward(const void*, int, const void*, const void*, const blocks::Blocks&, const blocks::Blocks&,
+                          void*, void*, const float*, const float*, int64_t, int64_t, float*, float*, hipStream_t);
 double gemv_gated_us(int64_t, int64_t, int64_t, int);
 size_t gemv_gated_workspace(int64_t, int64_t, int64_t, int);
 int gemv_gated(const void*, int, const uint8_t*, const float*, const float*, const uint8_t*, const float*,
@@ -565,7 +570,9 @@ int linear_backward_impl(const void* dy, int dtype, const uint8_t* packed_x, con
                          const float* x_scale, const uint8_t* packed_w, const float* scale, void* dx,
                          float* evidence, float* grad_scale, float* grad_bias, const float* offset_dot,
                          int64_t samples, int64_t rows, int64_t cols, void* workspace, size_t workspace_bytes,
-                         void* stream) {
+                         void* stream, const void* dy_evidence = nullptr, void* pad_evidence = nullptr) {
+  // dy_evidence: what the evidence takes for dy, if not dy itself (then with
+  // offset_dot and no grad_bias); pad_evidence: room for its padded copy
   if (!dtype_ok(dtype)) return QSTE_E_DTYPE;
   if (samples < 0 || rows <= 0 || cols <= 0) return QSTE_E_SHAPE;
   if (!evidence || !grad_scale || !scale || !packed_w) return QSTE_E_NULL;
@@ -601,6 +608,9 @@ int linear_backward_impl(const void* dy, int dtype, const uint8_t* packed_x, con
                                    v_part, grad_bias ? db_part : nullptr, v, grad_bias, s)))
         return rc;
       if (offset_dot && !grad_bias) v = const_cast<float*>(offset_dot);  // only read from here on
+      if (dy_evidence) {
+        if ((rc = launch_pad_rows(dy_evidence, pad_evidence, samples, 2 * rows, 2 * ldy, s))) return rc;
+      }
     } else if (offset_dot && !grad_bias) {
       v = const_cast<float*>(offset_dot);
     } else if (matrix) {
@@ -616,6 +626,7 @@ int linear_backward_impl(const void* dy, int dtype, const uint8_t* packed_x, con
     bool dgrad_done = false;
     if (matrix) {
       const EvidencePlan plan = mfma_evidence_plan(samples, rows, cols, dx != nullptr);
+      const void* dy_e = !dy_evidence ? dy_m : pad_dy ? pad_evidence : dy_evidence;
       float* partial = reinterpret_cast<float*>(base + l.partial);
       uint8_t* w_t = reinterpret_cast<uint8_t*>(base + l.w_t);
       uint8_t* x_t = reinterpret_cast<uint8_t*>(base + l.x_t);
@@ -640,7 +651,7 @@ int linear_backward_impl(const void* dy, int dtype, const uint8_t* packed_x, con
                dx ? ScaleJob{scale, s16, rows, up64(rows)} : no_ws, s)))
         return rc;
       if (plan.pair) {
-        rc = mfma_backward_pair(dy_m, ldy, dtype, x_t, l.x_t_pitch, xs16, evidence, w_t, l.w_t_pitch, s16, w_epi,
+        rc = mfma_backward_pair(dy_m, dy_e, ldy, dtype, x_t, l.x_t_pitch, xs16, evidence, w_t, l.w_t_pitch, s16, w_epi,
                                 w_epi_pb, dx, samples, rows, cols, v, scale, gs_part, plan, partial, s);
         if (rc == 0) return launch_sum_partials(gs_part, mfma_evidence_tiles(cols), rows, grad_scale, s);
         if (rc != 1) return rc;
@@ -651,7 +662,7 @@ int linear_backward_impl(const void* dy, int dtype, const uint8_t* packed_x, con
           if (rc) return rc;
         }
         dgrad_done = true;
-        rc = mfma_evidence_t(dy_m, ldy, dtype, x_t, l.x_t_pitch, xs16, evidence, samples, rows, cols, v, scale, w_epi,
+        rc = mfma_evidence_t(dy_e, ldy, dtype, x_t, l.x_t_pitch, xs16, evidence, samples, rows, cols, v, scale, w_epi,
                              w_epi_pb, gs_part, &plan, partial, s);
         if (rc == 0) return launch_sum_partials(gs_part, mfma_evidence_tiles(cols), rows, grad_scale, s);
         if (rc != 1) return rc;
@@ -679,8 +690,8 @@ int linear_backward_impl(const void* dy, int dtype, const uint8_t* packed_x, con
     if (grad_bias && (rc = fill_zero(grad_bias, rows, s))) return rc;
   }
   int64_t tiles = 0;
-  if ((rc = evidence_dispatch(dy, dtype, packed_x, x_scale, evidence, samples, rows, cols, v, scale, packed_w,
-                              gs_part, nullptr, nullptr, &tiles, s)))
+  if ((rc = evidence_dispatch(dy_evidence ? dy_evidence : dy, dtype, packed_x, x_scale, evidence, samples, rows, cols, v,
+                              scale, packed_w, gs_part, nullptr, nullptr, &tiles, s)))
     return rc;
   return launch_sum_partials(gs_part, tiles, rows, grad_scale, s);
 }
@@ -694,6 +705,28 @@ int qste_linear_backward(const void* dy, int dtype, const uint8_t* packed_x, con
                          void* stream) {
   return linear_backward_impl(dy, dtype, packed_x, x_offset, x_scale, packed_w, scale, dx, evidence, grad_scale,
                               grad_bias, nullptr, samples, rows, cols, workspace, workspace_bytes, stream);
+}
+
+size_t qste_linear_backward_operands_workspace_bytes(int64_t samples, int64_t rows, int64_t cols, int dtype) {
+  if (dtype == QSTE_F32 || samples <= 0 || rows <= 0 || cols <= 0) return 0;
+  return align_up(qste_linear_backward_workspace_bytes_dtype(samples, rows, cols, dtype)) +
+         (rows % 64 ? align_up(static_cast<size_t>(samples * up64(rows)) * 2) : 0);
+}
+
+int qste_linear_backward_operands(const void* dy, const void* dy_evidence, int dtype, const uint8_t* packed_x,
+                                  const float* x_scale, const uint8_t* packed_w, const float* scale, void* dx,
+                                  float* evidence, float* grad_scale, const float* offset_dot, int64_t samples,
+                                  int64_t rows, int64_t cols, void* workspace, size_t workspace_bytes, void* stream) {
+  if (dtype != QSTE_BF16 && dtype != QSTE_F16) return QSTE_E_DTYPE;
+  if (samples <= 0 || rows <= 0 || cols <= 0) return QSTE_E_SHAPE;
+  if (!dy_evidence || !offset_dot || !x_scale) return QSTE_E_NULL;
+  if (!workspace || workspace_bytes < qste_linear_backward_operands_workspace_bytes(samples, rows, cols, dtype))
+    return QSTE_E_WORKSPACE;
+  const size_t own = align_up(qste_linear_backward_workspace_bytes_dtype(samples, rows, cols, dtype));
+  // (x's offsets are in offset_dot: any pointer stands for them)
+  return linear_backward_impl(dy, dtype, packed_x, x_scale, x_scale, packed_w, scale, dx, evidence, grad_scale, nullptr,
+                              offset_dot, samples, rows, cols, workspace, own, stream, dy_evidence,
+                              static_cast<char*>(workspace) + own);
 }
 
 int qste_linear_backward_offset_dot(const void* dy, int dtype, const uint8_t* packed_x, const float* x_offset,
@@ -806,6 +839,32 @@ int qste_swiglu_backward_blocks_sums(const void* grad, int dtype, const int8_t* 
   return launch_swiglu_backward_blocks_sums(grad, dtype, gate_payload, gate_codes, up_payload, up_codes, grad_gate,
                                             grad_up, offset_gate, offset_up, rows, cols, sums,
                                             static_cast<float*>(workspace), s, ld);
+}
+
+size_t qste_gated_backward_workspace_bytes(int64_t rows, int64_t cols) {
+  if (rows <= 0 || cols <= 0) return 0;
+  return gated_backward_workspace(rows, cols);
+}
+
+int qste_gated_backward(const void* grad, int dtype, const void* gate, const void* up, const int8_t* gate_payload,
+                        const uint8_t* gate_codes, const int8_t* up_payload, const uint8_t* up_codes, void* grads,
+                        void* evidence_grads, const float* x_offset, const float* x_scale, float* sums, int64_t rows,
+                        int64_t cols, void* workspace, size_t workspace_bytes, void* stream) {
+  if (dtype != QSTE_BF16 && dtype != QSTE_F16) return QSTE_E_DTYPE;
+  if (rows <= 0 || cols <= 0 || cols % 8) return QSTE_E_SHAPE;
+  const bool blocks8 = gate_payload && gate_codes && up_payload && up_codes;
+  if (!grad || !grads || !evidence_grads || !x_offset || !x_scale || !sums || !gate != !up || blocks8 == (gate != nullptr))
+    return QSTE_E_NULL;
+  for (const void* p : {grad, gate, up, static_cast<const void*>(grads), static_cast<const void*>(evidence_grads)})
+    if (reinterpret_cast<uintptr_t>(p) & 15) return QSTE_E_ALIGN;
+  for (const void* p : {gate_payload, up_payload})
+    if (reinterpret_cast<uintptr_t>(p) & 7) return QSTE_E_ALIGN;
+  if (!workspace || workspace_bytes < gated_backward_workspace(rows, cols)) return QSTE_E_WORKSPACE;
+  return launch_gated_backward(grad, dtype, gate, up,
+                               blocks::Blocks{const_cast<int8_t*>(gate_payload), const_cast<uint8_t*>(gate_codes)},
+                               blocks::Blocks{const_cast<int8_t*>(up_payload), const_cast<uint8_t*>(up_codes)}, grads,
+                               evidence_grads, x_offset, x_scale, rows, cols, sums, static_cast<float*>(workspace),
+                               as_stream(stream));
 }
 
 namespace {

@@ -1790,20 +1790,21 @@ EvidencePlan mfma_evidence_plan(int64_t samples, int64_t rows, int64_t cols, boo
 // from transposed sign copies: x_t [cols][x_t_pitch] (bit k of row c = sign
 // of x[k][c]) and w_t [cols][w_t_pitch] (bit r of row c = sign of W[r][c]),
 // both zero past their K, and bf16 copies of x_scale and scale, zero-padded
-// to a multiple of 64 entries.  `plan` is mfma_evidence_plan's for the
+// to a multiple of 64 entries.  The evidence reads dy_evidence (dy, unless the
+// caller has it in another rounding).  `plan` is mfma_evidence_plan's for the
 // shape (with pair set); its split tiles need plan.partial_bytes at
 // `partial`.  Returns 1 when either product is not for this path.
-int mfma_backward_pair(const void* dy, int64_t ldy, int dtype, const uint8_t* x_t, int64_t x_t_pitch,
+int mfma_backward_pair(const void* dy, const void* dy_evidence, int64_t ldy, int dtype, const uint8_t* x_t, int64_t x_t_pitch,
                        const uint16_t* x_scale16, float* ev, const uint8_t* w_t, int64_t w_t_pitch,
                        const uint16_t* scale16, const uint8_t* packed_w, int64_t w_pb, void* dx, int64_t samples,
                        int64_t rows, int64_t cols, const float* m_add, const float* scale, float* gs_partial,
                        const EvidencePlan& plan, float* partial, hipStream_t stream) {
-  if (!dx || !backward_operands_ok(dy, ldy, dtype, x_t, x_t_pitch, samples, rows, cols) ||
+  if (!dx || !backward_operands_ok(dy_evidence, ldy, dtype, x_t, x_t_pitch, samples, rows, cols) ||
       !backward_operands_ok(dy, ldy, dtype, w_t, w_t_pitch, samples, rows, cols))
     return 1;
   if (plan.splits > 1 && !partial) return QSTE_E_WORKSPACE;
   mfma::Params pe{};
-  pe.a = static_cast<const uint16_t*>(dy);
+  pe.a = static_cast<const uint16_t*>(dy_evidence);
   pe.bits = x_t;
   pe.kscale16 = x_scale16;
   pe.out = ev;

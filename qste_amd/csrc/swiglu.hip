@@ -28,6 +28,8 @@
 // the backward takes the g and u that they stand for.  HBM-bound like the
 // rest: 16384 x 14336 in bf16 read and write 1.89 GB forward (1.41 without) and
 // 1.89 GB backward (2.35 without).
+#include <type_traits>
+
 #include "blocks.hpp"
 #include "common.hpp"
 #include "encode.hpp"
@@ -318,69 +320,123 @@ __global__ __launch_bounds__(kThreads) void backward_blocks_kernel(const typenam
   }
 }
 
-// The same with the sums over the rows of dg off_g and of du off_u, for the two
-// binary layers that made g and u: a workgroup takes 512 columns, eight a lane,
-// of `chunk` rows, each wave every fourth of them; its waves' sums meet in LDS in
-// wave order, and the chunks' [chunk][2][cols] are added in their order by
-// sum_partials_kernel.
-template <int DT, bool ONCE>
-__global__ __launch_bounds__(kThreads) void backward_blocks_sums_kernel(
-    const uint16_t* __restrict__ dh, Pair kept, uint16_t* __restrict__ dg, uint16_t* __restrict__ du,
-    const float* __restrict__ off_g, const float* __restrict__ off_u, int64_t rows, int64_t cols, int64_t per_row,
-    int64_t ld, int chunk, float* __restrict__ part) {
-  constexpr int kWaves = kThreads / kWave;
-  __shared__ float red[kWaves][2][512];
+// Where a backward finds eight values of g or u: in a 16-bit tensor, or in blocks.
+template <int DT>
+struct Values {
+  const uint16_t* p;
+  using Held = blocks::Eight<DT>;
+  __device__ __forceinline__ Held load(int64_t at, int64_t) const { return Held::load(p + at); }
+  __device__ __forceinline__ static void values(const Held& h, float (&x)[8]) { h.values(x); }
+};
+template <int DT>
+struct Kept {
+  blocks::Blocks b;
+  struct Held {
+    uint2 q;
+    uint32_t code;
+  };
+  __device__ __forceinline__ Held load(int64_t at, int64_t block) const {
+    return Held{*reinterpret_cast<const uint2*>(b.q + at), b.codes[block]};
+  }
+  __device__ __forceinline__ static void values(const Held& h, float (&x)[8]) { blocks::dequantize8(h.q, h.code, x); }
+};
+
+// What the backward of a gated block writes besides dg and du (GATED below): the
+// operands of its layers' evidence.  That product takes dg times x's
+// scale, a scale for each row, and takes it as a 16-bit operand of its own: dg
+// and the scale rounded each.  Here dg c is rounded instead, c = scale / scale
+// rounded to the type, so that one rounding is left (error of the evidence
+// against 64 bits, in bf16, before it is rounded itself: 2.6e-3 -> 1.7e-3).
+struct EvidenceOperands {
+  uint16_t *gate, *up;
+  const float* x_scale;
+};
+
+template <int DT>
+__device__ __forceinline__ float scale_left(float scale) {
+  const float held = Elem<DT>::round(scale), c = scale / held;
+  return held != 0.0f && __builtin_isfinite(c) ? c : 1.0f;
+}
+
+// The backward with sums over the rows for the two binary layers that made g and u:
+// of dg off_g and du off_u, and with GATED also of dg and du, [2 or 4][cols].  A
+// workgroup takes 512 columns, eight a lane, of `chunk` rows, each wave every fourth
+// of them; its waves' sums meet in LDS in wave order, and the chunks' are added in
+// their order by sum_partials_kernel.
+template <int DT, class SRC, bool GATED, bool ONCE>
+__global__ __launch_bounds__(kThreads) void backward_columns_kernel(
+    const uint16_t* __restrict__ dh, SRC g, SRC u, uint16_t* __restrict__ dg, uint16_t* __restrict__ du,
+    EvidenceOperands ev, const float* __restrict__ off_g, const float* __restrict__ off_u, int64_t rows, int64_t cols,
+    int64_t per_row, int64_t ld, int chunk, float* __restrict__ part) {
+  constexpr int kWaves = kThreads / kWave, kSums = GATED ? 4 : 2, kDeep = GATED ? 2 : 4;
+  __shared__ float red[kWaves][kSums][512];
   const int lane = static_cast<int>(threadIdx.x) % kWave, wave = static_cast<int>(threadIdx.x) / kWave;
   const int64_t base = static_cast<int64_t>(blockIdx.x) * 512, c = base + 8 * lane, block = c / blocks::kBlock;
   const int64_t first = static_cast<int64_t>(blockIdx.y) * chunk;
   const int64_t last = first + chunk < rows ? first + chunk : rows;
   struct Held {
     blocks::Eight<DT> dh;
-    uint2 gq, uq;
-    uint32_t gcode, ucode;
-    float og, ou;
+    typename SRC::Held g, u;
+    float og, ou, xs;
   };
   auto load = [&](int64_t t) {
-    const int64_t at = t * cols + c;
-    return Held{blocks::Eight<DT>::load(dh + at), *reinterpret_cast<const uint2*>(kept.gate.q + at),
-                *reinterpret_cast<const uint2*>(kept.up.q + at), kept.gate.codes[t * per_row + block],
-                kept.up.codes[t * per_row + block], off_g[t], off_u[t]};
+    const int64_t at = t * cols + c, b = t * per_row + block;
+    return Held{blocks::Eight<DT>::load(dh + at), g.load(at, b), u.load(at, b), off_g[t], off_u[t],
+                GATED ? ev.x_scale[t] : 0.0f};
   };
-  float sg[8] = {}, su[8] = {};
+  float sums[kSums][8] = {};
   auto take = [&](int64_t t, const Held& r) {
-    float a[8], b[8];
-    backward_quarter<DT>(r.dh, r.gq, r.gcode, r.uq, r.ucode, a, b);
-    blocks::store8<DT, ONCE>(dg + t * ld + c, a);
-    blocks::store8<DT, ONCE>(du + t * ld + c, b);
+    float h[8], gv[8], uv[8], a[8], b[8];
+    r.dh.values(h);
+    SRC::values(r.g, gv);
+    SRC::values(r.u, uv);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      sg[i] = fmaf(a[i], r.og, sg[i]);
-      su[i] = fmaf(b[i], r.ou, su[i]);
+      backward_at<DT>(h[i], gv[i], uv[i], a[i], b[i]);
+      sums[0][i] = fmaf(a[i], r.og, sums[0][i]);
+      sums[1][i] = fmaf(b[i], r.ou, sums[1][i]);
+      if constexpr (GATED) {
+        sums[2][i] += a[i];
+        sums[3][i] += b[i];
+      }
+    }
+    blocks::store8<DT, ONCE>(dg + t * ld + c, a);
+    blocks::store8<DT, ONCE>(du + t * ld + c, b);
+    if constexpr (GATED) {
+      const float left = scale_left<DT>(r.xs);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        a[i] *= left;
+        b[i] *= left;
+      }
+      blocks::store8<DT, ONCE>(ev.gate + t * ld + c, a);
+      blocks::store8<DT, ONCE>(ev.up + t * ld + c, b);
     }
   };
   if (c < cols) {
     int64_t t = first + wave;
-    for (; t + 3 * kWaves < last; t += 4 * kWaves) {  // four rows' loads in flight
-      Held r[4];
+    for (; t + (kDeep - 1) * kWaves < last; t += kDeep * kWaves) {  // several rows' loads in flight
+      Held r[kDeep];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) r[k] = load(t + k * kWaves);
+      for (int k = 0; k < kDeep; ++k) r[k] = load(t + k * kWaves);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) take(t + k * kWaves, r[k]);
+      for (int k = 0; k < kDeep; ++k) take(t + k * kWaves, r[k]);
     }
     for (; t < last; t += kWaves) take(t, load(t));
   }
 #pragma unroll
-  for (int i = 0; i < 8; i += 4) {
-    *reinterpret_cast<float4*>(&red[wave][0][8 * lane + i]) = make_float4(sg[i], sg[i + 1], sg[i + 2], sg[i + 3]);
-    *reinterpret_cast<float4*>(&red[wave][1][8 * lane + i]) = make_float4(su[i], su[i + 1], su[i + 2], su[i + 3]);
-  }
+  for (int k = 0; k < kSums; ++k)
+#pragma unroll
+    for (int i = 0; i < 8; i += 4)
+      *reinterpret_cast<float4*>(&red[wave][k][8 * lane + i]) =
+          make_float4(sums[k][i], sums[k][i + 1], sums[k][i + 2], sums[k][i + 3]);
   __syncthreads();
-  for (int j = static_cast<int>(threadIdx.x); j < 2 * 512; j += kThreads) {
+  for (int j = static_cast<int>(threadIdx.x); j < kSums * 512; j += kThreads) {
     const int which = j / 512, cc = j % 512;
     float sum = red[0][which][cc];
 #pragma unroll
     for (int w = 1; w < kWaves; ++w) sum += red[w][which][cc];
-    if (base + cc < cols) part[(static_cast<int64_t>(blockIdx.y) * 2 + which) * cols + base + cc] = sum;
+    if (base + cc < cols) part[(static_cast<int64_t>(blockIdx.y) * kSums + which) * cols + base + cc] = sum;
   }
 }
 
@@ -794,20 +850,20 @@ inline int chunk_of(int64_t rows, int64_t cols) {
   return chunk;
 }
 
-template <int DT>
-int run_backward_blocks_sums(const void* dh, const Pair& kept, void* dg, void* du, const float* off_g,
-                             const float* off_u, int64_t rows, int64_t cols, float* sums, float* part, hipStream_t s,
-                             int64_t ld_out) {
+template <int DT, bool GATED, class SRC>
+int run_backward_columns(const void* dh, const SRC& g, const SRC& u, void* dg, void* du, const EvidenceOperands& ev,
+                         const float* off_g, const float* off_u, int64_t rows, int64_t cols, float* sums, float* part,
+                         hipStream_t s, int64_t ld_out) {
   const int chunk = chunk_of(rows, cols);
   const int64_t chunks = (rows + chunk - 1) / chunk;
   const dim3 grid(static_cast<unsigned>((cols + 511) / 512), static_cast<unsigned>(chunks));
-  auto* kernel =
-      backward_once(rows, cols, DT) ? backward_blocks_sums_kernel<DT, true> : backward_blocks_sums_kernel<DT, false>;
-  kernel<<<grid, kThreads, 0, s>>>(
-      static_cast<const uint16_t*>(dh), kept, static_cast<uint16_t*>(dg), static_cast<uint16_t*>(du), off_g, off_u, rows,
-      cols, blocks::blocks_of(cols), ld_out, chunk, part);
+  auto* kernel = backward_once(rows, cols, DT) ? backward_columns_kernel<DT, SRC, GATED, true>
+                                               : backward_columns_kernel<DT, SRC, GATED, false>;
+  kernel<<<grid, kThreads, 0, s>>>(static_cast<const uint16_t*>(dh), g, u, static_cast<uint16_t*>(dg),
+                                   static_cast<uint16_t*>(du), ev, off_g, off_u, rows, cols, blocks::blocks_of(cols),
+                                   ld_out, chunk, part);
   const int rc = static_cast<int>(hipGetLastError());
-  return rc ? rc : launch_sum_partials(part, chunks, 2 * cols, sums, s);
+  return rc ? rc : launch_sum_partials(part, chunks, (GATED ? 4 : 2) * cols, sums, s);
 }
 
 }  // namespace swiglu
@@ -868,16 +924,45 @@ int launch_swiglu_backward_blocks_sums(const void* dh, int dtype, const int8_t* 
                   {const_cast<int8_t*>(uq), const_cast<uint8_t*>(ucodes)}};
   if ((dtype == QSTE_BF16 || dtype == QSTE_F16) && kept_ok(kept, cols) && aligned(dh) && aligned(dg) && aligned(du) &&
       ld_out % 8 == 0)
-    return dtype == QSTE_BF16 ? run_backward_blocks_sums<QSTE_BF16>(dh, kept, dg, du, off_g, off_u, rows, cols, sums,
-                                                                   part, s, ld_out)
-                              : run_backward_blocks_sums<QSTE_F16>(dh, kept, dg, du, off_g, off_u, rows, cols, sums,
-                                                                  part, s, ld_out);
+    return dtype == QSTE_BF16
+               ? run_backward_columns<QSTE_BF16, false>(dh, Kept<QSTE_BF16>{kept.gate}, Kept<QSTE_BF16>{kept.up}, dg, du,
+                                                        {}, off_g, off_u, rows, cols, sums, part, s, ld_out)
+               : run_backward_columns<QSTE_F16, false>(dh, Kept<QSTE_F16>{kept.gate}, Kept<QSTE_F16>{kept.up}, dg, du,
+                                                       {}, off_g, off_u, rows, cols, sums, part, s, ld_out);
   // outputs with a row pitch of their own are written by the 8-wide pass only
   if (ld_out != cols) return QSTE_E_ALIGN;
   int rc = launch_swiglu_backward_blocks(dh, dtype, gq, gcodes, uq, ucodes, dg, du, rows, cols, s);
   if (rc) return rc;
   if ((rc = launch_colsums(dg, dtype, off_g, rows, cols, part, nullptr, sums, nullptr, s))) return rc;
   return launch_colsums(du, dtype, off_u, rows, cols, part, nullptr, sums + cols, nullptr, s);
+}
+
+// A gated block's backward from h's gradient to its layers' products: dg and du side
+// by side in `grads` [rows, 2 cols], the same as the evidence takes them in `evidence`,
+// and sums [4][cols] of dg off, du off, dg and du, off and x_scale being what the two
+// layers keep of their input.  16-bit types, cols a multiple of 8, operands at
+// 16-byte steps; g and u as they are (`gate`, `up`) or in blocks.
+size_t gated_backward_workspace(int64_t rows, int64_t cols) {
+  const int64_t chunk = swiglu::chunk_of(rows, cols), chunks = (rows + chunk - 1) / chunk;
+  return static_cast<size_t>(chunks * 4 * cols) * sizeof(float);
+}
+
+int launch_gated_backward(const void* dh, int dtype, const void* gate, const void* up, const blocks::Blocks& gate8,
+                          const blocks::Blocks& up8, void* grads, void* evidence, const float* off,
+                          const float* x_scale, int64_t rows, int64_t cols, float* sums, float* part, hipStream_t s) {
+  using namespace swiglu;
+  uint16_t *dg = static_cast<uint16_t*>(grads), *eg = static_cast<uint16_t*>(evidence);
+  const EvidenceOperands ev{eg, eg + cols, x_scale};
+  auto run = [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+    if (gate)
+      return run_backward_columns<DT, true>(dh, Values<DT>{static_cast<const uint16_t*>(gate)},
+                                            Values<DT>{static_cast<const uint16_t*>(up)}, dg, dg + cols, ev, off, off,
+                                            rows, cols, sums, part, s, 2 * cols);
+    return run_backward_columns<DT, true>(dh, Kept<DT>{gate8}, Kept<DT>{up8}, dg, dg + cols, ev, off, off, rows, cols,
+                                          sums, part, s, 2 * cols);
+  };
+  return dtype == QSTE_BF16 ? run(std::integral_constant<int, QSTE_BF16>{}) : run(std::integral_constant<int, QSTE_F16>{});
 }
 
 }  // namespace qste

@@ -270,23 +270,28 @@ def _through_scale(grad_scale: Tensor, e: Tensor, surface: Surface) -> Tensor:
 
 
 def _gate_up_backward(ctx, dh: list, kept: tuple, payload_x: Tensor, aux_x: Tensor, packed_g: Tensor, packed_u: Tensor,
-                      scale_gu: Tensor, sg: Surface, su: Surface):
+                      scale_gu: Tensor, sg: Surface, su: Surface, plain: bool = False):
     """The gate's backward and that of the two layers before it as one layer of 2
     ffn rows, their evidence delivered: ``(dx, scale gradients [2 ffn], bias
     gradients [2 ffn] or None)``.  ``dh``: the gradient of h in a list, taken out of it
     so that it is free during the product; ``kept``: g and u, as tensors or ``Blocks8``;
-    ``scale_gu``: both layers' scales, fp32."""
+    ``scale_gu``: both layers' scales, fp32; ``plain``: round as the gate and the
+    layers one by one do, g and u being tensors."""
 
     d, ffn = sg.columns, sg.rows
-    backward = kernels.swiglu_backward_blocks if isinstance(kept[0], kernels.Blocks8) else kernels.swiglu_backward_sums
-    both, sums = backward(dh.pop(), *kept, aux_x[0], aux_x[0], side_by_side=True)
     # (a copy of their signs: the deliveries below may rewrite them)
     packed_gu = torch.cat((packed_g, packed_u))
-    dx, ev_gu, gs_gu, gb_gu = kernels.linear_backward(
-        both, payload_x, aux_x[0], aux_x[1], packed_gu, scale_gu, d,
-        need_bias=any(b is not None for b in ctx.bias_dtypes[:2]), need_input=ctx.needs_input_grad[0],
-        offset_dot=sums.reshape(-1))
-    del both
+    need_bias = any(b is not None for b in ctx.bias_dtypes[:2])
+    if plain:
+        both, sums = kernels.swiglu_backward_sums(dh.pop(), *kept, aux_x[0], aux_x[0], side_by_side=True)
+        dx, ev_gu, gs_gu, gb_gu = kernels.linear_backward(
+            both, payload_x, aux_x[0], aux_x[1], packed_gu, scale_gu, d, need_bias=need_bias,
+            need_input=ctx.needs_input_grad[0], offset_dot=sums.reshape(-1))
+        del both
+    else:
+        dx, ev_gu, gs_gu, gb_gu = kernels.gated_backward(
+            dh.pop(), *kept, payload_x, aux_x[0], aux_x[1], packed_gu, scale_gu, d, need_bias=need_bias,
+            need_input=ctx.needs_input_grad[0])
     if dx is not None:
         dx = dx.reshape(ctx.input_shape)
     sg.consume_evidence(ev_gu[:ffn])
@@ -455,7 +460,8 @@ class SwiGLUMLPFn(Function):
         del ev_d
         dh = [dh]
         scale_gu = torch.cat((scale_g.detach().float(), scale_u.detach().float()))
-        dx, gs_gu, gb_gu = _gate_up_backward(ctx, dh, kept, payload_x, aux_x, packed_g, packed_u, scale_gu, sg, su)
+        dx, gs_gu, gb_gu = _gate_up_backward(ctx, dh, kept, payload_x, aux_x, packed_g, packed_u, scale_gu, sg, su,
+                                             plain=not ctx.checkpoint)
         (gs_g, gs_u), (gb_g, gb_u) = _halves(gs_gu, ffn), _halves(gb_gu, ffn)
 
         return (dx, None, _through_scale(gs_g, e_g, sg), _cast(gb_g, bg), None, _through_scale(gs_u, e_u, su),

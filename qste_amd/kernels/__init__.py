@@ -43,6 +43,7 @@ __all__ = [
     "embedding_backward",
     "packed_embedding",
     "evidence_from_packed",
+    "gated_backward",
     "gated_forward",
     "linear_backward",
     "native_available",
@@ -1003,6 +1004,65 @@ def gated_forward(inputs: Tensor, gate: Tensor, gate_scale: Tensor, gate_bias: T
                                   us.data_ptr(), _ptr(ub), out.data_ptr(), *values, *blocks, m, rows, columns,
                                   _ptr(work), nbytes, _stream(device)), "gated_forward")
     return out, g, u
+
+
+def gated_backward(grad: Tensor, gate, up, packed_x: Tensor, x_offset: Tensor, x_scale: Tensor, packed_w: Tensor,
+                   scale: Tensor, columns: int, *, need_input: bool = True, need_bias: bool = False):
+    """The backward of ``gated_forward`` from out's gradient [samples, rows] (bf16 or
+    fp16, rows a multiple of 8): ``(dx, evidence, grad_scale, grad_bias)`` of the two
+    layers as one of 2 rows, dx None without ``need_input`` and grad_bias without ``need_bias``.
+
+    ``gate`` and ``up`` are what the forward kept, tensors or ``Blocks8``; ``packed_x``,
+    ``x_offset`` and ``x_scale`` the encoding of its input (``pack_affine_rows``), ``packed_w``
+    [2 rows, ...] and ``scale`` [2 rows] both layers' signs and scales, gate's first.
+    """
+
+    kept = isinstance(gate, Blocks8)
+    if kept != isinstance(up, Blocks8):
+        raise TypeError("gate and up are both tensors or both Blocks8")
+    if kept:
+        gate, up = _check_blocks(gate, "gate blocks"), _check_blocks(up, "up blocks")
+        parts, shapes = (*gate[:2], *up[:2]), (gate.payload.shape, up.payload.shape)
+    else:
+        parts, shapes = (gate, up), (gate.shape, up.shape)
+    device = _require_gpu(grad, *parts, packed_x, x_offset, x_scale, packed_w, scale)
+    if grad.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"gated_backward takes bfloat16 or float16, got {grad.dtype}")
+    if grad.dim() != 2 or grad.shape[1] % 8 or not grad.numel():
+        raise ValueError("gated_backward expects a rank-2 gradient with rows and whole eights of columns")
+    if not (grad.shape == shapes[0] == shapes[1]) or not (grad.dtype == gate.dtype == up.dtype):
+        raise ValueError("grad, gate and up must have the same shape and dtype")
+    samples, rows = (int(s) for s in grad.shape)
+    columns, code = int(columns), _DTYPES[grad.dtype]
+    packed_x, packed_w = _check_packed(packed_x, columns, samples), _check_packed(packed_w, columns, 2 * rows)
+    offset, xs = _layer_vector(x_offset, samples, "x_offset"), _layer_vector(x_scale, samples, "x_scale")
+    scale = _layer_vector(scale, 2 * rows, "scale")
+    dh = _aligned(grad)
+    if kept:
+        sources = (None, None, *(_ptr(t) for t in parts))
+    else:
+        parts = (_aligned(gate), _aligned(up))  # held until the launch is queued
+        sources = (_ptr(parts[0]), _ptr(parts[1]), None, None, None, None)
+    lib = _lib.load()
+    # dy and what the evidence takes for it
+    both, ev = torch.empty(2, samples, 2 * rows, dtype=grad.dtype, device=device).unbind(0)
+    sums = torch.empty(4 * rows, dtype=torch.float32, device=device)
+    dx = torch.empty(samples, columns, dtype=grad.dtype, device=device) if need_input else None
+    evidence = torch.empty(2 * rows, columns, dtype=torch.float32, device=device)
+    grad_scale = torch.empty(2 * rows, dtype=torch.float32, device=device)
+    # one workspace for both calls, which follow each other on the stream
+    nbytes = lib.qste_linear_backward_operands_workspace_bytes(samples, 2 * rows, columns, code)
+    work = _workspace(max(nbytes, lib.qste_gated_backward_workspace_bytes(samples, rows)), device)
+    with _device_of(device):
+        stream = _stream(device)
+        _lib.check(lib.qste_gated_backward(_ptr(dh), code, *sources, _ptr(both), _ptr(ev), _ptr(offset), _ptr(xs),
+                                           _ptr(sums), samples, rows, _ptr(work), work.numel(), stream),
+                   "gated_backward")
+        _lib.check(lib.qste_linear_backward_operands(
+            _ptr(both), _ptr(ev), code, _ptr(packed_x), _ptr(xs), _ptr(packed_w), _ptr(scale), _ptr(dx), _ptr(evidence),
+            _ptr(grad_scale), _ptr(sums), samples, 2 * rows, columns, _ptr(work), work.numel(), stream),
+            "linear_backward_operands")
+    return dx, evidence, grad_scale, (sums[2 * rows:] if need_bias else None)
 
 
 def _leading(t: Tensor) -> int:

@@ -84,6 +84,12 @@ SIGNATURES = {
     "qste_swiglu_backward_blocks_sums": (_int, [_vp, _int, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _i64,
                                                 _i64, _vp, _sz, _vp]),
     "qste_gated_workspace_bytes": (_sz, [_i64, _i64, _i64, _int, _int]),
+    "qste_gated_backward_workspace_bytes": (_sz, [_i64, _i64]),
+    "qste_gated_backward": (_int, [_vp, _int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp,
+                                   _sz, _vp]),
+    "qste_linear_backward_operands_workspace_bytes": (_sz, [_i64, _i64, _i64, _int]),
+    "qste_linear_backward_operands": (_int, [_vp, _vp, _int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64,
+                                             _vp, _sz, _vp]),
     "qste_gated_route": (_int, [_i64, _i64, _i64, _int, _int]),
     "qste_gated": (_int, [_vp, _int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64,
                           _vp, _sz, _vp]),

@@ -293,11 +293,9 @@ def test_training_node(m, rows, cols, dtype, bias, checkpoint):
     payload, offset, xscale = kernels.pack_affine_rows(flat)
     if checkpoint:
         g, u = kernels.quantize_blocks(g), kernels.quantize_blocks(u)
-    backward = kernels.swiglu_backward_blocks if checkpoint else kernels.swiglu_backward_sums
-    both, sums = backward(grad, g, u, offset, offset, side_by_side=True)
-    dx, evidence, grad_scale, grad_bias = kernels.linear_backward(
-        both, payload, offset, xscale, torch.cat((sides[0][0], sides[1][0])),
-        torch.cat((sides[0][1].float(), sides[1][1].float())), cols, need_bias=bias, offset_dot=sums.reshape(-1))
+    dx, evidence, grad_scale, grad_bias = kernels.gated_backward(
+        grad, g, u, payload, offset, xscale, torch.cat((sides[0][0], sides[1][0])),
+        torch.cat((sides[0][1].float(), sides[1][1].float())), cols, need_bias=bias)
     assert torch.equal(_bits(x.grad), _bits(dx))
     for i, layer in enumerate((gate, up)):
         part = slice(i * rows, (i + 1) * rows)
@@ -314,8 +312,86 @@ def test_training_node(m, rows, cols, dtype, bias, checkpoint):
             assert torch.equal(layer.bias.grad, grad_bias[i * rows:(i + 1) * rows])
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,rows,cols", [(1, 8, 64), (70, 40, 64), (250, 2048, 768), (513, 264, 128), (33, 1000, 192),
+                                         (2000, 512, 320)])
+@pytest.mark.parametrize("kept", ["values", "blocks"])
+def test_backward_kernels(m, rows, cols, dtype, kept):
+    """dx, evidence, scale and bias gradients against the formulas in 64 bits at the kept g and u.
+
+    e: half a step of the type, relative.  dg and du are within e of theirs (fp32 before that: 2^-24 times a few tens,
+    within another e / 16), the row scales are exact in the type here.  A sum in fp32 adds 2^-24 of its terms' magnitudes
+    for each of its terms, and dx is rounded again.  So every element is within e (1 + 1/16) of the sum of its terms'
+    magnitudes and that.  Over a tensor the errors are of random sign: a rounding is off by 0.42 e in the root mean
+    square for values spread evenly over a binade's logarithm, so evidence with one rounding in its terms is off by
+    0.42 e of itself, with two by 0.59 e: half of e is between them."""
+
+    from qste_amd import kernels
+
+    print(f"gated backward {m} x {rows} x {cols} {dtype} {kept}", flush=True)
+    e = torch.finfo(dtype).eps / 2
+    gen = torch.Generator(device=DEV).manual_seed(m + rows)
+    x = (torch.randn(m, cols, generator=gen, device=DEV) + 0.1).to(dtype)
+    x *= torch.rand(m, 1, generator=gen, device=DEV).add(0.5).to(dtype)
+    g, u, dh = (torch.randn(m, rows, generator=gen, device=DEV).to(dtype) for _ in range(3))
+    packed = torch.randint(0, 256, (2 * rows, cols // 8), generator=gen, device=DEV, dtype=torch.uint8)
+    scale = (torch.rand(2 * rows, generator=gen, device=DEV) + 0.2).to(dtype).float()
+    payload, offset, xs = kernels.pack_affine_rows(x)
+    operands = [kernels.quantize_blocks(t) if kept == "blocks" else t for t in (g, u)]
+    dx, evidence, grad_scale, grad_bias = kernels.gated_backward(dh, *operands, payload, offset, xs, packed, scale, cols,
+                                                                 need_bias=True)
+    if kept == "blocks":
+        g, u = (kernels.dequantize_blocks(t) for t in operands)
+    a, b, d = g.double(), u.double(), dh.double()
+    s = torch.sigmoid(a)
+    dy = torch.cat((d * b * s * (1 + a * (1 - s)), d * a * s), 1)
+    place = torch.arange(cols, device=DEV)
+    sign = ((packed[:, place // 8].int() >> (place % 8)) & 1).double() * 2 - 1
+    x_sign = ((payload[:, place // 8].int() >> (place % 8)) & 1).double() * 2 - 1
+    seen, wide = offset.double()[:, None] + xs.double()[:, None] * x_sign, scale.double()[:, None]
+    term = e * (1 + 1 / 16)
+    tiny = 2.0 ** -24 if dtype == torch.float16 else 1e-30
+
+    def close(got, want, sizes, terms, rounded=0.0):
+        bound = (term + terms * 2.0 ** -24) * sizes + rounded * (want.abs() + term * sizes) + tiny * (1 + terms)
+        assert bool(((got.double() - want).abs() <= bound).all())
+
+    close(dx, dy @ (sign * wide), dy.abs() @ wide.expand(-1, cols), 2 * rows, e)
+    whole = dy.t() @ seen
+    sizes = dy.abs().t() @ (offset.double().abs() + xs.double())[:, None].expand(-1, cols)
+    close(evidence, whole * wide, sizes * wide, m)
+    close(grad_scale, (whole * sign).sum(1), sizes.sum(1), m + cols)
+    close(grad_bias, dy.sum(0), dy.abs().sum(0), m)
+    if m * rows > 100000:
+        assert float((evidence.double() - whole * wide).norm() / (whole * wide).norm()) <= 0.5 * e
+    no_input = kernels.gated_backward(dh, *operands, payload, offset, xs, packed, scale, cols, need_input=False)
+    assert no_input[0] is None and no_input[3] is None
+    again = kernels.gated_backward(dh, *operands, payload, offset, xs, packed, scale, cols)
+    assert torch.equal(again[1], evidence) and torch.equal(_bits(again[0]), _bits(dx))
+
+
+def test_backward_refusals():
+    from qste_amd import kernels
+
+    x, layers = _operands(6, 32, 64, torch.bfloat16)
+    g = torch.zeros(6, 32, dtype=torch.bfloat16, device=DEV)
+    payload, offset, xs = kernels.pack_affine_rows(x)
+    packed, scale = torch.cat((layers[0], layers[3])), torch.cat((layers[1], layers[4]))
+    good = [g, g, g, payload, offset, xs, packed, scale, 64]
+    kernels.gated_backward(*good)
+    for at, bad, error in ((0, g.float(), TypeError), (0, g[:, :31].contiguous(), ValueError), (0, g[:0], ValueError),
+                           (1, g[:5], ValueError), (2, g.half(), ValueError), (3, payload[:5], ValueError),
+                           (4, offset[:5], ValueError), (5, xs[:5], ValueError), (6, layers[0], ValueError),
+                           (7, layers[1], ValueError), (1, kernels.quantize_blocks(g), TypeError)):
+        with pytest.raises(error):
+            kernels.gated_backward(*good[:at], bad, *good[at + 1:])
+
+
 def test_node_against_the_layers_one_by_one():
-    """Output, input gradient, evidence and scale gradients of the composition with the plain gate."""
+    """Output, input gradient, evidence and scale gradients of the composition with the plain gate.
+
+    The composition rounds dg (or du), twice on its way, and x's scale in the evidence's operand, the node dg and its
+    scale together: four roundings' root of squares, 0.42 e each (see above), bounds the evidence's difference by e."""
 
     import qste_amd as qste
 
@@ -337,7 +413,7 @@ def test_node_against_the_layers_one_by_one():
     assert float((one[0].double() - other[0].double()).norm() / other[0].double().norm()) <= 2 * e
     assert float((one[1].double() - other[1].double()).norm() / other[1].double().norm()) <= 2 * e
     for a, b in zip(one[2:], other[2:]):
-        assert float((a - b).norm() / b.norm()) <= 1e-5
+        assert float((a - b).norm() / b.norm()) <= e
 
 
 def test_node_against_differences():
