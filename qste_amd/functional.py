@@ -215,7 +215,12 @@ class SwiGLUFn(Function):
     def forward(ctx, gate, up, encode: bool, checkpoint: bool):
         forget_offers()
         ctx.checkpoint = checkpoint
+        # the encodings of the inputs of the binary layers that produced gate
+        # and up (one [2, tokens] aux each), when both did
+        aux_g, aux_u = getattr(gate, _AUX_ATTR, None), getattr(up, _AUX_ATTR, None)
         if checkpoint:
+            # (over other layers than binary ones the next is taken to be no binary one either)
+            encode = encode and aux_g is not None and aux_u is not None
             out, encoding, *kept = kernels.swiglu_forward_blocks(gate, up, encode=encode)
             _save_kept(ctx, *kept)
         else:
@@ -224,10 +229,7 @@ class SwiGLUFn(Function):
         if encoding is not None:
             packed, offset, scale = encoding
             remember_encoding(out, packed, kernels.stacked_pair(offset, scale))
-        # the encodings of the inputs of the binary layers that produced gate
-        # and up (one [2, tokens] aux each), when both did
         ctx.auxes = None
-        aux_g, aux_u = getattr(gate, _AUX_ATTR, None), getattr(up, _AUX_ATTR, None)
         tokens = gate.numel() // gate.shape[-1] if gate.dim() and gate.shape[-1] else 0
         if (aux_g is not None and aux_u is not None and tokens and aux_g.shape == (2, tokens)
                 and aux_u.shape == (2, tokens)):
@@ -305,29 +307,38 @@ def _halves(t: Tensor | None, rows: int) -> tuple:
     return (None, None) if t is None else (t[:rows], t[rows:])
 
 
-def _two_scales(log_g: Tensor, log_u: Tensor, sg: Surface, su: Surface) -> tuple[Tensor, Tensor, Tensor | None]:
-    """Both layers' scales (fp32 [2 ffn]) and their exponentials: one tensor and
-    None, or, where the log-scales' dtypes differ, one each."""
-
-    ffn, (g, u) = sg.rows, (sg.cfg, su.cfg)
-    if log_g.dtype != log_u.dtype:
-        scale_g, e_g = kernels.row_scale(log_g, g.scale_min, g.scale_max)
-        scale_u, e_u = kernels.row_scale(log_u, u.scale_min, u.scale_max)
-        return torch.cat((scale_g.float(), scale_u.float())), e_g, e_u
-    scale, e = (torch.empty(2 * ffn, dtype=log_g.dtype, device=log_g.device) for _ in range(2))
-    kernels.row_scale(log_g, g.scale_min, g.scale_max, (scale[:ffn], e[:ffn]))
-    kernels.row_scale(log_u, u.scale_min, u.scale_max, (scale[ffn:], e[ffn:]))
-    return scale.float(), e, None
-
-
-def _through_two_scales(grad: Tensor, e: Tensor, e_u: Tensor | None, sg: Surface, su: Surface) -> tuple[Tensor, Tensor]:
-    """``_through_scale`` of both layers, of what ``_two_scales`` returned; one launch where their bounds agree."""
+def _two_scales(log_g: Tensor, log_u: Tensor, sg: Surface, su: Surface) -> tuple[Tensor, Tensor]:
+    """Both layers' scales and their exponentials before the clamp, fp32 [2 ffn]
+    each, of values in the log-scales' dtypes."""
 
     ffn = sg.rows
-    if e_u is None and (sg.cfg.scale_min, sg.cfg.scale_max) == (su.cfg.scale_min, su.cfg.scale_max):
-        return _halves(_through_scale(grad, e, sg), ffn)
-    e_g, e_u = (e[:ffn], e[ffn:]) if e_u is None else (e, e_u)
-    return _through_scale(grad[:ffn], e_g, sg), _through_scale(grad[ffn:], e_u, su)
+    same = log_g.dtype == log_u.dtype
+    both = torch.empty(2, 2 * ffn, dtype=log_g.dtype if same else torch.float32, device=log_g.device)
+    for log, surface, at in ((log_g, sg, slice(0, ffn)), (log_u, su, slice(ffn, 2 * ffn))):
+        out = (both[0, at], both[1, at])
+        lo, hi = surface.cfg.scale_min, surface.cfg.scale_max
+        if same:
+            kernels.row_scale(log, lo, hi, out)
+        else:
+            for to, t in zip(out, kernels.row_scale(log, lo, hi)):
+                to.copy_(t)
+    scale, e = both.float().unbind(0)
+    return scale, e
+
+
+def _through_two_scales(grad: Tensor, e: Tensor, sg: Surface, su: Surface, dtypes: tuple) -> tuple[Tensor, Tensor]:
+    """The scales' gradients carried to the log-scales in fp32, rounded once to their dtypes."""
+
+    ffn, (g, u) = sg.rows, (sg.cfg, su.cfg)
+    if (g.scale_min, g.scale_max) == (u.scale_min, u.scale_max):
+        log = kernels.row_scale_backward(e, grad, g.scale_min, g.scale_max)
+        if dtypes[0] == dtypes[1]:
+            return _halves(log.to(dtypes[0]), ffn)
+        log_g, log_u = _halves(log, ffn)
+    else:
+        log_g = kernels.row_scale_backward(e[:ffn], grad[:ffn], g.scale_min, g.scale_max)
+        log_u = kernels.row_scale_backward(e[ffn:], grad[ffn:], u.scale_min, u.scale_max)
+    return log_g.to(dtypes[0]), log_u.to(dtypes[1])
 
 
 class GatedFn(Function):
@@ -344,13 +355,13 @@ class GatedFn(Function):
         sg, su = surfaces
         d, ffn = sg.columns, sg.rows
         flat = inputs.reshape(-1, d)
-        scale_gu, e, e_u = _two_scales(log_g, log_u, sg, su)
+        scale_gu, e = _two_scales(log_g, log_u, sg, su)
         keep = "" if not grad_on else "blocks" if checkpoint else "values"
         h, g, u = kernels.gated_forward(flat, packed_g, scale_gu[:ffn], bias_g, packed_u, scale_gu[ffn:], bias_u, d,
                                         keep=keep)
         if grad_on:
             payload_x, aux_x = _encoding_of(inputs, flat, d)
-            more = (payload_x, aux_x, packed_g, packed_u, scale_gu, e, e_u)
+            more = (payload_x, aux_x, packed_g, packed_u, scale_gu, e)
             if checkpoint:
                 _save_kept(ctx, g, u, *more)
             else:
@@ -358,6 +369,7 @@ class GatedFn(Function):
         ctx.checkpoint = checkpoint
         ctx.surfaces = surfaces
         ctx.input_shape = inputs.shape
+        ctx.log_dtypes = (log_g.dtype, log_u.dtype)
         ctx.bias_dtypes = tuple(None if b is None else b.dtype for b in (bias_g, bias_u))
         return h.reshape(*inputs.shape[:-1], ffn)
 
@@ -366,11 +378,11 @@ class GatedFn(Function):
     def backward(ctx, grad_output):
         forget_encodings()
         saved = ctx.saved_tensors
-        payload_x, aux_x, packed_g, packed_u, scale_gu, e, e_u = saved[-7:]
+        payload_x, aux_x, packed_g, packed_u, scale_gu, e = saved[-6:]
         sg, su = ctx.surfaces
         dx, gs_gu, gb_gu = _gate_up_backward(ctx, [grad_output.reshape(-1, sg.rows)], _kept(ctx, saved), payload_x,
                                              aux_x, packed_g, packed_u, scale_gu, sg, su)
-        log_g, log_u = _through_two_scales(gs_gu, e, e_u, sg, su)
+        log_g, log_u = _through_two_scales(gs_gu, e, sg, su, ctx.log_dtypes)
         gb_g, gb_u = _halves(gb_gu, sg.rows)
         bg, bu = ctx.bias_dtypes
         return dx, None, log_g, _cast(gb_g, bg), None, log_u, _cast(gb_u, bu), None, None, None

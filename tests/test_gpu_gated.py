@@ -300,16 +300,12 @@ def test_training_node(m, rows, cols, dtype, bias, checkpoint):
     for i, layer in enumerate((gate, up)):
         part = slice(i * rows, (i + 1) * rows)
         assert len(layer.evidence) == 1 and torch.equal(layer.evidence[0], evidence[part])
-        scale = layer.scale
-        scale.backward(grad_scale[part].to(scale.dtype))
-    once = [layer.surface.log_scale.grad for layer in (gate, up)]
-    # both the node's gradient and scale's own have been added: twice one of them
-    gate.surface.log_scale.grad = up.surface.log_scale.grad = None
-    for i, layer in enumerate((gate, up)):
-        layer.scale.backward(grad_scale[i * rows:(i + 1) * rows].to(layer.scale.dtype))
-        assert torch.equal(once[i], 2 * layer.surface.log_scale.grad)
+        # exp's value in the log-scale's type times the scale's gradient, rounded once
+        log_scale = layer.surface.log_scale
+        want = (log_scale.detach().exp().float() * grad_scale[part]).to(log_scale.dtype)
+        assert torch.equal(log_scale.grad, want)
         if bias:
-            assert torch.equal(layer.bias.grad, grad_bias[i * rows:(i + 1) * rows])
+            assert torch.equal(layer.bias.grad, grad_bias[part])
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
@@ -442,6 +438,38 @@ def test_node_against_differences():
     slope = float((value(x.detach().double() + step * v) - value(x.detach().double() - step * v)) / (2 * step))
     terms = x.grad.double() * v
     assert abs(float(terms.sum()) - slope) <= 4 * 2.0 ** -9 * float(terms.norm()) * math.sqrt(8)
+
+
+def test_log_scales_of_two_types_and_bounds():
+    """Log-scales in different types, at and past the clamp, and surfaces with bounds of their own."""
+
+    import qste_amd as qste
+    from qste_amd import kernels
+
+    x = torch.randn(40, 64, device=DEV, generator=torch.Generator(device=DEV).manual_seed(1)).bfloat16()
+    w = torch.randn(40, 96, device=DEV, generator=torch.Generator(device=DEV).manual_seed(2)).bfloat16()
+    for types, bounds in (((torch.float32, torch.bfloat16), (4.0, 4.0)), ((torch.bfloat16, torch.bfloat16), (4.0, 0.125)),
+                          ((torch.float32, torch.float32), (0.125, 4.0))):
+        gate, up = _pair(96, 64, 8)
+        for layer, dtype, hi in zip((gate, up), types, bounds):
+            layer.surface.cfg = qste.QSTEConfig(scale_max=hi)
+            layer.surface.log_scale.data = layer.surface.log_scale.data.to(dtype)
+        h = qste.nn.gated(x, gate, up)
+        h.backward(w)
+        scales = [layer.scale.detach().float() for layer in (gate, up)]
+        assert all(float(s.max()) <= hi for s, hi in zip(scales, bounds))
+        want, g, u = kernels.gated_forward(x, gate.packed_sign, scales[0], None, up.packed_sign, scales[1], None, 64,
+                                           keep="values")
+        assert torch.equal(h.detach(), want)
+        grad_scale = kernels.gated_backward(w, g, u, *kernels.pack_affine_rows(x),
+                                            torch.cat((gate.packed_sign.data, up.packed_sign.data)), torch.cat(scales),
+                                            64)[2]
+        for layer, part, hi in ((gate, grad_scale[:96], bounds[0]), (up, grad_scale[96:], bounds[1])):
+            log_scale = layer.surface.log_scale
+            e = log_scale.detach().exp()
+            inside = (e.float() >= 1e-6) & (e.float() <= hi)
+            assert log_scale.grad.dtype == log_scale.dtype
+            assert torch.equal(log_scale.grad, torch.where(inside, e.float() * part, 0.0).to(log_scale.dtype))
 
 
 def test_node_in_use():
