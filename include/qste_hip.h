@@ -492,9 +492,11 @@ int qste_swiglu_backward_blocks_sums(const void* grad, int dtype, const int8_t* 
  * What a backward needs is written where asked for: g and u as they are
  * (gate_out and up_out, both or neither) and as 8-bit blocks (the four blocks'
  * pointers, all or none).
- * One launch (two where K is cut into ranges) up to 64 rows of bf16 / fp16 and 21
- * of fp32 with nothing kept, and on the 16-bit tiles where cols is a multiple
- * of 64 and rows of 8; elsewhere the two products (qste_packed_linear_affine_ws)
+ * Both layers are one product, on the kernel for few rows (up to 64 of bf16 / fp16
+ * and 21 of fp32, nothing kept) or on the tiles (fp32 with nothing kept; 16-bit
+ * types, rows a multiple of 8 where something is), columns that are no multiple of
+ * 64 on padded copies.  Elsewhere (a few columns, too small an fp32 product) the two
+ * products (qste_packed_linear_affine_ws)
  * and qste_swiglu_forward (which rounds silu(g) too) one after the other, with g and
  * u in the workspace.  Sums are
  * fp32, in an order that may differ from the two products' called alone: g and u

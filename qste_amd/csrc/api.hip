@@ -91,7 +91,10 @@ double gemv_gated_us(int64_t, int64_t, int64_t, int);
 size_t gemv_gated_workspace(int64_t, int64_t, int64_t, int);
 int gemv_gated(const void*, int, const uint8_t*, const float*, const float*, const uint8_t*, const float*,
                const float*, void*, int64_t, int64_t, int64_t, void*, hipStream_t);
-bool mfma_gated_ok(int64_t, int64_t, int64_t, int);
+bool mfma_gated_ok(int64_t, int64_t, int64_t, int, bool);
+size_t f32_gated_workspace(int64_t, int64_t, int64_t);
+int mfma_f32_gated(const float*, const uint8_t*, const float*, const float*, const uint8_t*, const float*, const float*,
+                   float*, int64_t, int64_t, int64_t, void*, hipStream_t);
 double mfma_gated_us(int64_t, int64_t, int64_t);
 size_t mfma_gated_workspace(int64_t, int64_t, int64_t);
 int mfma_gated(const void*, int, const uint8_t*, const float*, const float*, const uint8_t*, const float*,
@@ -869,19 +872,44 @@ int qste_gated_backward(const void* grad, int dtype, const void* gate, const voi
 
 namespace {
 
-enum GatedRoute { kOneByOne = 0, kSkinny = 1, kTiles = 2 };
+// How a gated block runs: layer by layer, on the kernel for few rows or on the
+// tiles, the latter two on copies of x and the signs of `padded` columns if that is
+// not 0.
+enum GatedKind { kOneByOne = 0, kSkinny = 1, kTiles = 2 };
+struct GatedRoute {
+  GatedKind kind;
+  int64_t padded;
+};
 
-// How a gated block runs.  Few rows with nothing kept take the kernel for them
-// where its estimate is the lower one; what neither that nor the tiles take runs
-// layer by layer.
+// Few rows with nothing kept take the kernel for them where its estimate is the
+// lower one.  Ragged columns are copied from the width on from which a layer's
+// forward copies them (below it the scalar kernels are as fast).
 GatedRoute gated_route(int64_t m, int64_t rows, int64_t cols, int dtype, int keep) {
-  if (m <= 0 || rows <= 0 || cols <= 0) return kOneByOne;
-  const double skinny = keep ? -1.0 : gemv_gated_us(m, rows, cols, dtype);
-  if (mfma_gated_ok(m, rows, cols, dtype)) {
-    const double tiles = mfma_gated_us(m <= 16 ? m : (m + 15) / 16 * 16, rows, cols);
-    return skinny >= 0.0 && skinny < tiles ? kSkinny : kTiles;
+  if (m <= 0 || rows <= 0 || cols <= 0) return {kOneByOne, 0};
+  const int64_t wide = padded_cols(cols), copies = cols % 128 != 0 ? wide : 0;
+  const bool reach = static_cast<double>(m) * wide * elem_bytes(dtype) < 4294967296.0;
+  const double copying = copies ? padding_us(2 * rows, cols) : 0.0;
+  const double skinny = keep || cols <= 64 || (copies && !reach) ? -1.0 : gemv_gated_us(m, rows, wide, dtype);
+  if (dtype == QSTE_F32) {
+    if (keep) return {kOneByOne, 0};
+    // (past 21 rows; the limbs are padded copies of their own)
+    if (skinny >= 0.0) return {kSkinny, copies};
+    return {f32_gated_workspace(m, rows, cols) ? kTiles : kOneByOne, 0};
   }
-  return skinny >= 0.0 ? kSkinny : kOneByOne;
+  const bool whole = cols % 64 == 0;  // the tiles take it as it is
+  const int64_t tiled = whole ? cols : wide;
+  double tiles = -1.0;
+  if ((whole || (cols > 160 && reach)) && mfma_gated_ok(m, rows, tiled, dtype, keep != 0))
+    tiles = mfma_gated_us(m <= 16 ? m : (m + 15) / 16 * 16, rows, tiled) + (whole ? 0.0 : copying);
+  if (skinny >= 0.0 && (tiles < 0.0 || skinny + copying < tiles)) return {kSkinny, copies};
+  return tiles >= 0.0 ? GatedRoute{kTiles, whole ? 0 : wide} : GatedRoute{kOneByOne, 0};
+}
+
+// room for a route's padded copies
+size_t gated_copies(int64_t m, int64_t rows, int64_t padded, int dtype) {
+  return padded ? align_up(static_cast<size_t>(m * padded) * elem_bytes(dtype)) +
+                      2 * align_up(static_cast<size_t>(rows * padded / 8))
+                : 0;
 }
 
 bool aligned_to(const void* p, uintptr_t step) { return (reinterpret_cast<uintptr_t>(p) & (step - 1)) == 0; }
@@ -889,14 +917,18 @@ bool aligned_to(const void* p, uintptr_t step) { return (reinterpret_cast<uintpt
 }  // namespace
 
 int qste_gated_route(int64_t m, int64_t rows, int64_t cols, int dtype, int keep) {
-  return dtype_ok(dtype) ? gated_route(m, rows, cols, dtype, keep) : QSTE_E_DTYPE;
+  return dtype_ok(dtype) ? gated_route(m, rows, cols, dtype, keep).kind : QSTE_E_DTYPE;
 }
 
 size_t qste_gated_workspace_bytes(int64_t m, int64_t rows, int64_t cols, int dtype, int keep) {
   if (!dtype_ok(dtype) || m <= 0 || rows <= 0 || cols < 0) return 0;
-  switch (gated_route(m, rows, cols, dtype, keep)) {
-    case kSkinny: return gemv_gated_workspace(m, rows, cols, dtype);
-    case kTiles: return mfma_gated_workspace(m, rows, cols);
+  const GatedRoute route = gated_route(m, rows, cols, dtype, keep);
+  const size_t copies = gated_copies(m, rows, route.padded, dtype);
+  const int64_t taken = route.padded ? route.padded : cols;
+  switch (route.kind) {
+    case kSkinny: return copies + gemv_gated_workspace(m, rows, taken, dtype);
+    case kTiles:
+      return dtype == QSTE_F32 ? f32_gated_workspace(m, rows, cols) : copies + mfma_gated_workspace(m, rows, taken);
     default:
       return (keep & 1 ? 0 : 2 * align_up(static_cast<size_t>(m * rows) * elem_bytes(dtype))) +
              qste_packed_linear_affine_workspace_bytes(m, rows, cols, dtype);
@@ -921,16 +953,35 @@ int qste_gated(const void* x, int dtype, const uint8_t* gate, const float* gate_
   if (need && (!workspace || workspace_bytes < need)) return QSTE_E_WORKSPACE;
   if (need && !aligned_to(workspace, 16)) return QSTE_E_ALIGN;
   hipStream_t s = as_stream(stream);
-  switch (gated_route(m, rows, cols, dtype, keep)) {
+  const GatedRoute route = gated_route(m, rows, cols, dtype, keep);
+  char* ws = static_cast<char*>(workspace);
+  int rc;
+  if (const int64_t pc = route.padded) {
+    const int64_t eb = static_cast<int64_t>(elem_bytes(dtype)), pb = (cols + 7) / 8;
+    char* xp = ws;
+    char* gp = xp + align_up(static_cast<size_t>(m * pc * eb));
+    char* up_p = gp + align_up(static_cast<size_t>(rows * pc / 8));
+    if ((rc = launch_pad_rows(x, xp, m, eb * cols, eb * pc, s))) return rc;
+    if ((rc = launch_pad_rows(gate, gp, rows, pb, pc / 8, s))) return rc;
+    if ((rc = launch_pad_rows(up, up_p, rows, pb, pc / 8, s))) return rc;
+    x = xp;
+    gate = reinterpret_cast<const uint8_t*>(gp);
+    up = reinterpret_cast<const uint8_t*>(up_p);
+    cols = pc;
+    ws += gated_copies(m, rows, pc, dtype);
+  }
+  switch (route.kind) {
     case kSkinny:
-      return gemv_gated(x, dtype, gate, gate_scale, gate_bias, up, up_scale, up_bias, out, m, rows, cols, workspace, s);
+      return gemv_gated(x, dtype, gate, gate_scale, gate_bias, up, up_scale, up_bias, out, m, rows, cols, ws, s);
     case kTiles:
+      if (dtype == QSTE_F32)
+        return mfma_f32_gated(static_cast<const float*>(x), gate, gate_scale, gate_bias, up, up_scale, up_bias,
+                              static_cast<float*>(out), m, rows, cols, ws, s);
       return mfma_gated(x, dtype, gate, gate_scale, gate_bias, up, up_scale, up_bias, out, gate_out, up_out,
                         blocks::Blocks{gate_payload, gate_codes}, blocks::Blocks{up_payload, up_codes}, m, rows, cols,
-                        workspace, s);
+                        ws, s);
     default: break;
   }
-  char* ws = static_cast<char*>(workspace);
   const size_t hidden = align_up(static_cast<size_t>(m * rows) * elem_bytes(dtype));
   size_t left = workspace_bytes;
   if (!gate_out) {
@@ -939,7 +990,7 @@ int qste_gated(const void* x, int dtype, const uint8_t* gate, const float* gate_
     ws += 2 * hidden;
     left -= 2 * hidden;
   }
-  int rc = qste_packed_linear_affine_ws(x, dtype, gate, gate_scale, gate_bias, gate_out, m, rows, cols, ws, left, stream);
+  rc = qste_packed_linear_affine_ws(x, dtype, gate, gate_scale, gate_bias, gate_out, m, rows, cols, ws, left, stream);
   if (rc) return rc;
   rc = qste_packed_linear_affine_ws(x, dtype, up, up_scale, up_bias, up_out, m, rows, cols, ws, left, stream);
   if (rc) return rc;

@@ -48,8 +48,9 @@ enum { B_BITS_ALONG_K = 0, B_BITS_ALONG_N = 1, B_BITS_ALONG_K_SCALED = 2 };
 // forward's scale and bias, stored as fp32 (the fp32 products, whose dense
 // operand arrives as three bf16 limbs along K).  EPI_EVIDENCE_F32: the
 // evidence of such an operand.  Both undo the limbs' power of two per row.
-// EPI_GATED: two forwards of one input, g and u, that end in silu(g) * u (PairParams).
-enum { EPI_FORWARD = 0, EPI_PLAIN = 1, EPI_EVIDENCE = 2, EPI_PARTIAL = 3, EPI_FORWARD_F32 = 4, EPI_EVIDENCE_F32 = 5, EPI_GATED = 6 };
+// EPI_GATED: two forwards of one input, g and u, that end in silu(g) * u (PairParams);
+// EPI_GATED_F32: the same of an operand in limbs.
+enum { EPI_FORWARD = 0, EPI_PLAIN = 1, EPI_EVIDENCE = 2, EPI_PARTIAL = 3, EPI_FORWARD_F32 = 4, EPI_EVIDENCE_F32 = 5, EPI_GATED = 6, EPI_GATED_F32 = 7 };
 
 struct Params {
   const uint16_t* a;     // bf16 dense operand (x or dy)
@@ -275,12 +276,33 @@ constexpr int A_STAGE_K = (BK / 2) * APK;    // bytes
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
 
+// Eight outputs, of which `left` (or more) lie in the row, at `at`, which is at a
+// 16-byte step if `vec`.  Streaming stores, as the forward's: 500 x 8192 over 2048
+// 29.6 -> 28.6 us, large sizes within noise.
+template <int DT>
+__device__ __forceinline__ void store_gated(uint16_t* at, const float (&v)[8], int64_t left, bool vec) {
+  if (vec) {
+    blocks::store8<DT, true>(at, v);
+  } else if (left >= 8) {
+    struct __attribute__((packed)) Unaligned16 {
+      uint32_t w[4];
+    };
+    const blocks::Eight<DT> e = blocks::rounded<DT>(v);
+    *reinterpret_cast<Unaligned16*>(at) = Unaligned16{{e.w[0], e.w[1], e.w[2], e.w[3]}};
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < left) Elem<DT>::store(at, i, v[i]);
+  }
+}
+
 // The end of a gated block's tile: g and u from the accumulators (scale, bias,
 // rounded to the type, as the two layers alone give them), through LDS EPR rows
 // at a time, so that a lane holds eight features of g and of u of one row;
 // h = silu(g) u and what the backward keeps leave from there in 16-byte (8-bit:
 // 8-byte) pieces, 64 (32) bytes of a row by four lanes, which are a block of 32.
-// N is a multiple of 8: a piece lies inside the row or outside.
+// Where something is kept N is a multiple of 8: a piece lies inside the row or
+// outside.
 template <int DT, int MBN>
 __device__ __forceinline__ void gated_epilogue(const PairParams& p, f32x16 (&acc)[MBN][NBN], int64_t m0, int64_t n0,
                                                int wave, int lane, uint8_t* stg) {
@@ -345,8 +367,7 @@ __device__ __forceinline__ void gated_epilogue(const PairParams& p, f32x16 (&acc
       u8.values(u);
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = swiglu::gated_one<DT>(g[i], u[i]);
-      // streaming, as the forward's: 500 x 8192 over 2048 29.6 -> 28.6 us, large sizes within noise
-      blocks::store8<DT, true>(h + grow * p.N + gcol, v);
+      store_gated<DT>(h + grow * p.N + gcol, v, p.N - gcol, (p.N & 7) == 0);
     }
   }
 }
@@ -725,6 +746,33 @@ __device__ __forceinline__ void wide_tile(const P& p, int pid, uint8_t* A0, uint
     return;
   }
 
+  if constexpr (EPI == EPI_GATED_F32) {
+    // EPI_FORWARD_F32's two columns of a lane are g and u of one element
+    float* h = static_cast<float*>(p.out);
+    int* xst = reinterpret_cast<int*>(A0);  // [TM]
+    if (tid < TM) xst[tid] = m0 + tid < p.M ? -limb_shift(p.m_top[m0 + tid]) : 0;
+    stage_barrier<0>();
+    const int64_t col = n0 + 32 * wn + l32;
+    const bool in = col < p.N;
+    float gs = in ? p.n_scale[col] : 0.0f, us = in ? p.up_scale[col] : 0.0f;
+    float gb = in && p.n_bias ? p.n_bias[col] : 0.0f, ub = in && p.up_bias ? p.up_bias[col] : 0.0f;
+    asm volatile("" : "+v"(gs), "+v"(us), "+v"(gb), "+v"(ub));  // waited for here, as in EPI_FORWARD_F32
+#pragma unroll
+    for (int mb = 0; mb < MBN; ++mb) {
+      int back[16];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<int4*>(back + 4 * i) = *reinterpret_cast<const int4*>(xst + 32 * mb + 8 * i + 4 * kg);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int64_t row = m0 + 32 * mb + 8 * (r >> 2) + 4 * kg + (r & 3);
+        const float g = ldexpf(acc[mb][0][r], back[r]) * gs + gb, u = ldexpf(acc[mb][1][r], back[r]) * us + ub;
+        if (row < p.M && in) h[row * p.N + col] = swiglu::gated_one<QSTE_F32>(g, u);
+      }
+    }
+    return;
+  }
+
   if (EPI == EPI_EVIDENCE || EPI == EPI_EVIDENCE_F32) {
     // E0 = acc + v[m]; E = E0 * s[m] (fp32, 32 lanes x 4 bytes per row per
     // store); row partials of E0 * sign_w over this wave's columns.
@@ -914,18 +962,18 @@ __global__ __launch_bounds__(THREADS, 2) void half_kernel(Params p) {
 
 // The gated block on whole and on half tiles: two layers' products of 128
 // features from one reading of x.
-template <int DT>
+template <int DT, int EPI = EPI_GATED>
 __global__ __launch_bounds__(THREADS, 2) void gated_half_kernel(PairParams p) {
   using SZ = StageSizes<A_ROWS_M, B_BITS_ALONG_K>;
   QSTE_WIDE_STAGES(A_STAGE / 2, SZ::b, SZ::s)
-  wide_tile<A_ROWS_M, B_BITS_ALONG_K, EPI_GATED, DT, BM / 2>(p, blockIdx.x, A0, A1, A2, A3, B0, B1, B2, B3, Sc);
+  wide_tile<A_ROWS_M, B_BITS_ALONG_K, EPI, DT, BM / 2>(p, blockIdx.x, A0, A1, A2, A3, B0, B1, B2, B3, Sc);
 }
 
-template <int DT>
+template <int DT, int EPI = EPI_GATED>
 __global__ __launch_bounds__(THREADS, 1) void gated_wide_kernel(PairParams p) {
   using SZ = StageSizes<A_ROWS_M, B_BITS_ALONG_K>;
   QSTE_WIDE_STAGES(SZ::a, SZ::b, SZ::s)
-  wide_tile<A_ROWS_M, B_BITS_ALONG_K, EPI_GATED, DT>(p, blockIdx.x, A0, A1, A2, A3, B0, B1, B2, B3, Sc);
+  wide_tile<A_ROWS_M, B_BITS_ALONG_K, EPI, DT>(p, blockIdx.x, A0, A1, A2, A3, B0, B1, B2, B3, Sc);
 }
 
 template <int AKIND, int BKIND, int EPI, int DT>
@@ -1176,7 +1224,8 @@ __global__ __launch_bounds__(THREADS, 1) void gated_split_kernel(PairParams p, i
 
 // The ranges' sums in range order, then as gated_epilogue.  Workgroup (x, i):
 // rows 16x .. 16x + 15 of tile i, eight features a thread.
-template <int DT>
+// OUT: the outputs' type (fp32: the tiles summed bf16 limbs, whose power of two is undone).
+template <int OUT>
 __global__ __launch_bounds__(THREADS) void gated_combine_kernel(PairParams p, const float* __restrict__ partial,
                                                                 int tiles, int splits) {
   const int tiles_m = static_cast<int>((p.M + BM - 1) / BM), tiles_n = static_cast<int>((p.N + BN / 2 - 1) / (BN / 2));
@@ -1185,8 +1234,9 @@ __global__ __launch_bounds__(THREADS) void gated_combine_kernel(PairParams p, co
   tile_of<2>(i, tiles_m, tiles_n, tm, tn);  // the tiles' mapping
   const int lrow = static_cast<int>(blockIdx.x) * 16 + tid / 16, eight = tid % 16;
   const int64_t row = static_cast<int64_t>(tm) * BM + lrow, col = static_cast<int64_t>(tn) * (BN / 2) + 8 * eight;
-  const bool there = row < p.M && col < p.N;  // N is a multiple of 8
+  const bool there = row < p.M && col < p.N;
   float g[8] = {}, u[8] = {}, v[8];
+  const int back = OUT == QSTE_F32 && there ? -limb_shift(p.m_top[row]) : 0;
   if (there) {
     const float* src = partial + static_cast<int64_t>(i) * (BM * BN) + lrow * BN + 64 * (eight / 4) + 8 * (eight % 4);
     for (int j = 0; j < splits; ++j) {
@@ -1200,31 +1250,47 @@ __global__ __launch_bounds__(THREADS) void gated_combine_kernel(PairParams p, co
     }
 #pragma unroll
     for (int q = 0; q < 8; ++q) {
-      g[q] = Elem<DT>::round(g[q] * p.n_scale[col + q] + (p.n_bias ? p.n_bias[col + q] : 0.0f));
-      u[q] = Elem<DT>::round(u[q] * p.up_scale[col + q] + (p.up_bias ? p.up_bias[col + q] : 0.0f));
-    }
-  }
-  if (p.gate8.q) {
-    uint32_t gc, uc;
-    const uint2 gq = blocks::quantize8(blocks::rounded<DT>(g), gc), uq = blocks::quantize8(blocks::rounded<DT>(u), uc);
-    if (there) {
-      *reinterpret_cast<uint2*>(p.gate8.q + row * p.N + col) = gq;
-      *reinterpret_cast<uint2*>(p.up8.q + row * p.N + col) = uq;
-      if (eight % 4 == 0) {
-        const int64_t block = row * ((p.N + blocks::kBlock - 1) / blocks::kBlock) + col / blocks::kBlock;
-        p.gate8.codes[block] = static_cast<uint8_t>(gc);
-        p.up8.codes[block] = static_cast<uint8_t>(uc);
+      const bool in = col + q < p.N;
+      const float gs = in ? p.n_scale[col + q] : 0.0f, us = in ? p.up_scale[col + q] : 0.0f;
+      const float gb = in && p.n_bias ? p.n_bias[col + q] : 0.0f, ub = in && p.up_bias ? p.up_bias[col + q] : 0.0f;
+      if constexpr (OUT == QSTE_F32) {
+        g[q] = ldexpf(g[q], back) * gs + gb;
+        u[q] = ldexpf(u[q], back) * us + ub;
+      } else {
+        g[q] = Elem<OUT>::round(g[q] * gs + gb);
+        u[q] = Elem<OUT>::round(u[q] * us + ub);
       }
     }
   }
-  if (!there) return;
-  if (p.gate) {
-    blocks::store8<DT>(p.gate + row * p.N + col, g);
-    blocks::store8<DT>(p.up + row * p.N + col, u);
-  }
+  if constexpr (OUT == QSTE_F32) {
+    if (!there) return;
+    float* h = static_cast<float*>(p.out) + row * p.N + col;
 #pragma unroll
-  for (int q = 0; q < 8; ++q) v[q] = swiglu::gated_one<DT>(g[q], u[q]);
-  blocks::store8<DT>(static_cast<uint16_t*>(p.out) + row * p.N + col, v);
+    for (int q = 0; q < 8; ++q)
+      if (col + q < p.N) h[q] = swiglu::gated_one<QSTE_F32>(g[q], u[q]);
+  } else {
+    if (p.gate8.q) {
+      uint32_t gc, uc;
+      const uint2 gq = blocks::quantize8(blocks::rounded<OUT>(g), gc), uq = blocks::quantize8(blocks::rounded<OUT>(u), uc);
+      if (there) {
+        *reinterpret_cast<uint2*>(p.gate8.q + row * p.N + col) = gq;
+        *reinterpret_cast<uint2*>(p.up8.q + row * p.N + col) = uq;
+        if (eight % 4 == 0) {
+          const int64_t block = row * ((p.N + blocks::kBlock - 1) / blocks::kBlock) + col / blocks::kBlock;
+          p.gate8.codes[block] = static_cast<uint8_t>(gc);
+          p.up8.codes[block] = static_cast<uint8_t>(uc);
+        }
+      }
+    }
+    if (!there) return;
+    if (p.gate) {
+      blocks::store8<OUT>(p.gate + row * p.N + col, g);
+      blocks::store8<OUT>(p.up + row * p.N + col, u);
+    }
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[q] = swiglu::gated_one<OUT>(g[q], u[q]);
+    store_gated<OUT>(static_cast<uint16_t*>(p.out) + row * p.N + col, v, p.N - col, (p.N & 7) == 0);
+  }
 }
 #undef QSTE_WIDE_STAGES
 }  // namespace wide
@@ -1449,10 +1515,11 @@ int mfma_linear_forward_split(const void* x, int dtype, const uint8_t* packed, c
 // of 2 * rows columns, in tiles of 128 features of both.
 static int64_t gated_columns(int64_t rows) { return (rows + 127) / 128 * 256; }
 
-// Whether it is for this path: what the tiles need, and features in whole eights.
-bool mfma_gated_ok(int64_t m, int64_t rows, int64_t cols, int dtype) {
-  return mfma_dtype(dtype) && m > 0 && rows > 0 && rows % 8 == 0 && cols > 0 && cols % 64 == 0 && fits32(m * cols * 2) &&
-         fits32((rows + 128) * (cols / 8));
+// Whether it is for this path: what the tiles need, and with something kept
+// features in whole eights.
+bool mfma_gated_ok(int64_t m, int64_t rows, int64_t cols, int dtype, bool kept) {
+  return mfma_dtype(dtype) && m > 0 && rows > 0 && (!kept || rows % 8 == 0) && cols > 0 && cols % 64 == 0 &&
+         fits32(m * cols * 2) && fits32((rows + 128) * (cols / 8));
 }
 
 static ProductPlan gated_plan(int64_t m, int64_t rows, int64_t cols) {
@@ -1463,8 +1530,10 @@ size_t mfma_gated_workspace(int64_t m, int64_t rows, int64_t cols) {
   return split_bytes(gated_plan(m, rows, cols).split, wide_grid(m, gated_columns(rows)));
 }
 
-template <int DT>
+// DT: the operands' type, OUT: the outputs' (fp32: bf16 limbs)
+template <int DT, int OUT = DT>
 static int launch_gated(const mfma::PairParams& p, const ProductPlan& plan, float* partial, hipStream_t stream) {
+  constexpr int EPI = OUT == QSTE_F32 ? mfma::EPI_GATED_F32 : mfma::EPI_GATED;
   const int tiles = wide_grid(p.M, gated_columns(p.N));
   if (plan.split.splits > 1) {
     mfma::wide::gated_split_kernel<DT>
@@ -1472,13 +1541,13 @@ static int launch_gated(const mfma::PairParams& p, const ProductPlan& plan, floa
     const int rc = static_cast<int>(hipGetLastError());
     if (rc) return rc;
     const dim3 grid(mfma::wide::BM / 16, static_cast<unsigned>(tiles));
-    mfma::wide::gated_combine_kernel<DT>
+    mfma::wide::gated_combine_kernel<OUT>
         <<<grid, mfma::wide::THREADS, 0, stream>>>(p, partial, tiles, plan.split.splits);
   } else if (plan.half) {
     const int64_t grid = (p.M + 127) / 128 * ((p.N + 127) / 128);
-    mfma::wide::gated_half_kernel<DT><<<static_cast<unsigned>(grid), mfma::wide::THREADS, 0, stream>>>(p);
+    mfma::wide::gated_half_kernel<DT, EPI><<<static_cast<unsigned>(grid), mfma::wide::THREADS, 0, stream>>>(p);
   } else {
-    mfma::wide::gated_wide_kernel<DT><<<tiles, mfma::wide::THREADS, 0, stream>>>(p);
+    mfma::wide::gated_wide_kernel<DT, EPI><<<tiles, mfma::wide::THREADS, 0, stream>>>(p);
   }
   return static_cast<int>(hipGetLastError());
 }
@@ -2210,6 +2279,54 @@ int mfma_f32_forward(const float* x, const uint8_t* packed, const float* scale, 
   float* partial = reinterpret_cast<float*>(b + limbs::up256(static_cast<size_t>(rows) * 3 * kb));
   limbs::repeat_kernel<<<limbs::grid_for(rows * kb / 8), 256, 0, stream>>>(packed, rows, pb, pb, b, 3 * kb, kb, kb);
   return f32_product(x, nullptr, b, scale, bias, y, m, rows, cols, a, top, partial, true, stream);
+}
+
+// The gated block in fp32 through the limbs: both layers' signs three times, the
+// rest as a product of gated_columns(rows) columns.  0 where it is not for this path.
+size_t f32_gated_workspace(int64_t m, int64_t rows, int64_t cols) {
+  if (m <= 0 || rows <= 0 || cols <= 0) return 0;
+  const int64_t n = gated_columns(rows), kp = up64(cols);
+  const size_t product = f32_product_workspace(m, n, cols, true);
+  if (product == 0 || !fits32(f32_chunk_rows(m, cols) * 3 * kp * 2) || !fits32((rows + 128) * 3 * kp / 8)) return 0;
+  return product + 2 * limbs::up256(static_cast<size_t>(rows) * 3 * kp / 8);
+}
+
+int mfma_f32_gated(const float* x, const uint8_t* gate_bits, const float* gate_scale, const float* gate_bias,
+                   const uint8_t* up_bits, const float* up_scale, const float* up_bias, float* h, int64_t m,
+                   int64_t rows, int64_t cols, void* workspace, hipStream_t stream) {
+  const int64_t n = gated_columns(rows), kp = up64(cols), kb = kp / 8, mc = f32_chunk_rows(m, cols), pb = (cols + 7) / 8;
+  const size_t signs = limbs::up256(static_cast<size_t>(rows) * 3 * kb);
+  uint8_t* at = static_cast<uint8_t*>(workspace);
+  auto take = [&](size_t bytes) {
+    uint8_t* p = at;
+    at += limbs::up256(bytes);
+    return p;
+  };
+  uint16_t* a = reinterpret_cast<uint16_t*>(take(static_cast<size_t>(mc) * 3 * kp * 2));
+  int* top = reinterpret_cast<int*>(take(static_cast<size_t>(mc) * sizeof(int)));
+  uint8_t *gate = take(signs), *up = take(signs);
+  float* partial = reinterpret_cast<float*>(at);
+  limbs::repeat_kernel<<<limbs::grid_for(rows * kb / 8), 256, 0, stream>>>(gate_bits, rows, pb, pb, gate, 3 * kb, kb, kb);
+  limbs::repeat_kernel<<<limbs::grid_for(rows * kb / 8), 256, 0, stream>>>(up_bits, rows, pb, pb, up, 3 * kb, kb, kb);
+  for (int64_t i0 = 0; i0 < m; i0 += mc) {
+    const int64_t mi = m - i0 < mc ? m - i0 : mc;
+    int rc = launch_split_rows(x + i0 * cols, mi, cols, nullptr, a, 3 * kp, kp, kp, top, stream);
+    if (rc) return rc;
+    mfma::PairParams p{};
+    p.a = a;
+    p.bits = gate;
+    p.bits_up = up;
+    p.out = h + i0 * rows;
+    p.M = mi; p.N = rows; p.K = 3 * kp;
+    p.lda = 3 * kp; p.pb = 3 * kb;
+    p.a_rows = mi; p.bit_rows = rows;
+    p.n_scale = gate_scale; p.n_bias = gate_bias;
+    p.up_scale = up_scale; p.up_bias = up_bias;
+    p.m_top = top;
+    rc = launch_gated<QSTE_BF16, QSTE_F32>(p, f32_plan(mi, n, cols, true), partial, stream);
+    if (rc) return rc;
+  }
+  return 0;
 }
 
 size_t f32_dgrad_workspace(int64_t m, int64_t rows, int64_t cols) { return f32_product_workspace(m, cols, rows, false); }

@@ -499,12 +499,11 @@ def swiglu_mlp_fusable(inputs: Tensor, gate, up, down) -> bool:
 
 def gated_fusable(inputs: Tensor, gate, up) -> bool:
     """Whether ``GatedFn`` takes this block: a bf16 or fp16 input on the GPU,
-    its columns a multiple of 64 and the layers' rows of 8."""
+    the layers' rows a multiple of 8."""
 
     sg, su = gate.surface, up.surface
     return (inputs.is_cuda and inputs.dtype in (torch.bfloat16, torch.float16) and inputs.dim() >= 1
-            and inputs.shape[-1] == sg.columns == su.columns and sg.rows == su.rows and sg.columns % 64 == 0
-            and sg.rows % 8 == 0 and inputs.numel() > 0
+            and inputs.shape[-1] == sg.columns == su.columns and sg.rows == su.rows and sg.rows % 8 == 0 and inputs.numel() > 0
             and all(s.log_scale.is_cuda and s.log_scale.dtype in _SCALE_DTYPES for s in (sg, su)))
 
 

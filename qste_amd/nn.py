@@ -83,9 +83,8 @@ def gated(inputs: Tensor, gate, up, *, checkpoint: bool = False) -> Tensor:
     once, where the operators one by one round silu's value too.  With gradients it is one
     autograd node, whose backward runs the two layers as one; evidence and
     scale gradients go where the layers' own would.  ``checkpoint`` keeps gate and up
-    for the backward in 8-bit blocks (``quantize_blocks``) in place of 16 bits.  Sizes
-    that the one kernel does not take (columns that are no multiple of 64, rows that
-    are none of 8, fp32 past 21 rows) run layer by layer."""
+    for the backward in 8-bit blocks (``quantize_blocks``) in place of 16 bits.  With
+    gradients, fp32 and rows that are no multiple of 8 run layer by layer."""
 
     # a module's buffers and parts by their dicts: attributes of modules are looked up in Python, half a microsecond each
     try:

@@ -75,12 +75,27 @@ def test_c_entries_refuse_before_any_launch():
     assert _gated(lib, x=4098) == E_ALIGN
     assert _gated(lib, out=4104) == E_ALIGN
     assert _gated(lib, blocks=(4100, 4096, 4096, 4096)) == E_ALIGN
-    # rows that the one kernel does not take need room for g and u
-    assert lib.qste_gated_route(100, 63, 64, BF16, 0) == 0
-    assert _gated(lib, m=100, rows=63) == E_WORKSPACE
-    need = lib.qste_gated_workspace_bytes(100, 63, 64, BF16, 0)
+    # columns that the one kernel does not take need room for g and u
+    assert lib.qste_gated_route(100, 63, 60, BF16, 0) == 0
+    assert _gated(lib, m=100, rows=63, cols=60) == E_WORKSPACE
+    need = lib.qste_gated_workspace_bytes(100, 63, 60, BF16, 0)
     assert need >= 2 * 100 * 63 * 2
-    assert _gated(lib, m=100, rows=63, ws=4096, ws_bytes=need - 1) == E_WORKSPACE
+    assert _gated(lib, m=100, rows=63, cols=60, ws=4096, ws_bytes=need - 1) == E_WORKSPACE
+    assert _gated(lib, m=100, rows=63, cols=60, ws=4100, ws_bytes=need) == E_ALIGN
+    p = ctypes.c_void_p
+    ones = [p(4096)] * 9
+    back = lambda dtype=BF16, kept=(None,) * 6, rows=4, cols=64, grads=4096, ws=None, n=0: lib.qste_gated_backward(  # noqa: E731
+        p(4096), dtype, *kept, p(grads), *ones[:4], rows, cols, ws, n, None)
+    values = (p(4096), p(4096), None, None, None, None)
+    assert back(F32, values) == E_DTYPE and back(kept=values, cols=60) == E_SHAPE and back(kept=values, rows=0) == E_SHAPE
+    assert back() == E_NULL and back(kept=(p(4096), None, None, None, None, None)) == E_NULL
+    assert back(kept=tuple(ones[:6])) == E_NULL  # both
+    assert back(kept=values, grads=4104) == E_ALIGN
+    assert back(kept=values) == E_WORKSPACE
+    assert lib.qste_linear_backward_operands(*ones[:2], F32, *ones[:8], 4, 8, 8, None, 0, None) == E_DTYPE
+    assert lib.qste_linear_backward_operands(*ones[:2], F16, *ones[:8], 0, 8, 8, None, 0, None) == E_SHAPE
+    assert lib.qste_linear_backward_operands(p(4096), None, F16, *ones[:8], 4, 8, 8, None, 0, None) == E_NULL
+    assert lib.qste_linear_backward_operands(*ones[:2], F16, *ones[:8], 4, 8, 8, None, 0, None) == E_WORKSPACE
     assert lib.qste_quantize_blocks(None, 9, None, None, 1, 1, None) == E_DTYPE
     assert lib.qste_quantize_blocks(None, F32, None, None, -1, 1, None) == E_SHAPE
     assert lib.qste_quantize_blocks(None, F32, None, None, 1, 1, None) == E_NULL
@@ -99,9 +114,11 @@ def test_routes():
     assert route(1, 999, 4096, BF16, 0) == 1  # rows of any number
     assert route(500, 8192, 2048, BF16, 0) == 2 and route(8190, 14336, 4096, F16, 2) == 2
     assert route(1, 14336, 4096, BF16, 2) == 2  # with something kept
-    assert route(500, 8191, 2048, BF16, 0) == 0 and route(500, 8192, 2040, BF16, 0) == 0
-    assert route(500, 8192, 2048, F32, 0) == 0 and route(22, 8192, 2048, F32, 0) == 0
-    assert route(4, 64, 0, BF16, 0) == 0
+    assert route(500, 8191, 2048, BF16, 0) == 2 and route(500, 8192, 2041, BF16, 0) == 2  # ragged ones
+    assert route(500, 8191, 2048, BF16, 1) == 0 and route(500, 8192, 2041, BF16, 2) == 2
+    assert route(500, 8192, 2048, F32, 0) == 2 and route(22, 8192, 2048, F32, 0) == 2
+    assert route(500, 8192, 2048, F32, 1) == 0 and route(1, 2816, 1000, F32, 0) == 1
+    assert route(4, 64, 0, BF16, 0) == 0 and route(300, 64, 100, BF16, 0) == 0
     for m in (1, 16, 17, 64, 65, 300):
         for keep in (0, 1, 2):
             for dtype in (F32, F16, BF16):

@@ -118,6 +118,8 @@ def test_few_rows(m, rows, cols, dtype):
 def test_few_rows_take_their_kernel():
     assert _route(1, 14336, 4096, torch.bfloat16) == 1
     assert _route(3, 999, 128, torch.float16) == 1 and _route(21, 512, 2048, torch.float32) == 1
+    assert _route(131, 999, 2048, torch.bfloat16) == 2 and _route(200, 1000, 512, torch.float32) == 2
+    assert _route(100, 63, 60, torch.bfloat16) == 0
 
 
 def test_a_row_is_the_same_beside_others():
@@ -173,8 +175,10 @@ def test_the_same_bits_as_the_layers_one_by_one(m, rows, cols, dtype):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("m,rows,cols", [(100, 63, 64), (70, 1000, 100), (3, 33, 65), (1, 1, 1), (80, 264, 7),
-                                         (30, 128, 256), (5, 24, 0)])
-def test_sizes_that_go_layer_by_layer(m, rows, cols, dtype):
+                                         (30, 128, 256), (5, 24, 0), (300, 1001, 200), (129, 77, 1000), (513, 264, 333),
+                                         (40, 1000, 200), (1, 3000, 1000), (22, 300, 256), (200, 1000, 512),
+                                         (512, 4416, 1712), (131, 999, 2048)])
+def test_ragged_sizes(m, rows, cols, dtype):
     from qste_amd import kernels
 
     x, layers = _operands(m, rows, cols, dtype, bias=True)
@@ -270,7 +274,8 @@ def _pair(rows, cols, seed, bias=False, dtype=torch.float32):
 
 @pytest.mark.parametrize("checkpoint", [False, True])
 @pytest.mark.parametrize("dtype,bias", [(torch.bfloat16, False), (torch.float16, True)])
-@pytest.mark.parametrize("m,rows,cols", [(3, 64, 64), (250, 2048, 768), (300, 264, 128), (1030, 1000, 512)])
+@pytest.mark.parametrize("m,rows,cols", [(3, 64, 64), (250, 2048, 768), (300, 264, 128), (1030, 1000, 512), (70, 64, 72),
+                                         (300, 264, 333), (600, 1000, 1000), (5, 8, 3)])
 def test_training_node(m, rows, cols, dtype, bias, checkpoint):
     """Values and gradients are those of the kernels that the node stands for, at the g and u it kept."""
 
@@ -310,7 +315,7 @@ def test_training_node(m, rows, cols, dtype, bias, checkpoint):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("m,rows,cols", [(1, 8, 64), (70, 40, 64), (250, 2048, 768), (513, 264, 128), (33, 1000, 192),
-                                         (2000, 512, 320)])
+                                         (2000, 512, 320), (70, 64, 72), (600, 1000, 1001), (5, 8, 3)])
 @pytest.mark.parametrize("kept", ["values", "blocks"])
 def test_backward_kernels(m, rows, cols, dtype, kept):
     """dx, evidence, scale and bias gradients against the formulas in 64 bits at the kept g and u.
@@ -330,7 +335,9 @@ def test_backward_kernels(m, rows, cols, dtype, kept):
     x = (torch.randn(m, cols, generator=gen, device=DEV) + 0.1).to(dtype)
     x *= torch.rand(m, 1, generator=gen, device=DEV).add(0.5).to(dtype)
     g, u, dh = (torch.randn(m, rows, generator=gen, device=DEV).to(dtype) for _ in range(3))
-    packed = torch.randint(0, 256, (2 * rows, cols // 8), generator=gen, device=DEV, dtype=torch.uint8)
+    packed = torch.randint(0, 256, (2 * rows, -(-cols // 8)), generator=gen, device=DEV, dtype=torch.uint8)
+    if cols % 8:
+        packed[:, -1] &= (1 << (cols % 8)) - 1
     scale = (torch.rand(2 * rows, generator=gen, device=DEV) + 0.2).to(dtype).float()
     payload, offset, xs = kernels.pack_affine_rows(x)
     operands = [kernels.quantize_blocks(t) if kept == "blocks" else t for t in (g, u)]
@@ -510,8 +517,7 @@ def test_node_in_use():
             qste.nn.swiglu(dual, x, checkpoint=True)
 
 
-@pytest.mark.parametrize("dtype,cols,rows", [(torch.float32, 64, 128), (torch.bfloat16, 72, 128),
-                                             (torch.bfloat16, 64, 100)])
+@pytest.mark.parametrize("dtype,cols,rows", [(torch.float32, 64, 128), (torch.bfloat16, 64, 100)])
 def test_layers_that_the_node_does_not_take(dtype, cols, rows):
     import qste_amd as qste
 
