@@ -278,9 +278,10 @@ def _gate_up_backward(ctx, dh: list, kept: tuple, payload_x: Tensor, aux_x: Tens
     gradients [2 ffn] or None)``.  ``dh``: the gradient of h in a list, taken out of it
     so that it is free during the product; ``kept``: g and u, as tensors or ``Blocks8``;
     ``scale_gu``: both layers' scales, fp32; ``plain``: round as the gate and the
-    layers one by one do, g and u being tensors."""
+    layers one by one do, g and u being tensors.  ffn, the rows of ``packed_g`` and
+    ``packed_u``, may be more than the surfaces have."""
 
-    d, ffn = sg.columns, sg.rows
+    d, ffn = sg.columns, packed_g.shape[0]
     # (a copy of their signs: the deliveries below may rewrite them)
     packed_gu = torch.cat((packed_g, packed_u))
     need_bias = any(b is not None for b in ctx.bias_dtypes[:2])
@@ -296,8 +297,8 @@ def _gate_up_backward(ctx, dh: list, kept: tuple, payload_x: Tensor, aux_x: Tens
             need_input=ctx.needs_input_grad[0])
     if dx is not None:
         dx = dx.reshape(ctx.input_shape)
-    sg.consume_evidence(ev_gu[:ffn])
-    su.consume_evidence(ev_gu[ffn:])
+    sg.consume_evidence(ev_gu[:sg.rows])
+    su.consume_evidence(ev_gu[ffn:ffn + su.rows])
     return dx, gs_gu, gb_gu
 
 
@@ -307,14 +308,27 @@ def _halves(t: Tensor | None, rows: int) -> tuple:
     return (None, None) if t is None else (t[:rows], t[rows:])
 
 
+def _eights(rows: int) -> int:
+    return -(-rows // 8) * 8
+
+
+def _in_eights(t: Tensor | None, dim: int = 0) -> Tensor | None:
+    """``t`` with zeros behind it up to a whole number of eights along ``dim``."""
+
+    more = 0 if t is None else -t.shape[dim] % 8
+    return t if not more else torch.cat((t, t.new_zeros(*t.shape[:dim], more, *t.shape[dim + 1:])), dim)
+
+
 def _two_scales(log_g: Tensor, log_u: Tensor, sg: Surface, su: Surface) -> tuple[Tensor, Tensor]:
     """Both layers' scales and their exponentials before the clamp, fp32 [2 ffn]
-    each, of values in the log-scales' dtypes."""
+    each, of values in the log-scales' dtypes.  ffn, the layers' rows in whole
+    eights: behind a layer's own there are zeros."""
 
-    ffn = sg.rows
+    rows, ffn = sg.rows, _eights(sg.rows)
     same = log_g.dtype == log_u.dtype
-    both = torch.empty(2, 2 * ffn, dtype=log_g.dtype if same else torch.float32, device=log_g.device)
-    for log, surface, at in ((log_g, sg, slice(0, ffn)), (log_u, su, slice(ffn, 2 * ffn))):
+    make = torch.empty if rows == ffn else torch.zeros
+    both = make(2, 2 * ffn, dtype=log_g.dtype if same else torch.float32, device=log_g.device)
+    for log, surface, at in ((log_g, sg, slice(0, rows)), (log_u, su, slice(ffn, ffn + rows))):
         out = (both[0, at], both[1, at])
         lo, hi = surface.cfg.scale_min, surface.cfg.scale_max
         if same:
@@ -329,16 +343,15 @@ def _two_scales(log_g: Tensor, log_u: Tensor, sg: Surface, su: Surface) -> tuple
 def _through_two_scales(grad: Tensor, e: Tensor, sg: Surface, su: Surface, dtypes: tuple) -> tuple[Tensor, Tensor]:
     """The scales' gradients carried to the log-scales in fp32, rounded once to their dtypes."""
 
-    ffn, (g, u) = sg.rows, (sg.cfg, su.cfg)
+    rows, ffn = sg.rows, _eights(sg.rows)
+    (g, u), parts = (sg.cfg, su.cfg), (slice(0, rows), slice(ffn, ffn + rows))
     if (g.scale_min, g.scale_max) == (u.scale_min, u.scale_max):
         log = kernels.row_scale_backward(e, grad, g.scale_min, g.scale_max)
         if dtypes[0] == dtypes[1]:
-            return _halves(log.to(dtypes[0]), ffn)
-        log_g, log_u = _halves(log, ffn)
-    else:
-        log_g = kernels.row_scale_backward(e[:ffn], grad[:ffn], g.scale_min, g.scale_max)
-        log_u = kernels.row_scale_backward(e[ffn:], grad[ffn:], u.scale_min, u.scale_max)
-    return log_g.to(dtypes[0]), log_u.to(dtypes[1])
+            log = log.to(dtypes[0])
+        return log[parts[0]].to(dtypes[0]), log[parts[1]].to(dtypes[1])
+    return tuple(kernels.row_scale_backward(e[at], grad[at], cfg.scale_min, cfg.scale_max).to(dtype)
+                 for at, cfg, dtype in zip(parts, (g, u), dtypes))
 
 
 class GatedFn(Function):
@@ -346,19 +359,22 @@ class GatedFn(Function):
 
     The forward is one kernel over both layers' signs (``kernels.gated_forward``)
     and x's encoding; what it keeps of g and u is them, or with ``checkpoint``
-    their 8-bit blocks.  The backward is the gate and up layers' part of
-    SwiGLUMLPFn's."""
+    their 8-bit blocks.  The backward is ``kernels.gated_backward``.  Layers whose
+    rows are no whole eights run with zero rows behind them."""
 
     @staticmethod
     def forward(ctx, inputs, packed_g, log_g, bias_g, packed_u, log_u, bias_u, surfaces, checkpoint: bool,
                 grad_on: bool):
         sg, su = surfaces
-        d, ffn = sg.columns, sg.rows
+        d, rows, ffn = sg.columns, sg.rows, _eights(sg.rows)
         flat = inputs.reshape(-1, d)
         scale_gu, e = _two_scales(log_g, log_u, sg, su)
-        keep = "" if not grad_on else "blocks" if checkpoint else "values"
-        h, g, u = kernels.gated_forward(flat, packed_g, scale_gu[:ffn], bias_g, packed_u, scale_gu[ffn:], bias_u, d,
-                                        keep=keep)
+        signs, biases, keep = (packed_g, packed_u), (bias_g, bias_u), ""
+        scales = (scale_gu[:rows], scale_gu[ffn:ffn + rows])
+        if grad_on:
+            signs, biases = [_in_eights(t) for t in signs], [_in_eights(t) for t in biases]
+            scales, keep = _halves(scale_gu, ffn), "blocks" if checkpoint else "values"
+        h, g, u = kernels.gated_forward(flat, signs[0], scales[0], biases[0], signs[1], scales[1], biases[1], d, keep=keep)
         if grad_on:
             payload_x, aux_x = _encoding_of(inputs, flat, d)
             more = (payload_x, aux_x, packed_g, packed_u, scale_gu, e)
@@ -366,12 +382,14 @@ class GatedFn(Function):
                 _save_kept(ctx, g, u, *more)
             else:
                 ctx.save_for_backward(g, u, *more)
+            if rows != ffn:
+                h = h[:, :rows].contiguous()
         ctx.checkpoint = checkpoint
         ctx.surfaces = surfaces
         ctx.input_shape = inputs.shape
         ctx.log_dtypes = (log_g.dtype, log_u.dtype)
         ctx.bias_dtypes = tuple(None if b is None else b.dtype for b in (bias_g, bias_u))
-        return h.reshape(*inputs.shape[:-1], ffn)
+        return h.reshape(*inputs.shape[:-1], rows)
 
     @staticmethod
     @once_differentiable
@@ -380,11 +398,14 @@ class GatedFn(Function):
         saved = ctx.saved_tensors
         payload_x, aux_x, packed_g, packed_u, scale_gu, e = saved[-6:]
         sg, su = ctx.surfaces
-        dx, gs_gu, gb_gu = _gate_up_backward(ctx, [grad_output.reshape(-1, sg.rows)], _kept(ctx, saved), payload_x,
-                                             aux_x, packed_g, packed_u, scale_gu, sg, su)
+        dh = [_in_eights(grad_output.reshape(-1, sg.rows), 1)]
+        dx, gs_gu, gb_gu = _gate_up_backward(ctx, dh, _kept(ctx, saved), payload_x, aux_x, _in_eights(packed_g),
+                                             _in_eights(packed_u), scale_gu, sg, su)
         log_g, log_u = _through_two_scales(gs_gu, e, sg, su, ctx.log_dtypes)
-        gb_g, gb_u = _halves(gb_gu, sg.rows)
+        gb_g, gb_u = _halves(gb_gu, _eights(sg.rows))
         bg, bu = ctx.bias_dtypes
+        if gb_gu is not None:
+            gb_g, gb_u = gb_g[:sg.rows], gb_u[:su.rows]
         return dx, None, log_g, _cast(gb_g, bg), None, log_u, _cast(gb_u, bu), None, None, None
 
 
@@ -498,13 +519,12 @@ def swiglu_mlp_fusable(inputs: Tensor, gate, up, down) -> bool:
 
 
 def gated_fusable(inputs: Tensor, gate, up) -> bool:
-    """Whether ``GatedFn`` takes this block: a bf16 or fp16 input on the GPU,
-    the layers' rows a multiple of 8."""
+    """Whether ``GatedFn`` takes this block: a bf16 or fp16 input on the GPU."""
 
     sg, su = gate.surface, up.surface
     return (inputs.is_cuda and inputs.dtype in (torch.bfloat16, torch.float16) and inputs.dim() >= 1
-            and inputs.shape[-1] == sg.columns == su.columns and sg.rows == su.rows and sg.rows % 8 == 0 and inputs.numel() > 0
-            and all(s.log_scale.is_cuda and s.log_scale.dtype in _SCALE_DTYPES for s in (sg, su)))
+            and inputs.shape[-1] == sg.columns == su.columns and sg.rows == su.rows
+            and inputs.numel() > 0 and all(s.log_scale.is_cuda and s.log_scale.dtype in _SCALE_DTYPES for s in (sg, su)))
 
 
 def swiglu(gate: Tensor, up: Tensor, *, checkpoint: bool = False) -> Tensor:

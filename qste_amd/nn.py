@@ -83,8 +83,8 @@ def gated(inputs: Tensor, gate, up, *, checkpoint: bool = False) -> Tensor:
     once, where the operators one by one round silu's value too.  With gradients it is one
     autograd node, whose backward runs the two layers as one; evidence and
     scale gradients go where the layers' own would.  ``checkpoint`` keeps gate and up
-    for the backward in 8-bit blocks (``quantize_blocks``) in place of 16 bits.  With
-    gradients, fp32 and rows that are no multiple of 8 run layer by layer."""
+    for the backward in 8-bit blocks (``quantize_blocks``) in place of 16 bits.  fp32
+    runs layer by layer where it carries gradients."""
 
     # a module's buffers and parts by their dicts: attributes of modules are looked up in Python, half a microsecond each
     try:
