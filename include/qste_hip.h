@@ -549,6 +549,17 @@ int qste_row_scale(const void* log_scale, int dtype, void* scale, void* exp_valu
 int qste_row_scale_backward(const void* exp_value, const void* grad, int dtype, void* grad_log_scale, int64_t n,
                             float lo, float hi, void* stream);
 
+/* qste_row_scale of two layers that run as one (qste_gated): scale and exp_value
+ * fp32 [2 * padded], gate's rows first, up's from padded on, zeros behind a
+ * layer's rows; values are rounded in each log-scale's dtype.  Backward: grad fp32
+ * [2 * padded] times exp_value in fp32, rounded once to the log-scales' dtypes. */
+int qste_pair_scale(const void* log_gate, int gate_dtype, float gate_lo, float gate_hi, const void* log_up,
+                    int up_dtype, float up_lo, float up_hi, float* scale, float* exp_value, int64_t rows,
+                    int64_t padded, void* stream);
+int qste_pair_scale_backward(const float* exp_value, const float* grad, void* grad_log_gate, int gate_dtype,
+                             float gate_lo, float gate_hi, void* grad_log_up, int up_dtype, float up_lo, float up_hi,
+                             int64_t rows, int64_t padded, void* stream);
+
 /* The end of an optimizer step over `count` surfaces: log_scale[i], fp32 [n[i]],
  * is clamped to [lo, hi] in place (a NaN stays NaN) and, when nflips > 0,
  * *total = the sum of the nflips <= count counters flips[i].  The three arrays are host

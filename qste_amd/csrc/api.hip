@@ -103,6 +103,10 @@ int mfma_gated(const void*, int, const uint8_t*, const float*, const float*, con
 int launch_step_finish(float* const*, const int64_t*, int, const int64_t* const*, int, float, float, int64_t*,
                        hipStream_t);
 int launch_row_scale_backward(const void*, const void*, int, void*, int64_t, float, float, hipStream_t);
+int launch_pair_scale(const void*, int, float, float, const void*, int, float, float, float*, float*, int64_t, int64_t,
+                      hipStream_t);
+int launch_pair_scale_backward(const float*, const float*, void*, int, float, float, void*, int, float, float, int64_t,
+                               int64_t, hipStream_t);
 size_t token_logprobs_workspace(int64_t, int64_t, int, int64_t);
 int launch_token_logprobs(const vocab::Logits&, int, int64_t, const int64_t*, double, int64_t, float*, float*, float*,
                           int64_t*, float*, void*, hipStream_t);
@@ -1072,6 +1076,28 @@ int qste_row_scale(const void* log_scale, int dtype, void* scale, void* exp_valu
   if (n == 0) return 0;
   if (!log_scale || !scale || !exp_value) return QSTE_E_NULL;
   return launch_row_scale(log_scale, dtype, scale, exp_value, n, lo, hi, as_stream(stream));
+}
+
+int qste_pair_scale(const void* log_gate, int gate_dtype, float gate_lo, float gate_hi, const void* log_up,
+                    int up_dtype, float up_lo, float up_hi, float* scale, float* exp_value, int64_t rows,
+                    int64_t padded, void* stream) {
+  if (!dtype_ok(gate_dtype) || !dtype_ok(up_dtype)) return QSTE_E_DTYPE;
+  if (rows < 0 || padded < rows) return QSTE_E_SHAPE;
+  if (padded == 0) return 0;
+  if (!scale || !exp_value || (rows > 0 && (!log_gate || !log_up))) return QSTE_E_NULL;
+  return launch_pair_scale(log_gate, gate_dtype, gate_lo, gate_hi, log_up, up_dtype, up_lo, up_hi, scale, exp_value,
+                           rows, padded, as_stream(stream));
+}
+
+int qste_pair_scale_backward(const float* exp_value, const float* grad, void* grad_log_gate, int gate_dtype,
+                             float gate_lo, float gate_hi, void* grad_log_up, int up_dtype, float up_lo, float up_hi,
+                             int64_t rows, int64_t padded, void* stream) {
+  if (!dtype_ok(gate_dtype) || !dtype_ok(up_dtype)) return QSTE_E_DTYPE;
+  if (rows < 0 || padded < rows) return QSTE_E_SHAPE;
+  if (rows == 0) return 0;
+  if (!exp_value || !grad || !grad_log_gate || !grad_log_up) return QSTE_E_NULL;
+  return launch_pair_scale_backward(exp_value, grad, grad_log_gate, gate_dtype, gate_lo, gate_hi, grad_log_up, up_dtype,
+                                    up_lo, up_hi, rows, padded, as_stream(stream));
 }
 
 int qste_step_finish(float* const* log_scale, const int64_t* n, int count, const int64_t* const* flips, int nflips,

@@ -84,6 +84,82 @@ int launch_row_scale_backward(const void* e, const void* grad, int dtype, void* 
 }
 #undef QSTE_SCALE_DT_SWITCH
 
+// The scales of two layers that run as one (a gated block's gate and up), each in
+// its log-scale's type, as fp32 [2 padded] with zeros behind a layer's rows, and
+// the gradients back; bound by their launch, so one each way for both layers, with
+// the conversions that the products want.
+namespace pairscale {
+
+constexpr int kThreads = 256;
+
+struct Layer {
+  void* log;  // log-scales, or their gradients
+  int dtype;
+  float lo, hi;
+};
+
+template <int DT>
+__device__ __forceinline__ void forward_one(const Layer& l, int64_t i, float& scale, float& e) {
+  using E = Elem<DT>;
+  e = E::round(expf(E::load(static_cast<const typename E::T*>(l.log), i)));
+  scale = e != e ? e : E::round(fminf(fmaxf(e, l.lo), l.hi));
+}
+template <int DT>
+__device__ __forceinline__ void backward_one(const Layer& l, int64_t i, float e, float grad) {
+  using E = Elem<DT>;
+  const float pass = (e >= E::round(l.lo) && e <= E::round(l.hi)) ? grad : 0.0f;
+  E::store(static_cast<typename E::T*>(l.log), i, pass * e);
+}
+
+__global__ __launch_bounds__(kThreads) void forward_kernel(Layer gate, Layer up, float* __restrict__ scale,
+                                                           float* __restrict__ e_out, int64_t rows, int64_t padded) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  if (i >= padded) return;
+  const Layer l = blockIdx.y ? up : gate;
+  float s = 0.0f, e = 0.0f;
+  if (i < rows) {
+    if (l.dtype == QSTE_F32) forward_one<QSTE_F32>(l, i, s, e);
+    else if (l.dtype == QSTE_F16) forward_one<QSTE_F16>(l, i, s, e);
+    else forward_one<QSTE_BF16>(l, i, s, e);
+  }
+  const int64_t at = i + (blockIdx.y ? padded : 0);
+  scale[at] = s;
+  e_out[at] = e;
+}
+
+__global__ __launch_bounds__(kThreads) void backward_kernel(Layer gate, Layer up, const float* __restrict__ e,
+                                                            const float* __restrict__ grad, int64_t rows,
+                                                            int64_t padded) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  if (i >= rows) return;
+  const Layer l = blockIdx.y ? up : gate;
+  const int64_t at = i + (blockIdx.y ? padded : 0);
+  if (l.dtype == QSTE_F32) backward_one<QSTE_F32>(l, i, e[at], grad[at]);
+  else if (l.dtype == QSTE_F16) backward_one<QSTE_F16>(l, i, e[at], grad[at]);
+  else backward_one<QSTE_BF16>(l, i, e[at], grad[at]);
+}
+
+}  // namespace pairscale
+
+int launch_pair_scale(const void* log_gate, int gate_dtype, float gate_lo, float gate_hi, const void* log_up,
+                      int up_dtype, float up_lo, float up_hi, float* scale, float* e, int64_t rows, int64_t padded,
+                      hipStream_t stream) {
+  const pairscale::Layer gate{const_cast<void*>(log_gate), gate_dtype, gate_lo, gate_hi};
+  const pairscale::Layer up{const_cast<void*>(log_up), up_dtype, up_lo, up_hi};
+  pairscale::forward_kernel<<<dim3(ceil_div(padded, pairscale::kThreads), 2), pairscale::kThreads, 0, stream>>>(
+      gate, up, scale, e, rows, padded);
+  return static_cast<int>(hipGetLastError());
+}
+
+int launch_pair_scale_backward(const float* e, const float* grad, void* grad_gate, int gate_dtype, float gate_lo,
+                               float gate_hi, void* grad_up, int up_dtype, float up_lo, float up_hi, int64_t rows,
+                               int64_t padded, hipStream_t stream) {
+  const pairscale::Layer gate{grad_gate, gate_dtype, gate_lo, gate_hi}, up{grad_up, up_dtype, up_lo, up_hi};
+  pairscale::backward_kernel<<<dim3(ceil_div(rows, pairscale::kThreads), 2), pairscale::kThreads, 0, stream>>>(
+      gate, up, e, grad, rows, padded);
+  return static_cast<int>(hipGetLastError());
+}
+
 // The end of an optimizer step in one launch: every surface's log-scales
 // clamped in place (torch's clamp: NaN stays) and the surfaces' flip counts
 // added up.  Bound by the launch: a clamp per surface, a stack and a sum took

@@ -319,39 +319,8 @@ def _in_eights(t: Tensor | None, dim: int = 0) -> Tensor | None:
     return t if not more else torch.cat((t, t.new_zeros(*t.shape[:dim], more, *t.shape[dim + 1:])), dim)
 
 
-def _two_scales(log_g: Tensor, log_u: Tensor, sg: Surface, su: Surface) -> tuple[Tensor, Tensor]:
-    """Both layers' scales and their exponentials before the clamp, fp32 [2 ffn]
-    each, of values in the log-scales' dtypes.  ffn, the layers' rows in whole
-    eights: behind a layer's own there are zeros."""
-
-    rows, ffn = sg.rows, _eights(sg.rows)
-    same = log_g.dtype == log_u.dtype
-    make = torch.empty if rows == ffn else torch.zeros
-    both = make(2, 2 * ffn, dtype=log_g.dtype if same else torch.float32, device=log_g.device)
-    for log, surface, at in ((log_g, sg, slice(0, rows)), (log_u, su, slice(ffn, ffn + rows))):
-        out = (both[0, at], both[1, at])
-        lo, hi = surface.cfg.scale_min, surface.cfg.scale_max
-        if same:
-            kernels.row_scale(log, lo, hi, out)
-        else:
-            for to, t in zip(out, kernels.row_scale(log, lo, hi)):
-                to.copy_(t)
-    scale, e = both.float().unbind(0)
-    return scale, e
-
-
-def _through_two_scales(grad: Tensor, e: Tensor, sg: Surface, su: Surface, dtypes: tuple) -> tuple[Tensor, Tensor]:
-    """The scales' gradients carried to the log-scales in fp32, rounded once to their dtypes."""
-
-    rows, ffn = sg.rows, _eights(sg.rows)
-    (g, u), parts = (sg.cfg, su.cfg), (slice(0, rows), slice(ffn, ffn + rows))
-    if (g.scale_min, g.scale_max) == (u.scale_min, u.scale_max):
-        log = kernels.row_scale_backward(e, grad, g.scale_min, g.scale_max)
-        if dtypes[0] == dtypes[1]:
-            log = log.to(dtypes[0])
-        return log[parts[0]].to(dtypes[0]), log[parts[1]].to(dtypes[1])
-    return tuple(kernels.row_scale_backward(e[at], grad[at], cfg.scale_min, cfg.scale_max).to(dtype)
-                 for at, cfg, dtype in zip(parts, (g, u), dtypes))
+def _bounds(surface: Surface) -> tuple[float, float]:
+    return surface.cfg.scale_min, surface.cfg.scale_max
 
 
 class GatedFn(Function):
@@ -368,7 +337,7 @@ class GatedFn(Function):
         sg, su = surfaces
         d, rows, ffn = sg.columns, sg.rows, _eights(sg.rows)
         flat = inputs.reshape(-1, d)
-        scale_gu, e = _two_scales(log_g, log_u, sg, su)
+        scale_gu, e = kernels.pair_scale(log_g, _bounds(sg), log_u, _bounds(su), ffn)
         signs, biases, keep = (packed_g, packed_u), (bias_g, bias_u), ""
         scales = (scale_gu[:rows], scale_gu[ffn:ffn + rows])
         if grad_on:
@@ -401,11 +370,12 @@ class GatedFn(Function):
         dh = [_in_eights(grad_output.reshape(-1, sg.rows), 1)]
         dx, gs_gu, gb_gu = _gate_up_backward(ctx, dh, _kept(ctx, saved), payload_x, aux_x, _in_eights(packed_g),
                                              _in_eights(packed_u), scale_gu, sg, su)
-        log_g, log_u = _through_two_scales(gs_gu, e, sg, su, ctx.log_dtypes)
-        gb_g, gb_u = _halves(gb_gu, _eights(sg.rows))
+        (dt_g, dt_u), rows = ctx.log_dtypes, sg.rows
+        log_g, log_u = kernels.pair_scale_backward(e, gs_gu, dt_g, _bounds(sg), dt_u, _bounds(su), rows)
+        gb_g, gb_u = _halves(gb_gu, _eights(rows))
         bg, bu = ctx.bias_dtypes
         if gb_gu is not None:
-            gb_g, gb_u = gb_g[:sg.rows], gb_u[:su.rows]
+            gb_g, gb_u = gb_g[:rows], gb_u[:rows]
         return dx, None, log_g, _cast(gb_g, bg), None, log_u, _cast(gb_u, bu), None, None, None
 
 

@@ -1072,18 +1072,14 @@ def _leading(t: Tensor) -> int:
     return count
 
 
-def row_scale(log_scale: Tensor, lo: float, hi: float,
-              out: tuple[Tensor, Tensor] | None = None) -> tuple[Tensor, Tensor]:
+def row_scale(log_scale: Tensor, lo: float, hi: float) -> tuple[Tensor, Tensor]:
     """``(clamp(exp(log_scale), lo, hi), exp(log_scale))`` in log_scale's
     dtype (fp32, fp16 or bf16), one launch (surface.py:84-85), rounded as
-    torch's ``exp().clamp()`` on that dtype; in ``out``, two contiguous tensors of
-    that shape and dtype, if given."""
+    torch's ``exp().clamp()`` on that dtype."""
 
     device = _require_gpu(log_scale)
     ls = log_scale.detach().contiguous()
-    scale, e = (torch.empty_like(ls), torch.empty_like(ls)) if out is None else out
-    if out is not None and not all(t.shape == ls.shape and t.dtype == ls.dtype and t.is_contiguous() for t in out):
-        raise ValueError("row_scale's outputs must be contiguous and of log_scale's shape and dtype")
+    scale, e = torch.empty_like(ls), torch.empty_like(ls)
     code = _lib.load().qste_row_scale(_ptr(ls), _dtype_code(ls), _ptr(scale), _ptr(e), ls.numel(), float(lo),
                                       float(hi), _stream(device))
     _lib.check(code, "row_scale")
@@ -1103,6 +1099,43 @@ def row_scale_backward(exp_value: Tensor, grad: Tensor, lo: float, hi: float) ->
                                                float(hi), _stream(device))
     _lib.check(code, "row_scale_backward")
     return out
+
+
+def pair_scale(log_gate: Tensor, gate_bounds: tuple[float, float], log_up: Tensor, up_bounds: tuple[float, float],
+               padded: int) -> tuple[Tensor, Tensor]:
+    """``row_scale`` of two layers that run as one: ``(scale, exp)``, fp32 [2 padded]
+    of values in the log-scales' own dtypes, zeros behind each layer's rows."""
+
+    device = _require_gpu(log_gate, log_up)
+    rows, padded = log_gate.numel(), int(padded)
+    if log_up.numel() != rows or padded < rows:
+        raise ValueError(f"log-scales of {rows} and {log_up.numel()} rows in {padded}")
+    lg, lu = log_gate.detach().contiguous(), log_up.detach().contiguous()
+    out = torch.empty(2, 2 * padded, dtype=torch.float32, device=device)
+    scale, e = out.unbind(0)
+    with _device_of(device):
+        _lib.check(_lib.load().qste_pair_scale(_ptr(lg), _dtype_code(lg), *gate_bounds, _ptr(lu), _dtype_code(lu),
+                                               *up_bounds, _ptr(scale), _ptr(e), rows, padded, _stream(device)),
+                   "pair_scale")
+    return scale, e
+
+
+def pair_scale_backward(exp_value: Tensor, grad: Tensor, gate_dtype: torch.dtype, gate_bounds: tuple[float, float],
+                        up_dtype: torch.dtype, up_bounds: tuple[float, float], rows: int) -> tuple[Tensor, Tensor]:
+    """The log-scales' gradients [rows] for the gradient fp32 [2 padded] of
+    ``pair_scale``'s scales: in fp32, rounded once to their dtypes."""
+
+    device = _require_gpu(exp_value, grad)
+    if exp_value.shape != grad.shape or not exp_value.dtype == grad.dtype == torch.float32 or exp_value.dim() != 1:
+        raise ValueError("pair_scale_backward takes fp32 vectors of one shape")
+    e, g = exp_value.contiguous(), grad.contiguous()
+    log_g = torch.empty(rows, dtype=gate_dtype, device=device)
+    log_u = torch.empty(rows, dtype=up_dtype, device=device)
+    with _device_of(device):
+        _lib.check(_lib.load().qste_pair_scale_backward(
+            _ptr(e), _ptr(g), _ptr(log_g), _dtype_code(log_g), *gate_bounds, _ptr(log_u), _dtype_code(log_u), *up_bounds,
+            rows, e.numel() // 2, _stream(device)), "pair_scale_backward")
+    return log_g, log_u
 
 
 def step_finish(log_scales: list[Tensor], lo: float, hi: float, flips: list[Tensor]) -> Tensor | None:

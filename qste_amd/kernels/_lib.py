@@ -94,6 +94,8 @@ SIGNATURES = {
     "qste_gated": (_int, [_vp, _int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64,
                           _vp, _sz, _vp]),
     "qste_row_scale": (_int, [_vp, _int, _vp, _vp, _i64, _flt, _flt, _vp]),
+    "qste_pair_scale": (_int, [_vp, _int, _flt, _flt, _vp, _int, _flt, _flt, _vp, _vp, _i64, _i64, _vp]),
+    "qste_pair_scale_backward": (_int, [_vp, _vp, _vp, _int, _flt, _flt, _vp, _int, _flt, _flt, _i64, _i64, _vp]),
     "qste_step_finish": (_int, [_vp, _vp, _int, _vp, _int, _flt, _flt, _vp, _vp]),
     "qste_row_scale_backward": (_int, [_vp, _vp, _int, _vp, _i64, _flt, _flt, _vp]),
     "qste_packed_embedding": (_int, [_vp, _i64, _vp, _vp, _vp, _int, _i64, _i64, _vp]),

@@ -106,11 +106,11 @@ def gated(inputs: Tensor, gate, up, *, checkpoint: bool = False) -> Tensor:
     _no_tangent("gated", x)
     if not gated_fusable(x, gate, up):
         return swiglu(gate(inputs), up(inputs), checkpoint=checkpoint)
-    surfaces = (gate.surface, up.surface)
-    for s in surfaces:
-        s.note_forward()
-    return GatedFn.apply(x, gate.surface.packed_sign, gate.surface.log_scale, gate.bias, up.surface.packed_sign,
-                         up.surface.log_scale, up.bias, surfaces, checkpoint, torch.is_grad_enabled())
+    sg, su = gate.surface, up.surface
+    sg.note_forward()
+    su.note_forward()
+    return GatedFn.apply(x, sg.packed_sign, sg.log_scale, gate.bias, su.packed_sign, su.log_scale, up.bias, (sg, su),
+                         checkpoint, torch.is_grad_enabled())
 
 
 def swiglu_mlp(inputs: Tensor, gate, up, down, *, checkpoint: bool = False) -> Tensor:

@@ -96,6 +96,11 @@ def test_c_entries_refuse_before_any_launch():
     assert lib.qste_linear_backward_operands(*ones[:2], F16, *ones[:8], 0, 8, 8, None, 0, None) == E_SHAPE
     assert lib.qste_linear_backward_operands(p(4096), None, F16, *ones[:8], 4, 8, 8, None, 0, None) == E_NULL
     assert lib.qste_linear_backward_operands(*ones[:2], F16, *ones[:8], 4, 8, 8, None, 0, None) == E_WORKSPACE
+    bounds = (1e-6, 4.0)
+    assert lib.qste_pair_scale(p(4096), 5, *bounds, p(4096), F32, *bounds, p(4096), p(4096), 4, 8, None) == E_DTYPE
+    assert lib.qste_pair_scale(p(4096), F32, *bounds, p(4096), F32, *bounds, p(4096), p(4096), 9, 8, None) == E_SHAPE
+    assert lib.qste_pair_scale(p(4096), F32, *bounds, None, F32, *bounds, p(4096), p(4096), 4, 8, None) == E_NULL
+    assert lib.qste_pair_scale_backward(p(4096), p(4096), p(4096), F32, *bounds, None, F32, *bounds, 4, 8, None) == E_NULL
     assert lib.qste_quantize_blocks(None, 9, None, None, 1, 1, None) == E_DTYPE
     assert lib.qste_quantize_blocks(None, F32, None, None, -1, 1, None) == E_SHAPE
     assert lib.qste_quantize_blocks(None, F32, None, None, 1, 1, None) == E_NULL
