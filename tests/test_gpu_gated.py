@@ -592,6 +592,52 @@ def test_mlp_with_a_checkpoint():
     assert all(a > 0 and b > 0 for a, b in zip(moved0, moved1))
 
 
+def test_trained_then_served():
+    """One module whose block is a call of gated: trained by steps of both optimizers with its gate and up in 8 bits,
+    exported, and served a prompt and then token by token."""
+
+    import qste_amd as qste
+
+    class Block(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.gate, self.up = torch.nn.Linear(192, 520), torch.nn.Linear(192, 520, bias=False)
+            self.down = torch.nn.Linear(520, 192, bias=False)
+
+        def forward(self, x):
+            return self.down(qste.nn.gated(x, self.gate, self.up, checkpoint=True))
+
+    torch.manual_seed(0)
+    model = Block()
+    qste.convert(model, include=["*"])
+    model.to(DEV)
+    optimizer = torch.optim.SGD(qste.continuous_parameters(model), lr=1e-3)
+    coords = qste.QSTEOptimizer(model)
+    x = torch.randn(2, 150, 192, device=DEV, generator=torch.Generator(device=DEV).manual_seed(1)).bfloat16()
+    before = [s.coordinate.detach().clone() for s in qste.surfaces(model)]
+    for _ in range(3):
+        model(x).float().square().mean().backward()
+        # (of a mean over 57600 outputs: times the learning rate far below half a unit, 2^-23, of a log-scale of -3.3,
+        # so that they are looked at and not what the step makes of them)
+        assert all(bool(torch.isfinite(p.grad).all()) and bool((p.grad != 0).any()) for p in optimizer.param_groups[0]["params"])
+        optimizer.step(), optimizer.zero_grad()
+        coords.step()
+    for s, b in zip(qste.surfaces(model), before):
+        assert bool((s.coordinate.detach() != b).any())
+        assert torch.equal(s.packed_sign.data, qste.kernels.pack_coordinate(s.coordinate.data))
+    with torch.no_grad():
+        whole = model(x)
+    served = qste.export_packed(model)
+    assert isinstance(served.gate, qste.PackedLinear)
+    prompt = served(x)
+    # the same products; those of few tokens sum in another order, which g, u, h and the output's rounding show: four
+    # roundings of half a step each
+    assert torch.equal(prompt, whole)
+    for t in (0, 7, 149):
+        token = served(x[:, t])
+        assert float((token.double() - whole[:, t].double()).norm() / whole[:, t].double().norm()) <= 4 * 2.0 ** -8
+
+
 def test_streams_and_graphs():
     """On a side stream, and captured with two ways in one graph and replayed with eager work in between."""
 
