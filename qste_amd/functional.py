@@ -292,9 +292,10 @@ def _gate_up_backward(ctx, dh: list, kept: tuple, payload_x: Tensor, aux_x: Tens
             need_input=ctx.needs_input_grad[0], offset_dot=sums.reshape(-1))
         del both
     else:
-        dx, ev_gu, gs_gu, gb_gu = kernels.gated_backward(
-            dh.pop(), *kept, payload_x, aux_x[0], aux_x[1], packed_gu, scale_gu, d, need_bias=need_bias,
-            need_input=ctx.needs_input_grad[0])
+        grads = kernels._gated_grads(dh.pop(), *kept, aux_x[0], aux_x[1])
+        dx, ev_gu, gs_gu, gb_gu = kernels._gated_products(*grads, payload_x, aux_x[1], packed_gu, scale_gu, d,
+                                                          ctx.needs_input_grad[0], need_bias)
+        del grads
     if dx is not None:
         dx = dx.reshape(ctx.input_shape)
     sg.consume_evidence(ev_gu[:sg.rows])

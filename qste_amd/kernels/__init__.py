@@ -1017,6 +1017,17 @@ def gated_backward(grad: Tensor, gate, up, packed_x: Tensor, x_offset: Tensor, x
     [2 rows, ...] and ``scale`` [2 rows] both layers' signs and scales, gate's first.
     """
 
+    grads = _gated_grads(grad, gate, up, x_offset, x_scale)
+    return _gated_products(*grads, packed_x, x_scale, packed_w, scale, columns, need_input, need_bias)
+
+
+# In two halves for the autograd nodes: out's gradient is free once the first is queued.
+
+
+def _gated_grads(grad: Tensor, gate, up, x_offset: Tensor, x_scale: Tensor) -> tuple[Tensor, Tensor, Tensor]:
+    """gate's and up's gradients side by side [samples, 2 rows], the same as the
+    evidence takes them, and the sums over the samples (``qste_gated_backward``)."""
+
     kept = isinstance(gate, Blocks8)
     if kept != isinstance(up, Blocks8):
         raise TypeError("gate and up are both tensors or both Blocks8")
@@ -1025,7 +1036,7 @@ def gated_backward(grad: Tensor, gate, up, packed_x: Tensor, x_offset: Tensor, x
         parts, shapes = (*gate[:2], *up[:2]), (gate.payload.shape, up.payload.shape)
     else:
         parts, shapes = (gate, up), (gate.shape, up.shape)
-    device = _require_gpu(grad, *parts, packed_x, x_offset, x_scale, packed_w, scale)
+    device = _require_gpu(grad, *parts, x_offset, x_scale)
     if grad.dtype not in (torch.bfloat16, torch.float16):
         raise TypeError(f"gated_backward takes bfloat16 or float16, got {grad.dtype}")
     if grad.dim() != 2 or grad.shape[1] % 8 or not grad.numel():
@@ -1033,36 +1044,42 @@ def gated_backward(grad: Tensor, gate, up, packed_x: Tensor, x_offset: Tensor, x
     if not (grad.shape == shapes[0] == shapes[1]) or not (grad.dtype == gate.dtype == up.dtype):
         raise ValueError("grad, gate and up must have the same shape and dtype")
     samples, rows = (int(s) for s in grad.shape)
-    columns, code = int(columns), _DTYPES[grad.dtype]
-    packed_x, packed_w = _check_packed(packed_x, columns, samples), _check_packed(packed_w, columns, 2 * rows)
     offset, xs = _layer_vector(x_offset, samples, "x_offset"), _layer_vector(x_scale, samples, "x_scale")
-    scale = _layer_vector(scale, 2 * rows, "scale")
     dh = _aligned(grad)
-    if kept:
-        sources = (None, None, *(_ptr(t) for t in parts))
-    else:
-        parts = (_aligned(gate), _aligned(up))  # held until the launch is queued
-        sources = (_ptr(parts[0]), _ptr(parts[1]), None, None, None, None)
-    lib = _lib.load()
-    # dy and what the evidence takes for it
+    parts = tuple(_aligned(t) for t in parts)  # held until the launch is queued
+    sources = (None, None, *map(_ptr, parts)) if kept else (*map(_ptr, parts), None, None, None, None)
     both, ev = torch.empty(2, samples, 2 * rows, dtype=grad.dtype, device=device).unbind(0)
     sums = torch.empty(4 * rows, dtype=torch.float32, device=device)
-    dx = torch.empty(samples, columns, dtype=grad.dtype, device=device) if need_input else None
-    evidence = torch.empty(2 * rows, columns, dtype=torch.float32, device=device)
-    grad_scale = torch.empty(2 * rows, dtype=torch.float32, device=device)
-    # one workspace for both calls, which follow each other on the stream
-    nbytes = lib.qste_linear_backward_operands_workspace_bytes(samples, 2 * rows, columns, code)
-    work = _workspace(max(nbytes, lib.qste_gated_backward_workspace_bytes(samples, rows)), device)
+    lib = _lib.load()
+    work = _workspace(lib.qste_gated_backward_workspace_bytes(samples, rows), device)
     with _device_of(device):
-        stream = _stream(device)
-        _lib.check(lib.qste_gated_backward(_ptr(dh), code, *sources, _ptr(both), _ptr(ev), _ptr(offset), _ptr(xs),
-                                           _ptr(sums), samples, rows, _ptr(work), work.numel(), stream),
-                   "gated_backward")
+        _lib.check(lib.qste_gated_backward(_ptr(dh), _DTYPES[grad.dtype], *sources, _ptr(both), _ptr(ev), _ptr(offset),
+                                           _ptr(xs), _ptr(sums), samples, rows, _ptr(work), work.numel(),
+                                           _stream(device)), "gated_backward")
+    return both, ev, sums
+
+
+def _gated_products(both: Tensor, ev: Tensor, sums: Tensor, packed_x: Tensor, x_scale: Tensor, packed_w: Tensor,
+                    scale: Tensor, columns: int, need_input: bool, need_bias: bool):
+    """What ``gated_backward`` returns, from what ``_gated_grads`` does."""
+
+    device = _require_gpu(both, packed_x, x_scale, packed_w, scale)
+    samples, rows = both.shape
+    columns = int(columns)
+    packed_x, packed_w = _check_packed(packed_x, columns, samples), _check_packed(packed_w, columns, rows)
+    xs, scale = _layer_vector(x_scale, samples, "x_scale"), _layer_vector(scale, rows, "scale")
+    dx = torch.empty(samples, columns, dtype=both.dtype, device=device) if need_input else None
+    evidence = torch.empty(rows, columns, dtype=torch.float32, device=device)
+    grad_scale = torch.empty(rows, dtype=torch.float32, device=device)
+    lib, code = _lib.load(), _DTYPES[both.dtype]
+    nbytes = lib.qste_linear_backward_operands_workspace_bytes(samples, rows, columns, code)
+    work = _workspace(nbytes, device)
+    with _device_of(device):
         _lib.check(lib.qste_linear_backward_operands(
             _ptr(both), _ptr(ev), code, _ptr(packed_x), _ptr(xs), _ptr(packed_w), _ptr(scale), _ptr(dx), _ptr(evidence),
-            _ptr(grad_scale), _ptr(sums), samples, 2 * rows, columns, _ptr(work), work.numel(), stream),
+            _ptr(grad_scale), _ptr(sums), samples, rows, columns, _ptr(work), nbytes, _stream(device)),
             "linear_backward_operands")
-    return dx, evidence, grad_scale, (sums[2 * rows:] if need_bias else None)
+    return dx, evidence, grad_scale, (sums[rows:] if need_bias else None)
 
 
 def _leading(t: Tensor) -> int:
