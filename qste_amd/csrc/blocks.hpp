@@ -37,9 +37,9 @@ __device__ __forceinline__ float to_steps(uint32_t code) {
   return __uint_as_float(code == kBadCode ? 0u : (260u - code) << 23);
 }
 
-// a step, 2^(code - 133); NaN for a bad block
+// a step, 2^(code - 133); NaN for a bad block (and 0 for the codes below the least)
 __device__ __forceinline__ float step_of(uint32_t code) {
-  return __uint_as_float(code == kBadCode ? 0x7FC00000u : (code - 6u) << 23);
+  return __uint_as_float(code == kBadCode ? 0x7FC00000u : code < kLeastCode ? 0u : (code - 6u) << 23);
 }
 
 // rint(x * to) within +-127, in the low byte of what is returned: added to 1.5 *

@@ -133,9 +133,9 @@ struct Pair {
 
 // ONCE, here and below: what is written is stored without keeping its lines
 // (blocks::streamed).  us, kept / streamed, 16384 x 14336 in bf16: the forward with
-// blocks 404 / 393, with the encoding too 414 / 400, the backward 399 / 381, with the sums 380 / 372; 4096 x
-// 4096, whose gradients the next product finds in the cache, 30.6 / 31.3 with the
-// sums.
+// blocks 404 / 393, with the encoding too 414 / 400, the backward 399 / 381, with
+// the sums 380 / 372; 4096 x 4096, whose gradients the next product finds in the
+// cache, 30.6 / 31.3 with the sums.
 
 // Chunk q of a row of g and of u (zeros past the row) to their blocks, the four
 // lanes of a block together.
@@ -355,7 +355,7 @@ struct EvidenceOperands {
 template <int DT>
 __device__ __forceinline__ float scale_left(float scale) {
   const float held = Elem<DT>::round(scale), c = scale / held;
-  return held != 0.0f && __builtin_isfinite(c) ? c : 1.0f;
+  return held != 0.0f && __builtin_isfinite(held) ? c : 1.0f;
 }
 
 // The backward with sums over the rows for the two binary layers that made g and u:
@@ -909,9 +909,10 @@ int launch_swiglu_backward_blocks(const void* dh, int dtype, const int8_t* gq, c
 }
 
 size_t swiglu_backward_blocks_sums_workspace(int64_t rows, int64_t cols) {
-  // (the chunks of other dtypes and layouts are swiglu_backward_sums_workspace's, of 256 rows)
   const int64_t chunk = swiglu::chunk_of(rows, cols), chunks = (rows + chunk - 1) / chunk;
-  return static_cast<size_t>(chunks * 2 * cols) * sizeof(float);
+  const size_t mine = static_cast<size_t>(chunks * 2 * cols) * sizeof(float);
+  const size_t other = swiglu_backward_sums_workspace(rows, cols);  // for other dtypes and layouts
+  return mine > other ? mine : other;
 }
 
 // sums as launch_swiglu_backward_sums has them; part: swiglu_backward_blocks_sums_workspace of space

@@ -261,6 +261,12 @@ class SwiGLUFn(Function):
         return grad_gate, grad_up, None, None
 
 
+class SwiGLUKeptFn(SwiGLUFn):
+    """SwiGLUFn with a checkpoint: its gradients have none of their own."""
+
+    backward = staticmethod(once_differentiable(SwiGLUFn.backward))
+
+
 def _cast(grad: Tensor | None, dtype: torch.dtype | None) -> Tensor | None:
     return None if grad is None or dtype is None else grad.to(dtype)
 
@@ -490,11 +496,13 @@ def swiglu_mlp_fusable(inputs: Tensor, gate, up, down) -> bool:
 
 
 def gated_fusable(inputs: Tensor, gate, up) -> bool:
-    """Whether ``GatedFn`` takes this block: a bf16 or fp16 input on the GPU."""
+    """Whether ``GatedFn`` takes this block: a bf16 or fp16 input on the GPU, both
+    layers' gradients side by side within the matrix kernels' 32-bit offsets."""
 
     sg, su = gate.surface, up.surface
+    tokens = inputs.numel() // max(sg.columns, 1)
     return (inputs.is_cuda and inputs.dtype in (torch.bfloat16, torch.float16) and inputs.dim() >= 1
-            and inputs.shape[-1] == sg.columns == su.columns and sg.rows == su.rows
+            and tokens * 4 * _eights(sg.rows) < 1 << 32 and inputs.shape[-1] == sg.columns == su.columns and sg.rows == su.rows
             and inputs.numel() > 0 and all(s.log_scale.is_cuda and s.log_scale.dtype in _SCALE_DTYPES for s in (sg, su)))
 
 
@@ -511,10 +519,12 @@ def swiglu(gate: Tensor, up: Tensor, *, checkpoint: bool = False) -> Tensor:
     blocks of 32 columns, 33 bytes for 32 elements: the value is the same, the
     gradients are those at the blocks' values (``nn.quantize_blocks``)."""
 
+    grad_on = torch.is_grad_enabled()
     if checkpoint:
         _no_tangent("swiglu with a checkpoint", gate, up)
-    grad_on = torch.is_grad_enabled()
-    return SwiGLUFn.apply(gate, up, grad_on, checkpoint and grad_on and (gate.requires_grad or up.requires_grad))
+        if grad_on and (gate.requires_grad or up.requires_grad):
+            return SwiGLUKeptFn.apply(gate, up, True, True)
+    return SwiGLUFn.apply(gate, up, grad_on, False)
 
 
 def qste_weight(surface: Surface) -> Tensor:

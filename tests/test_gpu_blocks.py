@@ -295,6 +295,32 @@ def test_gradients_against_differences():
     assert bool(((u.grad.double() - slope_u).abs() <= bound).all())
 
 
+def test_no_second_derivative():
+    """A gradient that reached the node with a graph of its own is refused; one without any (a linear loss's) gives a
+    gradient without one."""
+
+    from qste_amd import nn as qnn
+
+    gate, up = _randn((4, 64), torch.float32, 1).requires_grad_(), _randn((4, 64), torch.float32, 2)
+    grad, = torch.autograd.grad(qnn.swiglu(gate, up, checkpoint=True).sum(), gate, create_graph=True)
+    with pytest.raises(RuntimeError, match="does not require grad"):
+        grad.sum().backward()
+    loss = qnn.swiglu(gate, up, checkpoint=True).square().sum()
+    grad, = torch.autograd.grad(loss, gate, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiate twice"):
+        grad.sum().backward()
+
+
+def test_codes_below_the_least_read_as_nothing():
+    from qste_amd import nn as qnn
+
+    payload = torch.full((2, 40), 100, dtype=torch.int8, device=DEV)
+    codes = torch.tensor([[0, 6], [7, 133]], dtype=torch.uint8, device=DEV)
+    for dtype in DTYPES:
+        x = qnn.dequantize_blocks(qnn.Blocks8(payload, codes, dtype), torch.float32)
+        assert bool((x[0] == 0).all()) and bool((x[1, :32] == 100 * 2.0 ** -126).all()) and bool((x[1, 32:] == 100).all())
+
+
 def test_checkpoint_is_what_is_kept():
     """33 bytes for 32 elements, and nothing where no gradient is asked for."""
 

@@ -378,6 +378,26 @@ def test_backward_kernels(m, rows, cols, dtype, kept):
     assert torch.equal(again[1], evidence) and torch.equal(_bits(again[0]), _bits(dx))
 
 
+def test_scales_that_the_type_does_not_hold():
+    """A sample whose scale is past fp16's range, or below its least, has evidence of infinities and of zeros, as the
+    operand of that scale gives; the others' stay what they are."""
+
+    from qste_amd import kernels
+
+    gen = torch.Generator(device=DEV).manual_seed(5)
+    g, u, dh = (torch.randn(40, 32, generator=gen, device=DEV).half() for _ in range(3))
+    x, layers = _operands(40, 32, 64, torch.float16)
+    packed, scale = torch.cat((layers[0], layers[3])), torch.cat((layers[1], layers[4]))
+    payload, offset, xs = kernels.pack_affine_rows(x)
+    dh[3] = 0
+    want = kernels.gated_backward(dh, g, u, payload, offset, xs, packed, scale, 64)
+    xs[3] = 1e-12  # of no gradient: nothing changes
+    assert torch.equal(kernels.gated_backward(dh, g, u, payload, offset, xs, packed, scale, 64)[1], want[1])
+    xs[4] = 1e6
+    large = kernels.gated_backward(dh, g, u, payload, offset, xs, packed, scale, 64)
+    assert torch.equal(_bits(large[0]), _bits(want[0])) and not bool(torch.isfinite(large[1]).any())
+
+
 def test_backward_refusals():
     from qste_amd import kernels
 
@@ -656,6 +676,9 @@ def test_streams_and_graphs():
     with torch.cuda.graph(graph):
         captured = [kernels.gated_forward(t, *layers, 512)[0] for t in (small, large)]
         kept = kernels.gated_forward(large, *layers, 512, keep="blocks")
+        encoding = kernels.pack_affine_rows(large)
+        packed, scale = torch.cat((layers[0], layers[3])), torch.cat((layers[1], layers[4]))
+        back = kernels.gated_backward(kept[0], *kept[1:], *encoding, packed, scale, 512, need_bias=True)
     for seed in (5, 6, 7):
         gen = torch.Generator(device=DEV).manual_seed(seed)
         for t in (small, large):
@@ -666,3 +689,6 @@ def test_streams_and_graphs():
         assert all(torch.equal(a, b) for a, b in zip(captured, want))
         eager = kernels.gated_forward(large, *layers, 512, keep="blocks")
         assert torch.equal(kept[0], eager[0]) and torch.equal(kept[1].payload, eager[1].payload)
+        want = kernels.gated_backward(eager[0], *eager[1:], *kernels.pack_affine_rows(large), packed, scale, 512,
+                                      need_bias=True)
+        assert all(torch.equal(a, b) for a, b in zip(back, want))
