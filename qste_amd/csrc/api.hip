@@ -54,8 +54,8 @@ int mfma_evidence_t(const void*, int64_t, int, const uint8_t*, int64_t, const ui
 int64_t mfma_evidence_tiles(int64_t cols);
 bool mfma_backward_ok(const void*, int64_t, int, int64_t, int64_t, int64_t);
 EvidencePlan mfma_evidence_plan(int64_t, int64_t, int64_t, bool);
-int mfma_backward_pair(const void*, const void*, int64_t, int, const uint8_t*, int64_t, const uint16_t*, float*, const uint8_t*,
-                       int64_t, const uint16_t*, const uint8_t*, int64_t, void*, int64_t, int64_t, int64_t,
+int mfma_backward_pair(const void*, const void*, int64_t, int, const uint8_t*, int64_t, const uint16_t*, float*,
+                       const uint8_t*, int64_t, const uint16_t*, const uint8_t*, int64_t, void*, int64_t, int64_t, int64_t,
                        const float*, const float*, float*, const EvidencePlan&, float*, hipStream_t);
 int launch_pad_rows(const void*, void*, int64_t, int64_t, int64_t, hipStream_t);
 int launch_colsums_pad(const void*, int, const float*, int64_t, int64_t, int64_t, uint16_t*, float*, float*, float*,

@@ -47,7 +47,9 @@
 // blocks in pairs: the first half of a workgroup's are 16 rows each of the gate's
 // weights, the second half the same rows of up's, so that the gate is formed
 // where the waves' sums meet, and one launch with one reading of x takes the
-// place of three with two.
+// place of three with two.  Bound by its latency (a chain of loads, products and the
+// waves' meeting) as the layers are: us, this / the two layers and the gate, 4096
+// columns to 14336 features in bf16: 1 row 7.6 / 13.8, 16 rows 9.3 / 16.4.
 #include <type_traits>
 
 #include "common.hpp"
@@ -305,7 +307,9 @@ __global__ __launch_bounds__(THREADS, 1) void skinny_kernel(Args p) {
   };
 
   u32x4 W[NBW];
-  auto issue_w1 = [&](int c, int b) { return ld128(PAIR && b >= FB ? rb_up : rb, c < c_last ? boff[b] + 64u * static_cast<uint32_t>(c) : kOob); };
+  auto issue_w1 = [&](int c, int b) {
+    return ld128(PAIR && b >= FB ? rb_up : rb, c < c_last ? boff[b] + 64u * static_cast<uint32_t>(c) : kOob);
+  };
 
   f32x4 acc[NBW][MT];
 #pragma unroll

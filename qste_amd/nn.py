@@ -82,9 +82,10 @@ def gated(inputs: Tensor, gate, up, *, checkpoint: bool = False) -> Tensor:
     layers called one by one up to the order of the fp32 sums; their gate is rounded
     once, where the operators one by one round silu's value too.  With gradients it is one
     autograd node, whose backward runs the two layers as one; evidence and
-    scale gradients go where the layers' own would.  ``checkpoint`` keeps gate and up
-    for the backward in 8-bit blocks (``quantize_blocks``) in place of 16 bits.  fp32
-    runs layer by layer where it carries gradients."""
+    scale gradients go where the layers' own would; hooks of the layers do not run.
+    ``checkpoint`` keeps gate and up for the backward in 8-bit blocks
+    (``quantize_blocks``) in place of 16 bits.  Training layers with fp32 inputs run
+    one by one."""
 
     # a module's buffers and parts by their dicts: attributes of modules are looked up in Python, half a microsecond each
     try:
@@ -825,7 +826,8 @@ __all__ = [
     "CELU", "Dropout", "ELU", "EXACT_REPLACEMENTS", "GELU", "Hardsigmoid", "Hardswish", "Hardtanh",
     "LeakyReLU", "Mish", "REPLACEMENTS", "ReLU", "ReLU6", "SELU", "SMOOTH_REPLACEMENTS", "SiLU",
     "Sigmoid", "Softplus", "Tanh", "celu", "dropout", "elementwise", "elu", "gelu", "hardsigmoid", "swiglu", "swiglu_mlp",
-    "Blocks8", "TokenScores", "dequantize_blocks", "gated", "quantize_blocks", "distillation_loss", "distillation_loss_and_grad", "token_logprobs",
+    "Blocks8", "TokenScores", "dequantize_blocks", "distillation_loss", "distillation_loss_and_grad", "gated",
+    "quantize_blocks", "token_logprobs",
     "hardswish", "hardtanh", "leaky_relu", "mish", "packed", "packed_activations", "relu",
     "relu6", "relu_square", "replace", "selu", "sigmoid", "silu", "softplus", "tanh",
 ]
