@@ -74,15 +74,17 @@ def _require_gpu(*tensors: Tensor) -> torch.device:
     for t in tensors:
         if t is None:
             continue
-        if t.device.type != "cuda":
+        own = t.device  # asked for once: a new object each time, a quarter of a microsecond
+        if own == device:
+            continue
+        if own.type != "cuda":
             raise RuntimeError(
-                f"qste_amd kernels run on the GPU only; got a tensor on {t.device} "
+                f"qste_amd kernels run on the GPU only; got a tensor on {own} "
                 "(move the model to the ROCm device first)"
             )
-        if device is None:
-            device = t.device
-        elif t.device != device:
-            raise RuntimeError(f"tensors on different devices: {device} and {t.device}")
+        if device is not None:
+            raise RuntimeError(f"tensors on different devices: {device} and {own}")
+        device = own
     if device is None:
         raise RuntimeError("no tensor argument to place the kernel on")
     return device
@@ -116,15 +118,16 @@ def _packed_width(columns: int) -> int:
 
 
 def _check_packed(packed: Tensor, columns: int, rows: int | None = None) -> Tensor:
-    if packed.dtype != torch.uint8 or packed.dim() != 2:
+    shape = packed.shape
+    if packed.dtype != torch.uint8 or len(shape) != 2:
         raise ValueError("packed signs must be a rank-2 uint8 tensor")
-    if packed.shape[1] != _packed_width(columns):
+    if shape[1] != _packed_width(columns):
         raise ValueError(
-            f"packed sign width {packed.shape[1]} does not match {columns} columns "
+            f"packed sign width {shape[1]} does not match {columns} columns "
             f"(expected {_packed_width(columns)})"
         )
-    if rows is not None and packed.shape[0] != rows:
-        raise ValueError(f"packed signs have {packed.shape[0]} rows, expected {rows}")
+    if rows is not None and shape[0] != rows:
+        raise ValueError(f"packed signs have {shape[0]} rows, expected {rows}")
     return packed.contiguous()
 
 
@@ -958,7 +961,7 @@ def _layer_vector(t: Tensor | None, rows: int, what: str) -> Tensor | None:
         return None
     if t.shape != (rows,):
         raise ValueError(f"{what} has shape {tuple(t.shape)}, expected ({rows},)")
-    return t if t.dtype == torch.float32 and t.is_contiguous() else _f32(t)
+    return t if t.dtype is torch.float32 and t.is_contiguous() else _f32(t)
 
 
 def gated_forward(inputs: Tensor, gate: Tensor, gate_scale: Tensor, gate_bias: Tensor | None, up: Tensor,
@@ -982,12 +985,12 @@ def gated_forward(inputs: Tensor, gate: Tensor, gate_scale: Tensor, gate_bias: T
     rows = gate.shape[0]
     if up.shape[0] != rows:
         raise ValueError(f"gate has {rows} rows and up {up.shape[0]}")
-    gs, gb = _layer_vector(gate_scale, rows, "gate_scale"), _layer_vector(gate_bias, rows, "gate_bias")
-    us, ub = _layer_vector(up_scale, rows, "up_scale"), _layer_vector(up_bias, rows, "up_bias")
+    gs, us = _layer_vector(gate_scale, rows, "gate_scale"), _layer_vector(up_scale, rows, "up_scale")
+    gb = None if gate_bias is None else _layer_vector(gate_bias, rows, "gate_bias")
+    ub = None if up_bias is None else _layer_vector(up_bias, rows, "up_bias")
     x, gate, up = _aligned(inputs), _aligned(gate), _aligned(up)
-    shape = (*inputs.shape[:-1], rows)
     m = x.numel() // columns if columns else _leading(inputs)
-    out = torch.empty(shape, dtype=inputs.dtype, device=device)
+    out = torch.empty((*x.shape[:-1], rows), dtype=x.dtype, device=device)
     g = u = None
     values, blocks = (None, None), (None, None, None, None)
     if keep == "values":

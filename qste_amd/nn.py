@@ -90,15 +90,15 @@ def gated(inputs: Tensor, gate, up, *, checkpoint: bool = False) -> Tensor:
     # a module's buffers and parts by their dicts: attributes of modules are looked up in Python, half a microsecond each
     try:
         served, other = gate._buffers, up._buffers
-        trained = all("surface" in m._modules and "bias" in m._parameters for m in (gate, up))
     except AttributeError:
-        served, other, trained = {}, {}, False
+        served, other = {}, {}
     if "packed_sign" in served and "packed_sign" in other and "bias" in served and "bias" in other:
         if gate.in_features != up.in_features:
             raise ValueError(f"gate takes {gate.in_features} columns and up {up.in_features}")
-        return kernels.gated_forward(inputs.detach(), served["packed_sign"], served["scale"], served["bias"],
-                                     other["packed_sign"], other["scale"], other["bias"], gate.in_features)[0]
-    if not trained:
+        x = inputs.detach() if inputs.requires_grad else inputs
+        return kernels.gated_forward(x, served["packed_sign"], served["scale"], served["bias"], other["packed_sign"],
+                                     other["scale"], other["bias"], gate.in_features)[0]
+    if not all("surface" in getattr(m, "_modules", ()) and "bias" in m._parameters for m in (gate, up)):
         raise TypeError("gated takes two QSTELinear or two PackedLinear layers, got "
                         f"{type(gate).__name__} and {type(up).__name__}")
     from .functional import GatedFn, _autocast, gated_fusable
