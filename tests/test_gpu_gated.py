@@ -378,6 +378,29 @@ def test_backward_kernels(m, rows, cols, dtype, kept):
     assert torch.equal(again[1], evidence) and torch.equal(_bits(again[0]), _bits(dx))
 
 
+@pytest.mark.parametrize("kept", ["values", "blocks"])
+def test_past_32_bit_offsets(kept):
+    """Outputs of 4.6 GB and gradients of 9.2: rows that repeat have results that repeat, bit for bit, wherever they lie
+    (256 rows are whole tiles, and whole rounds of the backward's waves)."""
+
+    from qste_amd import kernels
+
+    repeats, features = 625, 14336
+    x, layers = _operands(256, features, 64, torch.bfloat16)
+    h, g, u = kernels.gated_forward(x.repeat(repeats, 1), *layers, 64, keep=kept)
+    assert h.numel() * 2 > 1 << 32
+    parts = (h, g, u) if kept == "values" else (h, g.payload, g.codes, u.payload, u.codes)
+    for t in parts:
+        assert torch.equal(t[-256:], t[:256])
+    _, offset, scale = kernels.pack_affine_rows(x)
+    grads, evidence, _ = kernels._gated_grads(h, g, u, offset.repeat(repeats), scale.repeat(repeats))
+    for t in (grads, evidence):
+        assert torch.equal(t[-256:], t[:256]) and bool(t[:256].any())
+    small = (g[:256], u[:256]) if kept == "values" else [type(b)(b.payload[:256], b.codes[:256], b.dtype) for b in (g, u)]
+    want = kernels._gated_grads(h[:256].contiguous(), *small, offset, scale)
+    assert torch.equal(grads[:256], want[0]) and torch.equal(evidence[:256], want[1])
+
+
 def test_scales_that_the_type_does_not_hold():
     """A sample whose scale is past fp16's range, or below its least, has evidence of infinities and of zeros, as the
     operand of that scale gives; the others' stay what they are."""
