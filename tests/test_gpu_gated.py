@@ -715,3 +715,43 @@ def test_streams_and_graphs():
         want = kernels.gated_backward(eager[0], *eager[1:], *kernels.pack_affine_rows(large), packed, scale, 512,
                                       need_bias=True)
         assert all(torch.equal(a, b) for a, b in zip(back, want))
+
+
+@pytest.mark.parametrize("rows,checkpoint,dtype", [(192, True, torch.bfloat16), (203, True, torch.float16),
+                                                   (192, False, torch.bfloat16)])
+def test_node_captured(rows, checkpoint, dtype):
+    """A training step of the block in a graph: every replay, with eager steps and synchronizations between, equals the
+    eager step on what the inputs hold then."""
+
+    import qste_amd as qste
+
+    gate, up = _pair(rows, 96, 12, bias=True, dtype=dtype)
+    x = torch.randn(70, 96, device=DEV, generator=torch.Generator(device=DEV).manual_seed(1)).to(dtype).requires_grad_()
+    w = torch.randn(70, rows, device=DEV, generator=torch.Generator(device=DEV).manual_seed(2)).to(dtype)
+    leaves = (x, gate.surface.log_scale, up.surface.log_scale, gate.bias, up.bias)
+
+    def step():
+        h = qste.nn.gated(x, gate, up, checkpoint=checkpoint)
+        grads = torch.autograd.grad(h, leaves, w)
+        return (h.detach(), *grads, gate.evidence.pop(), up.evidence.pop())
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for seed in (3, 4, 5, 6):
+        gen = torch.Generator(device=DEV).manual_seed(seed)
+        x.detach().copy_(torch.randn(70, 96, device=DEV, generator=gen))
+        w.copy_(torch.randn(70, rows, device=DEV, generator=gen))
+        graph.replay()
+        torch.cuda.synchronize()
+        kept = [t.clone() for t in captured]
+        want = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(kept, want))
+        assert bool(want[0].any()) and bool(want[-1].any())
