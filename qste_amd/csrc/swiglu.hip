@@ -242,7 +242,7 @@ __global__ __launch_bounds__(kThreads) void forward_blocks_kernel(const typename
     g8.values(gv);
     u8.values(uv);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) hv[i] = forward_one<DT>(gv[i], uv[i]);
+    for (int i = 0; i < 8; ++i) hv[i] = forward_fast<DT>(gv[i], uv[i]);
     blocks::store8<DT, ONCE>(h + p.at(), hv);
   }
 }

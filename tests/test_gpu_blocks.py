@@ -295,6 +295,23 @@ def test_gradients_against_differences():
     assert bool(((u.grad.double() - slope_u).abs() <= bound).all())
 
 
+def test_value_of_every_gate():
+    """The value with a checkpoint is torch's, bit for bit, at every bf16 gate: each has a rounding of its own."""
+
+    import torch.nn.functional as F
+
+    from qste_amd import nn as qnn
+
+    every = torch.arange(-32768, 32768, dtype=torch.int32, device=DEV).to(torch.int16)
+    gate = every.view(torch.bfloat16).reshape(256, 256).requires_grad_()
+    for seed in (1, 2):
+        up = torch.ones_like(gate.detach()) if seed == 1 else _randn((256, 256), torch.bfloat16, seed)
+        got, want = qnn.swiglu(gate, up, checkpoint=True).detach(), (F.silu(gate) * up).detach()
+        number = ~torch.isnan(want)
+        assert torch.equal(torch.isnan(got), ~number) and torch.equal(got[number].view(torch.int16),
+                                                                      want[number].view(torch.int16))
+
+
 def test_no_second_derivative():
     """A gradient that reached the node with a graph of its own is refused; one without any (a linear loss's) gives a
     gradient without one."""
