@@ -363,6 +363,12 @@ __device__ __forceinline__ float scale_left(float scale) {
 // workgroup takes 512 columns, eight a lane, of `chunk` rows, each wave every fourth
 // of them; its waves' sums meet in LDS in wave order, and the chunks' are added in
 // their order by sum_partials_kernel.
+// The chunks of kTogether workgroups lie row by row between one another, so that what
+// they read and write at one time are neighbouring rows.  us, GATED, chunks of up to
+// 256 rows by themselves / of up to 64, eight together: 8192 x 14336 308 / 266
+// (4.6 -> 5.3 TB/s), 16384 x 14336 574 / 533, 4096 x 4096 43.6 / 39.8; 4, 16 and 64 together
+// 268, 274 and 306 at the first size.
+constexpr unsigned kTogether = 8;
 template <int DT, class SRC, bool GATED, bool ONCE>
 __global__ __launch_bounds__(kThreads) void backward_columns_kernel(
     const uint16_t* __restrict__ dh, SRC g, SRC u, uint16_t* __restrict__ dg, uint16_t* __restrict__ du,
@@ -372,8 +378,10 @@ __global__ __launch_bounds__(kThreads) void backward_columns_kernel(
   __shared__ float red[kWaves][kSums][512];
   const int lane = static_cast<int>(threadIdx.x) % kWave, wave = static_cast<int>(threadIdx.x) / kWave;
   const int64_t base = static_cast<int64_t>(blockIdx.x) * 512, c = base + 8 * lane, block = c / blocks::kBlock;
-  const int64_t first = static_cast<int64_t>(blockIdx.y) * chunk;
-  const int64_t last = first + chunk < rows ? first + chunk : rows;
+  const unsigned before = blockIdx.y / kTogether * kTogether;
+  const int64_t apart = gridDim.y - before < kTogether ? gridDim.y - before : kTogether;
+  const int64_t begin = static_cast<int64_t>(before) * chunk;
+  const int64_t last = begin + apart * chunk < rows ? begin + apart * chunk : rows, step = apart * kWaves;
   struct Held {
     blocks::Eight<DT> dh;
     typename SRC::Held g, u;
@@ -414,15 +422,15 @@ __global__ __launch_bounds__(kThreads) void backward_columns_kernel(
     }
   };
   if (c < cols) {
-    int64_t t = first + wave;
-    for (; t + (kDeep - 1) * kWaves < last; t += kDeep * kWaves) {  // several rows' loads in flight
+    int64_t t = begin + (blockIdx.y - before) + wave * apart;
+    for (; t + (kDeep - 1) * step < last; t += kDeep * step) {  // several rows' loads in flight
       Held r[kDeep];
 #pragma unroll
-      for (int k = 0; k < kDeep; ++k) r[k] = load(t + k * kWaves);
+      for (int k = 0; k < kDeep; ++k) r[k] = load(t + k * step);
 #pragma unroll
-      for (int k = 0; k < kDeep; ++k) take(t + k * kWaves, r[k]);
+      for (int k = 0; k < kDeep; ++k) take(t + k * step, r[k]);
     }
-    for (; t < last; t += kWaves) take(t, load(t));
+    for (; t < last; t += step) take(t, load(t));
   }
 #pragma unroll
   for (int k = 0; k < kSums; ++k)
@@ -839,13 +847,13 @@ void run_backward_blocks(const void* dh, const Pair& kept, void* dg, void* du, i
 }
 
 // Rows of a chunk: as many as leave two workgroups a CU, from 16 (four a wave)
-// to 256 (the chunks' sums are then under 1% of the bytes).  us a call, chunks of
-// 256 rows / of the rule's: 250 x 2048 34.6 / 19.0, 4096 x 4096 42 / 31, 8192 x 14336
-// the same.
+// to 64 (the chunks' sums are then 4% of the bytes).  us a call, chunks of 256
+// rows / of the rule's: 250 x 2048 34.6 / 19.0, 4096 x 4096 42 / 29; of 32 at the most / the
+// rule's: 4096 x 4096 40.7 / 39.8 (GATED), 8192 x 14336 268 / 266.
 inline int chunk_of(int64_t rows, int64_t cols) {
   const int64_t groups = (cols + 511) / 512;
   int chunk = 16;
-  while (chunk < 256 && (rows + 2 * chunk - 1) / (2 * chunk) * groups >= 512) chunk *= 2;
+  while (chunk < 64 && (rows + 2 * chunk - 1) / (2 * chunk) * groups >= 512) chunk *= 2;
   while ((rows + chunk - 1) / chunk > 65535) chunk *= 2;  // what a grid's second dimension holds
   return chunk;
 }
