@@ -26,8 +26,8 @@
 // With a checkpoint, what autograd keeps of g and u is 8 bits an element
 // (blocks.hpp): the forward writes them beside h from the values it holds, and
 // the backward takes the g and u that they stand for.  HBM-bound like the
-// rest: 16384 x 14336 in bf16 read and write 1.89 GB forward (1.41 without), 406 us,
-// and 1.89 GB backward (2.35 without), 373 us: 4.7 and 5.1 TB/s, a copy's rate being 5.0.
+// rest: 16384 x 14336 in bf16 read and write 1.89 GB forward (1.41 without), 385 us,
+// and 1.89 GB backward (2.35 without), 372 us: 4.9 and 5.1 TB/s, a copy's rate being 5.0.
 #include <type_traits>
 
 #include "blocks.hpp"
@@ -135,7 +135,7 @@ struct Pair {
 // (blocks::streamed).  us, kept / streamed, 16384 x 14336 in bf16: the forward with
 // blocks 404 / 393, with the encoding too 414 / 400, the backward 399 / 381, with
 // the sums 380 / 372; 4096 x 4096, whose gradients the next product finds in the
-// cache, 30.6 / 31.3 with the sums.
+// cache, 30.6 / 31.3 with the sums (all before later steps took a little off).
 
 // Chunk q of a row of g and of u (zeros past the row) to their blocks, the four
 // lanes of a block together.
