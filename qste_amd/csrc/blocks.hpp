@@ -194,22 +194,21 @@ struct Blocks {
 };
 
 // Work is handed out by quarters of blocks, eight values to a thread: quarter j
-// (of rows * per_row * 4, per_row the blocks of a row) as its row and first
-// column.  With cols a multiple of 32 the quarters lie end to end.
+// (of rows * per_row * 4, per_row the blocks of a row).  With cols a multiple of 32
+// the quarters lie end to end.  A row may have more than 2^31 columns.
 struct Quarter {
-  int64_t row, block;  // block: its index in the codes
-  int col;
+  int64_t block;  // its block's index in the codes
   __device__ __forceinline__ Quarter(int64_t j, int64_t cols, int64_t per_row) {
     block = j >> 2;
     if (cols % kBlock == 0) {
-      row = 0;  // one long row
-      col = 0;
       at_ = 8 * j;
       whole_ = true;
     } else {
       // 32-bit where it reaches: a 64-bit division is several times as long
-      row = (block >> 32) == 0 ? static_cast<int64_t>(static_cast<uint32_t>(block) / static_cast<uint32_t>(per_row)) : block / per_row;
-      col = static_cast<int>((block - row * per_row) * kBlock + 8 * (j & 3));
+      const int64_t row = (block >> 32) == 0
+                              ? static_cast<int64_t>(static_cast<uint32_t>(block) / static_cast<uint32_t>(per_row))
+                              : block / per_row;
+      const int64_t col = (block - row * per_row) * kBlock + 8 * (j & 3);
       at_ = row * cols + col;
       whole_ = col < cols;
     }
