@@ -478,6 +478,12 @@ class SwiGLUMLPFn(Function):
                 _cast(gb_u, bu), None, _through_scale(gs_d, e_d, sd), _cast(gb_d, bd), None, None, None)
 
 
+class SwiGLUMLPKeptFn(SwiGLUMLPFn):
+    """SwiGLUMLPFn with a checkpoint: its gradients have none of their own."""
+
+    backward = staticmethod(once_differentiable(SwiGLUMLPFn.backward))
+
+
 # log-scale dtypes the row-scale kernels take (surface.row_scale)
 _SCALE_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 

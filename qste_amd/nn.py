@@ -126,7 +126,7 @@ def swiglu_mlp(inputs: Tensor, gate, up, down, *, checkpoint: bool = False) -> T
     the layer-by-layer composition.  With ``checkpoint`` gate and up are one
     kernel (``gated``), which keeps them for the backward in 8-bit blocks."""
 
-    from .functional import SwiGLUMLPFn, _autocast, swiglu_mlp_fusable
+    from .functional import SwiGLUMLPFn, SwiGLUMLPKeptFn, _autocast, swiglu_mlp_fusable
 
     x = _autocast(inputs)
     if not swiglu_mlp_fusable(x, gate, up, down):
@@ -136,9 +136,11 @@ def swiglu_mlp(inputs: Tensor, gate, up, down, *, checkpoint: bool = False) -> T
     surfaces = (gate.surface, up.surface, down.surface)
     for s in surfaces:
         s.note_forward()
-    y = SwiGLUMLPFn.apply(x, gate.surface.packed_sign, gate.surface.log_scale, gate.bias, up.surface.packed_sign,
-                          up.surface.log_scale, up.bias, down.surface.packed_sign, down.surface.log_scale, down.bias,
-                          surfaces, checkpoint, torch.is_grad_enabled())
+    grad_on = torch.is_grad_enabled()
+    node = SwiGLUMLPKeptFn if checkpoint and grad_on else SwiGLUMLPFn
+    y = node.apply(x, gate.surface.packed_sign, gate.surface.log_scale, gate.bias, up.surface.packed_sign,
+                   up.surface.log_scale, up.bias, down.surface.packed_sign, down.surface.log_scale, down.bias,
+                   surfaces, checkpoint, grad_on)
     return _mark_activation_input(y)
 
 
