@@ -95,6 +95,7 @@ def gated(inputs: Tensor, gate, up, *, checkpoint: bool = False) -> Tensor:
     if "packed_sign" in served and "packed_sign" in other and "bias" in served and "bias" in other:
         if gate.in_features != up.in_features:
             raise ValueError(f"gate takes {gate.in_features} columns and up {up.in_features}")
+        _no_tangent("gated", inputs)
         x = inputs.detach() if inputs.requires_grad else inputs
         return kernels.gated_forward(x, served["packed_sign"], served["scale"], served["bias"], other["packed_sign"],
                                      other["scale"], other["bias"], gate.in_features)[0]
