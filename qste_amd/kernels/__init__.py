@@ -857,7 +857,8 @@ def _rows_of(t: Tensor) -> tuple[int, int]:
 
 
 def quantize_blocks(values: Tensor) -> Blocks8:
-    """``values`` (fp32, fp16 or bf16, any shape but a scalar's) in 8-bit blocks along the last dimension."""
+    """``values`` (fp32, fp16 or bf16, any shape but a scalar's) in 8-bit blocks along the last dimension;
+    without a gradient, as every call here."""
 
     device = _require_gpu(values)
     code = _dtype_code(values)

@@ -26,7 +26,7 @@ from torch.autograd import Function
 
 from . import kernels
 from .functional import swiglu
-from .kernels import Blocks8, dequantize_blocks, quantize_blocks
+from .kernels import Blocks8, dequantize_blocks
 from .losses import TokenScores, _no_tangent, distillation_loss, distillation_loss_and_grad, token_logprobs
 
 # The originals, bound before ``packed_activations`` can patch them: the
@@ -71,6 +71,17 @@ def _mark_activation_input(value: Tensor) -> Tensor:
 
 def _take_activation_input(value: Tensor) -> Tensor | None:
     return value if getattr(value, "_qste_activation_input", False) else None
+
+
+def quantize_blocks(values: Tensor) -> Blocks8:
+    """``values`` (fp32, fp16 or bf16, any shape but a scalar's) in 8-bit blocks along the last dimension;
+    ``dequantize_blocks`` reads them back.
+
+    What it returns carries no gradient: ``values`` that ask for one are taken as constants, as a backward's saved
+    values are.  Forward-mode tangents are refused."""
+
+    _no_tangent("quantize_blocks", values)
+    return kernels.quantize_blocks(values)
 
 
 def gated(inputs: Tensor, gate, up, *, checkpoint: bool = False) -> Tensor:

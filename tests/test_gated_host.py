@@ -30,3 +30,10 @@ def test_tangents_of_packed_layers_are_refused():
                 qste.nn.gated(torch.zeros(2, 64), layer, layer)
     with pytest.raises(RuntimeError, match="GPU only"):
         qste.nn.gated(torch.zeros(2, 64), layer, layer)
+
+
+def test_tangents_of_values_to_quantize_are_refused():
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(torch.zeros(2, 64), torch.ones(2, 64))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            qste.nn.quantize_blocks(dual)
