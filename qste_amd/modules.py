@@ -15,7 +15,7 @@ from torch import Tensor
 from . import kernels
 from .config import QSTEConfig, coerce_config
 from .functional import qste_embedding, qste_linear, qste_weight
-from .nn import _mark_activation_input
+from .nn import _LAYER_FORWARDS, _mark_activation_input
 from .surface import Surface
 
 
@@ -91,6 +91,9 @@ class PackedLinear(nn.Module):
 
     def extra_repr(self) -> str:
         return f"in_features={self.in_features}, out_features={self.out_features}"
+
+
+_LAYER_FORWARDS.update((QSTELinear.forward, PackedLinear.forward))
 
 
 class QSTEEmbedding(nn.Module):

@@ -84,6 +84,17 @@ def quantize_blocks(values: Tensor) -> Blocks8:
     return kernels.quantize_blocks(values)
 
 
+# QSTELinear's and PackedLinear's forward (put here where they are defined)
+_LAYER_FORWARDS: set = set()
+
+
+def _plain(layer) -> bool:
+    """Whether a layer computes what QSTELinear or PackedLinear does: a forward of a subclass's or an instance's own
+    is called, not stood for."""
+
+    return getattr(layer.forward, "__func__", None) in _LAYER_FORWARDS
+
+
 def gated(inputs: Tensor, gate, up, *, checkpoint: bool = False) -> Tensor:
     """``swiglu(gate(inputs), up(inputs))``, the gated feed-forward block, of two
     converted layers (QSTELinear) or two packed ones (PackedLinear, which carry no
@@ -93,7 +104,8 @@ def gated(inputs: Tensor, gate, up, *, checkpoint: bool = False) -> Tensor:
     layers called one by one up to the order of the fp32 sums; their gate is rounded
     once, where the operators one by one round silu's value too.  With gradients it is one
     autograd node, whose backward runs the two layers as one; evidence and
-    scale gradients go where the layers' own would; hooks of the layers do not run.
+    scale gradients go where the layers' own would; hooks of the layers do not run, and layers with a
+    ``forward`` of their own (a subclass's, or set on the layer) are called one by one.
     ``checkpoint`` keeps gate and up for the backward in 8-bit blocks
     (``quantize_blocks``) in place of 16 bits.  Training layers with fp32 inputs run
     one by one."""
@@ -103,16 +115,19 @@ def gated(inputs: Tensor, gate, up, *, checkpoint: bool = False) -> Tensor:
         served, other = gate._buffers, up._buffers
     except AttributeError:
         served, other = {}, {}
-    if "packed_sign" in served and "packed_sign" in other and "bias" in served and "bias" in other:
+    packed = "packed_sign" in served and "packed_sign" in other and "bias" in served and "bias" in other
+    if not packed and not all("surface" in getattr(m, "_modules", ()) and "bias" in m._parameters for m in (gate, up)):
+        raise TypeError("gated takes two QSTELinear or two PackedLinear layers, got "
+                        f"{type(gate).__name__} and {type(up).__name__}")
+    if not (_plain(gate) and _plain(up)):
+        return swiglu(gate(inputs), up(inputs), checkpoint=checkpoint)
+    if packed:
         if gate.in_features != up.in_features:
             raise ValueError(f"gate takes {gate.in_features} columns and up {up.in_features}")
         _no_tangent("gated", inputs)
         x = inputs.detach() if inputs.requires_grad else inputs
         return kernels.gated_forward(x, served["packed_sign"], served["scale"], served["bias"], other["packed_sign"],
                                      other["scale"], other["bias"], gate.in_features)[0]
-    if not all("surface" in getattr(m, "_modules", ()) and "bias" in m._parameters for m in (gate, up)):
-        raise TypeError("gated takes two QSTELinear or two PackedLinear layers, got "
-                        f"{type(gate).__name__} and {type(up).__name__}")
     from .functional import GatedFn, _autocast, gated_fusable
 
     x = _autocast(inputs)
@@ -134,14 +149,15 @@ def swiglu_mlp(inputs: Tensor, gate, up, down, *, checkpoint: bool = False) -> T
     scale gradients as the three layers and the gate called one by one; for
     bf16 inputs on the GPU with d and ffn multiples of 64 the whole MLP is
     one autograd node whose input gradient is one product over the gate and
-    up layers, rounded once (``functional.SwiGLUMLPFn``).  Anything else is
-    the layer-by-layer composition.  With ``checkpoint`` gate and up are one
-    kernel (``gated``), which keeps them for the backward in 8-bit blocks."""
+    up layers, rounded once (``functional.SwiGLUMLPFn``).  Anything else, layers
+    with a ``forward`` of their own among it, is the layer-by-layer composition.
+    With ``checkpoint`` gate and up are one kernel (``gated``), which keeps them
+    for the backward in 8-bit blocks."""
 
     from .functional import SwiGLUMLPFn, SwiGLUMLPKeptFn, _autocast, swiglu_mlp_fusable
 
     x = _autocast(inputs)
-    if not swiglu_mlp_fusable(x, gate, up, down):
+    if not all(map(_plain, (gate, up, down))) or not swiglu_mlp_fusable(x, gate, up, down):
         if checkpoint:
             return down(gated(inputs, gate, up, checkpoint=True))
         return down(swiglu(gate(inputs), up(inputs)))

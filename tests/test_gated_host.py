@@ -37,3 +37,37 @@ def test_tangents_of_values_to_quantize_are_refused():
         dual = forward_ad.make_dual(torch.zeros(2, 64), torch.ones(2, 64))
         with pytest.raises(NotImplementedError, match="forward-mode"):
             qste.nn.quantize_blocks(dual)
+
+
+class _Doubling(qste.PackedLinear):
+    """A packed layer with a forward of its own."""
+
+    calls = 0
+
+    def forward(self, inputs):
+        self.calls += 1
+        return inputs[..., :self.out_features] * 2
+
+
+class _Named(qste.PackedLinear):
+    """A packed layer that adds a name and no forward."""
+
+    name = "named"
+
+
+def test_a_forward_of_its_own_is_called(monkeypatch):
+    """A subclass's forward, and one set on a layer, run: the block's kernel does not stand for them."""
+
+    gates = []
+    monkeypatch.setattr(qste.nn, "swiglu", lambda g, u, *, checkpoint=False: gates.append((g, u, checkpoint)) or g * u)
+    x = torch.ones(2, 64)
+    packed, scale = torch.zeros(8, 8, dtype=torch.uint8), torch.ones(8)
+    own, plain = _Doubling(packed, scale, 64, None), _Doubling(packed, scale, 64, None)
+    assert torch.equal(qste.nn.gated(x, own, plain, checkpoint=True), torch.full((2, 8), 4.0))
+    assert own.calls == plain.calls == 1 and gates.pop()[2]
+    wrapped = _packed()
+    wrapped.forward = lambda inputs: inputs[..., :8] * 3
+    assert torch.equal(qste.nn.gated(x, own, wrapped), torch.full((2, 8), 6.0)) and not gates.pop()[2]
+    assert not gates
+    with pytest.raises(RuntimeError, match="GPU only"):  # a subclass without one takes the kernel
+        qste.nn.gated(x, _Named(packed, scale, 64, None), _packed())
