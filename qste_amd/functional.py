@@ -489,11 +489,13 @@ _SCALE_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 
 
 def swiglu_mlp_fusable(inputs: Tensor, gate, up, down) -> bool:
-    """Whether ``SwiGLUMLPFn`` takes this MLP: bf16 input on the GPU, the
-    gate and up layers d -> ffn and the down layer ffn -> d, d and ffn
-    multiples of 64."""
+    """Whether ``SwiGLUMLPFn`` takes this MLP: training layers (packed ones have
+    no surface), bf16 input on the GPU, the gate and up layers d -> ffn and the
+    down layer ffn -> d, d and ffn multiples of 64."""
 
-    sg, su, sd = gate.surface, up.surface, down.surface
+    sg, su, sd = (getattr(m, "surface", None) for m in (gate, up, down))
+    if sg is None or su is None or sd is None:
+        return False
     d, ffn = sg.columns, sg.rows
     return (inputs.is_cuda and inputs.dtype == torch.bfloat16 and inputs.dim() >= 1 and inputs.shape[-1] == d
             and su.columns == d and su.rows == ffn and sd.columns == ffn and sd.rows == d

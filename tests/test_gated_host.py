@@ -71,3 +71,12 @@ def test_a_forward_of_its_own_is_called(monkeypatch):
     assert not gates
     with pytest.raises(RuntimeError, match="GPU only"):  # a subclass without one takes the kernel
         qste.nn.gated(x, _Named(packed, scale, 64, None), _packed())
+
+
+def test_mlp_of_packed_layers_goes_layer_by_layer():
+    """What swiglu_mlp says of everything that its node does not take: an exported model's layers reach the kernels."""
+
+    gate, up, down = _packed(64, 128), _packed(64, 128), _packed(128, 64)
+    for checkpoint in (False, True):
+        with pytest.raises(RuntimeError, match="GPU only"):
+            qste.nn.swiglu_mlp(torch.zeros(2, 128), gate, up, down, checkpoint=checkpoint)

@@ -81,3 +81,29 @@ def test_no_second_derivative_of_the_gated_block():
         grad, = torch.autograd.grad(loss, x, create_graph=True)
         with pytest.raises(RuntimeError, match="differentiate twice"):
             grad.float().square().sum().backward()
+
+
+@pytest.mark.parametrize("checkpoint", [False, True])
+@pytest.mark.parametrize("d,ffn,dtype", [(64, 192, torch.bfloat16), (72, 200, torch.float16)])
+def test_mlp_trained_then_served(d, ffn, dtype, checkpoint):
+    """A model written with swiglu_mlp, exported: its packed layers give what its training layers give."""
+
+    import qste_amd as qste
+
+    class MLP(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.gate, self.up, self.down = _layer(ffn, d, 1, True), _layer(ffn, d, 2), _layer(d, ffn, 3)
+
+        def forward(self, x):
+            return qste.nn.swiglu_mlp(x, self.gate, self.up, self.down, checkpoint=checkpoint)
+
+    model = MLP()
+    x = _randn((150, d), dtype, 4)
+    with torch.no_grad():
+        want = qste.nn.gated(x, model.gate, model.up) if checkpoint else qste.nn.swiglu(model.gate(x), model.up(x))
+        want = model.down(want)
+    served = qste.export_packed(model)
+    assert isinstance(served.down, qste.PackedLinear)
+    got = served(x)
+    assert not got.requires_grad and torch.equal(got, want)
