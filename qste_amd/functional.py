@@ -352,7 +352,9 @@ class GatedFn(Function):
             scales, keep = _halves(scale_gu, ffn), "blocks" if checkpoint else "values"
         h, g, u = kernels.gated_forward(flat, signs[0], scales[0], biases[0], signs[1], scales[1], biases[1], d, keep=keep)
         if grad_on:
-            payload_x, aux_x = _encoding_of(inputs, flat, d)
+            # encoded here, where both layers are: not what is remembered of a tensor by its identity, which a write
+            # that its version does not count (a graph's replay, one through .data) would leave behind
+            payload_x, aux_x = encode_activation(flat)
             more = (payload_x, aux_x, packed_g, packed_u, scale_gu, e)
             if checkpoint:
                 _save_kept(ctx, g, u, *more)
@@ -435,7 +437,8 @@ class SwiGLUMLPFn(Function):
         scale_d, e_d = kernels.row_scale(log_d, sd.cfg.scale_min, sd.cfg.scale_max)
         y = kernels.packed_linear_affine(h, packed_d, scale_d, bias_d, ffn)
         if grad_on:
-            payload_x, aux_x = _encoding_of(inputs, flat, d)
+            # (with a checkpoint as GatedFn does)
+            payload_x, aux_x = encode_activation(flat) if checkpoint else _encoding_of(inputs, flat, d)
             aux_h = kernels.stacked_pair(enc[1], enc[2])
             more = (payload_x, aux_x, enc[0], aux_h, packed_g, scale_g, packed_u, scale_u, packed_d, scale_d, e_g, e_u,
                     e_d)

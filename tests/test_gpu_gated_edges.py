@@ -107,3 +107,65 @@ def test_mlp_trained_then_served(d, ffn, dtype, checkpoint):
     assert isinstance(served.down, qste.PackedLinear)
     got = served(x)
     assert not got.requires_grad and torch.equal(got, want)
+
+
+@pytest.mark.parametrize("call", ["gated", "gated kept", "mlp kept"])
+def test_the_input_as_it_is_now(call):
+    """A forward whose backward never came, a write to the input that its version does not count, a forward with a
+    backward: its gradients are those of a new tensor of the same values."""
+
+    import qste_amd as qste
+
+    layers = [_layer(192, 64, 1), _layer(192, 64, 2)]
+    if call == "mlp kept":
+        layers.append(_layer(64, 192, 6))
+    x, other = (_randn((30, 64), torch.bfloat16, seed) for seed in (3, 4))
+
+    def forward(t):
+        return (qste.nn.gated(t, *layers, checkpoint=call == "gated kept") if len(layers) == 2
+                else qste.nn.swiglu_mlp(t, *layers, checkpoint=True))
+
+    w = _randn(forward(x).shape, torch.bfloat16, 5)
+    x.data.copy_(other)
+    results = []
+    for t in (x, other):
+        for layer in layers:
+            layer.surface.reset_tracking()
+            layer.surface.log_scale.grad = None
+        forward(t).backward(w)
+        results.append([layer.evidence.pop() for layer in layers] + [layer.surface.log_scale.grad for layer in layers])
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+def test_captured_after_a_forward_alone():
+    """A graph of a step, captured after a forward of the same input whose backward never came, encodes its input
+    itself: every replay equals the eager step."""
+
+    import qste_amd as qste
+
+    gate, up = _layer(96, 64, 1), _layer(96, 64, 2)
+    x, w = _randn((30, 64), torch.bfloat16, 3), _randn((30, 96), torch.bfloat16, 4)
+    leaves = gate.surface.log_scale, up.surface.log_scale
+
+    def step():
+        grads = torch.autograd.grad(qste.nn.gated(x, gate, up, checkpoint=True), leaves, w)
+        return (*grads, gate.evidence.pop(), up.evidence.pop())
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+        qste.nn.gated(x, gate, up, checkpoint=True)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    for layer in (gate, up):
+        layer.surface.reset_tracking()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for seed in (5, 6, 7):
+        x.copy_(_randn((30, 64), torch.bfloat16, seed))
+        graph.replay()
+        torch.cuda.synchronize()
+        kept = [t.clone() for t in captured]
+        assert all(torch.equal(a, b) for a, b in zip(kept, step()))
