@@ -276,6 +276,10 @@ int qste_clock_probe(int64_t* out, int64_t spins, void* stream);
  * compute units, maximum shader clock (kHz), memory clock (kHz), LDS bytes
  * per compute unit.  No counterpart in the reference. */
 int qste_device_info(int64_t* out);
+/* The number of the graph capture that `stream` records into, 0 for none: work
+ * recorded into a capture has not run, so its outputs are of that capture alone.
+ * No counterpart in the reference. */
+uint64_t qste_capture_id(void* stream);
 int qste_coordinate_update(const float* evidence, int8_t* coordinate, uint8_t* packed,
                            int8_t* moment_q, uint16_t* moment_scale, uint16_t* row_v,
                            uint16_t* col_v, int64_t rows, int64_t cols, double beta1,

@@ -1029,6 +1029,16 @@ int qste_device_info(int64_t* out) {
   return device_info(out);
 }
 
+uint64_t qste_capture_id(void* stream) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (hipStreamGetCaptureInfo(as_stream(stream), &status, &id) != hipSuccess) {
+    (void)hipGetLastError();
+    return 0;
+  }
+  return status == hipStreamCaptureStatusNone ? 0 : id;
+}
+
 int qste_coordinate_update(const float* evidence, int8_t* coordinate, uint8_t* packed, int8_t* moment_q,
                            uint16_t* moment_scale, uint16_t* row_v, uint16_t* col_v, int64_t rows,
                            int64_t cols, double beta1, double beta2, double update_clip,

@@ -45,13 +45,15 @@ def encode_activation(flat: Tensor) -> tuple[Tensor, Tensor]:
 # Layers that read the same input in one forward (a SwiGLU's gate and up
 # projections) share its encoding: the last input encoded, held weakly, with
 # its version counter and address.  Any backward clears it, so a reuse never
-# spans a training step.
+# spans a training step; and it is of one graph capture, or of none: an encoding
+# recorded into a graph has not run yet, and a graph that read one from before
+# it would not follow its input.
 _last_encoding: tuple | None = None
 
 
 def _encoding_of(inputs: Tensor, flat: Tensor, columns: int) -> tuple[Tensor, Tensor]:
     global _last_encoding
-    key = (inputs._version, inputs.data_ptr(), tuple(inputs.shape), inputs.dtype, columns)
+    key = (inputs._version, inputs.data_ptr(), tuple(inputs.shape), inputs.dtype, columns, kernels.capture_id(inputs))
     if _last_encoding is not None:
         ref, last_key, payload, aux = _last_encoding
         if ref() is inputs and last_key == key:
@@ -72,7 +74,7 @@ def remember_encoding(value: Tensor, payload: Tensor, aux: Tensor) -> None:
 
     global _last_encoding
     columns = int(value.shape[-1])
-    key = (value._version, value.data_ptr(), tuple(value.shape), value.dtype, columns)
+    key = (value._version, value.data_ptr(), tuple(value.shape), value.dtype, columns, kernels.capture_id(value))
     _last_encoding = (weakref.ref(value), key, payload, aux)
 
 

@@ -202,6 +202,14 @@ def stream_read(src: Tensor, groups: int | None = None) -> None:
                                     _stream(device)), "stream_read")
 
 
+def capture_id(t: Tensor) -> int:
+    """The number of the graph capture that ``t``'s device records into now, 0 for none (or a tensor on no GPU)."""
+
+    if not t.is_cuda or not torch.cuda.is_current_stream_capturing():
+        return 0
+    return _lib.load().qste_capture_id(_stream(t.device))
+
+
 def device_info(device=None) -> dict:
     """What the runtime reports for ``device``: compute units, maximum shader
     clock and memory clock (MHz), LDS bytes per compute unit."""

@@ -57,6 +57,7 @@ SIGNATURES = {
     "qste_stream_read": (_int, [_vp, _i64, _vp, _i64, _vp]),
     "qste_clock_probe": (_int, [_vp, _i64, _vp]),
     "qste_device_info": (_int, [_vp]),
+    "qste_capture_id": (ctypes.c_uint64, [_vp]),
     "qste_coordinate_update_static_limit": (_sz, []),
     "qste_coordinate_update_static": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _dbl, _dbl,
                                              _dbl, _dbl, _i64, _i64, _i64, _vp, _vp, _vp, _vp]),
