@@ -358,6 +358,20 @@ __device__ __forceinline__ float scale_left(float scale) {
   return held != 0.0f && __builtin_isfinite(held) ? c : 1.0f;
 }
 
+// v c; in fp16, whose end a gradient under a loss scale can come near, finite
+// where v rounds to a finite value: c is past 1 by half a step of the type, and by
+// up to a half for scales that are subnormal in it, so that the largest gradients
+// would pass the end in the evidence alone.  Held at the end the operand is nearer
+// than v would be.  (us, 8192 x 14336: fp16 267 -> 268.)
+template <int DT>
+__device__ __forceinline__ float evidence_operand(float v, float c) {
+  const float scaled = v * c;
+  if constexpr (DT == QSTE_F16)
+    return fabsf(v) < 65520.0f ? __builtin_amdgcn_fmed3f(scaled, -65504.0f, 65504.0f) : scaled;
+  else
+    return scaled;
+}
+
 // The backward with sums over the rows for the two binary layers that made g and u:
 // of dg off_g and du off_u, and with GATED also of dg and du, [2 or 4][cols].  A
 // workgroup takes 512 columns, eight a lane, of `chunk` rows, each wave every fourth
@@ -414,8 +428,8 @@ __global__ __launch_bounds__(kThreads) void backward_columns_kernel(
       const float left = scale_left<DT>(r.xs);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        a[i] *= left;
-        b[i] *= left;
+        a[i] = evidence_operand<DT>(a[i], left);
+        b[i] = evidence_operand<DT>(b[i], left);
       }
       blocks::store8<DT, ONCE>(ev.gate + t * ld + c, a);
       blocks::store8<DT, ONCE>(ev.up + t * ld + c, b);

@@ -169,3 +169,48 @@ def test_captured_after_a_forward_alone():
         torch.cuda.synchronize()
         kept = [t.clone() for t in captured]
         assert all(torch.equal(a, b) for a, b in zip(kept, step()))
+
+
+def test_evidence_of_the_largest_gradients():
+    """fp16 gradients at the end of the type's range under scales that it rounds down: where dg and du are finite the
+    evidence's operands are, and stay at the type's largest value where dg c passes it.
+
+    dg and du are within 2^-24 (|g| + 10) of theirs, relative (the exponential's argument, two units each for it and
+    the reciprocal, one for an addition or a product), times 4 for dg, a sum of terms of up to that size of it; c and
+    its product add 2; the operand is then rounded, by half a step."""
+
+    from qste_amd import kernels
+
+    dtype = torch.float16
+    e, most = torch.finfo(dtype).eps / 2, torch.finfo(dtype).max
+    # scales just below the middle between two values of the type, and subnormal ones
+    scales = [1 + e * (1 - 2.0 ** -8), 3 + 2 * e * (1 - 2.0 ** -8), 1.49 * 2.0 ** -24, 5.4 * 2.0 ** -24]
+    xs = torch.tensor(scales, device=DEV).repeat_interleave(8)
+    m = xs.numel()
+    # dg is dh at g = 20, du nearly dh at g = 1.2783
+    g = torch.full((m, 16), -3.0, device=DEV, dtype=dtype)
+    g[:, :4], g[:, 4:8] = 20.0, 1.2783
+    u = torch.ones(m, 16, device=DEV, dtype=dtype)
+    dh = torch.linspace(0.3, 1.0, m * 16, device=DEV).double().view(m, 16)
+    dh[:, :4] = dh[:, 4:8] = torch.linspace(0.99, 1.0, 4, device=DEV).double()
+    dh[::2] *= -1
+    dh = dh.mul(most).to(dtype)
+    both, operand, _ = kernels._gated_grads(dh, g, u, torch.zeros(m, device=DEV), xs)
+    a, d = g.double(), dh.double()
+    s = torch.sigmoid(a)
+    dy = torch.cat((d * u.double() * s * (1 + a * (1 - s)), d * a * s), 1)
+    c = (xs.double() / xs.to(dtype).double())[:, None]
+    held = torch.isfinite(both)
+    past = held & ((dy * c).abs() > most)
+    assert bool(past[:16, :16].any()) and bool(past[:16, 16:].any())  # the end is passed, by dg c and by du c
+    assert bool(torch.isfinite(operand)[held].all())
+    want = (dy * c).clamp(-most, most)
+    near = (operand.double() - want).abs() <= (e + 2.0 ** -24 * (4 * 30 + 2)) * want.abs()
+    assert bool(near[held].all())
+    packed = torch.randint(0, 256, (32, 8), generator=torch.Generator(device=DEV).manual_seed(1), device=DEV, dtype=torch.uint8)
+    payload = torch.full((m, 8), 255, dtype=torch.uint8, device=DEV)
+    finite = held.all(0)
+    assert bool(finite.any())
+    evidence = kernels.gated_backward(dh, g, u, payload, torch.zeros(m, device=DEV), xs, packed,
+                                      torch.ones(32, device=DEV), 64)[1]
+    assert bool(torch.isfinite(evidence[finite]).all())
