@@ -214,3 +214,30 @@ def test_evidence_of_the_largest_gradients():
     evidence = kernels.gated_backward(dh, g, u, payload, torch.zeros(m, device=DEV), xs, packed,
                                       torch.ones(32, device=DEV), 64)[1]
     assert bool(torch.isfinite(evidence[finite]).all())
+
+
+@pytest.mark.parametrize("cols", [64, 63])  # the wide pass, and an element a thread
+def test_fp32_gradients_of_a_checkpoint(cols):
+    """dg and du in fp32 at gates of -80 to 80.
+
+    In units of 2^-24, relative: 2 for e^-g, 1 for 1 + e^-g and 1 for the division, so s has 4 (e^-g's share in the sum
+    is at most all of it), 6 + 1 for e^-g s and its product.  For g > 0 the sum 1 + g e^-g s, whose second term is at
+    most 0.28 of the first, has 0.28 * 7 + 1 < 3, times s 4 + 1, times dh u 1 + 1: 10 in all.  For g < 0 the difference
+    1 - s is off by 4 s + 1 units of 1, s at most 1/2: 3 units, and 1 + g (1 - s) by 3 |g| + 1 of 1: (3 |g| + 1) of dh u s
+    beside the 7 of dg.  du: 4 for s and 1 for each of two products."""
+
+    from qste_amd import kernels
+
+    rows = 4096
+    g = torch.linspace(-80, 80, rows * cols, device=DEV).view(rows, cols)
+    u, dh = (_randn((rows, cols), torch.float32, seed) for seed in (1, 2))
+    kept = kernels.quantize_blocks(g), kernels.quantize_blocks(u)
+    a, b = (kernels.dequantize_blocks(t).double() for t in kept)
+    dg, du = kernels.swiglu_backward_blocks(dh, *kept)
+    s, unit = torch.sigmoid(a), 2.0 ** -24
+    one = dh.double() * b * s
+    want = one * (1 + a * (1 - s))
+    off = torch.where(a > 0, 10 * want.abs(), 7 * want.abs() + (3 * a.abs() + 1) * one.abs()) * unit + 1e-37
+    assert bool(((dg.double() - want).abs() <= off).all())
+    want = dh.double() * a * s
+    assert bool(((du.double() - want).abs() <= 6 * unit * want.abs() + 1e-37).all())
