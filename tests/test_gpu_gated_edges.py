@@ -241,3 +241,40 @@ def test_fp32_gradients_of_a_checkpoint(cols):
     assert bool(((dg.double() - want).abs() <= off).all())
     want = dh.double() * a * s
     assert bool(((du.double() - want).abs() <= 6 * unit * want.abs() + 1e-37).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m", [1, 65])  # the kernel for few rows, and the tiles
+def test_the_gate_at_every_value(m, dtype):
+    """silu(g) u at every 16-bit g, from layers whose values are their biases.
+
+    For g > -87 in units of 2^-24, relative: e^-g has -g for its argument's rounding, which counts where g < 0, and 2; 1
+    for the addition, 2 for the reciprocal, 1 for each of two products and 4 for the constant's rounding: max(-g, 0) +
+    10, and below 1 for the argument where g > 0.  Then half a step of the type, relative or of its least one.  Below
+    -87 |silu(g)| is under 2^-118 and may go to 0."""
+
+    from qste_amd import kernels
+    from qste_amd.kernels import _lib
+
+    e, most = torch.finfo(dtype).eps / 2, torch.finfo(dtype).max
+    tiny = 2.0 ** -25 if dtype == torch.float16 else 2.0 ** -126
+    every = torch.arange(-32768, 32768, dtype=torch.int32, device=DEV).to(torch.int16).view(dtype)
+    every = every[torch.isfinite(every)]
+    gate, features = every.float(), every.numel()
+    assert _lib.load().qste_gated_route(m, features, 1024, {torch.float16: 1, torch.bfloat16: 2}[dtype], 0) == (1 if m == 1 else 2)
+    x = torch.zeros(m, 1024, dtype=dtype, device=DEV)
+    bits = torch.full((features, 128), 255, dtype=torch.uint8, device=DEV)
+    scale = torch.ones(features, device=DEV)
+    for value in (1.0, -0.75, 1000.0 if dtype == torch.float16 else 1e30):
+        up = torch.full((features,), value, device=DEV).to(dtype).float()
+        h = kernels.gated_forward(x, bits, scale, gate, bits, scale, up, 1024)[0]
+        assert torch.equal(h[-1], h[0])
+        g, got = gate.double(), h[0].double()
+        want = g * torch.sigmoid(g) * up.double()
+        past = want.abs() * (1 - 2 * e) > most
+        inside = ~past & (want.abs() * (1 + 2 * e) < most)
+        assert bool(torch.isinf(h[0])[past].all()) and bool(torch.isfinite(h[0])[inside].all())
+        off = 2.0 ** -24 * ((-g).clamp(min=0) + 11) * want.abs()
+        bound = torch.where(g > -87, off + e * (want.abs() + off), want.abs() * (1 + e)) + tiny
+        assert bool(((got - want).abs() <= bound)[inside].all())
+        assert bool((got * want >= 0)[inside].all())  # of want's sign, or 0
