@@ -964,12 +964,14 @@ def swiglu_backward_blocks(grad: Tensor, gate: Blocks8, up: Blocks8, offset_gate
 
 
 def _layer_vector(t: Tensor | None, rows: int, what: str) -> Tensor | None:
-    """A layer's scale or bias as contiguous fp32 [rows]."""
+    """A layer's scale or bias, an entry per row in any shape, as contiguous fp32 [rows]."""
 
     if t is None:
         return None
     if t.shape != (rows,):
-        raise ValueError(f"{what} has shape {tuple(t.shape)}, expected ({rows},)")
+        if t.numel() != rows:
+            raise ValueError(f"{what} has shape {tuple(t.shape)}, expected ({rows},)")
+        t = t.reshape(rows)
     return t if t.dtype is torch.float32 and t.is_contiguous() else _f32(t)
 
 

@@ -278,3 +278,18 @@ def test_the_gate_at_every_value(m, dtype):
         bound = torch.where(g > -87, off + e * (want.abs() + off), want.abs() * (1 + e)) + tiny
         assert bool(((got - want).abs() <= bound)[inside].all())
         assert bool((got * want >= 0)[inside].all())  # of want's sign, or 0
+
+
+def test_scales_and_biases_in_a_column():
+    """Packed layers whose scale or bias is a column, which the layers themselves take."""
+
+    import qste_amd as qste
+
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    x = _randn((5, 64), torch.bfloat16, 2)
+    bits = [torch.randint(0, 256, (40, 8), generator=gen, device=DEV, dtype=torch.uint8) for _ in range(2)]
+    scale, bias = (torch.rand(40, generator=gen, device=DEV) for _ in range(2))
+    flat = [qste.PackedLinear(b, scale, 64, bias) for b in bits]
+    column = [qste.PackedLinear(b, scale[:, None], 64, bias[:, None]) for b in bits]
+    assert torch.equal(column[0](x), flat[0](x))
+    assert torch.equal(qste.nn.gated(x, *column), qste.nn.gated(x, *flat))
