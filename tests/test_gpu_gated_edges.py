@@ -293,3 +293,42 @@ def test_scales_and_biases_in_a_column():
     column = [qste.PackedLinear(b, scale[:, None], 64, bias[:, None]) for b in bits]
     assert torch.equal(column[0](x), flat[0](x))
     assert torch.equal(qste.nn.gated(x, *column), qste.nn.gated(x, *flat))
+
+
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("m,d,ffn", [(70, 128, 192), (300, 256, 640), (5, 64, 64)])
+def test_checkpointed_mlp_piece_by_piece(m, d, ffn, bias):
+    """Output, input gradient, evidence, scale and bias gradients of the three layers, bit for bit those of the kernels
+    that the node stands for."""
+
+    import qste_amd as qste
+    from qste_amd import kernels
+
+    gate, up, down = layers = _layer(ffn, d, m + 1, bias), _layer(ffn, d, m + 2, bias), _layer(d, ffn, m + 3, bias)
+    up.surface.log_scale.data = up.surface.log_scale.data.bfloat16()
+    x = (_randn((m, d), torch.bfloat16, 4) + 0.1).requires_grad_()
+    w = _randn((m, d), torch.bfloat16, 5)
+    y = qste.nn.swiglu_mlp(x, *layers, checkpoint=True)
+    y.backward(w)
+    sides = [[None if t is None else t.detach() for t in (layer.surface.packed_sign, layer.scale, layer.bias)]
+             for layer in layers]
+    flat = x.detach()
+    h, g, u = kernels.gated_forward(flat, *sides[0], *sides[1], d, keep="values")
+    assert torch.equal(y.detach(), kernels.packed_linear_affine(h, *sides[2], ffn))
+    dh, evidence_d, scale_d, bias_d = kernels.linear_backward(w, *kernels.pack_affine_rows(h), sides[2][0], sides[2][1], ffn,
+                                                              need_bias=bias)
+    dx, evidence, scales, biases = kernels.gated_backward(
+        dh, kernels.quantize_blocks(g), kernels.quantize_blocks(u), *kernels.pack_affine_rows(flat),
+        torch.cat((sides[0][0], sides[1][0])), torch.cat((sides[0][1].float(), sides[1][1].float())), d, need_bias=bias)
+    assert torch.equal(x.grad, dx)
+    parts = [(evidence[:ffn], scales[:ffn], biases[:ffn] if bias else None),
+             (evidence[ffn:], scales[ffn:], biases[ffn:] if bias else None), (evidence_d, scale_d, bias_d)]
+    for layer, (e, grad_scale, grad_bias) in zip(layers, parts):
+        log_scale = layer.surface.log_scale
+        assert len(layer.evidence) == 1 and torch.equal(layer.evidence[0], e)
+        # (the scale's gradient in the log-scale's type, times exp's value in it)
+        want = grad_scale.to(log_scale.dtype).float() * log_scale.detach().exp().float()
+        assert log_scale.grad.dtype == log_scale.dtype and torch.equal(log_scale.grad, want.to(log_scale.dtype))
+        if bias:
+            assert torch.equal(layer.bias.grad, grad_bias)
+    assert not torch.equal(gate.evidence[0], up.evidence[0])
