@@ -999,7 +999,12 @@ def gated_forward(inputs: Tensor, gate: Tensor, gate_scale: Tensor, gate_bias: T
     gs, us = _layer_vector(gate_scale, rows, "gate_scale"), _layer_vector(up_scale, rows, "up_scale")
     gb = None if gate_bias is None else _layer_vector(gate_bias, rows, "gate_bias")
     ub = None if up_bias is None else _layer_vector(up_bias, rows, "up_bias")
-    x, gate, up = _aligned(inputs), _aligned(gate), _aligned(up)
+    x = _aligned(inputs)
+    # the signs are contiguous already: in place of a second look by _aligned, 0.3 us
+    if gate.data_ptr() % 16:
+        gate = gate.clone()
+    if up.data_ptr() % 16:
+        up = up.clone()
     m = x.numel() // columns if columns else _leading(inputs)
     out = torch.empty((*x.shape[:-1], rows), dtype=x.dtype, device=device)
     g = u = None

@@ -334,3 +334,20 @@ def test_checkpointed_mlp_piece_by_piece(m, d, ffn, bias):
         if bias:
             assert torch.equal(layer.bias.grad, grad_bias)
     assert not torch.equal(gate.evidence[0], up.evidence[0])
+
+
+def test_signs_off_16_byte_steps():
+    from qste_amd import kernels
+
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    scale = torch.rand(40, generator=gen, device=DEV)
+    for m in (3, 90):
+        x = _randn((m, 128), torch.bfloat16, 2)
+        bits = [torch.randint(0, 256, (40, 16), generator=gen, device=DEV, dtype=torch.uint8) for _ in range(2)]
+        moved = []
+        for b in bits:
+            room = torch.empty(b.numel() + 3, dtype=torch.uint8, device=DEV)
+            moved.append(room[3:].view(40, 16).copy_(b))
+            assert moved[-1].is_contiguous() and moved[-1].data_ptr() % 16
+        got = kernels.gated_forward(x, moved[0], scale, None, moved[1], scale, None, 128)[0]
+        assert torch.equal(got, kernels.gated_forward(x, bits[0], scale, None, bits[1], scale, None, 128)[0])
