@@ -474,11 +474,13 @@ int qste_swiglu_backward_blocks(const void* grad, int dtype, const int8_t* gate_
                                 int64_t rows, int64_t cols, void* stream);
 
 /* qste_swiglu_backward_blocks that also sums its outputs against the offsets, as
- * qste_swiglu_backward_sums does (in an order of its own, and before dg and du are
- * rounded).
+ * qste_swiglu_backward_sums does (in an order of its own; with 16-bit dtypes and
+ * cols a multiple of 8 before dg and du are rounded).
  * ld: elements between the gradients' rows, cols, or with 16-bit dtypes and cols
  * a multiple of 8 any larger multiple of 8 (both gradients side by side in one
- * [rows, 2 cols] tensor: grad_up = grad_gate + cols, ld = 2 cols). */
+ * [rows, 2 cols] tensor: grad_up = grad_gate + cols, ld = 2 cols; for callers that
+ * go on with the two layers as one, as the autograd nodes do by
+ * qste_gated_backward). */
 size_t qste_swiglu_backward_blocks_sums_workspace_bytes(int64_t rows, int64_t cols);
 int qste_swiglu_backward_blocks_sums(const void* grad, int dtype, const int8_t* gate_payload,
                                      const uint8_t* gate_codes, const int8_t* up_payload, const uint8_t* up_codes,

@@ -133,9 +133,9 @@ struct Pair {
 
 // ONCE, here and below: what is written is stored without keeping its lines
 // (blocks::streamed).  us, kept / streamed, 16384 x 14336 in bf16: the forward with
-// blocks 404 / 393, with the encoding too 414 / 400, the backward 399 / 381, with
-// the sums 380 / 372; 4096 x 4096, whose gradients the next product finds in the
-// cache, 30.6 / 31.3 with the sums (all before later steps took a little off).
+// blocks 403 / 389, with the encoding too 401 / 397, the backward 399 / 383, with
+// the sums 364 / 354, of a gated block 551 / 532; 4096 x 4096, whose gradients the
+// next product finds in the cache, 29.1 / 28.8 and 39.5 / 39.8.
 
 // Chunk q of a row of g and of u (zeros past the row) to their blocks, the four
 // lanes of a block together.
@@ -831,8 +831,12 @@ int launch_quantize_blocks(const void*, int, int8_t*, uint8_t*, int64_t, int64_t
 namespace swiglu {
 
 inline bool aligned8(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7) == 0; }
-// whether the forward, which writes h and two bytes an element, and the backward,
-// which writes two tensors, stream them
+// Whether the forward, which writes h and two bytes an element, and the backward,
+// which writes two tensors, stream them.  A gated block's backward writes four and
+// goes by two of them: between 256 and 512 MiB the pass by itself gains when it
+// streams, and the products that then read what it wrote lose as much.  us, kept /
+// streamed, pass and whole step: 8192 x 5120 (1024 inputs) 110 / 85 and 642 / 638, 8192 x
+// 7168 (2048) 147 / 116 and 1285 / 1290, 4096 x 14336 (4096) 145 / 116 and 2337 / 2341.
 inline bool forward_once(int64_t rows, int64_t cols, int dtype) {
   return blocks::streamed(static_cast<double>(rows) * cols * (dtype == QSTE_F32 ? 6 : 4));
 }

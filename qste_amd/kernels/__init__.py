@@ -922,7 +922,9 @@ def swiglu_backward_blocks(grad: Tensor, gate: Blocks8, up: Blocks8, offset_gate
                            offset_up: Tensor | None = None, *, side_by_side: bool = False):
     """The gradients of ``silu(gate) * up`` at the gate and up that 8-bit blocks stand
     for, ``(grad_gate, grad_up)``, rounded once; with offsets fp32 [rows] also their
-    sums, laid out as ``swiglu_backward_sums`` does (``side_by_side`` as there)."""
+    sums, laid out as ``swiglu_backward_sums`` does (``side_by_side`` as there, for
+    callers of these functions: the autograd nodes that run two layers as one take
+    ``gated_backward``'s pass)."""
 
     gate, up = _check_blocks(gate, "gate blocks"), _check_blocks(up, "up blocks")
     device = _require_gpu(grad, gate.payload, gate.codes, up.payload, up.codes, offset_gate, offset_up)
