@@ -92,7 +92,7 @@ def _plain(layer) -> bool:
     """Whether a layer computes what QSTELinear or PackedLinear does: a forward of a subclass's or an instance's own
     is called, not stood for."""
 
-    return getattr(layer.forward, "__func__", None) in _LAYER_FORWARDS
+    return getattr(getattr(layer, "forward", None), "__func__", None) in _LAYER_FORWARDS
 
 
 def gated(inputs: Tensor, gate, up, *, checkpoint: bool = False) -> Tensor:

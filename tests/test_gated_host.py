@@ -80,3 +80,11 @@ def test_mlp_of_packed_layers_goes_layer_by_layer():
     for checkpoint in (False, True):
         with pytest.raises(RuntimeError, match="GPU only"):
             qste.nn.swiglu_mlp(torch.zeros(2, 128), gate, up, down, checkpoint=checkpoint)
+
+
+def test_mlp_of_functions(monkeypatch):
+    """Anything that can be called is composed."""
+
+    monkeypatch.setattr(qste.nn, "swiglu", lambda g, u, *, checkpoint=False: g * u)
+    got = qste.nn.swiglu_mlp(torch.ones(2, 8), lambda x: x * 2, lambda x: x * 3, lambda x: x + 1)
+    assert torch.equal(got, torch.full((2, 8), 7.0))
