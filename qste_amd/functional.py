@@ -53,6 +53,8 @@ _last_encoding: tuple | None = None
 
 def _encoding_of(inputs: Tensor, flat: Tensor, columns: int) -> tuple[Tensor, Tensor]:
     global _last_encoding
+    if inputs.is_inference():  # has no version to be remembered by
+        return encode_activation(flat)
     key = (inputs._version, inputs.data_ptr(), tuple(inputs.shape), inputs.dtype, columns, kernels.capture_id(inputs))
     if _last_encoding is not None:
         ref, last_key, payload, aux = _last_encoding

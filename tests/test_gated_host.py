@@ -88,3 +88,17 @@ def test_mlp_of_functions(monkeypatch):
     monkeypatch.setattr(qste.nn, "swiglu", lambda g, u, *, checkpoint=False: g * u)
     got = qste.nn.swiglu_mlp(torch.ones(2, 8), lambda x: x * 2, lambda x: x * 3, lambda x: x + 1)
     assert torch.equal(got, torch.full((2, 8), 7.0))
+
+
+def test_encoding_of_an_inference_tensor(monkeypatch):
+    """Layers in inference mode: their inputs have no version counter, so no encoding is remembered of them."""
+
+    from qste_amd import functional
+
+    monkeypatch.setattr(functional, "encode_activation", lambda flat: (flat, flat + 1))
+    functional.forget_encodings()
+    with torch.inference_mode():
+        x = torch.zeros(2, 8)
+        payload, aux = functional._encoding_of(x, x, 8)
+        assert torch.equal(aux, payload + 1)
+    assert functional._last_encoding is None

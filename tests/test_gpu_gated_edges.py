@@ -351,3 +351,22 @@ def test_signs_off_16_byte_steps():
             assert moved[-1].is_contiguous() and moved[-1].data_ptr() % 16
         got = kernels.gated_forward(x, moved[0], scale, None, moved[1], scale, None, 128)[0]
         assert torch.equal(got, kernels.gated_forward(x, bits[0], scale, None, bits[1], scale, None, 128)[0])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_in_inference_mode(dtype):
+    """Training layers on inference tensors, as one node and one by one, give what they give without gradients."""
+
+    import qste_amd as qste
+
+    layers = _layer(192, 64, 1), _layer(192, 64, 2), _layer(64, 192, 3)
+    x = _randn((10, 64), dtype, 4)
+    for checkpoint in (False, True):
+        calls = (lambda t: qste.nn.gated(t, *layers[:2], checkpoint=checkpoint),
+                 lambda t: qste.nn.swiglu_mlp(t, *layers, checkpoint=checkpoint), lambda t: layers[2](layers[0](t)))
+        for call in calls:
+            with torch.no_grad():
+                want = call(x)
+            with torch.inference_mode():
+                assert torch.equal(call(x * 1), want)
+    assert all(layer.surface.ledger.open_uses == 0 for layer in layers)
